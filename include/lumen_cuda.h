@@ -500,6 +500,121 @@ int lc_ring_deep_clone(const lc_ring* ring, lc_ring** out);
 
 void lc_ring_destroy(lc_ring* ring);
 
+/* ---- the uncompressed paged cache ----------------------------------------
+ * The layers that a model keeps uncompressed (the reference's sliding layers
+ * and every layer with TurboQuant off: plain K and V buffers,
+ * native_cache.rs:65-335) next to the compressed ones, for many sequences:
+ * caller-owned pools of pages in f32, bf16 or f16, decode attention over them,
+ * eviction by accumulated attention weight, and the reordering of beams.
+ *
+ * Pools: k_pages and v_pages, the same shape and strides: row (layer, page,
+ * head, slot) of head_dim contiguous elements. Tables: int32 [n_seqs][width]
+ * of page ids, slot t of a sequence in its page t / page_tokens; lens: int32
+ * [n_seqs]. Pools, tables, lens and every tensor of these calls are memory of
+ * the handle's device (LC_ERR_INVALID for host memory); nothing is copied to
+ * the host and no call synchronises, so calls can be captured in a CUDA graph
+ * after a first one outside (which may allocate the handle's workspace).
+ * Lengths and page ids are read on the device: a length beyond the table is
+ * cut to it, a page id outside the pool is not accessed, and both are told by
+ * lc_paged_status. Calls of one handle are ordered across streams (replays of
+ * a captured graph are the caller's to order against other calls). */
+typedef struct lc_paged lc_paged;
+
+typedef struct lc_paged_config {
+  int32_t n_layers, n_kv_heads, head_dim, page_tokens; /* head_dim <= 256, page_tokens <= 4096 */
+  int64_t n_pages;
+  /* element strides of the pools; all 0: contiguous
+   * [n_layers][n_pages][n_kv_heads][page_tokens][head_dim] */
+  int64_t layer_stride, page_stride, head_stride, token_stride;
+  int32_t dtype;             /* LC_F32, LC_BF16 or LC_F16 */
+  int32_t device;
+  int32_t max_seqs;          /* rows of one call, <= 2048 */
+  int32_t max_pages_per_seq; /* widest table */
+  int32_t max_q_heads;
+  int32_t reserved;          /* 0 */
+} lc_paged_config;
+
+/* The pools are borrowed until lc_paged_destroy. */
+int lc_paged_create(const lc_paged_config* config, void* k_pages, void* v_pages, lc_paged** out);
+void lc_paged_destroy(lc_paged* p);
+
+/* LC_ERR_INVALID once a call met a length beyond its table, a page id outside
+ * the pool or a parent outside its group (that call's output is unspecified).
+ * Reads a host word: synchronise first to hear of calls in flight. */
+int lc_paged_status(const lc_paged* p);
+
+/* Write keys / values [n_seqs][n_kv_heads][n_tokens][head_dim] of `dtype` to
+ * slots lens[s] .. lens[s] + n_tokens - 1 of `layer` (rounded to the pool's
+ * type). lens is the caller's to advance, once for all layers. pos (may be
+ * NULL): int32 [n_seqs][n_kv_heads][pos_stride], slot's position pos0[s] + i
+ * of the i-th token (kept for lc_paged_evict). */
+int lc_paged_append(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* tables, int32_t width,
+                    const int32_t* lens, const void* keys, const void* values, int32_t dtype, int64_t n_tokens,
+                    int32_t* pos, int64_t pos_stride, const int32_t* pos0, void* stream);
+
+/* Decode attention, one query token per sequence: out = softmax(scale q K^T) V
+ * over the last `window` of the lens[s] slots (0: all of them), GQA as
+ * lc_decode_attn; q, out [n_seqs][n_q_heads][head_dim]. Sums and softmax in
+ * f32. A sequence of length 0, or without a finite score, gives zeros. */
+int lc_paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* tables, int32_t width,
+                  const int32_t* lens, const void* q, int32_t q_dtype, int32_t n_q_heads, float scale, int32_t window,
+                  void* out, int32_t out_dtype, void* stream);
+
+/* lc_paged_attn, and acc_out[s][h][t] = decay * acc_in[s][h][t] + the sum over
+ * kv head h's query heads of slot t's attention weight, for t < lens[s] (other
+ * entries are not written). acc: f32 [n_seqs][n_kv_heads][acc_stride]; acc_out
+ * may be acc_in. */
+int lc_paged_attn_weights(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* tables, int32_t width,
+                          const int32_t* lens, const void* q, int32_t q_dtype, int32_t n_q_heads, float scale,
+                          int32_t window, void* out, int32_t out_dtype, const float* acc_in, float* acc_out,
+                          int64_t acc_stride, float decay, void* stream);
+
+/* Cut every (sequence, kv head) of `layer` longer than `budget` to the budget
+ * slots with the largest accumulated weight (equal ones: the lower slot; NaN
+ * below all); positions below n_sink and the newest n_recent always stay
+ * (n_sink + n_recent <= budget). The i-th freed slot below budget takes the
+ * i-th kept slot at or past it: its K and V rows, acc and pos; other slots do
+ * not move, so slots are no longer in order of position (and a `window` no
+ * longer names the newest tokens). acc_out and pos_out of slots budget ..
+ * lens[s] - 1 become 0 and -1; shorter sequences are copied. The new length,
+ * min(lens[s], budget), is the caller's to set once all layers are cut.
+ * acc, pos: [n_seqs][n_kv_heads][stride]; the outputs may be the inputs. Pages
+ * must not be shared between sequences. */
+int lc_paged_evict(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* tables, int32_t width,
+                   const int32_t* lens, int32_t budget, int32_t n_sink, int32_t n_recent, const float* acc_in,
+                   const int32_t* pos_in, float* acc_out, int32_t* pos_out, int64_t stride, void* stream);
+
+/* Beams change places: row j of group g continues row parents[g][j]. tables
+ * and tables_out: [n_groups * n_beams][width], lens: [n_groups] (a group's
+ * beams are equally long). Pages before the one that the next token goes to
+ * are full, never written again, and shared: row j takes its parent's. The
+ * tail page (where it is partly filled) is every row's own: a parent's first
+ * child keeps it; the i-th other child takes the tail page of the i-th row
+ * without children, into which the parent's tokens are copied (all layers and
+ * heads). Later pages stay with row j. tables_out must not overlap tables. */
+int lc_paged_reorder(lc_paged* p, int32_t n_groups, int32_t n_beams, const int32_t* tables, int32_t width,
+                     const int32_t* lens, const int32_t* parents, int32_t* tables_out, void* stream);
+
+/* ---- beam search's selection ---------------------------------------------- */
+typedef struct lc_beam lc_beam;
+
+/* Workspace for lc_beam_select: up to n_groups groups of n_beams (<= 64) rows
+ * of `vocab` logits, n_out (<= 64) chosen of each group. */
+int lc_beam_create(int32_t n_groups, int32_t n_beams, int64_t vocab, int32_t n_out, int32_t device, lc_beam** out);
+void lc_beam_destroy(lc_beam* b);
+
+/* Of every group's totals scores[b] + log_softmax(logits[b])[v] the n_out
+ * largest, best first, equal ones by lower b * vocab + v: scores_out, parents,
+ * tokens, finished_out [n_groups][n_out]. logits [n_groups * n_beams] rows
+ * row_stride elements apart, scores f32. A row with finished set (may be NULL)
+ * has the one candidate (pad, its score); -inf and NaN totals are none.
+ * finished_out: the parent was finished, or the token is eos. A place without
+ * a candidate holds -inf, parent place % n_beams, pad, finished. All tensors
+ * are device memory; outputs must not overlap inputs. */
+int lc_beam_select(lc_beam* b, int32_t n_groups, const void* logits, int32_t dtype, int64_t row_stride,
+                   const float* scores, const uint8_t* finished, int32_t eos, int32_t pad, float* scores_out,
+                   int32_t* parents, int32_t* tokens, uint8_t* finished_out, void* stream);
+
 /* Library version string. */
 const char* lc_version(void);
 

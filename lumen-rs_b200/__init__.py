@@ -8,6 +8,8 @@ meaning and error behaviour follow rabbitson87/lumen-rs:
   KVCache (trait) / SimpleCache             crates/turboquant-cache/src/{traits,simple}.rs
   NativeRotatingKvCacheTurboQuant           crates/lumen-mlx/src/native_cache.rs:1517-1862
   CudaKvCache                               the multi-sequence device cache the above sit on
+  PagedKvCache / BeamSearch                 uncompressed layers over caller-owned pages, with eviction
+                                            by attention weight, and beam search (no counterpart)
 
 There is no CPU fallback: every operation runs the sm_100a kernels through
 the C ABI, and importing this package fails if the library is missing.
@@ -25,7 +27,7 @@ import numpy as np
 
 __all__ = [
     "LumenError", "lib", "TurboQuantConfig", "TurboQuantCompressor", "CudaKvCache", "KVCache", "SimpleCache",
-    "NativeRotatingKvCacheTurboQuant", "RawRing", "SplitGroup", "packed_words", "LC_F32", "LC_BF16", "LC_F16",
+    "NativeRotatingKvCacheTurboQuant", "RawRing", "SplitGroup", "PagedKvCache", "BeamSearch", "packed_words", "LC_F32", "LC_BF16", "LC_F16",
     "LC_Q_ROTATED", "LC_OUT_ROTATED", "LC_STORE_K_QJL", "LC_STORE_V_QJL",
 ]
 
@@ -54,6 +56,8 @@ ABI_SYMBOLS = [
     "lc_ring_create",
     "lc_ring_update", "lc_ring_truncate_to", "lc_ring_counters", "lc_ring_read", "lc_ring_clear",
     "lc_ring_deep_clone", "lc_ring_destroy", "lc_version", "lc_save_lkv2", "lc_load_lkv2", "lc_lkv2_info",
+    "lc_paged_create", "lc_paged_destroy", "lc_paged_status", "lc_paged_append", "lc_paged_attn", "lc_paged_attn_weights",
+    "lc_paged_evict", "lc_paged_reorder", "lc_beam_create", "lc_beam_destroy", "lc_beam_select",
 ]
 
 
@@ -77,6 +81,15 @@ class lc_cache_config(C.Structure):
 class lc_fetch_out(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in
                 ("k_words", "k_sigma", "v_words", "v_sigma", "k_qjl", "k_rnorm", "v_qjl", "v_rnorm")]
+
+
+class lc_paged_config(C.Structure):
+    _fields_ = [
+        ("n_layers", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_tokens", C.c_int32),
+        ("n_pages", C.c_int64), ("layer_stride", C.c_int64), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
+        ("token_stride", C.c_int64), ("dtype", C.c_int32), ("device", C.c_int32), ("max_seqs", C.c_int32),
+        ("max_pages_per_seq", C.c_int32), ("max_q_heads", C.c_int32), ("reserved", C.c_int32),
+    ]
 
 
 _lib = None
@@ -147,6 +160,18 @@ def lib():
         "lc_ring_clear": (C.c_int, [vp]),
         "lc_ring_deep_clone": (C.c_int, [vp, pp]),
         "lc_ring_destroy": (None, [vp]),
+        "lc_paged_create": (C.c_int, [C.POINTER(lc_paged_config), vp, vp, pp]),
+        "lc_paged_destroy": (None, [vp]),
+        "lc_paged_status": (C.c_int, [vp]),
+        "lc_paged_append": (C.c_int, [vp, i32, i32, vp, i32, vp, vp, vp, i32, i64, vp, i64, vp, vp]),
+        "lc_paged_attn": (C.c_int, [vp, i32, i32, vp, i32, vp, vp, i32, i32, C.c_float, i32, vp, i32, vp]),
+        "lc_paged_attn_weights": (C.c_int, [vp, i32, i32, vp, i32, vp, vp, i32, i32, C.c_float, i32, vp, i32, vp, vp, i64,
+                                            C.c_float, vp]),
+        "lc_paged_evict": (C.c_int, [vp, i32, i32, vp, i32, vp, i32, i32, i32, vp, vp, vp, vp, i64, vp]),
+        "lc_paged_reorder": (C.c_int, [vp, i32, i32, vp, i32, vp, vp, vp, vp]),
+        "lc_beam_create": (C.c_int, [i32, i32, i64, i32, i32, pp]),
+        "lc_beam_destroy": (None, [vp]),
+        "lc_beam_select": (C.c_int, [vp, i32, vp, i32, i64, vp, vp, i32, i32, vp, vp, vp, vp, vp]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)
@@ -799,3 +824,216 @@ class NativeRotatingKvCacheTurboQuant:
     def clear(self):
         if self._ring is not None:
             self._ring.clear()
+
+
+# ---------------------------------------------------------------------------
+# The uncompressed paged cache and beam search
+# ---------------------------------------------------------------------------
+def _dev(x, name: str, shape, dtype: str, device: int) -> int:
+    """Address of a contiguous CUDA tensor of this shape and type on `device`."""
+    if not x.is_cuda or x.device.index != device:
+        raise ValueError(f"{name} must be a tensor on cuda:{device}")
+    if x.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(x.shape)}")
+    if dtype is not None and _TORCH_NAMES.get(x.dtype) != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {x.dtype}")
+    if not x.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return x.data_ptr()
+
+
+class _TorchNames(dict):
+    """torch dtype -> short name, filled at first use (torch is not imported with the package)."""
+
+    def get(self, key, default=None):
+        if not self:
+            import torch
+
+            self.update({torch.float32: "f32", torch.bfloat16: "bf16", torch.float16: "f16", torch.int32: "int32",
+                         torch.uint8: "uint8"})
+        return dict.get(self, key, default)
+
+
+_TORCH_NAMES = _TorchNames()
+_FLOAT_CODES = {"f32": LC_F32, "bf16": LC_BF16, "f16": LC_F16}
+
+
+def _float_code(x, name: str) -> int:
+    code = _FLOAT_CODES.get(_TORCH_NAMES.get(x.dtype))
+    if code is None:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}")
+    return code
+
+
+class PagedKvCache:
+    """Decode over an uncompressed paged cache (lc_paged): pools k_pages and
+    v_pages [n_layers, n_pages, n_kv_heads, page_tokens, head_dim] on the GPU,
+    contiguous in the last dimension (a permuted view of another page layout
+    will do), owned by the caller and borrowed by this object. In every call
+    tables is int32 [n_seqs, pages] and lens int32 [n_seqs], on the GPU."""
+
+    def __init__(self, k_pages, v_pages, *, max_seqs: int, max_pages_per_seq: int, max_q_heads: int):
+        if k_pages.dim() != 5 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+            raise ValueError("k_pages and v_pages must be [n_layers, n_pages, n_kv_heads, page_tokens, head_dim] alike")
+        if not k_pages.is_cuda or v_pages.device != k_pages.device:
+            raise ValueError("k_pages and v_pages must be on one GPU")
+        if v_pages.stride() != k_pages.stride() or (k_pages.shape[4] > 1 and k_pages.stride(4) != 1):
+            raise ValueError("k_pages and v_pages must have the same strides, 1 in the last dimension")
+        self.k_pages, self.v_pages = k_pages, v_pages
+        self.n_layers, self.n_pages, self.n_kv_heads, self.page_tokens, self.head_dim = k_pages.shape
+        self.device = k_pages.device.index
+        cfg = lc_paged_config()
+        cfg.n_layers, cfg.n_kv_heads, cfg.head_dim, cfg.page_tokens = (self.n_layers, self.n_kv_heads, self.head_dim,
+                                                                       self.page_tokens)
+        cfg.n_pages = self.n_pages
+        cfg.layer_stride, cfg.page_stride, cfg.head_stride, cfg.token_stride = k_pages.stride()[:4]
+        cfg.dtype, cfg.device = _float_code(k_pages, "k_pages"), self.device
+        cfg.max_seqs, cfg.max_pages_per_seq, cfg.max_q_heads = max_seqs, max_pages_per_seq, max_q_heads
+        h = C.c_void_p()
+        _check(lib().lc_paged_create(C.byref(cfg), k_pages.data_ptr(), v_pages.data_ptr(), C.byref(h)))
+        self._h = h
+
+    def close(self):
+        h = getattr(self, "_h", None)
+        if h is not None and _lib is not None:
+            _lib.lc_paged_destroy(h)
+            self._h = None
+
+    __del__ = close
+
+    def _rows(self, tables, lens):
+        n = tables.shape[0]
+        return n, _dev(tables, "tables", (n, tables.shape[1]), "int32", self.device), tables.shape[1], \
+            _dev(lens, "lens", (n,), "int32", self.device)
+
+    def status(self) -> int:
+        """LC_OK, or LC_ERR_INVALID once a finished call met a length, page id or parent out of range."""
+        return lib().lc_paged_status(self._h)
+
+    def append(self, layer: int, tables, lens, keys, values, pos=None, pos0=None, stream=None):
+        """Write keys / values [n_seqs, n_kv_heads, n_tokens, head_dim] behind the lens[s] slots of
+        each sequence (lens is not advanced) and, with pos int32 [n_seqs, n_kv_heads, tokens] and pos0
+        int32 [n_seqs], the new slots' positions."""
+        n, t, width, ln = self._rows(tables, lens)
+        shape = (n, self.n_kv_heads, keys.shape[2], self.head_dim)
+        if values.dtype != keys.dtype:
+            raise TypeError("keys and values must have one type")
+        k, v = _dev(keys, "keys", shape, None, self.device), _dev(values, "values", shape, None, self.device)
+        at = p0 = None
+        span = 0
+        if pos is not None:
+            span = pos.shape[2]
+            at = _dev(pos, "pos", (n, self.n_kv_heads, span), "int32", self.device)
+            p0 = _dev(pos0, "pos0", (n,), "int32", self.device)
+        _check(lib().lc_paged_append(self._h, layer, n, t, width, ln, k, v, _float_code(keys, "keys"), keys.shape[2], at,
+                                     span, p0, _auto_stream(stream, keys)))
+
+    def attn(self, layer: int, tables, lens, q, scale: float, window: int = 0, out=None, stream=None):
+        """softmax(scale q K^T) V for one query token per sequence, q [n_seqs, n_q_heads, head_dim],
+        over the last `window` slots (0: all); out like q unless given."""
+        n, t, width, ln = self._rows(tables, lens)
+        heads = q.shape[1]
+        shape = (n, heads, self.head_dim)
+        if out is None:
+            out = q.new_empty(shape)
+        _check(lib().lc_paged_attn(self._h, layer, n, t, width, ln, _dev(q, "q", shape, None, self.device),
+                                   _float_code(q, "q"), heads, scale, window, _dev(out, "out", shape, None, self.device),
+                                   _float_code(out, "out"), _auto_stream(stream, q)))
+        return out
+
+    def attn_weights(self, layer: int, tables, lens, q, scale: float, acc_in, acc_out=None, decay: float = 1.0,
+                     window: int = 0, out=None, stream=None):
+        """attn(), and acc_out = decay * acc_in + each slot's attention weight summed over its kv head's
+        query heads; acc f32 [n_seqs, n_kv_heads, tokens], acc_out acc_in itself unless given."""
+        n, t, width, ln = self._rows(tables, lens)
+        heads, span = q.shape[1], acc_in.shape[2]
+        shape, rows = (n, heads, self.head_dim), (n, self.n_kv_heads, span)
+        if out is None:
+            out = q.new_empty(shape)
+        acc_out = acc_in if acc_out is None else acc_out
+        _check(lib().lc_paged_attn_weights(
+            self._h, layer, n, t, width, ln, _dev(q, "q", shape, None, self.device), _float_code(q, "q"), heads, scale,
+            window, _dev(out, "out", shape, None, self.device), _float_code(out, "out"),
+            _dev(acc_in, "acc_in", rows, "f32", self.device), _dev(acc_out, "acc_out", rows, "f32", self.device), span,
+            decay, _auto_stream(stream, q)))
+        return out
+
+    def evict(self, layer: int, tables, lens, budget: int, acc_in, pos_in, acc_out=None, pos_out=None, n_sink: int = 0,
+              n_recent: int = 0, stream=None):
+        """Cut sequences longer than `budget` to their budget heaviest slots (and the first n_sink and
+        newest n_recent positions), moving kept slots into freed ones; acc f32 and pos int32
+        [n_seqs, n_kv_heads, tokens], in place unless outputs are given. The lengths become
+        min(lens, budget), for the caller to set after the last layer."""
+        n, t, width, ln = self._rows(tables, lens)
+        span = acc_in.shape[2]
+        rows = (n, self.n_kv_heads, span)
+        acc_out = acc_in if acc_out is None else acc_out
+        pos_out = pos_in if pos_out is None else pos_out
+        _check(lib().lc_paged_evict(
+            self._h, layer, n, t, width, ln, budget, n_sink, n_recent, _dev(acc_in, "acc_in", rows, "f32", self.device),
+            _dev(pos_in, "pos_in", rows, "int32", self.device), _dev(acc_out, "acc_out", rows, "f32", self.device),
+            _dev(pos_out, "pos_out", rows, "int32", self.device), span, _auto_stream(stream, acc_in)))
+
+    def reorder(self, tables, lens, parents, tables_out=None, stream=None):
+        """Beams change places: row j of each group continues row parents[g, j] (int32 [n_groups, n_beams]);
+        tables int32 [n_groups * n_beams, pages], lens int32 [n_groups]. Full pages are shared, partly
+        filled ones kept or copied. Returns the new tables."""
+        groups, beams = parents.shape
+        shape = (groups * beams, tables.shape[1])
+        t = _dev(tables, "tables", shape, "int32", self.device)
+        if tables_out is None:
+            tables_out = tables.new_empty(shape)
+        _check(lib().lc_paged_reorder(self._h, groups, beams, t, shape[1],
+                                      _dev(lens, "lens", (groups,), "int32", self.device),
+                                      _dev(parents, "parents", (groups, beams), "int32", self.device),
+                                      _dev(tables_out, "tables_out", shape, "int32", self.device),
+                                      _auto_stream(stream, tables)))
+        return tables_out
+
+
+class BeamSearch:
+    """Beam search's selection over beams and vocabulary (lc_beam), for up to
+    n_groups groups of n_beams rows; n_out (n_beams unless given) are chosen."""
+
+    def __init__(self, n_groups: int, n_beams: int, vocab: int, n_out: Optional[int] = None, device: int = 0):
+        self.n_groups, self.n_beams, self.vocab, self.device = n_groups, n_beams, vocab, device
+        self.n_out = n_beams if n_out is None else n_out
+        h = C.c_void_p()
+        _check(lib().lc_beam_create(n_groups, n_beams, vocab, self.n_out, device, C.byref(h)))
+        self._h = h
+
+    def close(self):
+        h = getattr(self, "_h", None)
+        if h is not None and _lib is not None:
+            _lib.lc_beam_destroy(h)
+            self._h = None
+
+    __del__ = close
+
+    def select(self, logits, scores, finished=None, *, eos_id: int = -1, pad_id: int = 0, stream=None):
+        """The n_out best totals scores + log_softmax(logits) of each group, best first: (scores f32,
+        parents int32, tokens int32, finished uint8), each [groups, n_out]. logits [groups, n_beams, vocab]
+        (rows may be strided), scores f32 and finished uint8 [groups, n_beams]. A finished beam has the
+        one candidate pad_id at its score."""
+        g = logits.shape[0]
+        rows = (g, self.n_beams)
+        if not logits.is_cuda or logits.device.index != self.device:
+            raise ValueError(f"logits must be a tensor on cuda:{self.device}")
+        if logits.shape != (g, self.n_beams, self.vocab):
+            raise ValueError(f"logits must have shape {(g, self.n_beams, self.vocab)}, got {tuple(logits.shape)}")
+        stride = logits.stride()
+        row = stride[1] if self.n_beams > 1 else stride[0] if g > 1 else self.vocab
+        if (self.vocab > 1 and stride[2] != 1) or (g > 1 and self.n_beams > 1 and stride[0] != self.n_beams * row):
+            raise ValueError("logits must be rows of contiguous values, evenly apart")
+        import torch
+
+        shape = (g, self.n_out)
+        out = torch.empty((3,) + shape, dtype=torch.int32, device=logits.device)
+        fin = torch.empty(shape, dtype=torch.uint8, device=logits.device)
+        base, step = out.data_ptr(), 4 * g * self.n_out
+        _check(lib().lc_beam_select(
+            self._h, g, logits.data_ptr(), _float_code(logits, "logits"), row,
+            _dev(scores, "scores", rows, "f32", self.device),
+            None if finished is None else _dev(finished, "finished", rows, "uint8", self.device), eos_id, pad_id, base,
+            base + step, base + 2 * step, fin.data_ptr(), _auto_stream(stream, logits)))
+        return out[0].view(torch.float32), out[1], out[2], fin

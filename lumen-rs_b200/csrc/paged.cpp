@@ -1,0 +1,505 @@
+// Host side of the uncompressed paged cache (lc_paged_*) and of beam
+// selection (lc_beam_*): argument checks, workspaces, stream order.
+#include <algorithm>
+#include <memory>
+#include <string>
+
+#include "paged.h"
+
+using namespace lc;
+
+namespace {
+
+int element_size(int32_t dtype) { return dtype == LC_F32 ? 4 : 2; }
+
+void check_dtype(int32_t dtype, const char* what) {
+  LC_REQUIRE(dtype == LC_F32 || dtype == LC_BF16 || dtype == LC_F16, LC_ERR_INVALID,
+             std::string(what) + ": unknown dtype " + std::to_string(dtype));
+}
+
+// Memory that kernels on `device` may read: that device's own, or managed.
+void check_device(const void* p, int device, const char* what, size_t align) {
+  LC_REQUIRE(p, LC_ERR_INVALID, std::string(what) + ": null pointer");
+  cudaPointerAttributes at;
+  const cudaError_t e = cudaPointerGetAttributes(&at, p);
+  if (e != cudaSuccess) cudaGetLastError();
+  LC_REQUIRE(e == cudaSuccess && (at.type == cudaMemoryTypeManaged ||
+                                  (at.type == cudaMemoryTypeDevice && at.device == device)),
+             LC_ERR_INVALID, std::string(what) + ": not memory of the handle's device");
+  LC_REQUIRE((reinterpret_cast<uintptr_t>(p) & (align - 1)) == 0, LC_ERR_INVALID,
+             std::string(what) + ": pointer not aligned to its elements");
+}
+
+// The calling thread's device, put back at the end of a call.
+struct DeviceScope {
+  int before = -1;
+  explicit DeviceScope(int device) {
+    LC_CUDA(cudaGetDevice(&before));
+    if (before != device) LC_CUDA(cudaSetDevice(device));
+    now = device;
+  }
+  ~DeviceScope() {
+    if (before >= 0 && before != now) cudaSetDevice(before);
+  }
+  int now = -1;
+};
+
+// A device buffer that grows. Growing waits for the stream order (the
+// device) that cudaFree brings, so a shorter buffer is never freed in use.
+struct Workspace {
+  void* p = nullptr;
+  size_t bytes = 0;
+  ~Workspace() {
+    if (p) cudaFree(p);
+  }
+  void* get(size_t need, bool zeroed = false) {
+    if (need > bytes) {
+      if (p) cudaFree(p);
+      p = nullptr;
+      bytes = 0;
+      const cudaError_t e = cudaMalloc(&p, need);
+      if (e != cudaSuccess) {
+        cudaGetLastError();
+        p = nullptr;
+        LC_THROW(LC_ERR_NOMEM, "workspace of " + std::to_string(need) + " bytes: " + cudaGetErrorString(e));
+      }
+      bytes = need;
+      if (zeroed) {
+        LC_CUDA(cudaMemset(p, 0, need));
+        LC_CUDA(cudaStreamSynchronize(cudaStreamLegacy));
+      }
+    }
+    return p;
+  }
+};
+
+// Calls of one handle share its workspace: a call on another stream than the
+// last one's waits for it. A stream that is being captured takes no part: a
+// graph may not wait for work outside it, so its replays are the caller's to
+// order.
+struct Order {
+  cudaStream_t own = nullptr, last = nullptr;
+  cudaEvent_t ev = nullptr;
+  void open() {
+    LC_CUDA(cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking));
+    LC_CUDA(cudaEventCreateWithFlags(&ev, cudaEventDisableTiming));
+  }
+  ~Order() {
+    if (ev) cudaEventDestroy(ev);
+    if (own) cudaStreamDestroy(own);
+  }
+  cudaStream_t on(void* stream) {
+    cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : own;
+    if (last == s) return s;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    LC_CUDA(cudaStreamIsCapturing(s, &capture));
+    if (capture != cudaStreamCaptureStatusNone) return s;
+    if (last) {
+      LC_CUDA(cudaEventRecord(ev, last));
+      LC_CUDA(cudaStreamWaitEvent(s, ev, 0));
+    }
+    last = s;
+    return s;
+  }
+};
+
+int sm_count(int device) {
+  int n = 0;
+  LC_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device));
+  return n;
+}
+
+}  // namespace
+
+struct lc_paged {
+  lc_paged_config cfg{};
+  PagedView view{};
+  int sms = 0, esize = 0;
+  Order order;
+  Workspace part, counters, scores, evict;
+  int32_t* status = nullptr;  // mapped host word
+  ~lc_paged() {
+    if (status) cudaFreeHost(status);
+  }
+
+  PagedView call(const int32_t* tables, int32_t width, const int32_t* lens, int32_t rows) const {
+    LC_REQUIRE(rows >= 1 && rows <= cfg.max_seqs, LC_ERR_INVALID,
+               "n_seqs " + std::to_string(rows) + " outside 1.." + std::to_string(cfg.max_seqs));
+    LC_REQUIRE(width >= 1 && width <= cfg.max_pages_per_seq, LC_ERR_INVALID,
+               "table width " + std::to_string(width) + " outside 1.." + std::to_string(cfg.max_pages_per_seq));
+    check_device(tables, cfg.device, "tables", 4);
+    check_device(lens, cfg.device, "lens", 4);
+    PagedView v = view;
+    v.tables = tables;
+    v.lens = lens;
+    v.width = width;
+    return v;
+  }
+  void check_layer(int32_t layer) const {
+    LC_REQUIRE(layer >= 0 && layer < cfg.n_layers, LC_ERR_INVALID, "layer out of range");
+  }
+};
+
+struct lc_beam {
+  int32_t n_groups = 0, n_beams = 0, n_out = 0, device = 0;
+  int64_t vocab = 0;
+  Order order;
+  Workspace ws;
+  BeamArgs a{};
+};
+
+extern "C" {
+
+int lc_paged_create(const lc_paged_config* config, void* k_pages, void* v_pages, lc_paged** out) {
+  return abi_guard([&] {
+    LC_REQUIRE(out, LC_ERR_INVALID, "null out");
+    *out = nullptr;
+    LC_REQUIRE(config, LC_ERR_INVALID, "null config");
+    lc_paged_config c = *config;
+    check_dtype(c.dtype, "pool");
+    LC_REQUIRE(c.n_layers >= 1 && c.n_layers <= 65535 && c.n_kv_heads >= 1 && c.n_kv_heads <= 1024, LC_ERR_INVALID,
+               "n_layers must be 1..65535 and n_kv_heads 1..1024");
+    LC_REQUIRE(c.head_dim >= 1 && c.head_dim <= kPagedMaxDim, LC_ERR_INVALID,
+               "head_dim must be 1.." + std::to_string(kPagedMaxDim));
+    LC_REQUIRE(c.page_tokens >= 1 && c.page_tokens <= 4096, LC_ERR_INVALID, "page_tokens must be 1..4096");
+    LC_REQUIRE(c.n_pages >= 1 && c.n_pages <= INT32_MAX, LC_ERR_INVALID, "n_pages must be 1..2^31-1");
+    LC_REQUIRE(c.max_seqs >= 1 && c.max_seqs <= kPagedMaxSeqs, LC_ERR_INVALID,
+               "max_seqs must be 1.." + std::to_string(kPagedMaxSeqs));
+    LC_REQUIRE(c.max_pages_per_seq >= 1 && (int64_t)c.max_pages_per_seq * c.page_tokens < (1ll << 30), LC_ERR_INVALID,
+               "a sequence must hold 1..2^30-1 slots");
+    LC_REQUIRE(c.max_q_heads >= c.n_kv_heads && c.max_q_heads <= 8192, LC_ERR_INVALID,
+               "max_q_heads must be n_kv_heads..8192");
+    LC_REQUIRE(c.reserved == 0, LC_ERR_INVALID, "reserved must be 0");
+    if (!c.layer_stride && !c.page_stride && !c.head_stride && !c.token_stride) {
+      c.token_stride = c.head_dim;
+      c.head_stride = c.token_stride * c.page_tokens;
+      c.page_stride = c.head_stride * c.n_kv_heads;
+      c.layer_stride = c.page_stride * c.n_pages;
+    }
+    // rows must not overlap: the writing calls would race
+    std::pair<int64_t, int64_t> dims[4] = {{c.layer_stride, c.n_layers},
+                                           {c.page_stride, c.n_pages},
+                                           {c.head_stride, c.n_kv_heads},
+                                           {c.token_stride, c.page_tokens}};
+    std::sort(dims, dims + 4);
+    int64_t span = c.head_dim;
+    for (const auto& [stride, n] : dims) {
+      if (n == 1) continue;
+      LC_REQUIRE(stride >= span, LC_ERR_INVALID, "pool strides overlap");
+      LC_REQUIRE(stride <= (1ll << 60) / n, LC_ERR_INVALID, "pool strides too large");
+      span = stride * (n - 1) + span;
+    }
+    DeviceScope scope(c.device);
+    check_device(k_pages, c.device, "k_pages", element_size(c.dtype));
+    check_device(v_pages, c.device, "v_pages", element_size(c.dtype));
+    auto p = std::make_unique<lc_paged>();
+    p->cfg = c;
+    p->esize = element_size(c.dtype);
+    p->sms = sm_count(c.device);
+    p->order.open();
+    LC_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&p->status), 4, cudaHostAllocMapped));
+    *p->status = 0;
+    int32_t* dev_status = nullptr;
+    LC_CUDA(cudaHostGetDevicePointer(reinterpret_cast<void**>(&dev_status), p->status, 0));
+    p->view.k = k_pages;
+    p->view.v = v_pages;
+    p->view.layer = c.n_layers == 1 ? 0 : c.layer_stride;
+    p->view.page = c.n_pages == 1 ? 0 : c.page_stride;
+    p->view.head = c.n_kv_heads == 1 ? 0 : c.head_stride;
+    p->view.token = c.page_tokens == 1 ? 0 : c.token_stride;
+    p->view.n_layers = c.n_layers;
+    p->view.hkv = c.n_kv_heads;
+    p->view.d = c.head_dim;
+    p->view.page_tokens = c.page_tokens;
+    p->view.n_pages = c.n_pages;
+    p->view.status = dev_status;
+    p->part.get((size_t)paged_part_floats(p->sms) * 4);
+    p->counters.get((size_t)c.max_seqs * c.max_q_heads * 4, true);
+    *out = p.release();
+  });
+}
+
+void lc_paged_destroy(lc_paged* p) {
+  if (!p) return;
+  int before = -1;
+  cudaGetDevice(&before);
+  cudaSetDevice(p->cfg.device);
+  cudaDeviceSynchronize();
+  const int device = p->cfg.device;
+  delete p;
+  if (before >= 0 && before != device) cudaSetDevice(before);
+}
+
+int lc_paged_status(const lc_paged* p) {
+  return abi_guard([&] {
+    LC_REQUIRE(p, LC_ERR_INVALID, "null handle");
+    LC_REQUIRE(*static_cast<volatile int32_t*>(p->status) == 0, LC_ERR_INVALID,
+               "a call met a length beyond its table, a page id outside the pool or a parent outside its group");
+  });
+}
+
+int lc_paged_append(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* tables, int32_t width,
+                    const int32_t* lens, const void* keys, const void* values, int32_t dtype, int64_t n_tokens,
+                    int32_t* pos, int64_t pos_stride, const int32_t* pos0, void* stream) {
+  return abi_guard([&] {
+    LC_REQUIRE(p, LC_ERR_INVALID, "null handle");
+    check_dtype(dtype, "keys");
+    p->check_layer(layer);
+    LC_REQUIRE(n_tokens >= 0 && n_tokens < (1ll << 30), LC_ERR_INVALID, "n_tokens must be 0..2^30-1");
+    DeviceScope scope(p->cfg.device);
+    PagedAppendArgs a{};
+    a.c = p->call(tables, width, lens, n_seqs);
+    if (n_tokens == 0) return;
+    check_device(keys, p->cfg.device, "keys", element_size(dtype));
+    check_device(values, p->cfg.device, "values", element_size(dtype));
+    if (pos) {
+      check_device(pos, p->cfg.device, "pos", 4);
+      check_device(pos0, p->cfg.device, "pos0", 4);
+      LC_REQUIRE(pos_stride >= (int64_t)width * p->cfg.page_tokens, LC_ERR_INVALID, "pos rows shorter than the table");
+    }
+    a.keys = keys;
+    a.values = values;
+    a.dtype = dtype;
+    a.pool_dtype = p->cfg.dtype;
+    a.layer = layer;
+    a.n_seqs = n_seqs;
+    a.n_tokens = n_tokens;
+    a.pos = pos;
+    a.pos0 = pos0;
+    a.pos_stride = pos_stride;
+    launch_paged_append(a, p->order.on(stream));
+  });
+}
+
+static void paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* tables, int32_t width,
+                       const int32_t* lens, const void* q, int32_t q_dtype, int32_t n_q_heads, float scale,
+                       int32_t window, void* out, int32_t out_dtype, const float* acc_in, float* acc_out,
+                       int64_t acc_stride, float decay, void* stream) {
+  LC_REQUIRE(p, LC_ERR_INVALID, "null handle");
+  check_dtype(q_dtype, "q");
+  check_dtype(out_dtype, "out");
+  p->check_layer(layer);
+  LC_REQUIRE(n_q_heads >= 1 && n_q_heads <= p->cfg.max_q_heads && n_q_heads % p->cfg.n_kv_heads == 0, LC_ERR_INVALID,
+             "n_q_heads must be a multiple of n_kv_heads and at most max_q_heads");
+  LC_REQUIRE(window >= 0, LC_ERR_INVALID, "window must be >= 0");
+  LC_REQUIRE(scale == scale && scale - scale == 0.f, LC_ERR_INVALID, "scale must be finite");
+  DeviceScope scope(p->cfg.device);
+  PagedAttnArgs a{};
+  a.c = p->call(tables, width, lens, n_seqs);
+  check_device(q, p->cfg.device, "q", element_size(q_dtype));
+  check_device(out, p->cfg.device, "out", element_size(out_dtype));
+  a.q = q;
+  a.out = out;
+  a.q_dtype = q_dtype;
+  a.out_dtype = out_dtype;
+  a.n_seqs = n_seqs;
+  a.group = n_q_heads / p->cfg.n_kv_heads;
+  a.layer = layer;
+  a.window = window;
+  a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  a.part = static_cast<float*>(p->part.p);
+  a.counters = static_cast<int32_t*>(p->counters.p);
+  const int64_t cap = (int64_t)width * p->cfg.page_tokens;
+  if (acc_out) {
+    check_device(acc_in, p->cfg.device, "acc_in", 4);
+    check_device(acc_out, p->cfg.device, "acc_out", 4);
+    LC_REQUIRE(acc_stride >= cap, LC_ERR_INVALID, "acc rows shorter than the table");
+    const size_t rows = (size_t)n_seqs * n_q_heads;
+    a.score_tokens = cap;
+    float* ws = static_cast<float*>(p->scores.get((rows * cap + 2 * rows) * 4));
+    a.stats = ws;
+    a.scores = ws + 2 * rows;
+  }
+  const cudaStream_t s = p->order.on(stream);
+  launch_paged_attn(a, p->cfg.dtype, p->cfg.device, p->sms, s);
+  if (acc_out) {
+    PagedWeightArgs w{};
+    w.scores = a.scores;
+    w.stats = a.stats;
+    w.acc_in = acc_in;
+    w.acc_out = acc_out;
+    w.lens = lens;
+    w.score_tokens = cap;
+    w.acc_stride = acc_stride;
+    w.n_seqs = n_seqs;
+    w.hkv = p->cfg.n_kv_heads;
+    w.group = a.group;
+    w.window = window;
+    w.cap = (int32_t)cap;
+    w.decay = decay;
+    launch_paged_weights(w, s);
+  }
+}
+
+int lc_paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* tables, int32_t width,
+                  const int32_t* lens, const void* q, int32_t q_dtype, int32_t n_q_heads, float scale, int32_t window,
+                  void* out, int32_t out_dtype, void* stream) {
+  return abi_guard([&] {
+    paged_attn(p, layer, n_seqs, tables, width, lens, q, q_dtype, n_q_heads, scale, window, out, out_dtype, nullptr,
+               nullptr, 0, 0.f, stream);
+  });
+}
+
+int lc_paged_attn_weights(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* tables, int32_t width,
+                          const int32_t* lens, const void* q, int32_t q_dtype, int32_t n_q_heads, float scale,
+                          int32_t window, void* out, int32_t out_dtype, const float* acc_in, float* acc_out,
+                          int64_t acc_stride, float decay, void* stream) {
+  return abi_guard([&] {
+    LC_REQUIRE(acc_in && acc_out, LC_ERR_INVALID, "acc_in and acc_out must be given");
+    LC_REQUIRE(decay >= 0.f && decay <= 1.f, LC_ERR_INVALID, "decay must be in [0, 1]");
+    paged_attn(p, layer, n_seqs, tables, width, lens, q, q_dtype, n_q_heads, scale, window, out, out_dtype, acc_in,
+               acc_out, acc_stride, decay, stream);
+  });
+}
+
+int lc_paged_evict(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* tables, int32_t width,
+                   const int32_t* lens, int32_t budget, int32_t n_sink, int32_t n_recent, const float* acc_in,
+                   const int32_t* pos_in, float* acc_out, int32_t* pos_out, int64_t stride, void* stream) {
+  return abi_guard([&] {
+    LC_REQUIRE(p, LC_ERR_INVALID, "null handle");
+    p->check_layer(layer);
+    LC_REQUIRE(budget >= 1 && n_sink >= 0 && n_recent >= 0 && (int64_t)n_sink + n_recent <= budget, LC_ERR_INVALID,
+               "budget must be >= 1 and hold n_sink + n_recent");
+    DeviceScope scope(p->cfg.device);
+    PagedEvictArgs a{};
+    a.c = p->call(tables, width, lens, n_seqs);
+    check_device(acc_in, p->cfg.device, "acc_in", 4);
+    check_device(pos_in, p->cfg.device, "pos_in", 4);
+    check_device(acc_out, p->cfg.device, "acc_out", 4);
+    check_device(pos_out, p->cfg.device, "pos_out", 4);
+    const int64_t cap = (int64_t)width * p->cfg.page_tokens;
+    LC_REQUIRE(stride >= cap, LC_ERR_INVALID, "acc and pos rows shorter than the table");
+    a.layer = layer;
+    a.n_seqs = n_seqs;
+    a.esize = p->esize;
+    a.budget = budget;
+    a.n_sink = n_sink;
+    a.n_recent = n_recent;
+    a.stride = stride;
+    a.acc_in = acc_in;
+    a.pos_in = pos_in;
+    a.acc_out = acc_out;
+    a.pos_out = pos_out;
+    // at most min(budget, cap - budget) slots move in a row
+    const int64_t rows = (int64_t)n_seqs * p->cfg.n_kv_heads;
+    a.list_cap = std::max<int64_t>(1, std::min<int64_t>(budget, cap - budget));
+    const int cl = paged_evict_cluster((int32_t)rows, cap, p->sms);
+    const int64_t keys = paged_evict_keys_in_smem(cap, cl) ? 0 : rows * stride;
+    int32_t* ws = static_cast<int32_t*>(p->evict.get((size_t)(rows * 4 * a.list_cap + keys) * 4));
+    a.list = ws;
+    a.keys = reinterpret_cast<uint32_t*>(ws + rows * 4 * a.list_cap);
+    launch_paged_evict(a, p->cfg.device, p->sms, p->order.on(stream));
+  });
+}
+
+int lc_paged_reorder(lc_paged* p, int32_t n_groups, int32_t n_beams, const int32_t* tables, int32_t width,
+                     const int32_t* lens, const int32_t* parents, int32_t* tables_out, void* stream) {
+  return abi_guard([&] {
+    LC_REQUIRE(p, LC_ERR_INVALID, "null handle");
+    LC_REQUIRE(n_groups >= 1 && n_beams >= 1 && n_beams <= kBeamMaxBeams, LC_ERR_INVALID,
+               "n_groups must be >= 1 and n_beams 1.." + std::to_string(kBeamMaxBeams));
+    LC_REQUIRE((int64_t)n_groups * n_beams <= p->cfg.max_seqs, LC_ERR_INVALID, "more rows than max_seqs");
+    DeviceScope scope(p->cfg.device);
+    PagedReorderArgs a{};
+    a.c = p->call(tables, width, lens, n_groups * n_beams);
+    check_device(parents, p->cfg.device, "parents", 4);
+    check_device(tables_out, p->cfg.device, "tables_out", 4);
+    const int64_t entries = (int64_t)n_groups * n_beams * width;
+    LC_REQUIRE(tables_out + entries <= tables || tables + entries <= tables_out, LC_ERR_INVALID,
+               "tables_out overlaps tables");
+    a.n_groups = n_groups;
+    a.n_beams = n_beams;
+    a.esize = p->esize;
+    a.parents = parents;
+    a.tables_out = tables_out;
+    launch_paged_reorder(a, p->order.on(stream));
+  });
+}
+
+int lc_beam_create(int32_t n_groups, int32_t n_beams, int64_t vocab, int32_t n_out, int32_t device, lc_beam** out) {
+  return abi_guard([&] {
+    LC_REQUIRE(out, LC_ERR_INVALID, "null out");
+    *out = nullptr;
+    LC_REQUIRE(n_groups >= 1 && n_beams >= 1 && n_beams <= kBeamMaxBeams && (int64_t)n_groups * n_beams <= 65535,
+               LC_ERR_INVALID, "n_beams must be 1.." + std::to_string(kBeamMaxBeams) + " and the rows at most 65535");
+    LC_REQUIRE(n_out >= 1 && n_out <= kBeamMaxOut, LC_ERR_INVALID, "n_out must be 1.." + std::to_string(kBeamMaxOut));
+    LC_REQUIRE(vocab >= 1 && vocab < (1ll << 31) && (int64_t)n_beams * vocab < (1ll << 32), LC_ERR_INVALID,
+               "vocab must be >= 1 and n_beams * vocab below 2^32");
+    const int64_t slices = (vocab + 7 + beam_slice(LC_F32) - 1) / beam_slice(LC_F32);
+    LC_REQUIRE(slices <= 256 && slices * n_out <= kBeamMaxMerge, LC_ERR_INVALID, "vocab too large for this n_out");
+    DeviceScope scope(device);
+    auto b = std::make_unique<lc_beam>();
+    b->n_groups = n_groups;
+    b->n_beams = n_beams;
+    b->n_out = n_out;
+    b->device = device;
+    b->vocab = vocab;
+    b->order.open();
+    const size_t rows = (size_t)n_groups * n_beams, lists = rows * slices;
+    const size_t keys = (lists + rows) * n_out;
+    uint8_t* w = static_cast<uint8_t*>(
+        b->ws.get(keys * 8 + (2 * lists + lists + rows + rows + n_groups) * 4, true));
+    BeamArgs& a = b->a;
+    a.slice_key = reinterpret_cast<uint64_t*>(w);
+    a.row_key = a.slice_key + lists * n_out;
+    a.slice_stats = reinterpret_cast<float*>(a.row_key + rows * n_out);
+    a.slice_count = reinterpret_cast<int32_t*>(a.slice_stats + 2 * lists);
+    a.row_count = a.slice_count + lists;
+    a.counters = a.row_count + rows;
+    *out = b.release();
+  });
+}
+
+void lc_beam_destroy(lc_beam* b) {
+  if (!b) return;
+  int before = -1;
+  cudaGetDevice(&before);
+  const int device = b->device;
+  cudaSetDevice(device);
+  cudaDeviceSynchronize();
+  delete b;
+  if (before >= 0 && before != device) cudaSetDevice(before);
+}
+
+int lc_beam_select(lc_beam* b, int32_t n_groups, const void* logits, int32_t dtype, int64_t row_stride,
+                   const float* scores, const uint8_t* finished, int32_t eos, int32_t pad, float* scores_out,
+                   int32_t* parents, int32_t* tokens, uint8_t* finished_out, void* stream) {
+  return abi_guard([&] {
+    LC_REQUIRE(b, LC_ERR_INVALID, "null handle");
+    check_dtype(dtype, "logits");
+    LC_REQUIRE(n_groups >= 1 && n_groups <= b->n_groups, LC_ERR_INVALID,
+               "n_groups outside 1.." + std::to_string(b->n_groups));
+    LC_REQUIRE(row_stride >= b->vocab && row_stride < (1ll << 40), LC_ERR_INVALID, "row_stride shorter than vocab");
+    LC_REQUIRE(pad >= 0 && pad < b->vocab, LC_ERR_INVALID, "pad outside the vocabulary");
+    DeviceScope scope(b->device);
+    check_device(logits, b->device, "logits", element_size(dtype));
+    check_device(scores, b->device, "scores", 4);
+    if (finished) check_device(finished, b->device, "finished", 1);
+    check_device(scores_out, b->device, "scores_out", 4);
+    check_device(parents, b->device, "parents", 4);
+    check_device(tokens, b->device, "tokens", 4);
+    check_device(finished_out, b->device, "finished_out", 1);
+    LC_REQUIRE(finished_out != finished && scores_out != scores, LC_ERR_INVALID, "outputs overlap inputs");
+    BeamArgs a = b->a;
+    a.logits = logits;
+    a.dtype = dtype;
+    a.row_stride = row_stride;
+    a.n_groups = n_groups;
+    a.n_beams = b->n_beams;
+    a.n_out = b->n_out;
+    a.vocab = (int32_t)b->vocab;
+    a.slice = beam_slice(dtype);
+    a.slices = (int32_t)((b->vocab + 7 + a.slice - 1) / a.slice);
+    a.scores = scores;
+    a.finished = finished;
+    a.eos = eos;
+    a.pad = pad;
+    a.scores_out = scores_out;
+    a.parents = parents;
+    a.tokens = tokens;
+    a.finished_out = finished_out;
+    launch_beam(a, b->order.on(stream));
+  });
+}
+
+}  // extern "C"

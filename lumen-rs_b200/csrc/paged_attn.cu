@@ -1,0 +1,491 @@
+// Decode attention over the uncompressed paged cache (lc_paged_attn), the
+// accumulated attention weights (lc_paged_attn_weights) and the append.
+//
+//   s_gt = scale q_g . k_t,  p_gt = exp(s_gt - max_t s_gt) / sum_t,
+//   out_g = sum_t p_gt v_t          over the slots lo <= t < n of a sequence
+//
+// One pass over K and V with the running maximum m and sum l of a softmax:
+// a tile's scores rescale what was summed before by 2^(m_old - m_new). The
+// bytes of K and V bound it: a kv head's `group` query heads are computed
+// together so that each row is read once.
+//
+// Work split: the tiles of all (sequence, kv head, group of query heads)
+// items form one list, and every block takes an equal run of it, whatever
+// the sequences' lengths are: a long sequence alone fills the card and a
+// batch of ragged ones leaves no tail. The lengths are read on the device
+// (no host copy, and a captured graph follows them). An item that lies in
+// one run is finished by its block; of one that spans several, each block
+// leaves (m, l, o) in its slot and the last to arrive joins them, in slot
+// order, so results do not depend on the order of arrival.
+#include <algorithm>
+
+#include "devutil.cuh"
+#include "paged.h"
+
+namespace lc {
+namespace {
+
+constexpr float kNegInf = -INFINITY;
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+
+__device__ __forceinline__ float load_f32(const void* p, int64_t i, int dtype) {
+  if (dtype == LC_F32) return static_cast<const float*>(p)[i];
+  if (dtype == LC_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+
+__device__ __forceinline__ void store_f32(void* p, int64_t i, int dtype, float x) {
+  if (dtype == LC_F32)
+    static_cast<float*>(p)[i] = x;
+  else if (dtype == LC_BF16)
+    static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+  else
+    static_cast<__half*>(p)[i] = __float2half_rn(x);
+}
+
+// A sequence's length within what its table can hold.
+__device__ __forceinline__ int clamp_len(const PagedView& c, int s) {
+  const int cap = c.width * c.page_tokens, n = c.lens[s];
+  if (n < 0 || n > cap) {
+    *c.status = 1;
+    return n < 0 ? 0 : cap;
+  }
+  return n;
+}
+
+__device__ __forceinline__ int first_slot(int n, int window) { return window > 0 && n > window ? n - window : 0; }
+
+// Offset in elements of slot t's row (head 0, this call's layer), or -1 for a
+// page id outside the pool.
+__device__ __forceinline__ int64_t row_offset(const PagedView& c, int s, int t) {
+  const int page = c.tables[(int64_t)s * c.width + t / c.page_tokens];
+  if (page < 0 || page >= c.n_pages) {
+    *c.status = 1;
+    return -1;
+  }
+  return page * c.page + (int64_t)(t % c.page_tokens) * c.token;
+}
+
+// prefix[s] = tiles of the sequences before s (of one item each); prefix[n_seqs]
+// the total. Every thread of the block calls it.
+template <int THREADS>
+__device__ void build_prefix(const PagedAttnArgs& a, int tile, int* prefix) {
+  __shared__ int warp_sum[THREADS / 32];
+  const int tid = threadIdx.x, per = (a.n_seqs + THREADS - 1) / THREADS;
+  const int b = min(a.n_seqs, tid * per), e = min(a.n_seqs, b + per);
+  int sum = 0;
+  for (int s = b; s < e; ++s) {
+    const int n = clamp_len(a.c, s);
+    sum += (n - first_slot(n, a.window) + tile - 1) / tile;
+  }
+  int inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(~0u, inc, o);
+    if ((tid & 31) >= o) inc += up;
+  }
+  if ((tid & 31) == 31) warp_sum[tid >> 5] = inc;
+  __syncthreads();
+  int at = inc - sum;
+  for (int w = 0; w < (tid >> 5); ++w) at += warp_sum[w];
+  for (int s = b; s < e; ++s) {
+    prefix[s] = at;
+    const int n = clamp_len(a.c, s);
+    at += (n - first_slot(n, a.window) + tile - 1) / tile;
+  }
+  if (tid == THREADS - 1) prefix[a.n_seqs] = at;
+  __syncthreads();
+}
+
+// A block's share of one item: tiles [j0, j1) of sequence s, item hh (kv head
+// and head group) of it.
+struct Segment {
+  int s, hh, j0, j1, n, lo;
+  // the item's blocks are first .. first + parts - 1; block b's partial is in
+  // slot 2 b, or 2 b + 1 where the item does not begin its run (the first only)
+  int first, parts, slot0, slot;
+};
+
+__device__ __forceinline__ Segment find_segment(const PagedAttnArgs& a, const int* prefix, int hh_n, int per, int u,
+                                                int u_end) {
+  Segment g;
+  const int key = u / hh_n;
+  int b = 0, e = a.n_seqs;  // the last s with prefix[s] <= key
+  while (e - b > 1) {
+    const int mid = (b + e) >> 1;
+    if (prefix[mid] <= key)
+      b = mid;
+    else
+      e = mid;
+  }
+  g.s = b;
+  const int tiles = prefix[b + 1] - prefix[b], r = u - prefix[b] * hh_n;
+  g.hh = r / tiles;
+  g.j0 = r - g.hh * tiles;
+  g.j1 = min(tiles, g.j0 + (u_end - u));
+  g.n = clamp_len(a.c, b);
+  g.lo = first_slot(g.n, a.window);
+  const int start = prefix[b] * hh_n + g.hh * tiles;
+  g.first = start / per;
+  g.parts = (start + tiles - 1) / per - g.first + 1;
+  g.slot0 = 2 * g.first + (g.first * per < start ? 1 : 0);
+  g.slot = (int)blockIdx.x == g.first ? g.slot0 : 2 * (int)blockIdx.x;
+  return g;
+}
+
+// Joins the warps' (m, l, o) of a segment (shared memory: om, ol [warps][GP],
+// oo [warps][GP][DP]) and writes the item's rows, its partial, or, as the last
+// block of a split item, the join of all its partials. Block-wide.
+template <int THREADS, int GP, int DP>
+__device__ void finish_segment(const PagedAttnArgs& a, const Segment& g, int hg_n, const float* om, const float* ol,
+                               const float* oo) {
+  constexpr int W = THREADS / 32;
+  __shared__ int last;
+  const int tid = threadIdx.x, d = a.c.d;
+  const int h = g.hh / hg_n, head0 = (g.hh - h * hg_n) * GP, nh = min(GP, a.group - head0);
+  const int64_t row0 = (int64_t)g.s * a.c.hkv * a.group + (int64_t)h * a.group + head0;
+  __syncthreads();
+  auto put = [&](int i, int x, float m, float l, float o) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // no slot with a finite score: zeros
+    store_f32(a.out, (row0 + i) * d + x, a.out_dtype, o * inv);
+    if (a.stats && x == 0) {
+      a.stats[2 * (row0 + i)] = m == kNegInf ? 0.f : m;
+      a.stats[2 * (row0 + i) + 1] = inv;
+    }
+  };
+  constexpr int64_t kSlot = GP * (DP + 2);
+  float* part = a.part + g.slot * kSlot;
+  for (int e = tid; e < nh * d; e += THREADS) {
+    const int i = e / d, x = e - i * d;
+    float m = kNegInf;
+#pragma unroll
+    for (int w = 0; w < W; ++w) m = fmaxf(m, om[w * GP + i]);
+    const float mg = m == kNegInf ? 0.f : m;
+    float l = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float f = ex2(om[w * GP + i] - mg);
+      l += f * ol[w * GP + i];
+      o += f * oo[(w * GP + i) * DP + x];
+    }
+    if (g.parts == 1) {
+      put(i, x, m, l, o);
+    } else {
+      if (x == 0) {
+        part[i] = m;
+        part[GP + i] = l;
+      }
+      part[2 * GP + i * DP + x] = o;
+    }
+  }
+  if (g.parts > 1) {
+    int* counter = a.counters + (int64_t)g.s * a.c.hkv * hg_n + g.hh;
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      last = atomicAdd(counter, 1) == g.parts - 1;
+      if (last) *counter = 0;
+    }
+    __syncthreads();
+    if (last) {
+      __threadfence();
+      for (int e = tid; e < nh * d; e += THREADS) {
+        const int i = e / d, x = e - i * d;
+        float m = kNegInf, l = 0.f, o = 0.f;
+        for (int b = g.first; b < g.first + g.parts; ++b) {
+          const float* p = a.part + (b == g.first ? g.slot0 : 2 * b) * kSlot;
+          const float pm = __ldcg(p + i), pl = __ldcg(p + GP + i), po = __ldcg(p + 2 * GP + i * DP + x);
+          const float mn = fmaxf(m, pm), mg = mn == kNegInf ? 0.f : mn;
+          const float fa = ex2(m - mg), fb = ex2(pm - mg);
+          l = l * fa + pl * fb;
+          o = o * fa + po * fb;
+          m = mn;
+        }
+        put(i, x, m, l, o);
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// Rows of sequences with nothing to attend to: zeros.
+template <int THREADS>
+__device__ void zero_empty(const PagedAttnArgs& a) {
+  const int heads = a.c.hkv * a.group, d = a.c.d;
+  for (int s = blockIdx.x; s < a.n_seqs; s += gridDim.x) {
+    if (clamp_len(a.c, s) != 0) continue;
+    for (int e = threadIdx.x; e < heads * d; e += THREADS) store_f32(a.out, (int64_t)s * heads * d + e, a.out_dtype, 0.f);
+    if (a.stats)
+      for (int e = threadIdx.x; e < 2 * heads; e += THREADS) a.stats[2ll * s * heads + e] = 0.f;
+  }
+}
+
+// The general kernel: any of the three types in and out, any alignment, head
+// dimension up to DP, products and sums in f32 on the FMA units. A warp owns
+// whole tiles of TT = 32 / LPT slots: LPT = DP / 64 lanes share a slot's dot
+// product, 16 bytes at a time in turn, and for the values the lanes own
+// dimensions. Rows sit in shared memory as f32 with 4 LPT words of padding,
+// which keeps the eight lanes of a 16-byte read phase on different banks.
+template <typename T, int DP, int GP, int W>
+__global__ void __launch_bounds__(W * 32) k_paged_attn(const PagedAttnArgs a) {
+  constexpr int LPT = DP / 64, TT = 32 / LPT, PITCH = DP + 4 * LPT, VL = DP / 32;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* kt = reinterpret_cast<float*>(smem);  // [W][TT][PITCH]
+  float* vt = kt + W * TT * PITCH;
+  float* qs = vt + W * TT * PITCH;         // [GP][DP]
+  float* ps = qs + GP * DP;                // [W][TT][GP]
+  float* om = ps + W * TT * GP;            // [W][GP]
+  float* ol = om + W * GP;
+  int* prefix = reinterpret_cast<int*>(ol + W * GP);
+  float* oo = kt;  // [W][GP][DP]: the tiles' room, free when a segment ends
+  static_assert(GP * DP <= TT * PITCH, "the warps' outputs fit the key tiles");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int hg_n = (a.group + GP - 1) / GP, hh_n = a.c.hkv * hg_n;
+  zero_empty<W * 32>(a);
+  build_prefix<W * 32>(a, TT, prefix);
+  const int total = prefix[a.n_seqs] * hh_n;
+  const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, a.min_tiles);
+  const int u_end = min(total, ((int)blockIdx.x + 1) * per);
+  float* kw = kt + warp * TT * PITCH;
+  float* vw = vt + warp * TT * PITCH;
+  float* pw = ps + warp * TT * GP;
+  const int tok = lane / LPT, part = lane % LPT;
+  for (int u = blockIdx.x * per; u < u_end;) {
+    const Segment g = find_segment(a, prefix, hh_n, per, u, u_end);
+    u += g.j1 - g.j0;
+    const int h = g.hh / hg_n, head0 = (g.hh - h * hg_n) * GP, nh = min(GP, a.group - head0);
+    const int64_t qrow = ((int64_t)g.s * a.c.hkv + h) * a.group + head0;
+    for (int e = tid; e < GP * DP; e += W * 32) {
+      const int i = e / DP, x = e - i * DP;
+      qs[e] = i < nh && x < a.c.d ? load_f32(a.q, (qrow + i) * a.c.d + x, a.q_dtype) * a.scale_log2 : 0.f;
+    }
+    __syncthreads();
+    const T* kb = static_cast<const T*>(a.c.k) + a.layer * a.c.layer + h * a.c.head;
+    const T* vb = static_cast<const T*>(a.c.v) + a.layer * a.c.layer + h * a.c.head;
+    float m[GP], l[GP], o[GP][VL];
+#pragma unroll
+    for (int i = 0; i < GP; ++i) {
+      m[i] = kNegInf;
+      l[i] = 0.f;
+#pragma unroll
+      for (int x = 0; x < VL; ++x) o[i][x] = 0.f;
+    }
+    for (int j = g.j0 + warp; j < g.j1; j += W) {
+      const int t0 = g.lo + j * TT, nt = min(TT, g.n - t0);
+      const int64_t mine = lane < nt ? row_offset(a.c, g.s, t0 + lane) : -1;
+#pragma unroll 4
+      for (int r = 0; r < TT; ++r) {
+        const int64_t off = __shfl_sync(~0u, mine, r);
+#pragma unroll
+        for (int x = 0; x < VL; ++x) {
+          const int c = x * 32 + lane;
+          const bool in = off >= 0 && c < a.c.d;
+          kw[r * PITCH + c] = in ? to_f32(kb[off + c]) : 0.f;
+          vw[r * PITCH + c] = in ? to_f32(vb[off + c]) : 0.f;
+        }
+      }
+      __syncwarp();
+      float s[GP];
+#pragma unroll
+      for (int i = 0; i < GP; ++i) s[i] = 0.f;
+#pragma unroll 4
+      for (int c = 0; c < 16; ++c) {
+        const int x = 4 * (c * LPT + part);
+        const float4 kk = *reinterpret_cast<const float4*>(kw + tok * PITCH + x);
+#pragma unroll
+        for (int i = 0; i < GP; ++i) {
+          const float4 qq = *reinterpret_cast<const float4*>(qs + i * DP + x);
+          s[i] = fmaf(kk.x, qq.x, fmaf(kk.y, qq.y, fmaf(kk.z, qq.z, fmaf(kk.w, qq.w, s[i]))));
+        }
+      }
+      bool grow = false;
+#pragma unroll
+      for (int i = 0; i < GP; ++i) {
+#pragma unroll
+        for (int b = 1; b < LPT; b <<= 1) s[i] += __shfl_xor_sync(~0u, s[i], b);
+        if (tok >= nt) s[i] = kNegInf;
+        grow |= s[i] > m[i];
+      }
+      if (a.scores && part == 0 && tok < nt) {
+        float* to = a.scores + (((int64_t)g.s * a.c.hkv + h) * a.score_tokens + t0 + tok) * a.group + head0;
+#pragma unroll
+        for (int i = 0; i < GP; ++i)
+          if (i < nh) to[i] = s[i];
+      }
+      if (__any_sync(~0u, grow)) {
+#pragma unroll
+        for (int i = 0; i < GP; ++i) {
+          float top = s[i];
+#pragma unroll
+          for (int b = LPT; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, b));
+          top = fmaxf(top, m[i]);
+          const float f = ex2(m[i] - (top == kNegInf ? 0.f : top));
+          m[i] = top;
+          l[i] *= f;
+#pragma unroll
+          for (int x = 0; x < VL; ++x) o[i][x] *= f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < GP; ++i) {
+        const float p = ex2(s[i] - (m[i] == kNegInf ? 0.f : m[i]));
+        if (part == 0) {
+          l[i] += p;
+          pw[tok * GP + i] = p;
+        }
+      }
+      __syncwarp();
+#pragma unroll 4
+      for (int r = 0; r < TT; ++r) {
+        float v[VL];
+#pragma unroll
+        for (int x = 0; x < VL; ++x) v[x] = vw[r * PITCH + x * 32 + lane];
+#pragma unroll
+        for (int i = 0; i < GP; ++i) {
+          const float p = pw[r * GP + i];
+#pragma unroll
+          for (int x = 0; x < VL; ++x) o[i][x] = fmaf(p, v[x], o[i][x]);
+        }
+      }
+      __syncwarp();
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < GP; ++i) {
+      float sum = l[i];
+#pragma unroll
+      for (int b = 1; b < 32; b <<= 1) sum += __shfl_xor_sync(~0u, sum, b);
+      if (lane == 0) {
+        om[warp * GP + i] = m[i];
+        ol[warp * GP + i] = sum;
+      }
+#pragma unroll
+      for (int x = 0; x < VL; ++x) oo[(warp * GP + i) * DP + x * 32 + lane] = o[i][x];
+    }
+    finish_segment<W * 32, GP, DP>(a, g, hg_n, om, ol, oo);
+  }
+}
+
+constexpr int kWarps = 4;
+
+template <int DP, int GP>
+constexpr size_t general_smem(int n_seqs) {
+  constexpr int LPT = DP / 64, TT = 32 / LPT, PITCH = DP + 4 * LPT;
+  return (size_t)(2 * kWarps * TT * PITCH + GP * DP + kWarps * TT * GP + 2 * kWarps * GP) * 4 + (size_t)(n_seqs + 1) * 4;
+}
+
+// Blocks for the call: as many as run at once, fewer where even the table's
+// full width holds less than min_tiles tiles for each.
+int attn_grid(const PagedAttnArgs& a, int gp, int tile, int most) {
+  const int64_t cap = (int64_t)a.c.width * a.c.page_tokens;
+  const int64_t seen = a.window > 0 ? std::min<int64_t>(cap, a.window) : cap;
+  const int64_t items = (int64_t)a.n_seqs * a.c.hkv * ((a.group + gp - 1) / gp);
+  const int64_t tiles = items * ((seen + tile - 1) / tile);
+  LC_REQUIRE(tiles < (1ll << 31) - (1 << 20), LC_ERR_INVALID, "more slots than one call can split");
+  return (int)std::max<int64_t>(1, std::min<int64_t>(most, (tiles + a.min_tiles - 1) / a.min_tiles));
+}
+
+template <typename T, int DP>
+void launch_general(PagedAttnArgs& a, int device, int sms, cudaStream_t s) {
+  constexpr int GP = 4;
+  auto kernel = k_paged_attn<T, DP, GP, kWarps>;
+  const size_t smem = general_smem<DP, GP>(a.n_seqs);
+  static SmemOptIn opt;
+  opt(kernel, general_smem<DP, GP>(kPagedMaxSeqs), device);
+  a.min_tiles = 2 * kWarps;
+  const int grid = attn_grid(a, GP, 32 / (DP / 64), 2 * sms);
+  kernel<<<grid, kWarps * 32, smem, s>>>(a);
+}
+
+template <typename T>
+void launch_general(PagedAttnArgs& a, int device, int sms, cudaStream_t s) {
+  if (a.c.d <= 64)
+    launch_general<T, 64>(a, device, sms, s);
+  else if (a.c.d <= 128)
+    launch_general<T, 128>(a, device, sms, s);
+  else
+    launch_general<T, 256>(a, device, sms, s);
+}
+
+// acc_out[s, h, t] = decay acc_in + sum_g exp2(score_gt - m_g) / l_g. A thread
+// per slot; 4 (group + 2) bytes a slot are read and written, all of them in
+// rows of consecutive slots.
+__global__ void __launch_bounds__(256) k_paged_weights(const PagedWeightArgs a) {
+  extern __shared__ float st[];  // [group][2]
+  const int row = blockIdx.x, s = row / a.hkv;
+  for (int i = threadIdx.x; i < 2 * a.group; i += 256) st[i] = a.stats[2ll * row * a.group + i];
+  __syncthreads();
+  const int n = min(max(a.lens[s], 0), a.cap), lo = first_slot(n, a.window);
+  for (int t = blockIdx.y * 256 + threadIdx.x; t < n; t += gridDim.y * 256) {
+    float sum = 0.f;
+    if (t >= lo) {
+      const float* sc = a.scores + ((int64_t)row * a.score_tokens + t) * a.group;
+      for (int i = 0; i < a.group; ++i) sum += ex2(sc[i] - st[2 * i]) * st[2 * i + 1];
+    }
+    const int64_t at = row * a.acc_stride + t;
+    a.acc_out[at] = fmaf(a.decay, a.acc_in[at], sum);
+  }
+}
+
+// One warp a (token, head) row: converts and writes K and V into its page.
+template <typename T>
+__global__ void __launch_bounds__(256) k_paged_append(const PagedAppendArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = (int64_t)a.n_seqs * a.c.hkv * a.n_tokens;
+  for (int64_t r = blockIdx.x * 8ll + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8ll) {
+    const int64_t sh = r / a.n_tokens;
+    const int tok = (int)(r - sh * a.n_tokens), s = (int)(sh / a.c.hkv), h = (int)(sh - (int64_t)s * a.c.hkv);
+    const int64_t t = (int64_t)a.c.lens[s] + tok;
+    if (t < 0 || t >= (int64_t)a.c.width * a.c.page_tokens) {
+      *a.c.status = 1;
+      continue;
+    }
+    const int64_t off = row_offset(a.c, s, (int)t);
+    if (off < 0) continue;
+    T* k = static_cast<T*>(a.c.k) + a.layer * a.c.layer + h * a.c.head + off;
+    T* v = static_cast<T*>(a.c.v) + a.layer * a.c.layer + h * a.c.head + off;
+    for (int x = lane; x < a.c.d; x += 32) {
+      store_f32(k, x, a.pool_dtype, load_f32(a.keys, r * a.c.d + x, a.dtype));
+      store_f32(v, x, a.pool_dtype, load_f32(a.values, r * a.c.d + x, a.dtype));
+    }
+    if (a.pos && lane == 0) a.pos[sh * a.pos_stride + t] = a.pos0[s] + tok;
+  }
+}
+
+}  // namespace
+
+int64_t paged_part_floats(int32_t sms) { return 2ll * (2 * sms) * 8 * (kPagedMaxDim + 2); }
+
+void launch_paged_attn(PagedAttnArgs& a, int32_t pool_dtype, int32_t device, int32_t sms, cudaStream_t s) {
+  if (pool_dtype == LC_F32)
+    launch_general<float>(a, device, sms, s);
+  else if (pool_dtype == LC_BF16)
+    launch_general<__nv_bfloat16>(a, device, sms, s);
+  else
+    launch_general<__half>(a, device, sms, s);
+  LC_CUDA(cudaGetLastError());
+}
+
+void launch_paged_weights(const PagedWeightArgs& a, cudaStream_t s) {
+  const int rows = a.n_seqs * a.hkv;
+  const dim3 grid((unsigned)rows, (unsigned)std::min<int64_t>(64, (a.cap + 1023) / 1024));
+  k_paged_weights<<<grid, 256, 2 * a.group * 4, s>>>(a);
+  LC_CUDA(cudaGetLastError());
+}
+
+void launch_paged_append(const PagedAppendArgs& a, cudaStream_t s) {
+  const int64_t rows = (int64_t)a.n_seqs * a.c.hkv * a.n_tokens;
+  const int grid = (int)std::min<int64_t>(148 * 16, (rows + 7) / 8);
+  if (a.pool_dtype == LC_F32)
+    k_paged_append<float><<<grid, 256, 0, s>>>(a);
+  else if (a.pool_dtype == LC_BF16)
+    k_paged_append<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
+  else
+    k_paged_append<__half><<<grid, 256, 0, s>>>(a);
+  LC_CUDA(cudaGetLastError());
+}
+
+}  // namespace lc

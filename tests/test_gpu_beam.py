@@ -1,0 +1,120 @@
+"""Beam search's selection against its plain 64-bit form."""
+import numpy as np
+import pytest
+import torch
+
+import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def check(lc, logits, scores, finished, n_out, eos=2, pad=0):
+    """logits [groups, beams, vocab] on the GPU. Totals in f32 are off by about
+    four roundings of values below 100: 3e-5."""
+    g, beams, vocab = logits.shape
+    beam = lc.BeamSearch(g, beams, vocab, n_out)
+    fin = None if finished is None else torch.from_numpy(finished).cuda()
+    s, p, t, f = beam.select(logits, torch.from_numpy(scores).cuda(), fin, eos_id=eos, pad_id=pad)
+    s, p, t, f = s.cpu().numpy(), p.cpu().numpy(), t.cpu().numpy(), f.cpu().numpy()
+    x = logits.double().cpu().numpy()
+    for i in range(g):
+        want = ref.select(x[i], scores[i], None if finished is None else finished[i], n_out, eos, pad)
+        assert [int(v) for v in p[i]] == [w[1] for w in want]
+        assert [int(v) for v in t[i]] == [w[2] for w in want]
+        assert [int(v) for v in f[i]] == [w[3] for w in want]
+        a, b = s[i].astype(np.float64), np.array([w[0] for w in want])
+        assert np.array_equal(np.isinf(a), np.isinf(b))
+        assert np.allclose(a[np.isfinite(a)], b[np.isfinite(b)], rtol=0, atol=3e-5)
+
+
+def inputs(groups, beams, vocab, dtype, seed, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn((groups, beams, vocab), generator=g) * spread).to(ref.DTYPES[dtype]).cuda()
+    r = np.random.default_rng(seed)
+    return x, (-10 * r.random((groups, beams))).astype(np.float32), r
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("groups,beams,vocab,n_out", [(1, 1, 1, 1), (1, 1, 1, 3), (2, 4, 7, 8), (1, 3, 500, 3), (3, 4, 8191, 4),
+                                                      (2, 5, 8193, 10), (1, 8, 50021, 16), (2, 2, 100003, 17),
+                                                      (1, 64, 1000, 64), (4, 16, 20000, 33), (1, 2, 262144, 64)])
+def test_select_matches_plain(lc, gpu, dtype, groups, beams, vocab, n_out):
+    x, scores, r = inputs(groups, beams, vocab, dtype, groups * 7 + vocab)
+    pad = 0 if vocab < 3 else 1
+    check(lc, x, scores, None, n_out, eos=2, pad=pad)
+    check(lc, x, scores, (r.random((groups, beams)) < 0.4).astype(np.uint8), n_out, eos=2, pad=pad)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_select_ties(lc, gpu, dtype):
+    """Equal logits: the lower token; equal beams: the lower beam. Whole rows equal take the list's
+    long way."""
+    x = torch.zeros((3, 4, 30011), dtype=ref.DTYPES[dtype], device="cuda")
+    x[1, :, ::5] = 1.0
+    x[2, :, 17::4099] = 2.0
+    x[2, 1, 3] = -0.0
+    check(lc, x, np.zeros((3, 4), np.float32), None, 9)
+
+
+def test_select_first_step_and_dead_beams(lc, gpu):
+    """One live beam (the others at -inf), then none, then NaN scores."""
+    x, _, _ = inputs(3, 4, 1000, "f32", 5)
+    scores = np.full((3, 4), -np.inf, np.float32)
+    scores[0, 0] = 0.0
+    scores[2] = [np.nan, -1.0, np.nan, -2.0]
+    check(lc, x, scores, None, 4)
+
+
+def test_select_masked_rows(lc, gpu):
+    """Rows with few or no candidates left, NaN and infinite logits."""
+    x, scores, _ = inputs(5, 3, 20000, "f32", 6)
+    x[0, 0] = -float("inf")
+    x[1] = -float("inf")
+    x[1, 2, 19999] = 1.0
+    x[2, 1, 7] = float("nan")
+    x[3, 0, 9] = float("inf")
+    x[4, :, 100:] = -float("inf")
+    check(lc, x, scores, None, 8)
+    check(lc, x, scores, np.array([[0, 1, 0]] * 5, np.uint8), 8)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_select_strided_rows_and_fewer_groups(lc, gpu, dtype):
+    wide = torch.randn((3, 4, 1100), device="cuda").to(ref.DTYPES[dtype])
+    scores = -torch.rand((3, 4), device="cuda")
+    beam = lc.BeamSearch(5, 4, 1003)
+    got = beam.select(wide[:, :, 5:1008], scores)
+    same = beam.select(wide[:, :, 5:1008].contiguous(), scores)
+    for a, b in zip(got, same):
+        assert torch.equal(a, b)
+
+
+def test_select_repeats(lc, gpu):
+    x, scores, _ = inputs(4, 8, 70001, "bf16", 9)
+    beam = lc.BeamSearch(4, 8, 70001, 16)
+    s = torch.from_numpy(scores).cuda()
+    first = beam.select(x, s)
+    for _ in range(5):
+        for a, b in zip(beam.select(x, s), first):
+            assert torch.equal(a, b)
+
+
+def test_select_refusals(lc, gpu):
+    for args in ((0, 4, 100), (1, 65, 100), (1, 4, 0), (1, 4, 100, 65), (1, 4, 1 << 26), (70000, 1, 10)):
+        with pytest.raises(lc.LumenError) as e:
+            lc.BeamSearch(*args)
+        assert e.value.code == lc.LC_ERR_INVALID
+    beam = lc.BeamSearch(2, 4, 100)
+    x = torch.zeros((2, 4, 100), device="cuda")
+    s = torch.zeros((2, 4), device="cuda")
+    with pytest.raises(lc.LumenError):
+        beam.select(torch.zeros((3, 4, 100), device="cuda"), torch.zeros((3, 4), device="cuda"))
+    with pytest.raises(lc.LumenError):
+        beam.select(x, s, pad_id=100)
+    for bad in (x.cpu(), x.double(), x[:, :3], torch.zeros((2, 100, 4), device="cuda").transpose(1, 2)):
+        with pytest.raises((ValueError, TypeError)):
+            beam.select(bad, s)
+    with pytest.raises((ValueError, TypeError)):
+        beam.select(x, s.double())
+    with pytest.raises((ValueError, TypeError)):
+        beam.select(x, s, s)

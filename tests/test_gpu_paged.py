@@ -1,0 +1,384 @@
+"""The uncompressed paged cache against its plain 64-bit forms: attention,
+accumulated weights, append, eviction and reordering."""
+import numpy as np
+import pytest
+import torch
+
+import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def make(lc, lens, heads, kv, dim, page, dtype, *, layers=2, layer=1, layout="phtd", offset=0, seed=0, spare=3, slack=1):
+    width = max(1, max(-(-n // page) for n in lens)) + slack
+    pages = sum(-(-n // page) for n in lens) + spare
+    k, v = ref.pool(layers, pages, kv, page, dim, dtype, seed, layout, offset)
+    tables = ref.tables_for(lens, page, pages, width, seed)
+    rows = ref.fill_slots(k, v, layer, tables, lens, seed)
+    cache = lc.PagedKvCache(k, v, max_seqs=len(lens), max_pages_per_seq=width, max_q_heads=heads)
+    return cache, tables, torch.tensor(lens, dtype=torch.int32, device="cuda"), rows
+
+
+def queries(n, heads, dim, dtype, seed, gain=1.0):
+    g = torch.Generator().manual_seed(seed + 77)
+    return (torch.randn((n, heads, dim), generator=g) * gain).to(ref.DTYPES[dtype]).cuda()
+
+
+def check(out, want, dtype):
+    got = out.double().cpu()
+    assert not torch.isnan(got).any()
+    err = (got - want).abs() - ref.RTOL[dtype] * want.abs()
+    assert err.max().item() <= ref.ATOL, err.max().item()
+
+
+LENS = [[1], [0, 1, 2], [15, 16, 17, 33], [300, 0, 7, 129, 64, 1000]]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads,kv,dim,page", [(4, 2, 64, 16), (8, 1, 128, 32), (6, 2, 80, 20), (3, 3, 256, 64),
+                                               (12, 1, 96, 8), (20, 1, 128, 16), (5, 5, 20, 7), (2, 1, 33, 16),
+                                               (16, 2, 192, 256), (4, 4, 8, 1), (24, 3, 128, 48)])
+@pytest.mark.parametrize("lens", LENS)
+def test_attn_matches_plain(lc, gpu, dtype, heads, kv, dim, page, lens):
+    cache, tables, ln, rows = make(lc, lens, heads, kv, dim, page, dtype)
+    q = queries(len(lens), heads, dim, dtype, 1)
+    out = cache.attn(1, tables, ln, q, dim ** -0.5)
+    check(out, ref.attn(rows, q, dim ** -0.5)[0], dtype)
+    assert cache.status() == lc.LC_OK
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [1, 15, 64, 100, 5000])
+def test_attn_window(lc, gpu, dtype, window):
+    lens = [0, 1, 64, 65, 999, 2000]
+    cache, tables, ln, rows = make(lc, lens, 8, 2, 128, 32, dtype)
+    q = queries(len(lens), 8, 128, dtype, 2)
+    check(cache.attn(1, tables, ln, q, 0.1, window=window), ref.attn(rows, q, 0.1, window)[0], dtype)
+
+
+@pytest.mark.parametrize("layout,offset", [("pthd", 0), ("plhtd", 0), ("phtd", 1), ("phtd", 8)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_attn_strides_and_alignment(lc, gpu, dtype, layout, offset):
+    lens = [70, 3, 257]
+    cache, tables, ln, rows = make(lc, lens, 8, 4, 64, 16, dtype, layout=layout, offset=offset)
+    q = queries(3, 8, 64, dtype, 3)
+    check(cache.attn(1, tables, ln, q, 0.125), ref.attn(rows, q, 0.125)[0], dtype)
+
+
+@pytest.mark.parametrize("pool,qt,out", [("bf16", "f32", "f32"), ("f16", "f16", "f32"), ("bf16", "bf16", "f32"),
+                                         ("f32", "bf16", "f16"), ("f16", "bf16", "bf16"), ("f32", "f32", "bf16")])
+def test_attn_mixed_types(lc, gpu, pool, qt, out):
+    lens = [500, 31]
+    cache, tables, ln, rows = make(lc, lens, 8, 2, 128, 64, pool)
+    q = queries(2, 8, 128, qt, 4)
+    o = torch.full((2, 8, 128), float("nan"), dtype=ref.DTYPES[out], device="cuda")
+    check(cache.attn(1, tables, ln, q, 0.08, out=o), ref.attn(rows, q, 0.08)[0], out)
+
+
+def test_attn_q_at_odd_address(lc, gpu):
+    lens = [500, 31]
+    cache, tables, ln, rows = make(lc, lens, 8, 2, 128, 64, "bf16")
+    q = queries(2, 8, 128, "bf16", 4)
+    flat = torch.empty(q.numel() + 1, dtype=q.dtype, device="cuda")
+    flat[1:] = q.view(-1)
+    check(cache.attn(1, tables, ln, flat[1:].view(q.shape), 0.08), ref.attn(rows, q, 0.08)[0], "bf16")
+
+
+@pytest.mark.parametrize("dtype,dim,heads,kv", [("bf16", 128, 8, 1), ("f16", 256, 4, 2), ("f32", 64, 3, 1)])
+def test_attn_long_split(lc, gpu, dtype, dim, heads, kv):
+    """One long sequence beside short ones: many partials of one item; peaked scores (gain 3)."""
+    lens = [20011, 5, 0, 1203]
+    cache, tables, ln, rows = make(lc, lens, heads, kv, dim, 64, dtype)
+    q = queries(4, heads, dim, dtype, 5, gain=3.0)
+    out = cache.attn(1, tables, ln, q, dim ** -0.5)
+    check(out, ref.attn(rows, q, dim ** -0.5)[0], dtype)
+    for _ in range(3):  # the order in which blocks finish changes nothing
+        assert torch.equal(cache.attn(1, tables, ln, q, dim ** -0.5), out)
+
+
+def test_attn_many_sequences(lc, gpu):
+    """More sequences than threads of a block, mostly short and empty."""
+    g = np.random.default_rng(8)
+    lens = [int(x) for x in g.integers(0, 40, 700)]
+    cache, tables, ln, rows = make(lc, lens, 2, 1, 64, 16, "bf16", layers=1, layer=0)
+    q = queries(700, 2, 64, "bf16", 6)
+    check(cache.attn(0, tables, ln, q, 0.125), ref.attn(rows, q, 0.125)[0], "bf16")
+
+
+def test_attn_infinite_scores(lc, gpu):
+    """A key row of -inf drops out; where no score is finite the row is zeros."""
+    cache, tables, ln, rows = make(lc, [40, 16], 2, 1, 64, 16, "f32", layers=1, layer=0)
+    q = queries(2, 2, 64, "f32", 7).abs()
+    rows[0][0][0, 5] = -float("inf")
+    cache.k_pages[0, int(tables[0, 0]), 0, 5] = -float("inf")
+    cache.k_pages[0, int(tables[1, 0])] = -float("inf")
+    out = cache.attn(0, tables, ln, q, 0.125)
+    want = ref.attn(rows[:1], q[:1], 0.125)[0]
+    check(out[:1], want, "f32")
+    assert (out[1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,dim", [("f32", 64), ("bf16", 128), ("f16", 80)])
+@pytest.mark.parametrize("heads,kv", [(4, 4), (6, 2), (16, 2), (20, 1)])
+@pytest.mark.parametrize("window,decay", [(0, 1.0), (50, 0.5)])
+def test_weights_match_plain(lc, gpu, dtype, dim, heads, kv, window, decay):
+    lens = [0, 1, 33, 64, 1500]
+    cache, tables, ln, rows = make(lc, lens, heads, kv, dim, 16, dtype)
+    q = queries(len(lens), heads, dim, dtype, 9)
+    span = tables.shape[1] * 16 + 5
+    acc = torch.rand((len(lens), kv, span), device="cuda")
+    acc_out = torch.full_like(acc, 7.0)
+    out = cache.attn_weights(1, tables, ln, q, dim ** -0.5, acc, acc_out, decay=decay, window=window)
+    want, w = ref.attn(rows, q, dim ** -0.5, window)
+    check(out, want, dtype)
+    for s, n in enumerate(lens):
+        add = w[s].view(kv, heads // kv, n).sum(1)
+        got = acc_out[s, :, :n].double().cpu() - decay * acc[s, :, :n].double().cpu()
+        # a weight's relative error is twice its score's absolute error (about 1e-5); acc rounds at 2^-24 of values below 22
+        assert ((got - add).abs() <= 1e-4 * add + 2e-6).all()
+        assert (acc_out[s, :, n:] == 7.0).all()
+    same = acc.clone()
+    cache.attn_weights(1, tables, ln, q, dim ** -0.5, same, decay=decay, window=window)
+    for s, n in enumerate(lens):
+        assert torch.equal(same[s, :, :n], acc_out[s, :, :n]) and torch.equal(same[s, :, n:], acc[s, :, n:])
+
+
+@pytest.mark.parametrize("pool,src", [("bf16", "f32"), ("f16", "f16"), ("f32", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("n_tokens,dim,page", [(1, 128, 16), (37, 33, 8), (5, 256, 64)])
+def test_append(lc, gpu, pool, src, n_tokens, dim, page):
+    kv, lens = 3, [0, 1, page - 1, page, 2 * page + 3]
+    width = -(-(max(lens) + n_tokens) // page)
+    pages = len(lens) * width
+    k, v = ref.pool(2, pages, kv, page, dim, pool, 0)
+    tables = torch.randperm(pages, device="cuda").to(torch.int32).view(len(lens), width)
+    cache = lc.PagedKvCache(k, v, max_seqs=len(lens), max_pages_per_seq=width, max_q_heads=kv)
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    keys = torch.randn((len(lens), kv, n_tokens, dim), device="cuda").to(ref.DTYPES[src])
+    values = torch.randn((len(lens), kv, n_tokens, dim), device="cuda").to(ref.DTYPES[src])
+    pos = torch.full((len(lens), kv, width * page), -9, dtype=torch.int32, device="cuda")
+    pos0 = ln + 100
+    cache.append(1, tables, ln, keys, values, pos, pos0)
+    assert torch.isnan(k[0].float()).all()
+    for pool_t, new in ((k, keys), (v, values)):
+        flat = pool_t[1][tables.long()].transpose(1, 2).reshape(len(lens), kv, width * page, dim)
+        for s, n in enumerate(lens):
+            assert torch.equal(flat[s, :, n:n + n_tokens], new[s].to(k.dtype))
+            assert torch.isnan(flat[s, :, :n].float()).all() and torch.isnan(flat[s, :, n + n_tokens:].float()).all()
+    for s, n in enumerate(lens):
+        assert (pos[s, :, n:n + n_tokens].cpu() == torch.arange(n_tokens) + n + 100).all()
+        assert (pos[s, :, :n] == -9).all() and (pos[s, :, n + n_tokens:] == -9).all()
+
+
+def run_evict(lc, lens, budget, sink, recent, *, kv=2, dim=64, page=16, dtype="bf16", layout="phtd", offset=0, acc=None,
+              seed=3, inplace=False):
+    cache, tables, ln, rows = make(lc, lens, kv, kv, dim, page, dtype, layout=layout, offset=offset, seed=seed)
+    span = tables.shape[1] * page + 3
+    g = torch.Generator().manual_seed(seed)
+    if acc is None:
+        acc = torch.exp(2 * torch.randn((len(lens), kv, span), generator=g))
+    acc = acc.cuda()
+    pos = torch.stack([torch.stack([torch.randperm(span, generator=g) for _ in range(kv)]) for _ in lens]).to(torch.int32)
+    for s, n in enumerate(lens):  # positions 0 .. n - 1 in some order
+        pos[s, :, :n] = torch.argsort(torch.argsort(pos[s, :, :n], dim=1), dim=1).to(torch.int32)
+    pos = pos.cuda()
+    a0, p0 = acc.cpu(), pos.cpu()
+    k0, v0 = cache.k_pages.clone(), cache.v_pages.clone()
+    acc_out = acc if inplace else torch.full_like(acc, 5.0)
+    pos_out = pos if inplace else torch.full_like(pos, 5)
+    cache.evict(1, tables, ln, budget, acc, pos, acc_out, pos_out, n_sink=sink, n_recent=recent)
+    moved = 0
+    for s, n in enumerate(lens):
+        for h in range(kv):
+            a, p, pairs = ref.evict_row(a0[s, h, :n].tolist(), p0[s, h, :n].tolist(), budget, sink, recent)
+            got = acc_out[s, h, :n].cpu()
+            np.testing.assert_array_equal(got.numpy(), np.array(a, np.float32))
+            assert pos_out[s, h, :n].tolist() == p
+            for at, to in pairs:
+                sp, dp = int(tables[s, at // page]), int(tables[s, to // page])
+                k0[1, dp, h, to % page] = k0[1, sp, h, at % page]
+                v0[1, dp, h, to % page] = v0[1, sp, h, at % page]
+            moved += len(pairs)
+    if not inplace:
+        for s, n in enumerate(lens):
+            assert (acc_out[s, :, n:] == 5.0).all() and (pos_out[s, :, n:] == 5).all()
+    else:
+        for s, n in enumerate(lens):
+            np.testing.assert_array_equal(acc_out[s, :, n:].cpu().numpy(), a0[s, :, n:].numpy())
+    assert torch.equal(cache.k_pages.contiguous().view(torch.uint8), k0.contiguous().view(torch.uint8))
+    assert torch.equal(cache.v_pages.contiguous().view(torch.uint8), v0.contiguous().view(torch.uint8))
+    assert cache.status() == lc.LC_OK
+    return moved
+
+
+@pytest.mark.parametrize("lens,budget,sink,recent", [([0, 1, 5], 3, 0, 0), ([2], 1, 0, 1), ([17, 64, 65], 64, 4, 16),
+                                                     ([300, 100], 37, 4, 33), ([1025, 900], 1024, 4, 128),
+                                                     ([5000, 40, 2047], 900, 0, 0), ([9001], 8000, 10, 5)])
+@pytest.mark.parametrize("inplace", [False, True])
+def test_evict_matches_plain(lc, gpu, lens, budget, sink, recent, inplace):
+    run_evict(lc, lens, budget, sink, recent, inplace=inplace)
+
+
+@pytest.mark.parametrize("dtype,dim,layout,offset", [("f32", 128, "pthd", 0), ("f16", 33, "phtd", 0), ("bf16", 256, "plhtd", 0),
+                                                     ("f32", 20, "phtd", 1), ("bf16", 64, "phtd", 3)])
+def test_evict_layouts(lc, gpu, dtype, dim, layout, offset):
+    assert run_evict(lc, [200, 77], 50, 2, 10, dtype=dtype, dim=dim, layout=layout, offset=offset) > 0
+
+
+def test_evict_ties_and_odd_weights(lc, gpu):
+    """Equal weights keep the lower slots; NaN goes first, then -inf; -0 equals 0; +inf stays."""
+    n, kv = 3000, 2
+    acc = torch.zeros((1, kv, 3100))
+    acc[0, 1, ::3] = -0.0
+    acc[0, 0, 5:2000:7] = float("nan")
+    acc[0, 0, 6:2000:7] = -float("inf")
+    acc[0, 0, 2500:2510] = float("inf")
+    acc[0, 1, 100:2900:11] = 1e-42
+    assert run_evict(lc, [n], 1200, 0, 0, acc=acc[:, :, :span_for(n)], kv=kv) > 100
+
+
+def span_for(n, page=16, slack=1):
+    return (-(-n // page) + slack) * page + 3
+
+
+def test_evict_long_row(lc, gpu):
+    """A row over several blocks of a cluster, with runs of equal weights across their borders."""
+    n = 40000
+    g = torch.Generator().manual_seed(4)
+    acc = torch.randint(0, 5, (1, 1, span_for(n, 64)), generator=g).float()
+    assert run_evict(lc, [n], 15000, 4, 100, kv=1, page=64, acc=acc) > 1000
+
+
+def test_evict_keys_beyond_shared_memory(lc, gpu):
+    """So long that a row's keys do not fit the cluster's shared memory."""
+    n = 340000
+    assert run_evict(lc, [n], 2000, 4, 100, kv=1, dim=8, page=256) > 1000
+
+
+@pytest.mark.parametrize("dtype,dim,page,layout", [("bf16", 128, 16, "phtd"), ("f16", 33, 7, "phtd"), ("f32", 64, 32, "pthd"),
+                                                   ("bf16", 80, 100, "plhtd")])
+@pytest.mark.parametrize("groups,beams", [(1, 1), (1, 4), (3, 8), (2, 33)])
+def test_reorder_matches_plain(lc, gpu, dtype, dim, page, layout, groups, beams):
+    g = np.random.default_rng(groups * 100 + beams)
+    for lens in ([page * 2 + 1] * groups, [page] * groups, [0] * groups, [int(x) for x in g.integers(0, 3 * page, groups)]):
+        width, kv = 4, 2
+        pages = groups * beams * width
+        k, v = ref.pool(3, pages, kv, page, dim, dtype, 0, layout)
+        for t in (k, v):
+            t.copy_(torch.randn(t.shape, device="cuda"))
+        cache = lc.PagedKvCache(k, v, max_seqs=groups * beams, max_pages_per_seq=width, max_q_heads=kv)
+        tables = g.permutation(pages).astype(np.int32).reshape(groups * beams, width)
+        parents = g.integers(0, beams, (groups, beams)).astype(np.int32)
+        want, copies = ref.reorder(tables, lens, parents, page)
+        k0, v0 = k.clone(), v.clone()
+        for src, dst, fill in copies:
+            k0[:, dst, :, :fill] = k0[:, src, :, :fill]
+            v0[:, dst, :, :fill] = v0[:, src, :, :fill]
+        out = cache.reorder(torch.from_numpy(tables).cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                            torch.from_numpy(parents).cuda())
+        np.testing.assert_array_equal(out.cpu().numpy(), want)
+        assert torch.equal(k, k0) and torch.equal(v, v0)
+        assert cache.status() == lc.LC_OK
+
+
+def test_other_streams_and_graph(lc, gpu):
+    """Calls on a side stream after the current one, and a captured call replayed with other lengths."""
+    lens = [700, 90]
+    cache, tables, ln, rows = make(lc, lens, 8, 2, 128, 32, "bf16")
+    q = queries(2, 8, 128, "bf16", 11)
+    want = ref.attn(rows, q, 0.1)[0]
+    first = cache.attn(1, tables, ln, q, 0.1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = cache.attn(1, tables, ln, q, 0.1)
+    third = cache.attn(1, tables, ln, q, 0.1)
+    torch.cuda.synchronize()
+    check(first, want, "bf16")
+    assert torch.equal(first, second) and torch.equal(first, third)
+    graph = torch.cuda.CUDAGraph()
+    out = torch.empty_like(q)
+    with torch.cuda.graph(graph):
+        cache.attn(1, tables, ln, q, 0.1, out=out)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, first)
+    ln.copy_(torch.tensor([650, 3], dtype=torch.int32))
+    graph.replay()
+    torch.cuda.synchronize()
+    check(out, ref.attn([(k[:, :n], v[:, :n]) for (k, v), n in zip(rows, (650, 3))], q, 0.1)[0], "bf16")
+
+
+def test_refusals(lc, gpu):
+    k = torch.zeros((1, 4, 2, 16, 64), dtype=torch.bfloat16, device="cuda")
+    cache = lc.PagedKvCache(k, k.clone(), max_seqs=2, max_pages_per_seq=2, max_q_heads=8)
+    tables = torch.zeros((2, 2), dtype=torch.int32, device="cuda")
+    ln = torch.ones(2, dtype=torch.int32, device="cuda")
+    q = torch.zeros((2, 8, 64), dtype=torch.bfloat16, device="cuda")
+    acc, pos = torch.zeros((2, 2, 32), device="cuda"), torch.zeros((2, 2, 32), dtype=torch.int32, device="cuda")
+
+    def refused(f, *args, **kw):
+        with pytest.raises(lc.LumenError) as e:
+            f(*args, **kw)
+        assert e.value.code == lc.LC_ERR_INVALID
+        return str(e.value)
+
+    refused(cache.attn, 1, tables, ln, q, 1.0)  # layer
+    refused(cache.attn, 0, tables, ln, q[:, :7].contiguous(), 1.0)  # heads
+    refused(cache.attn, 0, tables, ln, torch.zeros((2, 16, 64), dtype=q.dtype, device="cuda"), 1.0)
+    refused(cache.attn, 0, tables, ln, q, float("nan"))
+    refused(cache.attn, 0, tables, ln, q, 1.0, window=-1)
+    wide = torch.zeros((2, 3), dtype=torch.int32, device="cuda")
+    refused(cache.attn, 0, wide, ln, q, 1.0)
+    refused(cache.attn_weights, 0, tables, ln, q, 1.0, acc[:, :, :31].contiguous())
+    refused(cache.attn_weights, 0, tables, ln, q, 1.0, acc, decay=1.5)
+    refused(cache.evict, 0, tables, ln, 0, acc, pos)
+    refused(cache.evict, 0, tables, ln, 8, acc, pos, n_sink=4, n_recent=5)
+    parents = torch.zeros((1, 2), dtype=torch.int32, device="cuda")
+    refused(cache.reorder, tables, ln[:1].contiguous(), parents, tables)
+    for bad in (q.cpu(), q.float().double(), q[:, :, :32], q.transpose(0, 1)):
+        with pytest.raises((ValueError, TypeError)):
+            cache.attn(0, tables, ln, bad, 1.0)
+    with pytest.raises((ValueError, TypeError)):
+        cache.attn(0, tables.long(), ln, q, 1.0)
+    with pytest.raises((ValueError, TypeError)):
+        cache.attn(0, tables.cpu(), ln, q, 1.0)
+    # host pointers at the C entry
+    L = lc.lib()
+    host = np.zeros((2, 8, 64), np.float32)
+    assert L.lc_paged_attn(cache._h, 0, 2, tables.data_ptr(), 2, ln.data_ptr(), host.ctypes.data, 0, 8, 1.0, 0, q.data_ptr(), 1,
+                           None) == lc.LC_ERR_INVALID
+    assert L.lc_paged_attn(None, 0, 2, tables.data_ptr(), 2, ln.data_ptr(), q.data_ptr(), 1, 8, 1.0, 0, q.data_ptr(), 1,
+                           None) == lc.LC_ERR_INVALID
+    with pytest.raises(lc.LumenError):  # overlapping rows
+        lc.PagedKvCache(k[:, :1].expand(1, 4, 2, 16, 64), k[:, :1].expand(1, 4, 2, 16, 64), max_seqs=1, max_pages_per_seq=1,
+                        max_q_heads=2)
+    big = torch.zeros((1, 1, 1, 1, 264), device="cuda")
+    with pytest.raises(lc.LumenError):
+        lc.PagedKvCache(big, big.clone(), max_seqs=1, max_pages_per_seq=1, max_q_heads=1)
+
+
+@pytest.mark.parametrize("what", ["len", "negative", "page", "page_low", "parent"])
+def test_status_tells_of_bad_tables(lc, gpu, what):
+    """Lengths, pages and parents out of range are not followed, and told."""
+    k = torch.zeros((1, 4, 2, 16, 64), dtype=torch.bfloat16, device="cuda")
+    cache = lc.PagedKvCache(k, k.clone(), max_seqs=2, max_pages_per_seq=2, max_q_heads=2)
+    tables = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device="cuda")
+    ln = torch.tensor([20, 20], dtype=torch.int32, device="cuda")
+    parents = torch.tensor([[0, 0]], dtype=torch.int32, device="cuda")
+    assert cache.status() == lc.LC_OK
+    if what == "len":
+        ln[1] = 33
+    elif what == "negative":
+        ln[0] = -1
+    elif what == "page":
+        tables[1, 1] = 4
+    elif what == "page_low":
+        tables[0, 1] = -1
+    else:
+        parents[0, 1] = 2
+    if what == "parent":
+        cache.reorder(tables, ln[:1].contiguous(), parents)
+    else:
+        cache.attn(0, tables, ln, torch.zeros((2, 2, 64), dtype=torch.bfloat16, device="cuda"), 1.0)
+    torch.cuda.synchronize()
+    assert cache.status() == lc.LC_ERR_INVALID
