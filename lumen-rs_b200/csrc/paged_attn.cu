@@ -369,6 +369,229 @@ __global__ void __launch_bounds__(W * 32) k_paged_attn(const PagedAttnArgs a) {
   }
 }
 
+// ---- 16-bit pools on the tensor cores --------------------------------------
+__device__ __forceinline__ void mma_16(float* c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+  mma16816(c, a[0], a[1], a[2], a[3], b0, b1);
+}
+__device__ __forceinline__ void mma_16(float* c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// (x, y) in 16 bits, and what that leaves of them
+__device__ __forceinline__ void split_16(float x, float y, uint32_t& hi, uint32_t& lo, __half) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  hi = h2_as_u32(h);
+  lo = h2_as_u32(__floats2half2_rn(x - f.x, y - f.y));
+}
+__device__ __forceinline__ void split_16(float x, float y, uint32_t& hi, uint32_t& lo, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  const float2 f = __bfloat1622float2(h);
+  const __nv_bfloat162 r = __floats2bfloat162_rn(x - f.x, y - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool read) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+
+// The tensor-core kernel: 16-bit pools whose rows are whole 16-byte units,
+// queries of the pool's type, head dimension up to DP.
+//
+// S^T = K Q^T and O^T = V^T P^T by m16n8k16 products: slots (then dimensions)
+// are the 16 rows and up to 8 query heads the 8 columns, so a group of 8 heads
+// wastes nothing and every K and V byte is read from shared memory once, as a
+// fragment of the larger operand. The products are below a tenth of what the
+// HBM-bound pace leaves room for, which is why these are warp-wide products
+// and not tcgen05's: its smallest tile has 64 rows of one operand against the
+// 8 here, and no two warps share a tile. P is fed as two 16-bit halves (value
+// and remainder), which keeps the weights to 2^-17 or better and makes the
+// output's own rounding the only one that shows.
+//
+// Each warp runs its own pipeline: tiles of 16 slots, ST stages of cp.async,
+// no block barrier inside a segment. Rows have 16 bytes of padding: eight
+// rows of an ldmatrix are on different banks. Slots past the end and
+// dimensions past d are filled with zeros, never read.
+template <typename T, int DP, int W, int ST>
+__global__ void __launch_bounds__(W * 32, 1) k_paged_attn_mma(const PagedAttnArgs a) {
+  constexpr int GP = 8, TT = 16, CH = DP / 8, PITCH = DP * 2 + 16, TILE = TT * PITCH;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* om = reinterpret_cast<float*>(smem + W * ST * 2 * TILE);
+  float* ol = om + W * GP;
+  int* prefix = reinterpret_cast<int*>(ol + W * GP);
+  float* oo = reinterpret_cast<float*>(smem);  // [W][GP][DP]: the stages' room, free when a segment ends
+  static_assert(GP * DP * 4 <= ST * 2 * TILE, "the warps' outputs fit the stages");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, tg = lane & 3;
+  const int hg_n = (a.group + GP - 1) / GP, hh_n = a.c.hkv * hg_n;
+  zero_empty<W * 32>(a);
+  build_prefix<W * 32>(a, TT, prefix);
+  const int total = prefix[a.n_seqs] * hh_n;
+  const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, a.min_tiles);
+  const int u_end = min(total, ((int)blockIdx.x + 1) * per);
+  const uint32_t stages = (uint32_t)__cvta_generic_to_shared(smem) + warp * ST * 2 * TILE;
+  const uint32_t k_at = (lane & 15) * PITCH + (lane >> 4) * 16;
+  const uint32_t v_at = ((lane & 7) + ((lane >> 4) << 3)) * PITCH + ((lane >> 3) & 1) * 16;
+  for (int u = blockIdx.x * per; u < u_end;) {
+    const Segment g = find_segment(a, prefix, hh_n, per, u, u_end);
+    u += g.j1 - g.j0;
+    const int h = g.hh / hg_n, head0 = (g.hh - h * hg_n) * GP, nh = min(GP, a.group - head0);
+    const T* kb = static_cast<const T*>(a.c.k) + a.layer * a.c.layer + h * a.c.head;
+    const T* vb = static_cast<const T*>(a.c.v) + a.layer * a.c.layer + h * a.c.head;
+    const int32_t* table = a.c.tables + (int64_t)g.s * a.c.width;
+
+    // lane r (and r + 16) looks up slot r of a tile
+    auto page_of = [&](int j) -> int {
+      const int t = g.lo + j * TT + (lane & 15);
+      return j < g.j1 && t < g.n ? table[t / a.c.page_tokens] : INT32_MIN;
+    };
+    auto issue = [&](int j, int stage, int page) {
+      if (j < g.j1) {
+        const int t = g.lo + j * TT + (lane & 15);
+        int64_t off = -1;
+        if (page >= 0 && page < a.c.n_pages)
+          off = page * a.c.page + (int64_t)(t % a.c.page_tokens) * a.c.token;
+        else if (page != INT32_MIN)
+          *a.c.status = 1;
+        const uint32_t to = stages + stage * 2 * TILE;
+#pragma unroll
+        for (int x = 0; x < TT * CH / 32; ++x) {
+          const int e = x * 32 + lane, r = e / CH, c = e - r * CH;
+          const int64_t o = __shfl_sync(~0u, off, r);
+          const bool read = o >= 0 && c * 8 < a.c.d;
+          const int64_t from = read ? o + c * 8 : 0;
+          cp_async16_or_zero(to + r * PITCH + c * 16, kb + from, read);
+          cp_async16_or_zero(to + TILE + r * PITCH + c * 16, vb + from, read);
+        }
+      }
+      cp_commit();
+    };
+
+    uint32_t qf[DP / 16][2];
+    {
+      const T* q = static_cast<const T*>(a.q) + (((int64_t)g.s * a.c.hkv + h) * a.group + head0 + gr) * a.c.d;
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int x = i * 16 + b * 8 + tg * 2;
+          qf[i][b] = gr < nh && x < a.c.d ? *reinterpret_cast<const uint32_t*>(q + x) : 0u;
+        }
+    }
+    float m0 = kNegInf, m1 = kNegInf, l0 = 0.f, l1 = 0.f, o[DP / 16][4];
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) o[i][x] = 0.f;
+
+    const int first = g.j0 + warp;
+    int page = page_of(first);
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) {
+      const int now = page;
+      page = page_of(first + (i + 1) * W);
+      issue(first + i * W, i, now);
+    }
+    int stage = 0, fill = ST - 1;
+    for (int j = first; j < g.j1; j += W) {
+      cp_wait<ST - 2>();
+      __syncwarp();
+      issue(j + (ST - 1) * W, fill, page);
+      page = page_of(j + ST * W);
+      const uint32_t kt = stages + stage * 2 * TILE, vt = kt + TILE;
+      fill = stage;
+      stage = stage + 1 == ST ? 0 : stage + 1;
+
+      float sa[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i) {
+        uint32_t f[4];
+        ldsm_x4(kt + k_at + i * 32, f);
+        mma_16(i & 1 ? sb : sa, f, qf[i][0], qf[i][1], T());
+      }
+      float s[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[x] = (sa[x] + sb[x]) * a.scale_log2;
+      const int t = g.lo + j * TT + gr;
+      if (t >= g.n) s[0] = s[1] = kNegInf;
+      if (t + 8 >= g.n) s[2] = s[3] = kNegInf;
+      if (a.scores) {
+        float* to = a.scores + (((int64_t)g.s * a.c.hkv + h) * a.score_tokens + t) * a.group + head0 + 2 * tg;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (t + (x >> 1) * 8 < g.n && 2 * tg + (x & 1) < nh) to[(x >> 1) * 8 * a.group + (x & 1)] = s[x];
+      }
+      if (__any_sync(~0u, s[0] > m0 || s[2] > m0 || s[1] > m1 || s[3] > m1)) {
+        float t0 = fmaxf(m0, fmaxf(s[0], s[2])), t1 = fmaxf(m1, fmaxf(s[1], s[3]));
+#pragma unroll
+        for (int b = 4; b < 32; b <<= 1) {
+          t0 = fmaxf(t0, __shfl_xor_sync(~0u, t0, b));
+          t1 = fmaxf(t1, __shfl_xor_sync(~0u, t1, b));
+        }
+        const float f0 = ex2(m0 - (t0 == kNegInf ? 0.f : t0)), f1 = ex2(m1 - (t1 == kNegInf ? 0.f : t1));
+        m0 = t0;
+        m1 = t1;
+        l0 *= f0;
+        l1 *= f1;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          o[i][0] *= f0;
+          o[i][1] *= f1;
+          o[i][2] *= f0;
+          o[i][3] *= f1;
+        }
+      }
+      const float g0 = m0 == kNegInf ? 0.f : m0, g1 = m1 == kNegInf ? 0.f : m1;
+      const float p0 = ex2(s[0] - g0), p1 = ex2(s[1] - g1), p2 = ex2(s[2] - g0), p3 = ex2(s[3] - g1);
+      l0 += p0 + p2;
+      l1 += p1 + p3;
+      uint32_t hi0, hi1, lo0, lo1;
+      split_16(p0, p1, hi0, lo0, T());
+      split_16(p2, p3, hi1, lo1, T());
+      hi0 = transpose_8x8(hi0);
+      hi1 = transpose_8x8(hi1);
+      lo0 = transpose_8x8(lo0);
+      lo1 = transpose_8x8(lo1);
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i) {
+        uint32_t f[4];
+        ldsm_x4_t(vt + v_at + i * 32, f);
+        mma_16(o[i], f, hi0, hi1, T());
+        mma_16(o[i], f, lo0, lo1, T());
+      }
+    }
+    cp_wait<0>();
+#pragma unroll
+    for (int b = 4; b < 32; b <<= 1) {
+      l0 += __shfl_xor_sync(~0u, l0, b);
+      l1 += __shfl_xor_sync(~0u, l1, b);
+    }
+    __syncthreads();
+    if (gr == 0) {
+      om[warp * GP + 2 * tg] = m0;
+      om[warp * GP + 2 * tg + 1] = m1;
+      ol[warp * GP + 2 * tg] = l0;
+      ol[warp * GP + 2 * tg + 1] = l1;
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        oo[(warp * GP + 2 * tg + (x & 1)) * DP + i * 16 + gr + (x >> 1) * 8] = o[i][x];
+    finish_segment<W * 32, GP, DP>(a, g, hg_n, om, ol, oo);
+  }
+}
+
 constexpr int kWarps = 4;
 
 template <int DP, int GP>
@@ -455,12 +678,50 @@ __global__ void __launch_bounds__(256) k_paged_append(const PagedAppendArgs a) {
   }
 }
 
+template <typename T, int DP, int W, int ST>
+void launch_mma(PagedAttnArgs& a, int device, int sms, cudaStream_t s) {
+  auto kernel = k_paged_attn_mma<T, DP, W, ST>;
+  constexpr size_t fixed = (size_t)W * ST * 2 * 16 * (DP * 2 + 16) + 2 * W * 8 * 4;
+  static_assert(fixed + (kPagedMaxSeqs + 1) * 4 <= 226 * 1024, "fits a block");
+  static SmemOptIn opt;
+  opt(kernel, fixed + (kPagedMaxSeqs + 1) * 4, device);
+  a.min_tiles = 2 * W;
+  kernel<<<attn_grid(a, 8, 16, sms), W * 32, fixed + (size_t)(a.n_seqs + 1) * 4, s>>>(a);
+}
+
+template <typename T>
+void launch_mma(PagedAttnArgs& a, int device, int sms, cudaStream_t s) {
+  if (a.c.d <= 64)
+    launch_mma<T, 64, 8, 5>(a, device, sms, s);
+  else if (a.c.d <= 96)
+    launch_mma<T, 96, 8, 4>(a, device, sms, s);
+  else if (a.c.d <= 128)
+    launch_mma<T, 128, 8, 3>(a, device, sms, s);
+  else if (a.c.d <= 192)
+    launch_mma<T, 192, 4, 4>(a, device, sms, s);
+  else
+    launch_mma<T, 256, 4, 3>(a, device, sms, s);
+}
+
+// Rows and strides of whole 16-byte units.
+bool vector_rows(const PagedView& c, int esize) {
+  const int64_t e = 16 / esize;
+  return c.d % e == 0 && c.layer % e == 0 && c.page % e == 0 && c.head % e == 0 && c.token % e == 0 &&
+         (reinterpret_cast<uintptr_t>(c.k) & 15) == 0 && (reinterpret_cast<uintptr_t>(c.v) & 15) == 0;
+}
+
 }  // namespace
 
 int64_t paged_part_floats(int32_t sms) { return 2ll * (2 * sms) * 8 * (kPagedMaxDim + 2); }
 
 void launch_paged_attn(PagedAttnArgs& a, int32_t pool_dtype, int32_t device, int32_t sms, cudaStream_t s) {
-  if (pool_dtype == LC_F32)
+  const bool mma = pool_dtype != LC_F32 && a.q_dtype == pool_dtype && vector_rows(a.c, 2) &&
+                   (reinterpret_cast<uintptr_t>(a.q) & 3) == 0;
+  if (mma && pool_dtype == LC_BF16)
+    launch_mma<__nv_bfloat16>(a, device, sms, s);
+  else if (mma)
+    launch_mma<__half>(a, device, sms, s);
+  else if (pool_dtype == LC_F32)
     launch_general<float>(a, device, sms, s);
   else if (pool_dtype == LC_BF16)
     launch_general<__nv_bfloat16>(a, device, sms, s);
