@@ -829,40 +829,48 @@ class NativeRotatingKvCacheTurboQuant:
 # ---------------------------------------------------------------------------
 # The uncompressed paged cache and beam search
 # ---------------------------------------------------------------------------
-def _dev(x, name: str, shape, dtype: str, device: int) -> int:
-    """Address of a contiguous CUDA tensor of this shape and type on `device`."""
-    if not x.is_cuda or x.device.index != device:
+# torch dtypes by short name and LC_* codes by torch dtype, filled when a handle
+# below is made (the package itself does not import torch)
+_TORCH: dict = {}
+_FLOAT_CODES: dict = {}
+
+
+def _need_torch():
+    if not _TORCH:
+        import torch
+
+        _FLOAT_CODES.update({torch.float32: LC_F32, torch.bfloat16: LC_BF16, torch.float16: LC_F16})
+        _TORCH.update({"f32": torch.float32, "int32": torch.int32, "uint8": torch.uint8,
+                       "raw_stream": torch._C._cuda_getCurrentRawStream})
+
+
+def _dev(x, name: str, shape, dtype, device: int) -> int:
+    """Address of a contiguous CUDA tensor of this shape (and type, unless None) on `device`."""
+    if x.get_device() != device:
         raise ValueError(f"{name} must be a tensor on cuda:{device}")
     if x.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(x.shape)}")
-    if dtype is not None and _TORCH_NAMES.get(x.dtype) != dtype:
+    if dtype is not None and x.dtype is not _TORCH[dtype]:
         raise TypeError(f"{name} must be {dtype}, got {x.dtype}")
     if not x.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return x.data_ptr()
 
 
-class _TorchNames(dict):
-    """torch dtype -> short name, filled at first use (torch is not imported with the package)."""
-
-    def get(self, key, default=None):
-        if not self:
-            import torch
-
-            self.update({torch.float32: "f32", torch.bfloat16: "bf16", torch.float16: "f16", torch.int32: "int32",
-                         torch.uint8: "uint8"})
-        return dict.get(self, key, default)
-
-
-_TORCH_NAMES = _TorchNames()
-_FLOAT_CODES = {"f32": LC_F32, "bf16": LC_BF16, "f16": LC_F16}
-
-
 def _float_code(x, name: str) -> int:
-    code = _FLOAT_CODES.get(_TORCH_NAMES.get(x.dtype))
+    code = _FLOAT_CODES.get(x.dtype)
     if code is None:
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}")
     return code
+
+
+def _stream_on(stream, device: int) -> int:
+    """_auto_stream for calls whose tensors are all on `device`: the caller's, else torch's current one."""
+    if stream is not None:
+        stream = getattr(stream, "cuda_stream", stream)
+    else:
+        stream = _TORCH["raw_stream"](device)
+    return stream if stream else CUDA_STREAM_LEGACY
 
 
 class PagedKvCache:
@@ -873,6 +881,7 @@ class PagedKvCache:
     tables is int32 [n_seqs, pages] and lens int32 [n_seqs], on the GPU."""
 
     def __init__(self, k_pages, v_pages, *, max_seqs: int, max_pages_per_seq: int, max_q_heads: int):
+        _need_torch()
         if k_pages.dim() != 5 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
             raise ValueError("k_pages and v_pages must be [n_layers, n_pages, n_kv_heads, page_tokens, head_dim] alike")
         if not k_pages.is_cuda or v_pages.device != k_pages.device:
@@ -902,8 +911,8 @@ class PagedKvCache:
     __del__ = close
 
     def _rows(self, tables, lens):
-        n = tables.shape[0]
-        return n, _dev(tables, "tables", (n, tables.shape[1]), "int32", self.device), tables.shape[1], \
+        n, width = shape = tables.shape
+        return n, _dev(tables, "tables", shape, "int32", self.device), width, \
             _dev(lens, "lens", (n,), "int32", self.device)
 
     def status(self) -> int:
@@ -926,7 +935,7 @@ class PagedKvCache:
             at = _dev(pos, "pos", (n, self.n_kv_heads, span), "int32", self.device)
             p0 = _dev(pos0, "pos0", (n,), "int32", self.device)
         _check(lib().lc_paged_append(self._h, layer, n, t, width, ln, k, v, _float_code(keys, "keys"), keys.shape[2], at,
-                                     span, p0, _auto_stream(stream, keys)))
+                                     span, p0, _stream_on(stream, self.device)))
 
     def attn(self, layer: int, tables, lens, q, scale: float, window: int = 0, out=None, stream=None):
         """softmax(scale q K^T) V for one query token per sequence, q [n_seqs, n_q_heads, head_dim],
@@ -938,7 +947,7 @@ class PagedKvCache:
             out = q.new_empty(shape)
         _check(lib().lc_paged_attn(self._h, layer, n, t, width, ln, _dev(q, "q", shape, None, self.device),
                                    _float_code(q, "q"), heads, scale, window, _dev(out, "out", shape, None, self.device),
-                                   _float_code(out, "out"), _auto_stream(stream, q)))
+                                   _float_code(out, "out"), _stream_on(stream, self.device)))
         return out
 
     def attn_weights(self, layer: int, tables, lens, q, scale: float, acc_in, acc_out=None, decay: float = 1.0,
@@ -955,7 +964,7 @@ class PagedKvCache:
             self._h, layer, n, t, width, ln, _dev(q, "q", shape, None, self.device), _float_code(q, "q"), heads, scale,
             window, _dev(out, "out", shape, None, self.device), _float_code(out, "out"),
             _dev(acc_in, "acc_in", rows, "f32", self.device), _dev(acc_out, "acc_out", rows, "f32", self.device), span,
-            decay, _auto_stream(stream, q)))
+            decay, _stream_on(stream, self.device)))
         return out
 
     def evict(self, layer: int, tables, lens, budget: int, acc_in, pos_in, acc_out=None, pos_out=None, n_sink: int = 0,
@@ -972,7 +981,7 @@ class PagedKvCache:
         _check(lib().lc_paged_evict(
             self._h, layer, n, t, width, ln, budget, n_sink, n_recent, _dev(acc_in, "acc_in", rows, "f32", self.device),
             _dev(pos_in, "pos_in", rows, "int32", self.device), _dev(acc_out, "acc_out", rows, "f32", self.device),
-            _dev(pos_out, "pos_out", rows, "int32", self.device), span, _auto_stream(stream, acc_in)))
+            _dev(pos_out, "pos_out", rows, "int32", self.device), span, _stream_on(stream, self.device)))
 
     def reorder(self, tables, lens, parents, tables_out=None, stream=None):
         """Beams change places: row j of each group continues row parents[g, j] (int32 [n_groups, n_beams]);
@@ -987,7 +996,7 @@ class PagedKvCache:
                                       _dev(lens, "lens", (groups,), "int32", self.device),
                                       _dev(parents, "parents", (groups, beams), "int32", self.device),
                                       _dev(tables_out, "tables_out", shape, "int32", self.device),
-                                      _auto_stream(stream, tables)))
+                                      _stream_on(stream, self.device)))
         return tables_out
 
 
@@ -996,6 +1005,7 @@ class BeamSearch:
     n_groups groups of n_beams rows; n_out (n_beams unless given) are chosen."""
 
     def __init__(self, n_groups: int, n_beams: int, vocab: int, n_out: Optional[int] = None, device: int = 0):
+        _need_torch()
         self.n_groups, self.n_beams, self.vocab, self.device = n_groups, n_beams, vocab, device
         self.n_out = n_beams if n_out is None else n_out
         h = C.c_void_p()
@@ -1015,25 +1025,25 @@ class BeamSearch:
         parents int32, tokens int32, finished uint8), each [groups, n_out]. logits [groups, n_beams, vocab]
         (rows may be strided), scores f32 and finished uint8 [groups, n_beams]. A finished beam has the
         one candidate pad_id at its score."""
-        g = logits.shape[0]
-        rows = (g, self.n_beams)
-        if not logits.is_cuda or logits.device.index != self.device:
+        g, beams, vocab = logits.shape
+        if logits.get_device() != self.device:
             raise ValueError(f"logits must be a tensor on cuda:{self.device}")
-        if logits.shape != (g, self.n_beams, self.vocab):
+        if beams != self.n_beams or vocab != self.vocab:
             raise ValueError(f"logits must have shape {(g, self.n_beams, self.vocab)}, got {tuple(logits.shape)}")
-        stride = logits.stride()
-        row = stride[1] if self.n_beams > 1 else stride[0] if g > 1 else self.vocab
-        if (self.vocab > 1 and stride[2] != 1) or (g > 1 and self.n_beams > 1 and stride[0] != self.n_beams * row):
-            raise ValueError("logits must be rows of contiguous values, evenly apart")
-        import torch
-
-        shape = (g, self.n_out)
-        out = torch.empty((3,) + shape, dtype=torch.int32, device=logits.device)
-        fin = torch.empty(shape, dtype=torch.uint8, device=logits.device)
-        base, step = out.data_ptr(), 4 * g * self.n_out
-        _check(lib().lc_beam_select(
-            self._h, g, logits.data_ptr(), _float_code(logits, "logits"), row,
-            _dev(scores, "scores", rows, "f32", self.device),
-            None if finished is None else _dev(finished, "finished", rows, "uint8", self.device), eos_id, pad_id, base,
-            base + step, base + 2 * step, fin.data_ptr(), _auto_stream(stream, logits)))
-        return out[0].view(torch.float32), out[1], out[2], fin
+        if logits.is_contiguous():
+            row = vocab
+        else:
+            stride = logits.stride()
+            row = stride[1] if beams > 1 else stride[0] if g > 1 else vocab
+            if (vocab > 1 and stride[2] != 1) or (g > 1 and beams > 1 and stride[0] != beams * row):
+                raise ValueError("logits must be rows of contiguous values, evenly apart")
+        rows, shape = (g, beams), (g, self.n_out)
+        at = _dev(scores, "scores", rows, "f32", self.device)
+        fin = None if finished is None else _dev(finished, "finished", rows, "uint8", self.device)
+        new = scores.new_empty(shape)
+        parents, tokens = scores.new_empty((2,) + shape, dtype=_TORCH["int32"]).unbind(0)
+        done = scores.new_empty(shape, dtype=_TORCH["uint8"])
+        _check(lib().lc_beam_select(self._h, g, logits.data_ptr(), _float_code(logits, "logits"), row, at, fin, eos_id, pad_id,
+                                    new.data_ptr(), parents.data_ptr(), tokens.data_ptr(), done.data_ptr(),
+                                    _stream_on(stream, self.device)))
+        return new, parents, tokens, done

@@ -59,6 +59,29 @@ __device__ __forceinline__ float elem<__half>(const uint4& r, int i) {
   return __half2float(__ushort_as_half((unsigned short)(i & 1 ? w >> 16 : w & 0xffffu)));
 }
 
+// The largest of a granule's values; NaN only where all are.
+template <typename T>
+__device__ __forceinline__ float granule_max(const uint4& r);
+template <>
+__device__ __forceinline__ float granule_max<float>(const uint4& r) {
+  return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+}
+template <typename T2>
+__device__ __forceinline__ T2 max_2x4(const uint4& r) {
+  const T2* h = reinterpret_cast<const T2*>(&r);
+  return __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+}
+template <>
+__device__ __forceinline__ float granule_max<__nv_bfloat16>(const uint4& r) {
+  const float2 f = __bfloat1622float2(max_2x4<__nv_bfloat162>(r));
+  return fmaxf(f.x, f.y);
+}
+template <>
+__device__ __forceinline__ float granule_max<__half>(const uint4& r) {
+  const float2 f = __half22float2(max_2x4<__half2>(r));
+  return fmaxf(f.x, f.y);
+}
+
 __device__ __forceinline__ uint64_t block_max_key(uint64_t k, uint64_t* warp_key) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
@@ -102,11 +125,11 @@ __device__ __forceinline__ bool arrive_last(int* counter, int of) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_beam_select(const BeamArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) k_beam_select(const BeamArgs a) {
   constexpr int E = 16 / sizeof(T);
-  __shared__ uint64_t list[kBeamMaxMerge];  // the slice's list, then the merges' candidates
+  __shared__ __align__(16) uint64_t list[kBeamMaxMerge];  // the slice's list, then the merges' candidates
   __shared__ uint64_t warp_key[kThreads / 32];
-  __shared__ float sets[kThreads];
+  __shared__ __align__(16) float sets[kThreads];
   __shared__ float red_m[kThreads / 32], red_s[kThreads / 32];
   __shared__ float sh_tau, sh_shift;
   __shared__ int sh_n, sh_at[kThreads + 1];
@@ -123,30 +146,36 @@ __global__ void __launch_bounds__(kThreads) k_beam_select(const BeamArgs a) {
     const T* base = x0 - mis;  // index i of the row sits at base[i + mis]
     const int i_end = mis + a.vocab;
     uint4 raw[kGran];
-    float top = kNegInf;
+    const int64_t at0 = (int64_t)slice * a.slice + tid * E;
+    if (at0 - tid * E >= mis && at0 - tid * E + a.slice <= i_end) {  // the whole slice is inside the row
 #pragma unroll
-    for (int r = 0; r < kGran; ++r) {
-      const int64_t at = (int64_t)slice * a.slice + (int64_t)(r * kThreads + tid) * E;
-      if (at >= mis && at + E <= i_end) {
-        raw[r] = __ldcs(reinterpret_cast<const uint4*>(base + at));
-      } else {
-        alignas(16) T part[E];
+      for (int r = 0; r < kGran; ++r) raw[r] = __ldcs(reinterpret_cast<const uint4*>(base + at0 + r * kThreads * E));
+    } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-          part[i] = at + i >= mis && at + i < i_end ? base[at + i] : T(kNegInf);
-        raw[r] = *reinterpret_cast<uint4*>(part);
+      for (int r = 0; r < kGran; ++r) {
+        const int64_t at = at0 + r * kThreads * E;
+        if (at >= mis && at + E <= i_end) {
+          raw[r] = __ldcs(reinterpret_cast<const uint4*>(base + at));
+        } else {
+          alignas(16) T part[E];
+#pragma unroll
+          for (int i = 0; i < E; ++i) part[i] = at + i >= mis && at + i < i_end ? base[at + i] : T(kNegInf);
+          raw[r] = *reinterpret_cast<uint4*>(part);
+        }
       }
     }
+    float top = kNegInf;
 #pragma unroll
-    for (int r = 0; r < kGran; ++r)
-#pragma unroll
-      for (int i = 0; i < E; ++i) top = fmaxf(top, elem<T>(raw[r], i));
+    for (int r = 0; r < kGran; ++r) top = fmaxf(top, granule_max<T>(raw[r]));
     const float tg = top == kNegInf ? 0.f : top;
     float sum = 0.f;
 #pragma unroll
-    for (int r = 0; r < kGran; ++r)
+    for (int r = 0; r < kGran; ++r) {
+      float part = 0.f;
 #pragma unroll
-      for (int i = 0; i < E; ++i) sum += ex2((elem<T>(raw[r], i) - tg) * kLog2e);
+      for (int i = 0; i < E; ++i) part += ex2((elem<T>(raw[r], i) - tg) * kLog2e);
+      sum += part;
+    }
     // maxima of 64 sets of four threads, or of 256
     const bool few = a.n_out <= 16;
     float set = top;
@@ -174,10 +203,17 @@ __global__ void __launch_bounds__(kThreads) k_beam_select(const BeamArgs a) {
     if (tid < n_sets) {
       int r = 0;
       const float v = sets[tid];
-      for (int i = 0; i < n_sets; ++i) r += sets[i] > v || (sets[i] == v && i < tid);
+#pragma unroll 4
+      for (int i = 0; i < n_sets; i += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(sets + i);
+        r += x.x > v || (x.x == v && i < tid);
+        r += x.y > v || (x.y == v && i + 1 < tid);
+        r += x.z > v || (x.z == v && i + 2 < tid);
+        r += x.w > v || (x.w == v && i + 3 < tid);
+      }
       if (r == a.n_out - 1) sh_tau = v;
     }
-    if (tid == 0) {
+    if (tid == kThreads - 1) {  // a warp that has no set to rank where there are 64
       float mm = kNegInf, ll = 0.f;
       for (int w = 0; w < kThreads / 32; ++w) {
         const float mn = fmaxf(mm, red_m[w]), mg = mn == kNegInf ? 0.f : mn;
@@ -190,16 +226,17 @@ __global__ void __launch_bounds__(kThreads) k_beam_select(const BeamArgs a) {
     __syncthreads();
     const float tau = sh_tau;
 #pragma unroll
-    for (int r = 0; r < kGran; ++r)
-#pragma unroll
+    for (int r = 0; r < kGran; ++r) {
+      if (!(granule_max<T>(raw[r]) >= tau)) continue;
+      const int64_t index = at0 + r * kThreads * E - mis;
       for (int i = 0; i < E; ++i) {
         const float x = elem<T>(raw[r], i);
         if (x >= tau && x > kNegInf) {
           const int at = atomicAdd(&sh_n, 1);
-          const int64_t index = (int64_t)slice * a.slice + (int64_t)(r * kThreads + tid) * E + i - mis;
-          if (at < kList) list[at] = make_key(x, (uint32_t)index);
+          if (at < kList) list[at] = make_key(x, (uint32_t)(index + i));
         }
       }
+    }
     __syncthreads();
     const int found = sh_n;
     uint64_t* keys = a.slice_key + srow * a.n_out;
@@ -211,19 +248,24 @@ __global__ void __launch_bounds__(kThreads) k_beam_select(const BeamArgs a) {
         if (r < a.n_out) keys[r] = k;
       }
     } else {
-      // many logits equal to the bound: one best after the other
+      // many logits equal to the bound: one best after the other, from shared memory
+      uint4* held = reinterpret_cast<uint4*>(list);
+      static_assert(sizeof(list) >= kGran * kThreads * 16, "the slice fits the list");
+#pragma unroll
+      for (int r = 0; r < kGran; ++r) held[r * kThreads + tid] = raw[r];
       uint64_t before = ~0ull;
       for (int o = 0; o < a.n_out; ++o) {
         uint64_t best = 0;
-#pragma unroll
-        for (int r = 0; r < kGran; ++r)
-#pragma unroll
+#pragma unroll 1
+        for (int r = 0; r < kGran; ++r) {
+          const uint4 x4 = held[r * kThreads + tid];
+#pragma unroll 1
           for (int i = 0; i < E; ++i) {
-            const float x = elem<T>(raw[r], i);
-            const int64_t index = (int64_t)slice * a.slice + (int64_t)(r * kThreads + tid) * E + i - mis;
-            const uint64_t k = make_key(x, (uint32_t)index);
+            const float x = elem<T>(x4, i);
+            const uint64_t k = make_key(x, (uint32_t)(at0 + r * kThreads * E + i - mis));
             if (x >= tau && k < before && k > best) best = k;
           }
+        }
         before = block_max_key(best, warp_key);
         if (tid == 0) keys[o] = before;
       }

@@ -412,7 +412,7 @@ int lc_paged_reorder(lc_paged* p, int32_t n_groups, int32_t n_beams, const int32
     a.esize = p->esize;
     a.parents = parents;
     a.tables_out = tables_out;
-    launch_paged_reorder(a, p->order.on(stream));
+    launch_paged_reorder(a, p->sms, p->order.on(stream));
   });
 }
 

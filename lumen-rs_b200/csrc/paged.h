@@ -132,7 +132,7 @@ void launch_paged_weights(const PagedWeightArgs& a, cudaStream_t s);
 int paged_evict_cluster(int32_t rows, int64_t cap, int32_t sms);
 bool paged_evict_keys_in_smem(int64_t cap, int cluster);
 void launch_paged_evict(const PagedEvictArgs& a, int32_t device, int32_t sms, cudaStream_t s);
-void launch_paged_reorder(const PagedReorderArgs& a, cudaStream_t s);
+void launch_paged_reorder(const PagedReorderArgs& a, int32_t sms, cudaStream_t s);
 int beam_slice(int32_t dtype);
 void launch_beam(const BeamArgs& a, cudaStream_t s);
 

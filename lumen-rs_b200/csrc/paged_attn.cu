@@ -70,17 +70,19 @@ __device__ __forceinline__ int64_t row_offset(const PagedView& c, int s, int t) 
 }
 
 // prefix[s] = tiles of the sequences before s (of one item each); prefix[n_seqs]
-// the total. Every thread of the block calls it.
+// the total. Sequences with nothing to attend to get their zeros here. Every
+// thread of the block calls it.
 template <int THREADS>
 __device__ void build_prefix(const PagedAttnArgs& a, int tile, int* prefix) {
   __shared__ int warp_sum[THREADS / 32];
   const int tid = threadIdx.x, per = (a.n_seqs + THREADS - 1) / THREADS;
   const int b = min(a.n_seqs, tid * per), e = min(a.n_seqs, b + per);
-  int sum = 0;
-  for (int s = b; s < e; ++s) {
+  auto tiles_of = [&](int s) {
     const int n = clamp_len(a.c, s);
-    sum += (n - first_slot(n, a.window) + tile - 1) / tile;
-  }
+    return (n - first_slot(n, a.window) + tile - 1) / tile;
+  };
+  int sum = 0;
+  for (int s = b; s < e; ++s) sum += tiles_of(s);
   int inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -90,14 +92,22 @@ __device__ void build_prefix(const PagedAttnArgs& a, int tile, int* prefix) {
   if ((tid & 31) == 31) warp_sum[tid >> 5] = inc;
   __syncthreads();
   int at = inc - sum;
-  for (int w = 0; w < (tid >> 5); ++w) at += warp_sum[w];
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w)
+    if (w < (tid >> 5)) at += warp_sum[w];
   for (int s = b; s < e; ++s) {
     prefix[s] = at;
-    const int n = clamp_len(a.c, s);
-    at += (n - first_slot(n, a.window) + tile - 1) / tile;
+    at += per == 1 ? sum : tiles_of(s);
   }
   if (tid == THREADS - 1) prefix[a.n_seqs] = at;
   __syncthreads();
+  const int heads = a.c.hkv * a.group, d = a.c.d;
+  for (int s = blockIdx.x; s < a.n_seqs; s += gridDim.x) {
+    if (prefix[s + 1] != prefix[s]) continue;
+    for (int x = tid; x < heads * d; x += THREADS) store_f32(a.out, (int64_t)s * heads * d + x, a.out_dtype, 0.f);
+    if (a.stats)
+      for (int x = tid; x < 2 * heads; x += THREADS) a.stats[2ll * s * heads + x] = 0.f;
+  }
 }
 
 // A block's share of one item: tiles [j0, j1) of sequence s, item hh (kv head
@@ -138,48 +148,57 @@ __device__ __forceinline__ Segment find_segment(const PagedAttnArgs& a, const in
 
 // Joins the warps' (m, l, o) of a segment (shared memory: om, ol [warps][GP],
 // oo [warps][GP][DP]) and writes the item's rows, its partial, or, as the last
-// block of a split item, the join of all its partials. Block-wide.
+// block of a split item, the join of all its partials. Block-wide; the weights
+// of the sums are worked out once a head, in om and (for the partials) in oo.
 template <int THREADS, int GP, int DP>
-__device__ void finish_segment(const PagedAttnArgs& a, const Segment& g, int hg_n, const float* om, const float* ol,
-                               const float* oo) {
+__device__ void finish_segment(const PagedAttnArgs& a, const Segment& g, int hg_n, float* om, const float* ol,
+                               float* oo) {
   constexpr int W = THREADS / 32;
+  constexpr int64_t kSlot = GP * (DP + 2);
   __shared__ int last;
-  const int tid = threadIdx.x, d = a.c.d;
+  __shared__ float scale[GP];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, d = a.c.d;
   const int h = g.hh / hg_n, head0 = (g.hh - h * hg_n) * GP, nh = min(GP, a.group - head0);
   const int64_t row0 = (int64_t)g.s * a.c.hkv * a.group + (int64_t)h * a.group + head0;
-  __syncthreads();
-  auto put = [&](int i, int x, float m, float l, float o) {
+  float* part = a.part + g.slot * kSlot;
+  auto row_stats = [&](int i, float m, float l) {
     const float inv = l == 0.f ? 0.f : 1.f / l;  // no slot with a finite score: zeros
-    store_f32(a.out, (row0 + i) * d + x, a.out_dtype, o * inv);
-    if (a.stats && x == 0) {
+    scale[i] = inv;
+    if (a.stats && i < nh) {
       a.stats[2 * (row0 + i)] = m == kNegInf ? 0.f : m;
       a.stats[2 * (row0 + i) + 1] = inv;
     }
   };
-  constexpr int64_t kSlot = GP * (DP + 2);
-  float* part = a.part + g.slot * kSlot;
-  for (int e = tid; e < nh * d; e += THREADS) {
-    const int i = e / d, x = e - i * d;
-    float m = kNegInf;
+  __syncthreads();
+  if (tid < GP) {
+    float m = kNegInf, l = 0.f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) m = fmaxf(m, om[w * GP + i]);
+    for (int w = 0; w < W; ++w) m = fmaxf(m, om[w * GP + tid]);
     const float mg = m == kNegInf ? 0.f : m;
-    float l = 0.f, o = 0.f;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float f = ex2(om[w * GP + i] - mg);
-      l += f * ol[w * GP + i];
-      o += f * oo[(w * GP + i) * DP + x];
+      const float f = ex2(om[w * GP + tid] - mg);
+      l += f * ol[w * GP + tid];
+      om[w * GP + tid] = f;
     }
     if (g.parts == 1) {
-      put(i, x, m, l, o);
+      row_stats(tid, m, l);
     } else {
-      if (x == 0) {
-        part[i] = m;
-        part[GP + i] = l;
-      }
-      part[2 * GP + i * DP + x] = o;
+      part[tid] = m;
+      part[GP + tid] = l;
     }
+  }
+  __syncthreads();
+  for (int e = tid; e < nh * DP; e += THREADS) {
+    const int i = e / DP, x = e % DP;
+    if (x >= d) continue;
+    float o = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) o = fmaf(om[w * GP + i], oo[(w * GP + i) * DP + x], o);
+    if (g.parts == 1)
+      store_f32(a.out, (row0 + i) * d + x, a.out_dtype, o * scale[i]);
+    else
+      part[2 * GP + i * DP + x] = o;
   }
   if (g.parts > 1) {
     int* counter = a.counters + (int64_t)g.s * a.c.hkv * hg_n + g.hh;
@@ -192,35 +211,35 @@ __device__ void finish_segment(const PagedAttnArgs& a, const Segment& g, int hg_
     __syncthreads();
     if (last) {
       __threadfence();
-      for (int e = tid; e < nh * d; e += THREADS) {
-        const int i = e / d, x = e - i * d;
-        float m = kNegInf, l = 0.f, o = 0.f;
-        for (int b = g.first; b < g.first + g.parts; ++b) {
-          const float* p = a.part + (b == g.first ? g.slot0 : 2 * b) * kSlot;
-          const float pm = __ldcg(p + i), pl = __ldcg(p + GP + i), po = __ldcg(p + 2 * GP + i * DP + x);
-          const float mn = fmaxf(m, pm), mg = mn == kNegInf ? 0.f : mn;
-          const float fa = ex2(m - mg), fb = ex2(pm - mg);
-          l = l * fa + pl * fb;
-          o = o * fa + po * fb;
-          m = mn;
+      auto slot = [&](int b) { return a.part + (b == 0 ? g.slot0 : 2 * (g.first + b)) * kSlot; };
+      for (int i = warp; i < nh; i += W) {
+        float m = kNegInf, l = 0.f;
+        for (int b = lane; b < g.parts; b += 32) m = fmaxf(m, __ldcg(slot(b) + i));
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+        const float mg = m == kNegInf ? 0.f : m;
+        for (int b = lane; b < g.parts; b += 32) {
+          const float f = ex2(__ldcg(slot(b) + i) - mg);
+          l += f * __ldcg(slot(b) + GP + i);
+          oo[b * GP + i] = f;
         }
-        put(i, x, m, l, o);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+        if (lane == 0) row_stats(i, m, l);
+      }
+      __syncthreads();
+      for (int e = tid; e < nh * DP; e += THREADS) {
+        const int i = e / DP, x = e % DP;
+        if (x >= d) continue;
+        float o = oo[i] * __ldcg(slot(0) + 2 * GP + e);
+#pragma unroll 8
+        for (int b = 1; b < g.parts; ++b)
+          o = fmaf(oo[b * GP + i], __ldcg(a.part + 2 * (g.first + b) * kSlot + 2 * GP + e), o);
+        store_f32(a.out, (row0 + i) * d + x, a.out_dtype, o * scale[i]);
       }
     }
   }
   __syncthreads();
-}
-
-// Rows of sequences with nothing to attend to: zeros.
-template <int THREADS>
-__device__ void zero_empty(const PagedAttnArgs& a) {
-  const int heads = a.c.hkv * a.group, d = a.c.d;
-  for (int s = blockIdx.x; s < a.n_seqs; s += gridDim.x) {
-    if (clamp_len(a.c, s) != 0) continue;
-    for (int e = threadIdx.x; e < heads * d; e += THREADS) store_f32(a.out, (int64_t)s * heads * d + e, a.out_dtype, 0.f);
-    if (a.stats)
-      for (int e = threadIdx.x; e < 2 * heads; e += THREADS) a.stats[2ll * s * heads + e] = 0.f;
-  }
 }
 
 // The general kernel: any of the three types in and out, any alignment, head
@@ -241,10 +260,9 @@ __global__ void __launch_bounds__(W * 32) k_paged_attn(const PagedAttnArgs a) {
   float* ol = om + W * GP;
   int* prefix = reinterpret_cast<int*>(ol + W * GP);
   float* oo = kt;  // [W][GP][DP]: the tiles' room, free when a segment ends
-  static_assert(GP * DP <= TT * PITCH, "the warps' outputs fit the key tiles");
+  static_assert(2 * 148 * 2 * GP <= W * TT * PITCH && GP * DP <= TT * PITCH, "the warps' outputs fit the key tiles");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hg_n = (a.group + GP - 1) / GP, hh_n = a.c.hkv * hg_n;
-  zero_empty<W * 32>(a);
   build_prefix<W * 32>(a, TT, prefix);
   const int total = prefix[a.n_seqs] * hh_n;
   const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, a.min_tiles);
@@ -434,7 +452,6 @@ __global__ void __launch_bounds__(W * 32, 1) k_paged_attn_mma(const PagedAttnArg
   static_assert(GP * DP * 4 <= ST * 2 * TILE, "the warps' outputs fit the stages");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, tg = lane & 3;
   const int hg_n = (a.group + GP - 1) / GP, hh_n = a.c.hkv * hg_n;
-  zero_empty<W * 32>(a);
   build_prefix<W * 32>(a, TT, prefix);
   const int total = prefix[a.n_seqs] * hh_n;
   const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, a.min_tiles);

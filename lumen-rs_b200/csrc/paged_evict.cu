@@ -40,28 +40,31 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Exclusive sum over the block of x; *total gets the block's sum.
-__device__ __forceinline__ int block_scan(int x, int* warp_sum, int* total) {
+// Exclusive sum over the block of x (two counts in one word where a caller
+// needs two); *total gets the block's sum.
+__device__ __forceinline__ uint64_t block_scan(uint64_t x, uint64_t* warp_sum, uint64_t* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int inc = x;
+  uint64_t inc = x;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(~0u, inc, o);
+    const uint64_t up = __shfl_up_sync(~0u, inc, o);
     if (lane >= o) inc += up;
   }
   __syncthreads();
   if (lane == 31) warp_sum[warp] = inc;
   __syncthreads();
-  int before = 0, all = 0;
+  uint64_t before = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < kEvictThreads / 32; ++w) {
-    if (w < warp) before += warp_sum[w];
-    all += warp_sum[w];
+    const uint64_t v = warp_sum[w];
+    if (w < warp) before += v;
+    all += v;
   }
   *total = all;
   return before + inc - x;
 }
 
+// Offset in copy units of slot t's row, or -1 for a page id outside the pool.
 __device__ __forceinline__ int64_t page_row(const PagedView& c, int s, int t) {
   const int page = c.tables[(int64_t)s * c.width + t / c.page_tokens];
   if (page < 0 || page >= c.n_pages) {
@@ -71,29 +74,39 @@ __device__ __forceinline__ int64_t page_row(const PagedView& c, int s, int t) {
   return page * c.page + (int64_t)(t % c.page_tokens) * c.token;
 }
 
-// U: the unit of a copy (uint4 where rows and strides are 16-byte aligned,
-// else the element).
-template <typename U>
-__global__ void __launch_bounds__(kEvictThreads) k_paged_evict(const PagedEvictArgs a, const int cl, const int use_smem) {
+// CL: the row has a cluster of blocks (else one). U: the unit of a copy, in
+// which the view's strides and d are given.
+template <typename U, bool CL>
+__global__ void __launch_bounds__(kEvictThreads) k_paged_evict(const PagedEvictArgs a, const int cl_arg,
+                                                               const int use_smem) {
   extern __shared__ uint32_t smem_keys[];
-  __shared__ int hist[3][kBins];
-  __shared__ int warp_sum[kEvictThreads / 32];
-  __shared__ int sh_max, sh_bin, sh_need, sh_eq, sh_hole, sh_move;
+  __shared__ __align__(16) int hist[3][kBins];
+  __shared__ uint64_t warp_sum[kEvictThreads / 32];
+  __shared__ uint64_t sh_count;
+  __shared__ int sh_max, sh_bin, sh_need, sh_equal, sh_eq;
   cg::cluster_group cluster = cg::this_cluster();
+  const int cl = CL ? cl_arg : 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rank = blockIdx.x % cl;
-  const int row = blockIdx.x / cl, s = row / a.c.hkv, h = row - s * a.c.hkv;
+  const int rank = CL ? blockIdx.x % cl : 0;
+  const int row = CL ? blockIdx.x / cl : blockIdx.x, s = row / a.c.hkv, h = row - s * a.c.hkv;
   const int cap = a.c.width * a.c.page_tokens;
+  auto sync = [&] {
+    if (CL)
+      cluster.sync();
+    else
+      __syncthreads();
+  };
+  auto remote = [&](auto* p, int r) { return CL ? cluster.map_shared_rank(p, r) : p; };
   int n = a.c.lens[s];
-  if (n < 0 || n > cap || n > a.stride) {
+  if (n < 0 || n > cap) {
     *a.c.status = 1;
-    n = n < 0 ? 0 : (int)min((int64_t)cap, a.stride);
+    n = n < 0 ? 0 : cap;
   }
   const float* acc_in = a.acc_in + row * a.stride;
   const int* pos_in = a.pos_in + row * a.stride;
   float* acc_out = a.acc_out + row * a.stride;
   int* pos_out = a.pos_out + row * a.stride;
-  const int per = (n + cl - 1) / cl, b = min(n, rank * per), e = min(n, b + per);
+  const int per = CL ? (n + cl - 1) / cl : n, b = min(n, rank * per), e = min(n, b + per);
   if (n <= a.budget) {  // the same for every block of the cluster
     for (int t = b + tid; t < e; t += kEvictThreads) {
       acc_out[t] = acc_in[t];
@@ -105,16 +118,20 @@ __global__ void __launch_bounds__(kEvictThreads) k_paged_evict(const PagedEvictA
 
   // the newest position
   int newest = INT32_MIN;
+#pragma unroll 4
   for (int t = b + tid; t < e; t += kEvictThreads) newest = max(newest, pos_in[t]);
   if (tid == 0) sh_max = INT32_MIN;
-  for (int i = tid; i < 3 * kBins; i += kEvictThreads) (&hist[0][0])[i] = 0;
+  for (int i = tid; i < 3 * kBins / 4; i += kEvictThreads) reinterpret_cast<int4*>(hist)[i] = make_int4(0, 0, 0, 0);
   __syncthreads();
   newest = __reduce_max_sync(~0u, newest);
   if (lane == 0) atomicMax(&sh_max, newest);
-  cluster.sync();
+  sync();
   newest = INT32_MIN;
-  for (int r = 0; r < cl; ++r) newest = max(newest, *cluster.map_shared_rank(&sh_max, r));
+#pragma unroll
+  for (int r = 0; r < kEvictMaxCluster; ++r)
+    if (r < cl) newest = max(newest, *remote(&sh_max, r));
 
+#pragma unroll 4
   for (int t = b + tid; t < e; t += kEvictThreads) {
     const int p = pos_in[t];
     const bool held = p < a.n_sink || (int64_t)p > (int64_t)newest - a.n_recent;
@@ -128,25 +145,31 @@ __global__ void __launch_bounds__(kEvictThreads) k_paged_evict(const PagedEvictA
   int need = a.budget;
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
-    cluster.sync();
-    constexpr int kPer = kBins / kEvictThreads;
+    sync();
+    static_assert(kBins == 4 * kEvictThreads, "four bins a thread");
     const int bins = pass == 2 ? 1024 : kBins, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    int mine[kPer], sum = 0;
+    const int quad = bins / 4 - 1 - tid;  // the highest bins first
+    int4 q = make_int4(0, 0, 0, 0);
+    if (quad >= 0) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int bin = bins - 1 - (tid * kPer + i);
-      mine[i] = 0;
-      if (bin >= 0)
-        for (int r = 0; r < cl; ++r) mine[i] += *cluster.map_shared_rank(&hist[pass][bin], r);
-      sum += mine[i];
+      for (int r = 0; r < kEvictMaxCluster; ++r)
+        if (r < cl) {
+          const int4 x = *remote(reinterpret_cast<const int4*>(hist[pass]) + quad, r);
+          q.x += x.x;
+          q.y += x.y;
+          q.z += x.z;
+          q.w += x.w;
+        }
     }
-    int total;
-    int above = block_scan(sum, warp_sum, &total);
+    uint64_t total;
+    int above = (int)block_scan((uint64_t)(q.x + q.y + q.z + q.w), warp_sum, &total);
+    const int mine[4] = {q.w, q.z, q.y, q.x};
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
+    for (int i = 0; i < 4; ++i) {
       if (above < need && need <= above + mine[i]) {
-        sh_bin = bins - 1 - (tid * kPer + i);
+        sh_bin = 4 * quad + 3 - i;
         sh_need = need - above;
+        sh_equal = mine[i];
       }
       above += mine[i];
     }
@@ -156,6 +179,7 @@ __global__ void __launch_bounds__(kEvictThreads) k_paged_evict(const PagedEvictA
     if (pass < 2) {
       const uint32_t mask = ~0u << shift;
       const int next = pass == 0 ? 10 : 0, width = pass == 0 ? kBins : 1024;
+#pragma unroll 4
       for (int i = tid; i < e - b; i += kEvictThreads) {
         const uint32_t key = keys[i];
         if ((key & mask) == prefix) atomicAdd(&hist[pass + 1][(key >> next) & (width - 1)], 1);
@@ -166,48 +190,59 @@ __global__ void __launch_bounds__(kEvictThreads) k_paged_evict(const PagedEvictA
   // each thread owns a run of slots (odd length: one bank each)
   const int run = ((e - b + kEvictThreads - 1) / kEvictThreads) | 1;
   const int i0 = min(e - b, tid * run), i1 = min(e - b, i0 + run);
-  int eq = 0, total;
-  for (int i = i0; i < i1; ++i) eq += keys[i] == prefix;
-  int eq_at = block_scan(eq, warp_sum, &total);
-  if (tid == 0) sh_eq = total;
-  cluster.sync();
-  for (int r = 0; r < rank; ++r) eq_at += *cluster.map_shared_rank(&sh_eq, r);
-  int holes = 0, movers = 0;
+  uint64_t total;
+  int eq_at = 0;
+  if (need < sh_equal) {  // the first `need` of equal keys stay (the same for every block)
+    int eq = 0;
+    for (int i = i0; i < i1; ++i) eq += keys[i] == prefix;
+    eq_at = (int)block_scan((uint64_t)eq, warp_sum, &total);
+    if (tid == 0) sh_eq = (int)total;
+    sync();
+    for (int r = 0; r < rank; ++r) eq_at += *remote(&sh_eq, r);
+  } else {
+    need = INT32_MAX;
+    __syncthreads();  // the run's keys were written by other threads' strides
+  }
+  uint64_t counts = 0;  // holes below, movers above 32 bits
   for (int i = i0; i < i1; ++i) {
     const uint32_t key = keys[i];
     bool stay = key > prefix;
     if (key == prefix) stay = eq_at++ < need;
     keys[i] = stay;
-    holes += b + i < a.budget && !stay;
-    movers += b + i >= a.budget && stay;
+    if (b + i < a.budget)
+      counts += !stay;
+    else
+      counts += (uint64_t)stay << 32;
   }
-  int hole_at = block_scan(holes, warp_sum, &total);
-  if (tid == 0) sh_hole = total;
-  int move_at = block_scan(movers, warp_sum, &total);
-  if (tid == 0) sh_move = total;
-  cluster.sync();
-  int pairs = 0;
-  for (int r = 0; r < cl; ++r) {
-    const int x = *cluster.map_shared_rank(&sh_hole, r);
-    if (r < rank) {
-      hole_at += x;
-      move_at += *cluster.map_shared_rank(&sh_move, r);
-    }
-    pairs += x;
+  uint64_t at = block_scan(counts, warp_sum, &total);
+  if (CL) {
+    if (tid == 0) sh_count = total;
+    sync();
+    total = 0;
+#pragma unroll
+    for (int r = 0; r < kEvictMaxCluster; ++r)
+      if (r < cl) {
+        const uint64_t x = *remote(&sh_count, r);
+        if (r < rank) at += x;
+        total += x;
+      }
   }
-  int* hole = a.list + row * 4 * a.list_cap;
-  int* mover = hole + a.list_cap;
+  const int pairs = (int)(total & 0xffffffffu);
+  int* hole = a.list + row * 4 * a.list_cap + (uint32_t)at;
+  int* mover = a.list + row * 4 * a.list_cap + a.list_cap + (at >> 32);
   for (int i = i0; i < i1; ++i) {
     const int t = b + i;
-    if (t < a.budget && !keys[i]) hole[hole_at++] = t;
-    if (t >= a.budget && keys[i]) {
-      mover[move_at] = t;
-      mover[a.list_cap + move_at] = __float_as_int(acc_in[t]);
-      mover[2 * a.list_cap + move_at] = pos_in[t];
-      ++move_at;
+    if (t < a.budget) {
+      if (!keys[i]) *hole++ = t;
+    } else if (keys[i]) {
+      mover[0] = t;
+      mover[a.list_cap] = __float_as_int(acc_in[t]);
+      mover[2 * a.list_cap] = pos_in[t];
+      ++mover;
     }
   }
   __syncthreads();  // acc_out may be acc_in: the movers' values are read above
+#pragma unroll 4
   for (int t = b + tid; t < e; t += kEvictThreads) {
     if (t >= a.budget) {
       acc_out[t] = 0.f;
@@ -217,87 +252,89 @@ __global__ void __launch_bounds__(kEvictThreads) k_paged_evict(const PagedEvictA
       pos_out[t] = pos_in[t];
     }
   }
-  cluster.sync();
+  sync();
 
   // the moves: eight pairs a warp at a time
-  const int units = a.c.d * a.esize / (int)sizeof(U);
-  const int64_t per_u = sizeof(U) / a.esize;
-  U* kb = static_cast<U*>(a.c.k) + (a.layer * a.c.layer + h * a.c.head) / per_u;
-  U* vb = static_cast<U*>(a.c.v) + (a.layer * a.c.layer + h * a.c.head) / per_u;
-  for (int p0 = (rank * (kEvictThreads / 32) + warp) * 8; p0 < pairs; p0 += cl * (kEvictThreads / 32) * 8) {
+  const int* list = a.list + row * 4 * a.list_cap;
+  U* kb = static_cast<U*>(a.c.k) + a.layer * a.c.layer + h * a.c.head;
+  U* vb = static_cast<U*>(a.c.v) + a.layer * a.c.layer + h * a.c.head;
+  const int units = a.c.d;
+  constexpr int kWarps = kEvictThreads / 32;
+  for (int p0 = (rank * kWarps + warp) * 8; p0 < pairs; p0 += cl * kWarps * 8) {
     int64_t src = -1, dst = -1;
     if (lane < 8 && p0 + lane < pairs) {
-      const int to = hole[p0 + lane], from = mover[p0 + lane];
+      const int* pair = list + p0 + lane;
+      const int to = pair[0], from = pair[a.list_cap];
       dst = page_row(a.c, s, to);
       src = page_row(a.c, s, from);
-      acc_out[to] = __int_as_float(mover[a.list_cap + p0 + lane]);
-      pos_out[to] = mover[2 * a.list_cap + p0 + lane];
+      acc_out[to] = __int_as_float(pair[2 * a.list_cap]);
+      pos_out[to] = pair[3 * a.list_cap];
       if (src < 0) dst = -1;
     }
     int64_t from[8], to[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      from[i] = __shfl_sync(~0u, src, i) / per_u;
+      from[i] = __shfl_sync(~0u, src, i);
       to[i] = __shfl_sync(~0u, dst, i);
     }
     for (int x = lane; x < 2 * units; x += 32) {
       U* base = x >= units ? vb : kb;
-      const int at = x >= units ? x - units : x;
+      const int at_u = x >= units ? x - units : x;
       U got[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (to[i] >= 0) got[i] = base[from[i] + at];
+        if (to[i] >= 0) got[i] = base[from[i] + at_u];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (to[i] >= 0) base[to[i] / per_u + at] = got[i];
+        if (to[i] >= 0) base[to[i] + at_u] = got[i];
     }
   }
 }
 
-// Reordering: block (row j, layer, part). The group's mapping (who inherits
-// which tail page) is worked out by every block from the parents; blocks of
-// layer 0's first part write row j's table, and where row j is a later child
-// of its parent, its blocks copy the first `fill` slots of the parent's tail
-// page into the spare tail page that it takes.
+// Reordering: block (row j, share of the copies). Every block works out the
+// group's mapping (who inherits which tail page) from the parents; a row's
+// first block writes its table, and where row j is a later child of its
+// parent, its blocks copy the first `fill` slots of the parent's tail page
+// into the spare tail page that it takes, four units a thread at a time.
 template <typename U>
 __global__ void __launch_bounds__(256) k_paged_reorder(const PagedReorderArgs a) {
   __shared__ int parent[kBeamMaxBeams], first[kBeamMaxBeams];
   __shared__ int owner;
   const int tid = threadIdx.x, w = a.n_beams;
   const int row = blockIdx.x, g = row / w, j = row - g * w;
-  if (tid < w) first[tid] = INT32_MAX;
-  __syncthreads();
-  if (tid < w) {
-    int p = a.parents[(int64_t)g * w + tid];
-    if (p < 0 || p >= w) {
-      *a.c.status = 1;
-      p = tid;
-    }
-    parent[tid] = p;
-    atomicMin(&first[p], tid);
-  }
-  __syncthreads();
-  if (tid == 0) {
-    int own = parent[j];
-    if (first[own] != j) {  // the i-th later child takes the i-th childless beam's tail
-      int i = 0;
-      for (int x = 0; x < j; ++x) i += first[parent[x]] != x;
-      own = -1;
-      while (i >= 0) i -= first[++own] == INT32_MAX;
-    }
-    owner = own;
-  }
-  __syncthreads();
-  const int p = parent[j], own = owner;
   const int cap = a.c.width * a.c.page_tokens;
   int n = a.c.lens[g];
   if (n < 0 || n > cap) {
     *a.c.status = 1;
     n = n < 0 ? 0 : cap;
   }
+  int p = -1;
+  if (tid < w) {
+    first[tid] = INT32_MAX;
+    p = a.parents[(int64_t)g * w + tid];
+    if (p < 0 || p >= w) {
+      *a.c.status = 1;
+      p = tid;
+    }
+    parent[tid] = p;
+  }
+  __syncthreads();
+  if (tid < w) atomicMin(&first[p], tid);
+  __syncthreads();
+  p = parent[j];
+  if (first[p] != j && tid == 0) {  // the i-th later child takes the i-th childless beam's tail
+    int i = 0, own = -1;
+    for (int x = 0; x < j; ++x) i += first[parent[x]] != x;
+    while (i >= 0) i -= first[++own] == INT32_MAX;
+    owner = own;
+  } else if (tid == 0) {
+    owner = p;
+  }
+  __syncthreads();
+  const int own = owner;
   const int full = n / a.c.page_tokens, fill = n - full * a.c.page_tokens;
   const int32_t* tables = a.c.tables + (int64_t)g * w * a.c.width;
-  if (blockIdx.y == 0 && blockIdx.z == 0)
+  if (blockIdx.y == 0)
     for (int i = tid; i < a.c.width; i += 256) {
       const int from = i < full ? p : i == full && fill > 0 ? own : j;
       a.tables_out[(int64_t)row * a.c.width + i] = tables[(int64_t)from * a.c.width + i];
@@ -308,16 +345,26 @@ __global__ void __launch_bounds__(256) k_paged_reorder(const PagedReorderArgs a)
     if (tid == 0) *a.c.status = 1;
     return;
   }
-  const int64_t per_u = sizeof(U) / a.esize;
-  const int units = (int)(a.c.d / per_u);
-  const int is_v = blockIdx.z & 1, part = blockIdx.z >> 1, parts = gridDim.z >> 1;
-  U* base = static_cast<U*>(is_v ? a.c.v : a.c.k) + blockIdx.y * a.c.layer / per_u;
-  const int64_t total = (int64_t)a.c.hkv * fill * units;
-  for (int64_t x = (int64_t)part * 256 + tid; x < total; x += (int64_t)parts * 256) {
-    const int64_t r = x / units;
-    const int c = (int)(x - r * units), h = (int)(r / fill), t = (int)(r - (int64_t)h * fill);
-    const int64_t at = (h * a.c.head + t * a.c.token) / per_u + c;
-    base[dst * a.c.page / per_u + at] = base[src * a.c.page / per_u + at];
+  // the copy's rows, (layer, K or V, head, slot), shared out evenly
+  const uint32_t units = a.c.d, per_head = units * fill, per_pool = per_head * a.c.hkv;
+  const int64_t total = (int64_t)per_pool * 2 * a.c.n_layers, step = (int64_t)gridDim.y * 256;
+  for (int64_t x0 = (int64_t)blockIdx.y * 256 + tid; x0 < total; x0 += 4 * step) {
+    U got[4];
+    U* to[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t x = x0 + i * step;
+      to[i] = nullptr;
+      if (x >= total) continue;
+      const uint32_t lp = (uint32_t)(x / per_pool), y = (uint32_t)(x - (int64_t)lp * per_pool);
+      const uint32_t h = y / per_head, z = y - h * per_head, t = z / units, c = z - t * units;
+      U* base = static_cast<U*>(lp & 1 ? a.c.v : a.c.k) + (lp >> 1) * a.c.layer + h * a.c.head + t * a.c.token + c;
+      got[i] = base[src * a.c.page];
+      to[i] = base + dst * a.c.page;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (to[i]) *to[i] = got[i];
   }
 }
 
@@ -328,18 +375,38 @@ bool vector_rows(const PagedView& c, int esize) {
          (reinterpret_cast<uintptr_t>(c.k) & 15) == 0 && (reinterpret_cast<uintptr_t>(c.v) & 15) == 0;
 }
 
+// The view with strides and d in units of U.
 template <typename U>
-void launch_evict(const PagedEvictArgs& a, int device, int sms, cudaStream_t s) {
-  auto kernel = k_paged_evict<U>;
-  static SmemOptIn opt;
-  opt(kernel, kEvictSmemKeys * 4, device);
+PagedView in_units(PagedView c, int esize) {
+  const int64_t e = sizeof(U) / esize;
+  c.layer /= e;
+  c.page /= e;
+  c.head /= e;
+  c.token /= e;
+  c.d = (int32_t)(c.d / e);
+  return c;
+}
+
+template <typename U>
+void launch_evict(PagedEvictArgs a, int device, int sms, cudaStream_t s) {
   const int64_t cap = std::min<int64_t>((int64_t)a.c.width * a.c.page_tokens, a.stride);
   const int rows = a.n_seqs * a.c.hkv, cl = paged_evict_cluster(rows, cap, sms);
   const bool in_smem = paged_evict_keys_in_smem(cap, cl);
+  const size_t smem = in_smem ? (size_t)((cap + cl - 1) / cl) * 4 : 0;
+  a.c = in_units<U>(a.c, a.esize);
+  if (cl == 1) {
+    static SmemOptIn opt;
+    opt(k_paged_evict<U, false>, kEvictSmemKeys * 4, device);
+    k_paged_evict<U, false><<<rows, kEvictThreads, smem, s>>>(a, 1, in_smem);
+    LC_CUDA(cudaGetLastError());
+    return;
+  }
+  static SmemOptIn opt;
+  opt(k_paged_evict<U, true>, kEvictSmemKeys * 4, device);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * cl));
   cfg.blockDim = dim3(kEvictThreads);
-  cfg.dynamicSmemBytes = in_smem ? (size_t)((cap + cl - 1) / cl) * 4 : 0;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -347,7 +414,17 @@ void launch_evict(const PagedEvictArgs& a, int device, int sms, cudaStream_t s) 
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  LC_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, cl, in_smem ? 1 : 0));
+  LC_CUDA(cudaLaunchKernelEx(&cfg, k_paged_evict<U, true>, a, cl, in_smem ? 1 : 0));
+}
+
+template <typename U>
+void launch_reorder(PagedReorderArgs a, int sms, cudaStream_t s) {
+  a.c = in_units<U>(a.c, a.esize);
+  // blocks a row: enough that one row in four copying fills the card, and none with less than 16 units a thread
+  const int64_t rows = (int64_t)a.n_groups * a.n_beams;
+  const int64_t units = 2ll * a.c.n_layers * a.c.hkv * a.c.page_tokens * a.c.d;
+  const int64_t y = std::max<int64_t>(1, std::min<int64_t>((units + 4095) / 4096, (32ll * sms + rows - 1) / rows));
+  k_paged_reorder<U><<<dim3((unsigned)rows, (unsigned)std::min<int64_t>(y, 65535)), 256, 0, s>>>(a);
 }
 
 }  // namespace
@@ -372,16 +449,13 @@ void launch_paged_evict(const PagedEvictArgs& a, int32_t device, int32_t sms, cu
     launch_evict<uint16_t>(a, device, sms, s);
 }
 
-void launch_paged_reorder(const PagedReorderArgs& a, cudaStream_t s) {
-  const int64_t bytes = (int64_t)a.c.hkv * a.c.page_tokens * a.c.d * a.esize;  // of a whole page
-  const unsigned parts = (unsigned)std::max<int64_t>(1, std::min<int64_t>(16, bytes / (32 << 10)));
-  const dim3 grid((unsigned)(a.n_groups * a.n_beams), (unsigned)a.c.n_layers, 2 * parts);
+void launch_paged_reorder(const PagedReorderArgs& a, int32_t sms, cudaStream_t s) {
   if (vector_rows(a.c, a.esize))
-    k_paged_reorder<uint4><<<grid, 256, 0, s>>>(a);
+    launch_reorder<uint4>(a, sms, s);
   else if (a.esize == 4)
-    k_paged_reorder<uint32_t><<<grid, 256, 0, s>>>(a);
+    launch_reorder<uint32_t>(a, sms, s);
   else
-    k_paged_reorder<uint16_t><<<grid, 256, 0, s>>>(a);
+    launch_reorder<uint16_t>(a, sms, s);
   LC_CUDA(cudaGetLastError());
 }
 
