@@ -383,11 +383,12 @@ int lc_paged_evict(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* ta
     // at most min(budget, cap - budget) slots move in a row
     const int64_t rows = (int64_t)n_seqs * p->cfg.n_kv_heads;
     a.list_cap = std::max<int64_t>(1, std::min<int64_t>(budget, cap - budget));
-    const int cl = paged_evict_cluster((int32_t)rows, cap, p->sms);
+    const int cl = paged_evict_cluster(cap);
     const int64_t keys = paged_evict_keys_in_smem(cap, cl) ? 0 : rows * stride;
-    int32_t* ws = static_cast<int32_t*>(p->evict.get((size_t)(rows * 4 * a.list_cap + keys) * 4));
+    int32_t* ws = static_cast<int32_t*>(p->evict.get((size_t)(rows * (4 * a.list_cap + 1) + keys) * 4));
     a.list = ws;
-    a.keys = reinterpret_cast<uint32_t*>(ws + rows * 4 * a.list_cap);
+    a.pairs = ws + rows * 4 * a.list_cap;
+    a.keys = reinterpret_cast<uint32_t*>(a.pairs + rows);
     launch_paged_evict(a, p->cfg.device, p->sms, p->order.on(stream));
   });
 }

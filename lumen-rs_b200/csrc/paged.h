@@ -87,6 +87,8 @@ struct PagedEvictArgs {
   int32_t* pos_out;
   int32_t* list;   // workspace: per row [4][list_cap]: holes, movers, the movers' acc and pos
   int64_t list_cap;
+  int32_t* pairs;  // workspace: [rows], the lists' lengths
+  int32_t fused;
   uint32_t* keys;  // workspace: [rows][stride], used where a row's keys do not fit shared memory
 };
 
@@ -129,7 +131,7 @@ void launch_paged_append(const PagedAppendArgs& a, cudaStream_t s);
 void launch_paged_attn(PagedAttnArgs& a, int32_t pool_dtype, int32_t device, int32_t sms, cudaStream_t s);
 int64_t paged_part_floats(int32_t sms);
 void launch_paged_weights(const PagedWeightArgs& a, cudaStream_t s);
-int paged_evict_cluster(int32_t rows, int64_t cap, int32_t sms);
+int paged_evict_cluster(int64_t cap);
 bool paged_evict_keys_in_smem(int64_t cap, int cluster);
 void launch_paged_evict(const PagedEvictArgs& a, int32_t device, int32_t sms, cudaStream_t s);
 void launch_paged_reorder(const PagedReorderArgs& a, int32_t sms, cudaStream_t s);

@@ -28,10 +28,12 @@ namespace cg = cooperative_groups;
 namespace lc {
 namespace {
 
-constexpr int kEvictThreads = 512;
 constexpr int kBins = 2048;  // 11 + 11 + 10 bits of the key
 constexpr int kEvictMaxCluster = 8;
 constexpr int64_t kEvictSmemKeys = 40 * 1024;  // 160 KB of keys a block
+constexpr int kFusedMoves = 64;  // longest list that a row's own blocks move (a second launch costs more)
+constexpr int kMoveBatch = 16;
+constexpr int kHeld = 8;  // slots whose acc and pos a thread of a row's only block holds in registers
 
 // Monotone map to unsigned; NaN below everything, -0 as 0.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -42,6 +44,7 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 
 // Exclusive sum over the block of x (two counts in one word where a caller
 // needs two); *total gets the block's sum.
+template <int THREADS>
 __device__ __forceinline__ uint64_t block_scan(uint64_t x, uint64_t* warp_sum, uint64_t* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint64_t inc = x;
@@ -53,15 +56,16 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t x, uint64_t* warp_sum, u
   __syncthreads();
   if (lane == 31) warp_sum[warp] = inc;
   __syncthreads();
-  uint64_t before = 0, all = 0;
+  constexpr int W = THREADS / 32;
+  uint64_t sums = lane < W ? warp_sum[lane] : 0;
 #pragma unroll
-  for (int w = 0; w < kEvictThreads / 32; ++w) {
-    const uint64_t v = warp_sum[w];
-    if (w < warp) before += v;
-    all += v;
+  for (int o = 1; o < W; o <<= 1) {
+    const uint64_t up = __shfl_up_sync(~0u, sums, o);
+    if (lane >= o) sums += up;
   }
-  *total = all;
-  return before + inc - x;
+  *total = __shfl_sync(~0u, sums, W - 1);
+  const uint64_t before = __shfl_sync(~0u, sums, warp > 0 ? warp - 1 : 0);
+  return (warp > 0 ? before : 0) + inc - x;
 }
 
 // Offset in copy units of slot t's row, or -1 for a page id outside the pool.
@@ -74,14 +78,54 @@ __device__ __forceinline__ int64_t page_row(const PagedView& c, int s, int t) {
   return page * c.page + (int64_t)(t % c.page_tokens) * c.token;
 }
 
+// Moves pairs [0, pairs) of a row's list: warp `first` of `warps`, B pairs at
+// a time: their lookups by B lanes, then N copies in flight a lane.
+template <typename U, int B, int N>
+__device__ __forceinline__ void move_pairs(const PagedEvictArgs& a, int row, int pairs, int first, int warps) {
+  const int lane = threadIdx.x & 31, s = row / a.c.hkv, h = row - s * a.c.hkv;
+  const int* list = a.list + row * 4 * a.list_cap;
+  U* kb = static_cast<U*>(a.c.k) + a.layer * a.c.layer + h * a.c.head;
+  U* vb = static_cast<U*>(a.c.v) + a.layer * a.c.layer + h * a.c.head;
+  const int units = a.c.d;
+  for (int p0 = first * B; p0 < pairs; p0 += warps * B) {
+    int64_t src = -1, dst = -1;
+    if (lane < B && p0 + lane < pairs) {
+      const int* pair = list + p0 + lane;
+      const int to = pair[0], from = pair[a.list_cap];
+      const int acc = pair[2 * a.list_cap], pos = pair[3 * a.list_cap];
+      dst = page_row(a.c, s, to);
+      src = page_row(a.c, s, from);
+      a.acc_out[row * a.stride + to] = __int_as_float(acc);
+      a.pos_out[row * a.stride + to] = pos;
+      if (src < 0) dst = -1;
+    }
+    for (int q = 0; q < B && p0 + q < pairs; q += N)
+      for (int x0 = 0; x0 < 2 * units; x0 += 32) {
+        const int x = x0 + lane;
+        U* base = x >= units ? vb + (x - units) : kb + x;
+        U got[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int64_t from = __shfl_sync(~0u, src, q + i), to = __shfl_sync(~0u, dst, q + i);
+          if (to >= 0 && x < 2 * units) got[i] = base[from];
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int64_t to = __shfl_sync(~0u, dst, q + i);
+          if (to >= 0 && x < 2 * units) base[to] = got[i];
+        }
+      }
+  }
+}
+
 // CL: the row has a cluster of blocks (else one). U: the unit of a copy, in
 // which the view's strides and d are given.
-template <typename U, bool CL>
-__global__ void __launch_bounds__(kEvictThreads) k_paged_evict(const PagedEvictArgs a, const int cl_arg,
-                                                               const int use_smem) {
+template <typename U, int THREADS, bool CL>
+__global__ void __launch_bounds__(THREADS, CL ? 2 : 1)
+    k_paged_evict(const PagedEvictArgs a, const int cl_arg, const int use_smem) {
   extern __shared__ uint32_t smem_keys[];
   __shared__ __align__(16) int hist[3][kBins];
-  __shared__ uint64_t warp_sum[kEvictThreads / 32];
+  __shared__ uint64_t warp_sum[THREADS / 32];
   __shared__ uint64_t sh_count;
   __shared__ int sh_max, sh_bin, sh_need, sh_equal, sh_eq;
   cg::cluster_group cluster = cg::this_cluster();
@@ -97,48 +141,86 @@ __global__ void __launch_bounds__(kEvictThreads) k_paged_evict(const PagedEvictA
       __syncthreads();
   };
   auto remote = [&](auto* p, int r) { return CL ? cluster.map_shared_rank(p, r) : p; };
-  int n = a.c.lens[s];
-  if (n < 0 || n > cap) {
-    *a.c.status = 1;
-    n = n < 0 ? 0 : cap;
-  }
   const float* acc_in = a.acc_in + row * a.stride;
   const int* pos_in = a.pos_in + row * a.stride;
   float* acc_out = a.acc_out + row * a.stride;
   int* pos_out = a.pos_out + row * a.stride;
-  const int per = CL ? (n + cl - 1) / cl : n, b = min(n, rank * per), e = min(n, b + per);
-  if (n <= a.budget) {  // the same for every block of the cluster
-    for (int t = b + tid; t < e; t += kEvictThreads) {
-      acc_out[t] = acc_in[t];
-      pos_out[t] = pos_in[t];
+  // a row's only block need not wait for its length to read ahead
+  float held_acc[kHeld];
+  int held_pos[kHeld];
+  if (!CL) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int t = tid + i * THREADS;
+      if (t < cap) {
+        held_acc[i] = acc_in[t];
+        held_pos[i] = pos_in[t];
+      }
     }
+  }
+  int n = a.c.lens[s];
+  if (tid == 0) sh_max = INT32_MIN;
+#pragma unroll
+  for (int i = tid; i < 3 * kBins / 4; i += THREADS) reinterpret_cast<int4*>(hist)[i] = make_int4(0, 0, 0, 0);
+  if (n < 0 || n > cap) {
+    *a.c.status = 1;
+    n = n < 0 ? 0 : cap;
+  }
+  const int per = CL ? (n + cl - 1) / cl : n, b = min(n, rank * per), e = min(n, b + per);
+  // each slot of the block's range, in strides: f(slot, acc, pos)
+  auto each = [&](auto&& f) {
+    int t = b + tid;
+    if (!CL) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i, t += THREADS)
+        if (t < e) f(t, held_acc[i], held_pos[i]);
+    }
+    // four loads before the first f, which may write where the compiler cannot tell them apart
+    for (; t < e; t += 4 * THREADS) {
+      float acc[4];
+      int pos[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (t + i * THREADS < e) {
+          acc[i] = acc_in[t + i * THREADS];
+          pos[i] = pos_in[t + i * THREADS];
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (t + i * THREADS < e) f(t + i * THREADS, acc[i], pos[i]);
+    }
+  };
+  if (n <= a.budget) {  // the same for every block of the cluster
+    each([&](int t, float acc, int pos) {
+      acc_out[t] = acc;
+      pos_out[t] = pos;
+    });
+    if (!a.fused && rank == 0 && tid == 0) a.pairs[row] = 0;
     return;
   }
   uint32_t* keys = use_smem ? smem_keys : a.keys + row * a.stride + b;
 
   // the newest position
   int newest = INT32_MIN;
-#pragma unroll 4
-  for (int t = b + tid; t < e; t += kEvictThreads) newest = max(newest, pos_in[t]);
-  if (tid == 0) sh_max = INT32_MIN;
-  for (int i = tid; i < 3 * kBins / 4; i += kEvictThreads) reinterpret_cast<int4*>(hist)[i] = make_int4(0, 0, 0, 0);
+  each([&](int, float, int pos) { newest = max(newest, pos); });
   __syncthreads();
   newest = __reduce_max_sync(~0u, newest);
   if (lane == 0) atomicMax(&sh_max, newest);
   sync();
-  newest = INT32_MIN;
+  newest = sh_max;
+  if (CL) {
 #pragma unroll
-  for (int r = 0; r < kEvictMaxCluster; ++r)
-    if (r < cl) newest = max(newest, *remote(&sh_max, r));
-
-#pragma unroll 4
-  for (int t = b + tid; t < e; t += kEvictThreads) {
-    const int p = pos_in[t];
-    const bool held = p < a.n_sink || (int64_t)p > (int64_t)newest - a.n_recent;
-    const uint32_t key = held ? 0xffffffffu : order_key(acc_in[t]);
+    for (int r = 0; r < kEvictMaxCluster; ++r)
+      if (r < cl) newest = max(newest, *remote(&sh_max, r));
+  }
+  each([&](int t, float acc, int pos) {
+    const bool held = pos < a.n_sink || (int64_t)pos > (int64_t)newest - a.n_recent;
+    const uint32_t key = held ? 0xffffffffu : order_key(acc);
     keys[t - b] = key;
     atomicAdd(&hist[0][key >> 21], 1);
-  }
+  });
+
+  pdl_launch_dependents();
 
   // radix select of the budget-th largest key
   uint32_t prefix = 0;
@@ -146,28 +228,28 @@ __global__ void __launch_bounds__(kEvictThreads) k_paged_evict(const PagedEvictA
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     sync();
-    static_assert(kBins == 4 * kEvictThreads, "four bins a thread");
+    constexpr int kPer = kBins / THREADS;
     const int bins = pass == 2 ? 1024 : kBins, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    const int quad = bins / 4 - 1 - tid;  // the highest bins first
-    int4 q = make_int4(0, 0, 0, 0);
-    if (quad >= 0) {
+    const int top = bins - 1 - tid * kPer;  // the highest bins first
+    int mine[kPer], sum = 0;
 #pragma unroll
-      for (int r = 0; r < kEvictMaxCluster; ++r)
-        if (r < cl) {
-          const int4 x = *remote(reinterpret_cast<const int4*>(hist[pass]) + quad, r);
-          q.x += x.x;
-          q.y += x.y;
-          q.z += x.z;
-          q.w += x.w;
-        }
-    }
+    for (int i = 0; i < kPer; ++i) mine[i] = 0;
+#pragma unroll
+    for (int r = 0; r < (CL ? kEvictMaxCluster : 1); ++r)
+      if (r < cl) {
+        const int* from = remote(hist[pass], r);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (top - i >= 0) mine[i] += from[top - i];
+      }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sum += mine[i];
     uint64_t total;
-    int above = (int)block_scan((uint64_t)(q.x + q.y + q.z + q.w), warp_sum, &total);
-    const int mine[4] = {q.w, q.z, q.y, q.x};
+    int above = (int)block_scan<THREADS>((uint64_t)sum, warp_sum, &total);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kPer; ++i) {
       if (above < need && need <= above + mine[i]) {
-        sh_bin = 4 * quad + 3 - i;
+        sh_bin = top - i;
         sh_need = need - above;
         sh_equal = mine[i];
       }
@@ -180,7 +262,7 @@ __global__ void __launch_bounds__(kEvictThreads) k_paged_evict(const PagedEvictA
       const uint32_t mask = ~0u << shift;
       const int next = pass == 0 ? 10 : 0, width = pass == 0 ? kBins : 1024;
 #pragma unroll 4
-      for (int i = tid; i < e - b; i += kEvictThreads) {
+      for (int i = tid; i < e - b; i += THREADS) {
         const uint32_t key = keys[i];
         if ((key & mask) == prefix) atomicAdd(&hist[pass + 1][(key >> next) & (width - 1)], 1);
       }
@@ -188,14 +270,14 @@ __global__ void __launch_bounds__(kEvictThreads) k_paged_evict(const PagedEvictA
   }
 
   // each thread owns a run of slots (odd length: one bank each)
-  const int run = ((e - b + kEvictThreads - 1) / kEvictThreads) | 1;
+  const int run = ((e - b + THREADS - 1) / THREADS) | 1;
   const int i0 = min(e - b, tid * run), i1 = min(e - b, i0 + run);
   uint64_t total;
   int eq_at = 0;
   if (need < sh_equal) {  // the first `need` of equal keys stay (the same for every block)
     int eq = 0;
     for (int i = i0; i < i1; ++i) eq += keys[i] == prefix;
-    eq_at = (int)block_scan((uint64_t)eq, warp_sum, &total);
+    eq_at = (int)block_scan<THREADS>((uint64_t)eq, warp_sum, &total);
     if (tid == 0) sh_eq = (int)total;
     sync();
     for (int r = 0; r < rank; ++r) eq_at += *remote(&sh_eq, r);
@@ -214,7 +296,7 @@ __global__ void __launch_bounds__(kEvictThreads) k_paged_evict(const PagedEvictA
     else
       counts += (uint64_t)stay << 32;
   }
-  uint64_t at = block_scan(counts, warp_sum, &total);
+  uint64_t at = block_scan<THREADS>(counts, warp_sum, &total);
   if (CL) {
     if (tid == 0) sh_count = total;
     sync();
@@ -242,53 +324,29 @@ __global__ void __launch_bounds__(kEvictThreads) k_paged_evict(const PagedEvictA
     }
   }
   __syncthreads();  // acc_out may be acc_in: the movers' values are read above
-#pragma unroll 4
-  for (int t = b + tid; t < e; t += kEvictThreads) {
+  each([&](int t, float acc, int pos) {
     if (t >= a.budget) {
       acc_out[t] = 0.f;
       pos_out[t] = -1;
     } else if (keys[t - b]) {
-      acc_out[t] = acc_in[t];
-      pos_out[t] = pos_in[t];
+      acc_out[t] = acc;
+      pos_out[t] = pos;
     }
-  }
+  });
   sync();
 
-  // the moves: eight pairs a warp at a time
-  const int* list = a.list + row * 4 * a.list_cap;
-  U* kb = static_cast<U*>(a.c.k) + a.layer * a.c.layer + h * a.c.head;
-  U* vb = static_cast<U*>(a.c.v) + a.layer * a.c.layer + h * a.c.head;
-  const int units = a.c.d;
-  constexpr int kWarps = kEvictThreads / 32;
-  for (int p0 = (rank * kWarps + warp) * 8; p0 < pairs; p0 += cl * kWarps * 8) {
-    int64_t src = -1, dst = -1;
-    if (lane < 8 && p0 + lane < pairs) {
-      const int* pair = list + p0 + lane;
-      const int to = pair[0], from = pair[a.list_cap];
-      dst = page_row(a.c, s, to);
-      src = page_row(a.c, s, from);
-      acc_out[to] = __int_as_float(pair[2 * a.list_cap]);
-      pos_out[to] = pair[3 * a.list_cap];
-      if (src < 0) dst = -1;
-    }
-    int64_t from[8], to[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      from[i] = __shfl_sync(~0u, src, i);
-      to[i] = __shfl_sync(~0u, dst, i);
-    }
-    for (int x = lane; x < 2 * units; x += 32) {
-      U* base = x >= units ? vb : kb;
-      const int at_u = x >= units ? x - units : x;
-      U got[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (to[i] >= 0) got[i] = base[from[i] + at_u];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (to[i] >= 0) base[to[i] + at_u] = got[i];
-    }
+  if (a.fused) {
+    move_pairs<U, 2, 2>(a, row, pairs, rank * (THREADS / 32) + warp, cl * (THREADS / 32));
+  } else if (rank == 0 && tid == 0) {
+    a.pairs[row] = pairs;
   }
+}
+
+// The moves of rows whose lists can be long, over the whole card.
+template <typename U>
+__global__ void __launch_bounds__(256, 4) k_paged_move(const PagedEvictArgs a) {
+  pdl_wait();
+  move_pairs<U, kMoveBatch, 8>(a, blockIdx.x, a.pairs[blockIdx.x], blockIdx.y * 8 + (threadIdx.x >> 5), gridDim.y * 8);
 }
 
 // Reordering: block (row j, share of the copies). Every block works out the
@@ -388,24 +446,39 @@ PagedView in_units(PagedView c, int esize) {
 }
 
 template <typename U>
+void launch_move(const PagedEvictArgs& a, int rows, int sms, cudaStream_t s) {
+  if (a.fused) return;
+  const int64_t most = (a.list_cap + 8 * kMoveBatch - 1) / (8 * kMoveBatch), fill = (4ll * sms + rows - 1) / rows;
+  launch_pdl(k_paged_move<U>, dim3((unsigned)rows, (unsigned)std::min<int64_t>(most, fill)), dim3(256), 0, s, a);
+}
+
+template <typename U>
 void launch_evict(PagedEvictArgs a, int device, int sms, cudaStream_t s) {
   const int64_t cap = std::min<int64_t>((int64_t)a.c.width * a.c.page_tokens, a.stride);
-  const int rows = a.n_seqs * a.c.hkv, cl = paged_evict_cluster(rows, cap, sms);
+  const int rows = a.n_seqs * a.c.hkv, cl = paged_evict_cluster(cap);
   const bool in_smem = paged_evict_keys_in_smem(cap, cl);
   const size_t smem = in_smem ? (size_t)((cap + cl - 1) / cl) * 4 : 0;
   a.c = in_units<U>(a.c, a.esize);
+  a.fused = a.list_cap <= kFusedMoves;
   if (cl == 1) {
-    static SmemOptIn opt;
-    opt(k_paged_evict<U, false>, kEvictSmemKeys * 4, device);
-    k_paged_evict<U, false><<<rows, kEvictThreads, smem, s>>>(a, 1, in_smem);
+    auto one = [&](auto kernel, int threads, SmemOptIn& opt) {
+      opt(kernel, kEvictSmemKeys * 4, device);
+      kernel<<<rows, threads, smem, s>>>(a, 1, in_smem);
+    };
+    static SmemOptIn small, large;
+    if (cap <= 2048)
+      one(k_paged_evict<U, 256, false>, 256, small);
+    else
+      one(k_paged_evict<U, 1024, false>, 1024, large);
     LC_CUDA(cudaGetLastError());
+    launch_move<U>(a, rows, sms, s);
     return;
   }
   static SmemOptIn opt;
-  opt(k_paged_evict<U, true>, kEvictSmemKeys * 4, device);
+  opt(k_paged_evict<U, 512, true>, kEvictSmemKeys * 4, device);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * cl));
-  cfg.blockDim = dim3(kEvictThreads);
+  cfg.blockDim = dim3(512);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
@@ -414,7 +487,8 @@ void launch_evict(PagedEvictArgs a, int device, int sms, cudaStream_t s) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  LC_CUDA(cudaLaunchKernelEx(&cfg, k_paged_evict<U, true>, a, cl, in_smem ? 1 : 0));
+  LC_CUDA(cudaLaunchKernelEx(&cfg, k_paged_evict<U, 512, true>, a, cl, in_smem ? 1 : 0));
+  launch_move<U>(a, rows, sms, s);
 }
 
 template <typename U>
@@ -429,11 +503,12 @@ void launch_reorder(PagedReorderArgs a, int sms, cudaStream_t s) {
 
 }  // namespace
 
-// Blocks per row: enough that the rows fill the card, none with less than
-// 1024 slots to itself.
-int paged_evict_cluster(int32_t rows, int64_t cap, int32_t sms) {
+// Blocks per row: one where it holds the row's keys in shared memory. A
+// cluster's barriers cost more than its blocks bring while one block can do
+// it: 8 rows of 8192 slots took 18 us with one block each, 22 with 2 and 28
+// with 4; 8 rows of 32768, 42, 40 and 37.
+int paged_evict_cluster(int64_t cap) {
   int cl = 1;
-  while (cl < kEvictMaxCluster && (int64_t)rows * cl < 2 * sms && cap / (2 * cl) >= 1024) cl *= 2;
   while (cl < kEvictMaxCluster && !paged_evict_keys_in_smem(cap, cl)) cl *= 2;
   return cl;
 }
