@@ -307,8 +307,8 @@ static void paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t
     const size_t rows = (size_t)n_seqs * n_q_heads;
     a.score_tokens = cap;
     float* ws = static_cast<float*>(p->scores.get((rows * cap + 2 * rows) * 4));
-    a.stats = ws;
-    a.scores = ws + 2 * rows;
+    a.scores = ws;
+    a.stats = ws + rows * cap;
   }
   const cudaStream_t s = p->order.on(stream);
   launch_paged_attn(a, p->cfg.dtype, p->cfg.device, p->sms, s);

@@ -61,7 +61,7 @@ struct PagedWeightArgs {
   float* acc_out;
   const int32_t* lens;
   int64_t score_tokens, acc_stride;
-  int32_t n_seqs, hkv, group, window, cap;
+  int32_t n_seqs, hkv, group, window, cap, chunks;
   float decay;
 };
 
@@ -121,6 +121,7 @@ struct BeamArgs {
 };
 
 constexpr int kPagedMaxSeqs = 2048;
+constexpr int kPagedMaxBlocks = 320;  // of an attention launch
 constexpr int kPagedMaxDim = 256;
 constexpr int kBeamMaxBeams = 64;
 constexpr int kBeamMaxOut = 64;
@@ -130,7 +131,7 @@ void launch_paged_append(const PagedAppendArgs& a, cudaStream_t s);
 // pool_dtype: LC_F32 / LC_BF16 / LC_F16.
 void launch_paged_attn(PagedAttnArgs& a, int32_t pool_dtype, int32_t device, int32_t sms, cudaStream_t s);
 int64_t paged_part_floats(int32_t sms);
-void launch_paged_weights(const PagedWeightArgs& a, cudaStream_t s);
+void launch_paged_weights(PagedWeightArgs a, cudaStream_t s);
 int paged_evict_cluster(int64_t cap);
 bool paged_evict_keys_in_smem(int64_t cap, int cluster);
 void launch_paged_evict(const PagedEvictArgs& a, int32_t device, int32_t sms, cudaStream_t s);

@@ -26,6 +26,12 @@ namespace lc {
 namespace {
 
 constexpr float kNegInf = -INFINITY;
+// What an item costs a block beyond its tiles, in tiles (see build_prefix):
+// 0, 8, 16 and 32 took 128, 119, 110 and 97 us for 32 sequences of 1 to 8192
+// slots on the tensor cores, 37, 30, 30 and 29 for a window of 1024; the
+// general kernel's tiles cost more each, and 64 sequences of 128 to 512 f32
+// slots took 150, 144, 156 and 180.
+constexpr int kMmaCost = 32, kGeneralCost = 8;
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -69,20 +75,23 @@ __device__ __forceinline__ int64_t row_offset(const PagedView& c, int s, int t) 
   return page * c.page + (int64_t)(t % c.page_tokens) * c.token;
 }
 
-// prefix[s] = tiles of the sequences before s (of one item each); prefix[n_seqs]
-// the total. Sequences with nothing to attend to get their zeros here. Every
-// thread of the block calls it.
+// prefix[s] = length in the list of the sequences before s (of one item each);
+// prefix[n_seqs] the total. An item of t tiles takes cost + t places: the
+// first ones are no tiles but stand for what beginning and ending an item
+// costs, so that a block's share holds less of others the more items it has.
+// Sequences with nothing to attend to take no place and get their zeros here.
+// Every thread of the block calls it.
 template <int THREADS>
-__device__ void build_prefix(const PagedAttnArgs& a, int tile, int* prefix) {
+__device__ void build_prefix(const PagedAttnArgs& a, int tile, int cost, int* prefix) {
   __shared__ int warp_sum[THREADS / 32];
   const int tid = threadIdx.x, per = (a.n_seqs + THREADS - 1) / THREADS;
   const int b = min(a.n_seqs, tid * per), e = min(a.n_seqs, b + per);
-  auto tiles_of = [&](int s) {
+  auto places_of = [&](int s) {
     const int n = clamp_len(a.c, s);
-    return (n - first_slot(n, a.window) + tile - 1) / tile;
+    return n == 0 ? 0 : cost + (n - first_slot(n, a.window) + tile - 1) / tile;
   };
   int sum = 0;
-  for (int s = b; s < e; ++s) sum += tiles_of(s);
+  for (int s = b; s < e; ++s) sum += places_of(s);
   int inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -97,7 +106,7 @@ __device__ void build_prefix(const PagedAttnArgs& a, int tile, int* prefix) {
     if (w < (tid >> 5)) at += warp_sum[w];
   for (int s = b; s < e; ++s) {
     prefix[s] = at;
-    at += per == 1 ? sum : tiles_of(s);
+    at += per == 1 ? sum : places_of(s);
   }
   if (tid == THREADS - 1) prefix[a.n_seqs] = at;
   __syncthreads();
@@ -113,14 +122,15 @@ __device__ void build_prefix(const PagedAttnArgs& a, int tile, int* prefix) {
 // A block's share of one item: tiles [j0, j1) of sequence s, item hh (kv head
 // and head group) of it.
 struct Segment {
-  int s, hh, j0, j1, n, lo;
+  int s, hh, j0, j1, n, lo;  // j1 <= j0: places only
+  int next;                  // where the block goes on in the list
   // the item's blocks are first .. first + parts - 1; block b's partial is in
   // slot 2 b, or 2 b + 1 where the item does not begin its run (the first only)
   int first, parts, slot0, slot;
 };
 
-__device__ __forceinline__ Segment find_segment(const PagedAttnArgs& a, const int* prefix, int hh_n, int per, int u,
-                                                int u_end) {
+__device__ __forceinline__ Segment find_segment(const PagedAttnArgs& a, const int* prefix, int cost, int hh_n, int per,
+                                                int u, int u_end) {
   Segment g;
   const int key = u / hh_n;
   int b = 0, e = a.n_seqs;  // the last s with prefix[s] <= key
@@ -132,16 +142,19 @@ __device__ __forceinline__ Segment find_segment(const PagedAttnArgs& a, const in
       e = mid;
   }
   g.s = b;
-  const int tiles = prefix[b + 1] - prefix[b], r = u - prefix[b] * hh_n;
-  g.hh = r / tiles;
-  g.j0 = r - g.hh * tiles;
-  g.j1 = min(tiles, g.j0 + (u_end - u));
+  const int places = prefix[b + 1] - prefix[b], r = u - prefix[b] * hh_n;
+  g.hh = r / places;
+  const int start = prefix[b] * hh_n + g.hh * places + cost;  // the item's first tile
+  const int end = start + places - cost;
+  g.j0 = max(u, start) - start;
+  g.j1 = min(end, u_end) - start;
+  g.next = min(end, u_end);
   g.n = clamp_len(a.c, b);
   g.lo = first_slot(g.n, a.window);
-  const int start = prefix[b] * hh_n + g.hh * tiles;
   g.first = start / per;
-  g.parts = (start + tiles - 1) / per - g.first + 1;
-  g.slot0 = 2 * g.first + (g.first * per < start ? 1 : 0);
+  g.parts = (end - 1) / per - g.first + 1;
+  // an item begins its first block's run unless other places are before its own
+  g.slot0 = 2 * g.first + (g.first * per < start - cost ? 1 : 0);
   g.slot = (int)blockIdx.x == g.first ? g.slot0 : 2 * (int)blockIdx.x;
   return g;
 }
@@ -228,61 +241,146 @@ __device__ void finish_segment(const PagedAttnArgs& a, const Segment& g, int hg_
         if (lane == 0) row_stats(i, m, l);
       }
       __syncthreads();
-      for (int e = tid; e < nh * DP; e += THREADS) {
-        const int i = e / DP, x = e % DP;
-        if (x >= d) continue;
-        float o = oo[i] * __ldcg(slot(0) + 2 * GP + e);
+      // four dimensions a thread, the parts shared out where threads are left
+      constexpr int kVecs = GP * DP / 4, kShare = THREADS > kVecs ? THREADS / kVecs : 1;
+      float4* sums = reinterpret_cast<float4*>(oo + kPagedMaxBlocks * GP);
+      const int share = kShare > 1 ? tid / kVecs : 0;
+      for (int v = tid - share * kVecs; v < nh * DP / 4 && share < kShare; v += THREADS) {
+        const int i = v * 4 / DP, x = v * 4 % DP;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-        for (int b = 1; b < g.parts; ++b)
-          o = fmaf(oo[b * GP + i], __ldcg(a.part + 2 * (g.first + b) * kSlot + 2 * GP + e), o);
-        store_f32(a.out, (row0 + i) * d + x, a.out_dtype, o * scale[i]);
+        for (int b = share; b < g.parts; b += kShare) {
+          const float f = oo[b * GP + i];
+          const float4 p = __ldcg(reinterpret_cast<const float4*>(slot(b) + 2 * GP) + v);
+          o.x = fmaf(f, p.x, o.x);
+          o.y = fmaf(f, p.y, o.y);
+          o.z = fmaf(f, p.z, o.z);
+          o.w = fmaf(f, p.w, o.w);
+        }
+        if (kShare > 1) {
+          sums[share * kVecs + v] = o;
+          continue;
+        }
+        const float r[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (x + c < d) store_f32(a.out, (row0 + i) * d + x + c, a.out_dtype, r[c] * scale[i]);
+      }
+      if (kShare > 1) {
+        __syncthreads();
+        for (int e = tid; e < nh * DP; e += THREADS) {
+          const int i = e / DP, x = e % DP;
+          if (x >= d) continue;
+          float o = 0.f;
+#pragma unroll
+          for (int b = 0; b < kShare; ++b) o += reinterpret_cast<const float*>(sums + b * kVecs)[e];
+          store_f32(a.out, (row0 + i) * d + x, a.out_dtype, o * scale[i]);
+        }
       }
     }
   }
   __syncthreads();
 }
 
-// The general kernel: any of the three types in and out, any alignment, head
-// dimension up to DP, products and sums in f32 on the FMA units. A warp owns
-// whole tiles of TT = 32 / LPT slots: LPT = DP / 64 lanes share a slot's dot
-// product, 16 bytes at a time in turn, and for the values the lanes own
-// dimensions. Rows sit in shared memory as f32 with 4 LPT words of padding,
-// which keeps the eight lanes of a 16-byte read phase on different banks.
-template <typename T, int DP, int GP, int W>
-__global__ void __launch_bounds__(W * 32) k_paged_attn(const PagedAttnArgs a) {
-  constexpr int LPT = DP / 64, TT = 32 / LPT, PITCH = DP + 4 * LPT, VL = DP / 32;
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool read) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+
+// The FMA kernel: products and sums in f32 for pools of any of the three
+// types, head dimension up to DP. A warp owns whole tiles of TT = 32 / LPT
+// slots: LPT = DP / 64 lanes share a slot's dot product, 16 bytes at a time in
+// turn, and for the values the lanes own dimensions. Rows sit in shared memory
+// as f32 with 4 LPT words of padding, which keeps the eight lanes of a 16-byte
+// read phase on different banks.
+//
+// ST > 1: f32 pools whose rows are whole 16-byte units, through ST stages of
+// cp.async a warp; per tile of 16 KB some 750 instructions (4 heads, d = 128)
+// against the 2800 that the SM issues while its share of the HBM delivers one.
+// ST = 1: any alignment and type, loaded value by value.
+template <typename T, int DP, int GP, int W, int ST>
+__global__ void __launch_bounds__(W * 32, ST > 1 ? 1 : 2) k_paged_attn(const PagedAttnArgs a) {
+  constexpr int LPT = DP / 64, TT = 32 / LPT, PITCH = DP + 4 * LPT, VL = DP / 32, kCost = kGeneralCost;
+  constexpr int TILE = TT * PITCH, CH = DP / 4;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* kt = reinterpret_cast<float*>(smem);  // [W][TT][PITCH]
-  float* vt = kt + W * TT * PITCH;
-  float* qs = vt + W * TT * PITCH;         // [GP][DP]
-  float* ps = qs + GP * DP;                // [W][TT][GP]
-  float* om = ps + W * TT * GP;            // [W][GP]
+  float* tiles = reinterpret_cast<float*>(smem);  // [W][ST][K, V][TT][PITCH]
+  float* qs = tiles + W * ST * 2 * TILE;          // [GP][DP]
+  float* ps = qs + GP * DP;                       // [W][TT][GP]
+  float* om = ps + W * TT * GP;                   // [W][GP]
   float* ol = om + W * GP;
   int* prefix = reinterpret_cast<int*>(ol + W * GP);
-  float* oo = kt;  // [W][GP][DP]: the tiles' room, free when a segment ends
-  static_assert(2 * 148 * 2 * GP <= W * TT * PITCH && GP * DP <= TT * PITCH, "the warps' outputs fit the key tiles");
+  float* oo = tiles;  // [W][GP][DP]: the tiles' room, free when a segment ends
+  static_assert(GP * DP <= 2 * TILE && kPagedMaxBlocks * GP + W * 128 <= W * ST * 2 * TILE,
+                "the warps' outputs, and the joins' weights and sums, fit the tiles");
+  static_assert(ST == 1 || sizeof(T) == 4, "cp.async does not convert");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hg_n = (a.group + GP - 1) / GP, hh_n = a.c.hkv * hg_n;
-  build_prefix<W * 32>(a, TT, prefix);
+  if (a.scores) pdl_launch_dependents();
+  build_prefix<W * 32>(a, TT, kCost, prefix);
   const int total = prefix[a.n_seqs] * hh_n;
   const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, a.min_tiles);
   const int u_end = min(total, ((int)blockIdx.x + 1) * per);
-  float* kw = kt + warp * TT * PITCH;
-  float* vw = vt + warp * TT * PITCH;
+  float* mine = tiles + warp * ST * 2 * TILE;
+  const uint32_t mine_at = (uint32_t)__cvta_generic_to_shared(mine);
   float* pw = ps + warp * TT * GP;
   const int tok = lane / LPT, part = lane % LPT;
+  auto dim = [&](int x) { return DP == 64 ? lane * 2 + x : (x >> 2) * 128 + lane * 4 + (x & 3); };
   for (int u = blockIdx.x * per; u < u_end;) {
-    const Segment g = find_segment(a, prefix, hh_n, per, u, u_end);
-    u += g.j1 - g.j0;
+    const Segment g = find_segment(a, prefix, kCost, hh_n, per, u, u_end);
+    u = g.next;
+    if (g.j1 <= g.j0) continue;
     const int h = g.hh / hg_n, head0 = (g.hh - h * hg_n) * GP, nh = min(GP, a.group - head0);
+    const T* kb = static_cast<const T*>(a.c.k) + a.layer * a.c.layer + h * a.c.head;
+    const T* vb = static_cast<const T*>(a.c.v) + a.layer * a.c.layer + h * a.c.head;
+    const int32_t* table = a.c.tables + (int64_t)g.s * a.c.width;
+
+    // lane r looks up slot r of a tile
+    auto page_of = [&](int j) -> int {
+      const int t = g.lo + j * TT + lane;
+      return j < g.j1 && lane < TT && t < g.n ? table[t / a.c.page_tokens] : INT32_MIN;
+    };
+    auto row_of = [&](int j, int page) -> int64_t {
+      const int t = g.lo + j * TT + lane;
+      if (page >= 0 && page < a.c.n_pages) return page * a.c.page + (int64_t)(t % a.c.page_tokens) * a.c.token;
+      if (page != INT32_MIN) *a.c.status = 1;
+      return -1;
+    };
+    auto issue = [&](int j, int stage, int page) {
+      if (j < g.j1) {
+        const int64_t off = row_of(j, page);
+        const uint32_t to = mine_at + stage * 2 * TILE * 4;
+#pragma unroll
+        for (int x = 0; x < TT * CH / 32; ++x) {
+          const int e = x * 32 + lane, r = e / CH, c = e - r * CH;
+          const int64_t o = __shfl_sync(~0u, off, r);
+          const bool read = o >= 0 && c * 4 < a.c.d;
+          const int64_t from = read ? o + c * 4 : 0;
+          cp_async16_or_zero(to + (r * PITCH + c * 4) * 4, kb + from, read);
+          cp_async16_or_zero(to + (TILE + r * PITCH + c * 4) * 4, vb + from, read);
+        }
+      }
+      cp_commit();
+    };
+
+    const int first = g.j0 + warp;
+    int page = page_of(first);
+    if constexpr (ST > 1) {
+#pragma unroll
+      for (int i = 0; i < ST - 1; ++i) {
+        const int now = page;
+        page = page_of(first + (i + 1) * W);
+        issue(first + i * W, i, now);
+      }
+    }
     const int64_t qrow = ((int64_t)g.s * a.c.hkv + h) * a.group + head0;
     for (int e = tid; e < GP * DP; e += W * 32) {
       const int i = e / DP, x = e - i * DP;
       qs[e] = i < nh && x < a.c.d ? load_f32(a.q, (qrow + i) * a.c.d + x, a.q_dtype) * a.scale_log2 : 0.f;
     }
     __syncthreads();
-    const T* kb = static_cast<const T*>(a.c.k) + a.layer * a.c.layer + h * a.c.head;
-    const T* vb = static_cast<const T*>(a.c.v) + a.layer * a.c.layer + h * a.c.head;
     float m[GP], l[GP], o[GP][VL];
 #pragma unroll
     for (int i = 0; i < GP; ++i) {
@@ -291,21 +389,35 @@ __global__ void __launch_bounds__(W * 32) k_paged_attn(const PagedAttnArgs a) {
 #pragma unroll
       for (int x = 0; x < VL; ++x) o[i][x] = 0.f;
     }
-    for (int j = g.j0 + warp; j < g.j1; j += W) {
+    int stage = 0, fill = ST - 1;
+    for (int j = first; j < g.j1; j += W) {
       const int t0 = g.lo + j * TT, nt = min(TT, g.n - t0);
-      const int64_t mine = lane < nt ? row_offset(a.c, g.s, t0 + lane) : -1;
+      if constexpr (ST > 1) {
+        cp_wait<(ST > 1 ? ST - 2 : 0)>();
+        __syncwarp();
+        issue(j + (ST - 1) * W, fill, page);
+        page = page_of(j + ST * W);
+      } else {
+        const int64_t row = row_of(j, page);
+        page = page_of(j + W);
 #pragma unroll 4
-      for (int r = 0; r < TT; ++r) {
-        const int64_t off = __shfl_sync(~0u, mine, r);
+        for (int r = 0; r < TT; ++r) {
+          const int64_t off = __shfl_sync(~0u, row, r);
 #pragma unroll
-        for (int x = 0; x < VL; ++x) {
-          const int c = x * 32 + lane;
-          const bool in = off >= 0 && c < a.c.d;
-          kw[r * PITCH + c] = in ? to_f32(kb[off + c]) : 0.f;
-          vw[r * PITCH + c] = in ? to_f32(vb[off + c]) : 0.f;
+          for (int x = 0; x < VL; ++x) {
+            const int c = x * 32 + lane;
+            const bool in = off >= 0 && c < a.c.d;
+            mine[r * PITCH + c] = in ? to_f32(kb[off + c]) : 0.f;
+            mine[TILE + r * PITCH + c] = in ? to_f32(vb[off + c]) : 0.f;
+          }
         }
+        __syncwarp();
       }
-      __syncwarp();
+      const float* kw = mine + stage * 2 * TILE;
+      const float* vw = kw + TILE;
+      fill = stage;
+      stage = stage + 1 == ST ? 0 : stage + 1;
+
       float s[GP];
 #pragma unroll
       for (int i = 0; i < GP; ++i) s[i] = 0.f;
@@ -358,18 +470,26 @@ __global__ void __launch_bounds__(W * 32) k_paged_attn(const PagedAttnArgs a) {
       __syncwarp();
 #pragma unroll 4
       for (int r = 0; r < TT; ++r) {
-        float v[VL];
+        float v[VL], p[GP];
+        if constexpr (DP == 64) {
+          *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(vw + r * PITCH + lane * 2);
+        } else {
 #pragma unroll
-        for (int x = 0; x < VL; ++x) v[x] = vw[r * PITCH + x * 32 + lane];
-#pragma unroll
-        for (int i = 0; i < GP; ++i) {
-          const float p = pw[r * GP + i];
-#pragma unroll
-          for (int x = 0; x < VL; ++x) o[i][x] = fmaf(p, v[x], o[i][x]);
+          for (int x = 0; x < VL / 4; ++x)
+            *reinterpret_cast<float4*>(v + 4 * x) =
+                *reinterpret_cast<const float4*>(vw + r * PITCH + x * 128 + lane * 4);
         }
+#pragma unroll
+        for (int i = 0; i < GP / 4; ++i)
+          *reinterpret_cast<float4*>(p + 4 * i) = *reinterpret_cast<const float4*>(pw + r * GP + 4 * i);
+#pragma unroll
+        for (int i = 0; i < GP; ++i)
+#pragma unroll
+          for (int x = 0; x < VL; ++x) o[i][x] = fmaf(p[i], v[x], o[i][x]);
       }
       __syncwarp();
     }
+    if constexpr (ST > 1) cp_wait<0>();
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < GP; ++i) {
@@ -381,7 +501,7 @@ __global__ void __launch_bounds__(W * 32) k_paged_attn(const PagedAttnArgs a) {
         ol[warp * GP + i] = sum;
       }
 #pragma unroll
-      for (int x = 0; x < VL; ++x) oo[(warp * GP + i) * DP + x * 32 + lane] = o[i][x];
+      for (int x = 0; x < VL; ++x) oo[(warp * GP + i) * DP + dim(x)] = o[i][x];
     }
     finish_segment<W * 32, GP, DP>(a, g, hg_n, om, ol, oo);
   }
@@ -416,14 +536,6 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool read) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
-}
-
 // The tensor-core kernel: 16-bit pools whose rows are whole 16-byte units,
 // queries of the pool's type, head dimension up to DP.
 //
@@ -443,16 +555,18 @@ __device__ __forceinline__ void cp_wait() {
 // dimensions past d are filled with zeros, never read.
 template <typename T, int DP, int W, int ST>
 __global__ void __launch_bounds__(W * 32, 1) k_paged_attn_mma(const PagedAttnArgs a) {
-  constexpr int GP = 8, TT = 16, CH = DP / 8, PITCH = DP * 2 + 16, TILE = TT * PITCH;
+  constexpr int GP = 8, TT = 16, CH = DP / 8, PITCH = DP * 2 + 16, TILE = TT * PITCH, kCost = kMmaCost;
   extern __shared__ __align__(16) uint8_t smem[];
   float* om = reinterpret_cast<float*>(smem + W * ST * 2 * TILE);
   float* ol = om + W * GP;
   int* prefix = reinterpret_cast<int*>(ol + W * GP);
   float* oo = reinterpret_cast<float*>(smem);  // [W][GP][DP]: the stages' room, free when a segment ends
-  static_assert(GP * DP * 4 <= ST * 2 * TILE, "the warps' outputs fit the stages");
+  static_assert(GP * DP * 4 <= ST * 2 * TILE && (kPagedMaxBlocks * GP + W * 128) * 4 <= W * ST * 2 * TILE,
+                "the warps' outputs, and the joins' weights and sums, fit the stages");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, tg = lane & 3;
   const int hg_n = (a.group + GP - 1) / GP, hh_n = a.c.hkv * hg_n;
-  build_prefix<W * 32>(a, TT, prefix);
+  if (a.scores) pdl_launch_dependents();
+  build_prefix<W * 32>(a, TT, kCost, prefix);
   const int total = prefix[a.n_seqs] * hh_n;
   const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, a.min_tiles);
   const int u_end = min(total, ((int)blockIdx.x + 1) * per);
@@ -460,8 +574,9 @@ __global__ void __launch_bounds__(W * 32, 1) k_paged_attn_mma(const PagedAttnArg
   const uint32_t k_at = (lane & 15) * PITCH + (lane >> 4) * 16;
   const uint32_t v_at = ((lane & 7) + ((lane >> 4) << 3)) * PITCH + ((lane >> 3) & 1) * 16;
   for (int u = blockIdx.x * per; u < u_end;) {
-    const Segment g = find_segment(a, prefix, hh_n, per, u, u_end);
-    u += g.j1 - g.j0;
+    const Segment g = find_segment(a, prefix, kCost, hh_n, per, u, u_end);
+    u = g.next;
+    if (g.j1 <= g.j0) continue;
     const int h = g.hh / hg_n, head0 = (g.hh - h * hg_n) * GP, nh = min(GP, a.group - head0);
     const T* kb = static_cast<const T*>(a.c.k) + a.layer * a.c.layer + h * a.c.head;
     const T* vb = static_cast<const T*>(a.c.v) + a.layer * a.c.layer + h * a.c.head;
@@ -611,62 +726,106 @@ __global__ void __launch_bounds__(W * 32, 1) k_paged_attn_mma(const PagedAttnArg
 
 constexpr int kWarps = 4;
 
-template <int DP, int GP>
-constexpr size_t general_smem(int n_seqs) {
-  constexpr int LPT = DP / 64, TT = 32 / LPT, PITCH = DP + 4 * LPT;
-  return (size_t)(2 * kWarps * TT * PITCH + GP * DP + kWarps * TT * GP + 2 * kWarps * GP) * 4 + (size_t)(n_seqs + 1) * 4;
-}
-
 // Blocks for the call: as many as run at once, fewer where even the table's
-// full width holds less than min_tiles tiles for each.
-int attn_grid(const PagedAttnArgs& a, int gp, int tile, int most) {
+// full width holds less than min_tiles places of the list for each.
+int attn_grid(const PagedAttnArgs& a, int gp, int tile, int cost, int most) {
   const int64_t cap = (int64_t)a.c.width * a.c.page_tokens;
   const int64_t seen = a.window > 0 ? std::min<int64_t>(cap, a.window) : cap;
   const int64_t items = (int64_t)a.n_seqs * a.c.hkv * ((a.group + gp - 1) / gp);
-  const int64_t tiles = items * ((seen + tile - 1) / tile);
+  const int64_t tiles = items * ((seen + tile - 1) / tile + cost);
   LC_REQUIRE(tiles < (1ll << 31) - (1 << 20), LC_ERR_INVALID, "more slots than one call can split");
+  most = std::min(most, kPagedMaxBlocks);
   return (int)std::max<int64_t>(1, std::min<int64_t>(most, (tiles + a.min_tiles - 1) / a.min_tiles));
 }
 
-template <typename T, int DP>
-void launch_general(PagedAttnArgs& a, int device, int sms, cudaStream_t s) {
-  constexpr int GP = 4;
-  auto kernel = k_paged_attn<T, DP, GP, kWarps>;
-  const size_t smem = general_smem<DP, GP>(a.n_seqs);
+template <typename T, int DP, int GP, int ST>
+void launch_fma(PagedAttnArgs& a, int device, int sms, cudaStream_t s) {
+  constexpr int LPT = DP / 64, TT = 32 / LPT, PITCH = DP + 4 * LPT;
+  constexpr size_t fixed = (size_t)(kWarps * ST * 2 * TT * PITCH + GP * DP + kWarps * TT * GP + 2 * kWarps * GP) * 4;
+  static_assert(fixed + (kPagedMaxSeqs + 1) * 4 <= 226 * 1024, "fits a block");
+  auto kernel = k_paged_attn<T, DP, GP, kWarps, ST>;
   static SmemOptIn opt;
-  opt(kernel, general_smem<DP, GP>(kPagedMaxSeqs), device);
-  a.min_tiles = 2 * kWarps;
-  const int grid = attn_grid(a, GP, 32 / (DP / 64), 2 * sms);
-  kernel<<<grid, kWarps * 32, smem, s>>>(a);
+  opt(kernel, fixed + (kPagedMaxSeqs + 1) * 4, device);
+  a.min_tiles = kWarps;
+  const int grid = attn_grid(a, GP, TT, kGeneralCost, ST > 1 ? sms : 2 * sms);
+  kernel<<<grid, kWarps * 32, fixed + (size_t)(a.n_seqs + 1) * 4, s>>>(a);
+}
+
+// 16-byte rows of f32: the pipeline, for as many heads at a time as the group
+// has (up to 8). Anything else that the tensor cores do not take: the plain
+// loads.
+template <typename T, int DP>
+void launch_fma(PagedAttnArgs& a, bool vec, int device, int sms, cudaStream_t s) {
+  if constexpr (sizeof(T) == 4) {
+    if (vec && a.group <= 4) return launch_fma<T, DP, 4, 3>(a, device, sms, s);
+    if (vec) return launch_fma<T, DP, 8, 3>(a, device, sms, s);
+  }
+  launch_fma<T, DP, 4, 1>(a, device, sms, s);
 }
 
 template <typename T>
-void launch_general(PagedAttnArgs& a, int device, int sms, cudaStream_t s) {
+void launch_fma(PagedAttnArgs& a, bool vec, int device, int sms, cudaStream_t s) {
   if (a.c.d <= 64)
-    launch_general<T, 64>(a, device, sms, s);
+    launch_fma<T, 64>(a, vec, device, sms, s);
   else if (a.c.d <= 128)
-    launch_general<T, 128>(a, device, sms, s);
+    launch_fma<T, 128>(a, vec, device, sms, s);
   else
-    launch_general<T, 256>(a, device, sms, s);
+    launch_fma<T, 256>(a, vec, device, sms, s);
 }
 
-// acc_out[s, h, t] = decay acc_in + sum_g exp2(score_gt - m_g) / l_g. A thread
-// per slot; 4 (group + 2) bytes a slot are read and written, all of them in
-// rows of consecutive slots.
+// acc_out[s, h, t] = decay acc_in + sum_g exp2(score_gt - m_g) / l_g. A block
+// does 1024 slots of a row, four a thread, so that a thread has all its loads
+// in flight at once; 4 (group + 2) bytes a slot, the scores still in L2.
+template <bool VEC>
 __global__ void __launch_bounds__(256) k_paged_weights(const PagedWeightArgs a) {
   extern __shared__ float st[];  // [group][2]
-  const int row = blockIdx.x, s = row / a.hkv;
-  for (int i = threadIdx.x; i < 2 * a.group; i += 256) st[i] = a.stats[2ll * row * a.group + i];
-  __syncthreads();
+  const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks, s = row / a.hkv, tid = threadIdx.x;
   const int n = min(max(a.lens[s], 0), a.cap), lo = first_slot(n, a.window);
-  for (int t = blockIdx.y * 256 + threadIdx.x; t < n; t += gridDim.y * 256) {
-    float sum = 0.f;
-    if (t >= lo) {
-      const float* sc = a.scores + ((int64_t)row * a.score_tokens + t) * a.group;
-      for (int i = 0; i < a.group; ++i) sum += ex2(sc[i] - st[2 * i]) * st[2 * i + 1];
+  const int t0 = chunk * 1024 + tid;
+  if (chunk * 1024 >= n) return;
+  const float* acc_in = a.acc_in + row * a.acc_stride;
+  float acc[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (t0 + i * 256 < n) acc[i] = acc_in[t0 + i * 256];
+  pdl_wait();  // what follows reads the attention's scores and statistics
+  for (int i = tid; i < 2 * a.group; i += 256) st[i] = a.stats[2ll * row * a.group + i];
+  const float* sc = a.scores + (int64_t)row * a.score_tokens * a.group;
+  if (VEC) {
+    for (int g = 0; g < a.group; g += 4) {
+      float4 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + i * 256;
+        if (t >= lo && t < n) x[i] = *reinterpret_cast<const float4*>(sc + (int64_t)t * a.group + g);
+      }
+      if (g == 0) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float* e = st + 2 * g;
+        sum[i] += ex2(x[i].x - e[0]) * e[1] + ex2(x[i].y - e[2]) * e[3] + ex2(x[i].z - e[4]) * e[5] +
+                  ex2(x[i].w - e[6]) * e[7];
+      }
     }
-    const int64_t at = row * a.acc_stride + t;
-    a.acc_out[at] = fmaf(a.decay, a.acc_in[at], sum);
+  } else {
+    __syncthreads();
+#pragma unroll 2
+    for (int g = 0; g < a.group; ++g) {
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + i * 256;
+        if (t >= lo && t < n) x[i] = sc[(int64_t)t * a.group + g];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] += ex2(x[i] - st[2 * g]) * st[2 * g + 1];
+    }
+  }
+  float* out = a.acc_out + row * a.acc_stride;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = t0 + i * 256;
+    if (t < n) out[t] = fmaf(a.decay, acc[i], t >= lo ? sum[i] : 0.f);
   }
 }
 
@@ -702,8 +861,8 @@ void launch_mma(PagedAttnArgs& a, int device, int sms, cudaStream_t s) {
   static_assert(fixed + (kPagedMaxSeqs + 1) * 4 <= 226 * 1024, "fits a block");
   static SmemOptIn opt;
   opt(kernel, fixed + (kPagedMaxSeqs + 1) * 4, device);
-  a.min_tiles = 2 * W;
-  kernel<<<attn_grid(a, 8, 16, sms), W * 32, fixed + (size_t)(a.n_seqs + 1) * 4, s>>>(a);
+  a.min_tiles = W;
+  kernel<<<attn_grid(a, 8, 16, kMmaCost, sms), W * 32, fixed + (size_t)(a.n_seqs + 1) * 4, s>>>(a);
 }
 
 template <typename T>
@@ -732,26 +891,28 @@ bool vector_rows(const PagedView& c, int esize) {
 int64_t paged_part_floats(int32_t sms) { return 2ll * (2 * sms) * 8 * (kPagedMaxDim + 2); }
 
 void launch_paged_attn(PagedAttnArgs& a, int32_t pool_dtype, int32_t device, int32_t sms, cudaStream_t s) {
-  const bool mma = pool_dtype != LC_F32 && a.q_dtype == pool_dtype && vector_rows(a.c, 2) &&
-                   (reinterpret_cast<uintptr_t>(a.q) & 3) == 0;
+  const bool vec = vector_rows(a.c, pool_dtype == LC_F32 ? 4 : 2);
+  const bool mma = pool_dtype != LC_F32 && a.q_dtype == pool_dtype && vec && (reinterpret_cast<uintptr_t>(a.q) & 3) == 0;
   if (mma && pool_dtype == LC_BF16)
     launch_mma<__nv_bfloat16>(a, device, sms, s);
   else if (mma)
     launch_mma<__half>(a, device, sms, s);
   else if (pool_dtype == LC_F32)
-    launch_general<float>(a, device, sms, s);
+    launch_fma<float>(a, vec, device, sms, s);
   else if (pool_dtype == LC_BF16)
-    launch_general<__nv_bfloat16>(a, device, sms, s);
+    launch_fma<__nv_bfloat16>(a, vec, device, sms, s);
   else
-    launch_general<__half>(a, device, sms, s);
+    launch_fma<__half>(a, vec, device, sms, s);
   LC_CUDA(cudaGetLastError());
 }
 
-void launch_paged_weights(const PagedWeightArgs& a, cudaStream_t s) {
-  const int rows = a.n_seqs * a.hkv;
-  const dim3 grid((unsigned)rows, (unsigned)std::min<int64_t>(64, (a.cap + 1023) / 1024));
-  k_paged_weights<<<grid, 256, 2 * a.group * 4, s>>>(a);
-  LC_CUDA(cudaGetLastError());
+void launch_paged_weights(PagedWeightArgs a, cudaStream_t s) {
+  a.chunks = (a.cap + 1023) / 1024;
+  const int64_t blocks = (int64_t)a.n_seqs * a.hkv * a.chunks;
+  LC_REQUIRE(blocks < (1ll << 31), LC_ERR_INVALID, "more slots than one call can weigh");
+  const bool vec = a.group % 4 == 0;  // a slot's scores are whole float4s (the workspace is 256-byte aligned)
+  launch_pdl(vec ? k_paged_weights<true> : k_paged_weights<false>, dim3((unsigned)blocks), dim3(256),
+             2 * a.group * 4, s, a);
 }
 
 void launch_paged_append(const PagedAppendArgs& a, cudaStream_t s) {
