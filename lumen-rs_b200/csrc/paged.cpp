@@ -114,6 +114,7 @@ int sm_count(int device) {
 struct lc_paged {
   lc_paged_config cfg{};
   PagedView view{};
+  PagedMaps maps{};
   int sms = 0, esize = 0;
   Order order;
   Workspace part, counters, scores, evict;
@@ -213,6 +214,7 @@ int lc_paged_create(const lc_paged_config* config, void* k_pages, void* v_pages,
     p->view.page_tokens = c.page_tokens;
     p->view.n_pages = c.n_pages;
     p->view.status = dev_status;
+    p->maps = make_paged_maps(p->view, c.dtype);
     p->part.get((size_t)paged_part_floats(p->sms) * 4);
     p->counters.get((size_t)c.max_seqs * c.max_q_heads * 4, true);
     *out = p.release();
@@ -311,7 +313,7 @@ static void paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t
     a.stats = ws + rows * cap;
   }
   const cudaStream_t s = p->order.on(stream);
-  launch_paged_attn(a, p->cfg.dtype, p->cfg.device, p->sms, s);
+  launch_paged_attn(a, p->maps, p->cfg.dtype, p->cfg.device, p->sms, s);
   if (acc_out) {
     PagedWeightArgs w{};
     w.scores = a.scores;

@@ -2,6 +2,7 @@
 // kernel argument blocks and launchers shared by paged.cpp and the kernels.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -38,6 +39,12 @@ struct PagedView {
   int32_t* status;  // mapped host word: set when a length or a page id is out of range
 };
 
+// TMA descriptors of the two pools; box: slots of a load, 0 where there are none.
+struct PagedMaps {
+  CUtensorMap k, v;
+  int32_t box;
+};
+
 struct PagedAttnArgs {
   PagedView c;
   const void* q;
@@ -47,6 +54,7 @@ struct PagedAttnArgs {
   int32_t layer, window;
   float scale_log2;  // scale * log2(e)
   int32_t min_tiles;
+  int32_t box;       // slots of a TMA box
   float* part;       // split partials: [2 * grid] slots of [heads][d + 2]
   int32_t* counters; // one per (sequence, kv head, head group); zero between calls
   float* scores;     // [n_seqs][hkv][score_tokens][group] (log2 domain), or null
@@ -129,7 +137,9 @@ constexpr int kBeamMaxMerge = 4096;  // candidates of one merge
 
 void launch_paged_append(const PagedAppendArgs& a, cudaStream_t s);
 // pool_dtype: LC_F32 / LC_BF16 / LC_F16.
-void launch_paged_attn(PagedAttnArgs& a, int32_t pool_dtype, int32_t device, int32_t sms, cudaStream_t s);
+void launch_paged_attn(PagedAttnArgs& a, const PagedMaps& maps, int32_t pool_dtype, int32_t device, int32_t sms,
+                       cudaStream_t s);
+PagedMaps make_paged_maps(const PagedView& c, int32_t dtype);
 int64_t paged_part_floats(int32_t sms);
 void launch_paged_weights(PagedWeightArgs a, cudaStream_t s);
 int paged_evict_cluster(int64_t cap);

@@ -88,7 +88,7 @@ __device__ void build_prefix(const PagedAttnArgs& a, int tile, int cost, int* pr
   const int b = min(a.n_seqs, tid * per), e = min(a.n_seqs, b + per);
   auto places_of = [&](int s) {
     const int n = clamp_len(a.c, s);
-    return n == 0 ? 0 : cost + (n - first_slot(n, a.window) + tile - 1) / tile;
+    return n == 0 ? 0 : cost + (n - 1) / tile - first_slot(n, a.window) / tile + 1;
   };
   int sum = 0;
   for (int s = b; s < e; ++s) sum += places_of(s);
@@ -123,14 +123,15 @@ __device__ void build_prefix(const PagedAttnArgs& a, int tile, int cost, int* pr
 // and head group) of it.
 struct Segment {
   int s, hh, j0, j1, n, lo;  // j1 <= j0: places only
+  int t0;                    // tile 0's first slot: lo, down to whole tiles
   int next;                  // where the block goes on in the list
   // the item's blocks are first .. first + parts - 1; block b's partial is in
   // slot 2 b, or 2 b + 1 where the item does not begin its run (the first only)
   int first, parts, slot0, slot;
 };
 
-__device__ __forceinline__ Segment find_segment(const PagedAttnArgs& a, const int* prefix, int cost, int hh_n, int per,
-                                                int u, int u_end) {
+__device__ __forceinline__ Segment find_segment(const PagedAttnArgs& a, const int* prefix, int tile, int cost, int hh_n,
+                                                int per, int u, int u_end) {
   Segment g;
   const int key = u / hh_n;
   int b = 0, e = a.n_seqs;  // the last s with prefix[s] <= key
@@ -151,6 +152,7 @@ __device__ __forceinline__ Segment find_segment(const PagedAttnArgs& a, const in
   g.next = min(end, u_end);
   g.n = clamp_len(a.c, b);
   g.lo = first_slot(g.n, a.window);
+  g.t0 = g.lo - g.lo % tile;
   g.first = start / per;
   g.parts = (end - 1) / per - g.first + 1;
   // an item begins its first block's run unless other places are before its own
@@ -329,7 +331,7 @@ __global__ void __launch_bounds__(W * 32, ST > 1 ? 1 : 2) k_paged_attn(const Pag
   const int tok = lane / LPT, part = lane % LPT;
   auto dim = [&](int x) { return DP == 64 ? lane * 2 + x : (x >> 2) * 128 + lane * 4 + (x & 3); };
   for (int u = blockIdx.x * per; u < u_end;) {
-    const Segment g = find_segment(a, prefix, kCost, hh_n, per, u, u_end);
+    const Segment g = find_segment(a, prefix, TT, kCost, hh_n, per, u, u_end);
     u = g.next;
     if (g.j1 <= g.j0) continue;
     const int h = g.hh / hg_n, head0 = (g.hh - h * hg_n) * GP, nh = min(GP, a.group - head0);
@@ -339,11 +341,11 @@ __global__ void __launch_bounds__(W * 32, ST > 1 ? 1 : 2) k_paged_attn(const Pag
 
     // lane r looks up slot r of a tile
     auto page_of = [&](int j) -> int {
-      const int t = g.lo + j * TT + lane;
-      return j < g.j1 && lane < TT && t < g.n ? table[t / a.c.page_tokens] : INT32_MIN;
+      const int t = g.t0 + j * TT + lane;
+      return j < g.j1 && lane < TT && t >= g.lo && t < g.n ? table[t / a.c.page_tokens] : INT32_MIN;
     };
     auto row_of = [&](int j, int page) -> int64_t {
-      const int t = g.lo + j * TT + lane;
+      const int t = g.t0 + j * TT + lane;
       if (page >= 0 && page < a.c.n_pages) return page * a.c.page + (int64_t)(t % a.c.page_tokens) * a.c.token;
       if (page != INT32_MIN) *a.c.status = 1;
       return -1;
@@ -391,7 +393,8 @@ __global__ void __launch_bounds__(W * 32, ST > 1 ? 1 : 2) k_paged_attn(const Pag
     }
     int stage = 0, fill = ST - 1;
     for (int j = first; j < g.j1; j += W) {
-      const int t0 = g.lo + j * TT, nt = min(TT, g.n - t0);
+      const int t0 = g.t0 + j * TT;
+      const bool seen = t0 + tok >= g.lo && t0 + tok < g.n;
       if constexpr (ST > 1) {
         cp_wait<(ST > 1 ? ST - 2 : 0)>();
         __syncwarp();
@@ -436,10 +439,10 @@ __global__ void __launch_bounds__(W * 32, ST > 1 ? 1 : 2) k_paged_attn(const Pag
       for (int i = 0; i < GP; ++i) {
 #pragma unroll
         for (int b = 1; b < LPT; b <<= 1) s[i] += __shfl_xor_sync(~0u, s[i], b);
-        if (tok >= nt) s[i] = kNegInf;
+        if (!seen) s[i] = kNegInf;
         grow |= s[i] > m[i];
       }
-      if (a.scores && part == 0 && tok < nt) {
+      if (a.scores && part == 0 && seen) {
         float* to = a.scores + (((int64_t)g.s * a.c.hkv + h) * a.score_tokens + t0 + tok) * a.group + head0;
 #pragma unroll
         for (int i = 0; i < GP; ++i)
@@ -536,6 +539,16 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+// One box of a pool into shared memory, completing on an mbarrier.
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int token, int head, int page,
+                                         int layer, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+      "%6}], [%7];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(token), "r"(head), "r"(page), "r"(layer), "r"(bar)
+      : "memory");
+}
+
 // The tensor-core kernel: 16-bit pools whose rows are whole 16-byte units,
 // queries of the pool's type, head dimension up to DP.
 //
@@ -549,32 +562,57 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
 // and remainder), which keeps the weights to 2^-17 or better and makes the
 // output's own rounding the only one that shows.
 //
-// Each warp runs its own pipeline: tiles of 16 slots, ST stages of cp.async,
-// no block barrier inside a segment. Rows have 16 bytes of padding: eight
-// rows of an ldmatrix are on different banks. Slots past the end and
-// dimensions past d are filled with zeros, never read.
-template <typename T, int DP, int W, int ST>
-__global__ void __launch_bounds__(W * 32, 1) k_paged_attn_mma(const PagedAttnArgs a) {
-  constexpr int GP = 8, TT = 16, CH = DP / 8, PITCH = DP * 2 + 16, TILE = TT * PITCH, kCost = kMmaCost;
-  extern __shared__ __align__(16) uint8_t smem[];
+// Each warp runs its own pipeline over tiles of 16 slots in ST stages, no block
+// barrier inside a segment. Slots outside the sequence or its window weigh
+// nothing and their V rows are zeros in shared memory, whatever memory holds.
+//
+// TMA: pages of whole 8 slots, d >= 64. One lane fetches a tile with boxes of
+// BR slots x 64 dimensions in the 128-byte swizzle, which puts the eight rows
+// of an ldmatrix on different banks. Else: cp.async of 16 bytes a lane into
+// rows with 16 bytes of padding. The latter's addresses are half of the
+// instructions of a tile, and a warp that has eight to share an SM with must
+// not take longer than the SM's share of the HBM does.
+template <typename T, int DP, int W, int ST, bool TMA>
+__global__ void __launch_bounds__(W * 32, 1)
+    k_paged_attn_mma(const PagedAttnArgs a, const __grid_constant__ CUtensorMap k_map,
+                     const __grid_constant__ CUtensorMap v_map) {
+  constexpr int GP = 8, TT = 16, CH = DP / 8, PITCH = TMA ? DP * 2 : DP * 2 + 16, TILE = TT * PITCH, kCost = kMmaCost;
+  extern __shared__ __align__(1024) uint8_t smem[];
   float* om = reinterpret_cast<float*>(smem + W * ST * 2 * TILE);
   float* ol = om + W * GP;
-  int* prefix = reinterpret_cast<int*>(ol + W * GP);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ol + W * GP);  // [W][ST], TMA
+  int* prefix = reinterpret_cast<int*>(bars + W * ST);
   float* oo = reinterpret_cast<float*>(smem);  // [W][GP][DP]: the stages' room, free when a segment ends
   static_assert(GP * DP * 4 <= ST * 2 * TILE && (kPagedMaxBlocks * GP + W * 128) * 4 <= W * ST * 2 * TILE,
                 "the warps' outputs, and the joins' weights and sums, fit the stages");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, tg = lane & 3;
   const int hg_n = (a.group + GP - 1) / GP, hh_n = a.c.hkv * hg_n;
   if (a.scores) pdl_launch_dependents();
+  const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars + warp * ST);
+  if (TMA && lane == 0) {
+#pragma unroll
+    for (int i = 0; i < ST; ++i) mbar_init(bar + 8 * i, 1);
+    mbar_init_fence();
+  }
   build_prefix<W * 32>(a, TT, kCost, prefix);
   const int total = prefix[a.n_seqs] * hh_n;
   const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, a.min_tiles);
   const int u_end = min(total, ((int)blockIdx.x + 1) * per);
-  const uint32_t stages = (uint32_t)__cvta_generic_to_shared(smem) + warp * ST * 2 * TILE;
-  const uint32_t k_at = (lane & 15) * PITCH + (lane >> 4) * 16;
-  const uint32_t v_at = ((lane & 7) + ((lane >> 4) << 3)) * PITCH + ((lane >> 3) & 1) * 16;
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem), stages = base + warp * ST * 2 * TILE;
+  // this lane's row and 16-byte half in the fragments of K (slots x dimensions)
+  // and V (transposed); under the swizzle a row's chunk c is at c ^ (row & 7)
+  const int k_row = lane & 15, k_half = lane >> 4, v_row = (lane & 7) + ((lane >> 4) << 3), v_half = (lane >> 3) & 1;
+  uint32_t k_at[TMA ? 4 : 1], v_at[TMA ? 4 : 1];
+#pragma unroll
+  for (int i = 0; i < (TMA ? 4 : 1); ++i) {
+    k_at[i] = TMA ? k_row * 128 + (((2 * i + k_half) ^ (k_row & 7)) << 4) : k_row * PITCH + k_half * 16;
+    v_at[i] = TMA ? v_row * 128 + (((2 * i + v_half) ^ (v_row & 7)) << 4) : v_row * PITCH + v_half * 16;
+  }
+  auto k_frag = [&](int i) -> uint32_t { return TMA ? (i >> 2) * 2048 + k_at[i & (TMA ? 3 : 0)] : k_at[0] + i * 32; };
+  auto v_frag = [&](int i) -> uint32_t { return TMA ? (i >> 2) * 2048 + v_at[i & (TMA ? 3 : 0)] : v_at[0] + i * 32; };
+  uint32_t phases = 0;
   for (int u = blockIdx.x * per; u < u_end;) {
-    const Segment g = find_segment(a, prefix, kCost, hh_n, per, u, u_end);
+    const Segment g = find_segment(a, prefix, TT, kCost, hh_n, per, u, u_end);
     u = g.next;
     if (g.j1 <= g.j0) continue;
     const int h = g.hh / hg_n, head0 = (g.hh - h * hg_n) * GP, nh = min(GP, a.group - head0);
@@ -582,31 +620,58 @@ __global__ void __launch_bounds__(W * 32, 1) k_paged_attn_mma(const PagedAttnArg
     const T* vb = static_cast<const T*>(a.c.v) + a.layer * a.c.layer + h * a.c.head;
     const int32_t* table = a.c.tables + (int64_t)g.s * a.c.width;
 
-    // lane r (and r + 16) looks up slot r of a tile
+    // cp.async: lane r (and r + 16) looks up slot r of a tile; TMA: lane b that
+    // of box row b (those past either end fetch page 0, to be masked)
     auto page_of = [&](int j) -> int {
-      const int t = g.lo + j * TT + (lane & 15);
-      return j < g.j1 && t < g.n ? table[t / a.c.page_tokens] : INT32_MIN;
+      if (TMA) {
+        const int t = g.t0 + j * TT + lane * a.box;
+        return j < g.j1 && lane * a.box < TT && t < g.n && t + a.box > g.lo ? table[t / a.c.page_tokens] : 0;
+      }
+      const int t = g.t0 + j * TT + (lane & 15);
+      return j < g.j1 && t >= g.lo && t < g.n ? table[t / a.c.page_tokens] : INT32_MIN;
     };
     auto issue = [&](int j, int stage, int page) {
-      if (j < g.j1) {
-        const int t = g.lo + j * TT + (lane & 15);
-        int64_t off = -1;
-        if (page >= 0 && page < a.c.n_pages)
-          off = page * a.c.page + (int64_t)(t % a.c.page_tokens) * a.c.token;
-        else if (page != INT32_MIN)
+      const uint32_t to = stages + stage * 2 * TILE;
+      if constexpr (TMA) {
+        if (j >= g.j1) return;
+        if (page < 0 || page >= a.c.n_pages) {
           *a.c.status = 1;
-        const uint32_t to = stages + stage * 2 * TILE;
-#pragma unroll
-        for (int x = 0; x < TT * CH / 32; ++x) {
-          const int e = x * 32 + lane, r = e / CH, c = e - r * CH;
-          const int64_t o = __shfl_sync(~0u, off, r);
-          const bool read = o >= 0 && c * 8 < a.c.d;
-          const int64_t from = read ? o + c * 8 : 0;
-          cp_async16_or_zero(to + r * PITCH + c * 16, kb + from, read);
-          cp_async16_or_zero(to + TILE + r * PITCH + c * 16, vb + from, read);
+          page = 0;
         }
+        const int page1 = __shfl_sync(~0u, page, 1);
+        if (lane != 0) return;
+        const int t = g.t0 + j * TT;
+        mbar_expect_tx(bar + 8 * stage, 2 * TILE);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (half * a.box >= TT) break;
+          const int tok = (t + half * a.box) % a.c.page_tokens, pg = half ? page1 : page;
+#pragma unroll
+          for (int b = 0; b < DP / 64; ++b) {
+            tma_load(to + b * 2048 + half * 1024, &k_map, b * 64, tok, h, pg, a.layer, bar + 8 * stage);
+            tma_load(to + TILE + b * 2048 + half * 1024, &v_map, b * 64, tok, h, pg, a.layer, bar + 8 * stage);
+          }
+        }
+      } else {
+        if (j < g.j1) {
+          const int t = g.t0 + j * TT + (lane & 15);
+          int64_t off = -1;
+          if (page >= 0 && page < a.c.n_pages)
+            off = page * a.c.page + (int64_t)(t % a.c.page_tokens) * a.c.token;
+          else if (page != INT32_MIN)
+            *a.c.status = 1;
+#pragma unroll
+          for (int x = 0; x < TT * CH / 32; ++x) {
+            const int e = x * 32 + lane, r = e / CH, c = e - r * CH;
+            const int64_t o = __shfl_sync(~0u, off, r);
+            const bool read = o >= 0 && c * 8 < a.c.d;
+            const int64_t from = read ? o + c * 8 : 0;
+            cp_async16_or_zero(to + r * PITCH + c * 16, kb + from, read);
+            cp_async16_or_zero(to + TILE + r * PITCH + c * 16, vb + from, read);
+          }
+        }
+        cp_commit();
       }
-      cp_commit();
     };
 
     uint32_t qf[DP / 16][2];
@@ -636,11 +701,27 @@ __global__ void __launch_bounds__(W * 32, 1) k_paged_attn_mma(const PagedAttnArg
     }
     int stage = 0, fill = ST - 1;
     for (int j = first; j < g.j1; j += W) {
-      cp_wait<ST - 2>();
-      __syncwarp();
-      issue(j + (ST - 1) * W, fill, page);
-      page = page_of(j + ST * W);
       const uint32_t kt = stages + stage * 2 * TILE, vt = kt + TILE;
+      if constexpr (TMA) {
+        __syncwarp();  // the stage to fill has been read
+        issue(j + (ST - 1) * W, fill, page);
+        if (!mbar_wait(bar + 8 * stage, phases >> stage & 1)) *a.c.status = 2;
+        phases ^= 1u << stage;
+        const int t = g.t0 + j * TT;
+        if (t < g.lo || t + TT > g.n) {  // rows outside: zeros in place of what memory held
+          for (int e = lane; e < TT * CH; e += 32) {
+            const int r = e % TT, c = e / TT;
+            if (t + r < g.lo || t + r >= g.n) *reinterpret_cast<uint4*>(smem + (vt - base) + (c >> 3) * 2048 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+          __syncwarp();
+        }
+      } else {
+        cp_wait<ST - 2>();
+        __syncwarp();
+        issue(j + (ST - 1) * W, fill, page);
+      }
+      page = page_of(j + ST * W);
       fill = stage;
       stage = stage + 1 == ST ? 0 : stage + 1;
 
@@ -648,20 +729,20 @@ __global__ void __launch_bounds__(W * 32, 1) k_paged_attn_mma(const PagedAttnArg
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i) {
         uint32_t f[4];
-        ldsm_x4(kt + k_at + i * 32, f);
+        ldsm_x4(kt + k_frag(i), f);
         mma_16(i & 1 ? sb : sa, f, qf[i][0], qf[i][1], T());
       }
       float s[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) s[x] = (sa[x] + sb[x]) * a.scale_log2;
-      const int t = g.lo + j * TT + gr;
-      if (t >= g.n) s[0] = s[1] = kNegInf;
-      if (t + 8 >= g.n) s[2] = s[3] = kNegInf;
+      const int t = g.t0 + j * TT + gr;
+      if (t < g.lo || t >= g.n) s[0] = s[1] = kNegInf;
+      if (t + 8 < g.lo || t + 8 >= g.n) s[2] = s[3] = kNegInf;
       if (a.scores) {
         float* to = a.scores + (((int64_t)g.s * a.c.hkv + h) * a.score_tokens + t) * a.group + head0 + 2 * tg;
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-          if (t + (x >> 1) * 8 < g.n && 2 * tg + (x & 1) < nh) to[(x >> 1) * 8 * a.group + (x & 1)] = s[x];
+          if (t + (x >> 1) * 8 >= g.lo && t + (x >> 1) * 8 < g.n && 2 * tg + (x & 1) < nh) to[(x >> 1) * 8 * a.group + (x & 1)] = s[x];
       }
       if (__any_sync(~0u, s[0] > m0 || s[2] > m0 || s[1] > m1 || s[3] > m1)) {
         float t0 = fmaxf(m0, fmaxf(s[0], s[2])), t1 = fmaxf(m1, fmaxf(s[1], s[3]));
@@ -697,12 +778,12 @@ __global__ void __launch_bounds__(W * 32, 1) k_paged_attn_mma(const PagedAttnArg
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i) {
         uint32_t f[4];
-        ldsm_x4_t(vt + v_at + i * 32, f);
+        ldsm_x4_t(vt + v_frag(i), f);
         mma_16(o[i], f, hi0, hi1, T());
         mma_16(o[i], f, lo0, lo1, T());
       }
     }
-    cp_wait<0>();
+    if constexpr (!TMA) cp_wait<0>();
 #pragma unroll
     for (int b = 4; b < 32; b <<= 1) {
       l0 += __shfl_xor_sync(~0u, l0, b);
@@ -721,6 +802,10 @@ __global__ void __launch_bounds__(W * 32, 1) k_paged_attn_mma(const PagedAttnArg
       for (int x = 0; x < 4; ++x)
         oo[(warp * GP + 2 * tg + (x & 1)) * DP + i * 16 + gr + (x >> 1) * 8] = o[i][x];
     finish_segment<W * 32, GP, DP>(a, g, hg_n, om, ol, oo);
+    if (TMA && u < u_end) {  // the sums were written where the next loads go
+      fence_proxy_async();
+      __syncthreads();
+    }
   }
 }
 
@@ -854,29 +939,36 @@ __global__ void __launch_bounds__(256) k_paged_append(const PagedAppendArgs a) {
   }
 }
 
-template <typename T, int DP, int W, int ST>
-void launch_mma(PagedAttnArgs& a, int device, int sms, cudaStream_t s) {
-  auto kernel = k_paged_attn_mma<T, DP, W, ST>;
-  constexpr size_t fixed = (size_t)W * ST * 2 * 16 * (DP * 2 + 16) + 2 * W * 8 * 4;
+template <typename T, int DP, int W, int ST, bool TMA>
+void launch_mma(PagedAttnArgs& a, const PagedMaps& maps, int device, int sms, cudaStream_t s) {
+  auto kernel = k_paged_attn_mma<T, DP, W, ST, TMA>;
+  constexpr size_t fixed = (size_t)W * ST * (2 * 16 * (TMA ? DP * 2 : DP * 2 + 16) + 8) + 2 * W * 8 * 4;
   static_assert(fixed + (kPagedMaxSeqs + 1) * 4 <= 226 * 1024, "fits a block");
   static SmemOptIn opt;
   opt(kernel, fixed + (kPagedMaxSeqs + 1) * 4, device);
   a.min_tiles = W;
-  kernel<<<attn_grid(a, 8, 16, kMmaCost, sms), W * 32, fixed + (size_t)(a.n_seqs + 1) * 4, s>>>(a);
+  a.box = maps.box;
+  kernel<<<attn_grid(a, 8, 16, kMmaCost, sms), W * 32, fixed + (size_t)(a.n_seqs + 1) * 4, s>>>(a, maps.k, maps.v);
 }
 
 template <typename T>
-void launch_mma(PagedAttnArgs& a, int device, int sms, cudaStream_t s) {
-  if (a.c.d <= 64)
-    launch_mma<T, 64, 8, 5>(a, device, sms, s);
-  else if (a.c.d <= 96)
-    launch_mma<T, 96, 8, 4>(a, device, sms, s);
-  else if (a.c.d <= 128)
-    launch_mma<T, 128, 8, 3>(a, device, sms, s);
-  else if (a.c.d <= 192)
-    launch_mma<T, 192, 4, 4>(a, device, sms, s);
-  else
-    launch_mma<T, 256, 4, 3>(a, device, sms, s);
+void launch_mma(PagedAttnArgs& a, const PagedMaps& maps, int device, int sms, cudaStream_t s) {
+  if (maps.box) {
+    if (a.c.d <= 64)
+      launch_mma<T, 64, 8, 6, true>(a, maps, device, sms, s);
+    else if (a.c.d <= 128)
+      launch_mma<T, 128, 8, 3, true>(a, maps, device, sms, s);
+    else if (a.c.d <= 192)
+      launch_mma<T, 192, 4, 4, true>(a, maps, device, sms, s);
+    else
+      launch_mma<T, 256, 4, 3, true>(a, maps, device, sms, s);
+  } else if (a.c.d <= 64) {
+    launch_mma<T, 64, 8, 5, false>(a, maps, device, sms, s);
+  } else if (a.c.d <= 128) {
+    launch_mma<T, 128, 8, 3, false>(a, maps, device, sms, s);
+  } else {
+    launch_mma<T, 256, 4, 3, false>(a, maps, device, sms, s);
+  }
 }
 
 // Rows and strides of whole 16-byte units.
@@ -890,13 +982,45 @@ bool vector_rows(const PagedView& c, int esize) {
 
 int64_t paged_part_floats(int32_t sms) { return 2ll * (2 * sms) * 8 * (kPagedMaxDim + 2); }
 
-void launch_paged_attn(PagedAttnArgs& a, int32_t pool_dtype, int32_t device, int32_t sms, cudaStream_t s) {
+// Tensor maps for the TMA loads: pages of whole boxes of 16 or 8 slots, rows of
+// at least the 64 dimensions of a box; box 0 where the pool has no such shape.
+PagedMaps make_paged_maps(const PagedView& c, int32_t dtype) {
+  PagedMaps m{};
+  if (dtype == LC_F32 || !vector_rows(c, 2) || c.page_tokens % 8 != 0 || c.d < 64) return m;
+  void* fn = nullptr;
+  cudaDriverEntryPointQueryResult found;
+  LC_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found));
+  LC_REQUIRE(found == cudaDriverEntryPointSuccess && fn, LC_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+  const int box = c.page_tokens % 16 == 0 ? 16 : 8;
+  const cuuint64_t dims[5] = {(cuuint64_t)c.d, (cuuint64_t)c.page_tokens, (cuuint64_t)c.hkv, (cuuint64_t)c.n_pages,
+                              (cuuint64_t)c.n_layers};
+  const int64_t strides[4] = {c.token, c.head, c.page, c.layer};
+  cuuint64_t bytes[4];
+  for (int i = 0; i < 4; ++i) {
+    bytes[i] = 2 * (cuuint64_t)(dims[i + 1] == 1 ? (c.d + 7) / 8 * 8 : strides[i]);  // a lone row's stride is never used
+    if (bytes[i] >= 1ull << 40) return m;
+  }
+  const cuuint32_t shape[5] = {64, (cuuint32_t)box, 1, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
+  const auto type = dtype == LC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  auto encode = reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(fn);
+  for (int i = 0; i < 2; ++i) {
+    const CUresult r = encode(i ? &m.v : &m.k, type, 5, i ? c.v : c.k, dims, bytes, shape, ones,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return PagedMaps{};
+  }
+  m.box = box;
+  return m;
+}
+
+void launch_paged_attn(PagedAttnArgs& a, const PagedMaps& maps, int32_t pool_dtype, int32_t device, int32_t sms,
+                       cudaStream_t s) {
   const bool vec = vector_rows(a.c, pool_dtype == LC_F32 ? 4 : 2);
   const bool mma = pool_dtype != LC_F32 && a.q_dtype == pool_dtype && vec && (reinterpret_cast<uintptr_t>(a.q) & 3) == 0;
   if (mma && pool_dtype == LC_BF16)
-    launch_mma<__nv_bfloat16>(a, device, sms, s);
+    launch_mma<__nv_bfloat16>(a, maps, device, sms, s);
   else if (mma)
-    launch_mma<__half>(a, device, sms, s);
+    launch_mma<__half>(a, maps, device, sms, s);
   else if (pool_dtype == LC_F32)
     launch_fma<float>(a, vec, device, sms, s);
   else if (pool_dtype == LC_BF16)
