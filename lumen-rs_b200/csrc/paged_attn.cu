@@ -228,15 +228,25 @@ __device__ void finish_segment(const PagedAttnArgs& a, const Segment& g, int hg_
       __threadfence();
       auto slot = [&](int b) { return a.part + (b == 0 ? g.slot0 : 2 * (g.first + b)) * kSlot; };
       for (int i = warp; i < nh; i += W) {
-        float m = kNegInf, l = 0.f;
-        for (int b = lane; b < g.parts; b += 32) m = fmaxf(m, __ldcg(slot(b) + i));
+        constexpr int kEach = (kPagedMaxBlocks + 31) / 32;  // parts a lane: all their loads at once
+        float m = kNegInf, l = 0.f, ms[kEach], ls[kEach];
+#pragma unroll
+        for (int b = 0; b < kEach; ++b) {
+          const bool in = b * 32 + lane < g.parts;
+          const float* from = slot(in ? b * 32 + lane : 0) + i;
+          ms[b] = in ? __ldcg(from) : kNegInf;
+          ls[b] = in ? __ldcg(from + GP) : 0.f;
+        }
+#pragma unroll
+        for (int b = 0; b < kEach; ++b) m = fmaxf(m, ms[b]);
 #pragma unroll
         for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
         const float mg = m == kNegInf ? 0.f : m;
-        for (int b = lane; b < g.parts; b += 32) {
-          const float f = ex2(__ldcg(slot(b) + i) - mg);
-          l += f * __ldcg(slot(b) + GP + i);
-          oo[b * GP + i] = f;
+#pragma unroll
+        for (int b = 0; b < kEach; ++b) {
+          const float f = ex2(ms[b] - mg);
+          l = fmaf(f, ls[b], l);
+          if (b * 32 + lane < g.parts) oo[(b * 32 + lane) * GP + i] = f;
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
@@ -250,14 +260,22 @@ __device__ void finish_segment(const PagedAttnArgs& a, const Segment& g, int hg_
       for (int v = tid - share * kVecs; v < nh * DP / 4 && share < kShare; v += THREADS) {
         const int i = v * 4 / DP, x = v * 4 % DP;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int b = share; b < g.parts; b += kShare) {
-          const float f = oo[b * GP + i];
-          const float4 p = __ldcg(reinterpret_cast<const float4*>(slot(b) + 2 * GP) + v);
-          o.x = fmaf(f, p.x, o.x);
-          o.y = fmaf(f, p.y, o.y);
-          o.z = fmaf(f, p.z, o.z);
-          o.w = fmaf(f, p.w, o.w);
+        constexpr int kAhead = 16;  // loads in flight
+        for (int b = share; b < g.parts; b += kShare * kAhead) {
+          float4 got[kAhead];
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k)
+            if (b + k * kShare < g.parts)
+              got[k] = __ldcg(reinterpret_cast<const float4*>(slot(b + k * kShare) + 2 * GP) + v);
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k)
+            if (b + k * kShare < g.parts) {
+              const float f = oo[(b + k * kShare) * GP + i];
+              o.x = fmaf(f, got[k].x, o.x);
+              o.y = fmaf(f, got[k].y, o.y);
+              o.z = fmaf(f, got[k].z, o.z);
+              o.w = fmaf(f, got[k].w, o.w);
+            }
         }
         if (kShare > 1) {
           sums[share * kVecs + v] = o;
@@ -572,8 +590,8 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
 // rows with 16 bytes of padding. The latter's addresses are half of the
 // instructions of a tile, and a warp that has eight to share an SM with must
 // not take longer than the SM's share of the HBM does.
-template <typename T, int DP, int W, int ST, bool TMA>
-__global__ void __launch_bounds__(W * 32, 1)
+template <typename T, int DP, int W, int ST, bool TMA, int PER_SM>
+__global__ void __launch_bounds__(W * 32, PER_SM)
     k_paged_attn_mma(const PagedAttnArgs a, const __grid_constant__ CUtensorMap k_map,
                      const __grid_constant__ CUtensorMap v_map) {
   constexpr int GP = 8, TT = 16, CH = DP / 8, PITCH = TMA ? DP * 2 : DP * 2 + 16, TILE = TT * PITCH, kCost = kMmaCost;
@@ -939,21 +957,33 @@ __global__ void __launch_bounds__(256) k_paged_append(const PagedAppendArgs a) {
   }
 }
 
-template <typename T, int DP, int W, int ST, bool TMA>
+template <typename T, int DP, int W, int ST, bool TMA, int PER_SM = 1>
 void launch_mma(PagedAttnArgs& a, const PagedMaps& maps, int device, int sms, cudaStream_t s) {
-  auto kernel = k_paged_attn_mma<T, DP, W, ST, TMA>;
+  auto kernel = k_paged_attn_mma<T, DP, W, ST, TMA, PER_SM>;
   constexpr size_t fixed = (size_t)W * ST * (2 * 16 * (TMA ? DP * 2 : DP * 2 + 16) + 8) + 2 * W * 8 * 4;
-  static_assert(fixed + (kPagedMaxSeqs + 1) * 4 <= 226 * 1024, "fits a block");
+  static_assert(PER_SM * (fixed + (kPagedMaxSeqs + 1) * 4 + 2048) <= 228 * 1024, "the blocks fit an SM");
   static SmemOptIn opt;
   opt(kernel, fixed + (kPagedMaxSeqs + 1) * 4, device);
   a.min_tiles = W;
   a.box = maps.box;
-  kernel<<<attn_grid(a, 8, 16, kMmaCost, sms), W * 32, fixed + (size_t)(a.n_seqs + 1) * 4, s>>>(a, maps.k, maps.v);
+  kernel<<<attn_grid(a, 8, 16, kMmaCost, PER_SM * sms), W * 32, fixed + (size_t)(a.n_seqs + 1) * 4, s>>>(a, maps.k, maps.v);
 }
 
 template <typename T>
 void launch_mma(PagedAttnArgs& a, const PagedMaps& maps, int device, int sms, cudaStream_t s) {
-  if (maps.box) {
+  // More short items than SMs: two blocks an SM of half the warps each, whose
+  // items' beginnings and ends overlap (64 sequences of 1 to 64 slots: 12 us
+  // against 18.5; one 131072-slot sequence 96 against 94).
+  const int64_t cap = (int64_t)a.c.width * a.c.page_tokens, seen = a.window > 0 ? std::min<int64_t>(cap, a.window) : cap;
+  const bool halves = seen <= 256 && (int64_t)a.n_seqs * a.c.hkv > sms;
+  if (maps.box && halves) {
+    if (a.c.d <= 64)
+      launch_mma<T, 64, 4, 5, true, 2>(a, maps, device, sms, s);
+    else if (a.c.d <= 128)
+      launch_mma<T, 128, 4, 3, true, 2>(a, maps, device, sms, s);
+    else
+      launch_mma<T, 256, 2, 3, true, 2>(a, maps, device, sms, s);
+  } else if (maps.box) {
     if (a.c.d <= 64)
       launch_mma<T, 64, 8, 6, true>(a, maps, device, sms, s);
     else if (a.c.d <= 128)
