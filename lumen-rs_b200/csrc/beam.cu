@@ -7,13 +7,20 @@
 // into registers, and takes from it both the softmax sums and the slice's
 // n_out best.
 //
-// A block takes a slice of one row. The n_out-th largest of the maxima of 64
-// (or 256) disjoint sets of its logits is a lower bound of the slice's n_out-th
-// largest logit, and few logits besides the best reach it; they are gathered
-// and ranked by counting. The last slice of a row to finish has the row's sum,
-// turns the slices' candidates into totals and ranks them; the last row of a
-// group ranks the rows' candidates and writes the answer. One launch; ranks
-// are by value and index only, so the order of arrival changes nothing.
+// A block takes a part of a row (all of it where there are rows enough for the
+// card) slice by slice through a ring of shared memory that one thread fills
+// with bulk copies. Rows that begin off 16 bytes are put right as they are
+// read from the ring, so that a thread's logits, and with them the order of
+// the sums, do not depend on the row's address. A thread keeps a running
+// maximum and sum of its own. The n_out-th largest of the maxima of 64 (or
+// 256) disjoint sets of the logits so far is a lower bound of the n_out-th
+// largest: it is taken after 1, 2, 4 ... slices, and the logits that reach it,
+// some n_out for every doubling, are gathered, to be ranked by counting at the
+// end. The last part of a row to finish has the row's sum, turns the parts'
+// candidates into totals and ranks them; the last row of a group ranks the
+// rows' candidates and writes the answer. One launch; ranks are by value and
+// index only, so the order of arrival changes nothing. The chain of those
+// steps is what a small call takes, and a good half of a large one.
 #include <algorithm>
 
 #include "devutil.cuh"
@@ -22,9 +29,13 @@
 namespace lc {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kGran = 8;      // 16-byte granules a thread holds
-constexpr int kList = 1024;   // gathered candidates of a slice
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kGran = 2;      // 16-byte granules of a slice for each thread
+constexpr int kStages = 4;    // slices of the ring
+constexpr int kStage = kGran * kThreads + 8;  // granules of a stage: a slice, and one more for rows off 16 bytes
+constexpr int kBeamPerSm = 2;
+constexpr int kList = 1024;   // gathered candidates of a part
 constexpr float kNegInf = -INFINITY;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -57,6 +68,20 @@ template <>
 __device__ __forceinline__ float elem<__half>(const uint4& r, int i) {
   const uint32_t w = (i >> 1) == 0 ? r.x : (i >> 1) == 1 ? r.y : (i >> 1) == 2 ? r.z : r.w;
   return __half2float(__ushort_as_half((unsigned short)(i & 1 ? w >> 16 : w & 0xffffu)));
+}
+
+// The 16 bytes that begin `off` bytes into (lo, hi).
+__device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, int off) {
+  uint32_t w0, w1, w2, w3, w4;
+  switch (off >> 2) {
+    case 0: w0 = lo.x, w1 = lo.y, w2 = lo.z, w3 = lo.w, w4 = hi.x; break;
+    case 1: w0 = lo.y, w1 = lo.z, w2 = lo.w, w3 = hi.x, w4 = hi.y; break;
+    case 2: w0 = lo.z, w1 = lo.w, w2 = hi.x, w3 = hi.y, w4 = hi.z; break;
+    default: w0 = lo.w, w1 = hi.x, w2 = hi.y, w3 = hi.z, w4 = hi.w; break;
+  }
+  const int bits = (off & 3) * 8;
+  return make_uint4(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits), __funnelshift_r(w2, w3, bits),
+                    __funnelshift_r(w3, w4, bits));
 }
 
 // The largest of a granule's values; NaN only where all are.
@@ -93,291 +118,340 @@ __device__ __forceinline__ uint64_t block_max_key(uint64_t k, uint64_t* warp_key
   __syncthreads();
   k = warp_key[0];
 #pragma unroll
-  for (int w = 1; w < kThreads / 32; ++w) k = warp_key[w] > k ? warp_key[w] : k;
+  for (int w = 1; w < kWarps; ++w) k = warp_key[w] > k ? warp_key[w] : k;
   return k;
 }
 
-// Entries of the descending list[0 .. n) above key.
-__device__ __forceinline__ int count_above(const uint64_t* list, int n, uint64_t key) {
-  int b = 0, e = n;
-  while (b < e) {
-    const int m = (b + e) >> 1;
-    if (list[m] > key)
-      b = m + 1;
-    else
-      e = m;
-  }
-  return b;
-}
-
 // true in every thread of the block that arrives last of `of`
-__device__ __forceinline__ bool arrive_last(int* counter, int of) {
-  __shared__ int last;
-  __threadfence();
+__device__ __forceinline__ bool arrive_last(int* counter, int of, int& flag) {
   __syncthreads();
   if (threadIdx.x == 0) {
-    last = atomicAdd(counter, 1) == of - 1;
+    __threadfence();  // the block's writes, which the barrier put before this thread
+    const bool last = atomicAdd(counter, 1) == of - 1;
     if (last) *counter = 0;
+    __threadfence();
+    flag = last;
   }
   __syncthreads();
-  if (last) __threadfence();
-  return last;
+  return flag;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) k_beam_select(const BeamArgs a) {
-  constexpr int E = 16 / sizeof(T);
-  __shared__ __align__(16) uint64_t list[kBeamMaxMerge];  // the slice's list, then the merges' candidates
-  __shared__ uint64_t warp_key[kThreads / 32];
-  __shared__ __align__(16) float sets[kThreads];
-  __shared__ float red_m[kThreads / 32], red_s[kThreads / 32];
-  __shared__ float sh_tau, sh_shift;
-  __shared__ int sh_n, sh_at[kThreads + 1];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.y, slice = blockIdx.x, group = row / a.n_beams, beam = row - group * a.n_beams;
-  const float score = a.scores[row];
-  const bool done = a.finished && a.finished[row];
-  const bool dead = done || !(score > kNegInf);  // its logits do not matter
-  const int64_t srow = (int64_t)row * a.slices + slice;
-
-  if (!dead) {
-    const T* x0 = static_cast<const T*>(a.logits) + row * a.row_stride;
-    const int mis = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));
-    const T* base = x0 - mis;  // index i of the row sits at base[i + mis]
-    const int i_end = mis + a.vocab;
-    uint4 raw[kGran];
-    const int64_t at0 = (int64_t)slice * a.slice + tid * E;
-    if (at0 - tid * E >= mis && at0 - tid * E + a.slice <= i_end) {  // the whole slice is inside the row
-#pragma unroll
-      for (int r = 0; r < kGran; ++r) raw[r] = __ldcs(reinterpret_cast<const uint4*>(base + at0 + r * kThreads * E));
-    } else {
-#pragma unroll
-      for (int r = 0; r < kGran; ++r) {
-        const int64_t at = at0 + r * kThreads * E;
-        if (at >= mis && at + E <= i_end) {
-          raw[r] = __ldcs(reinterpret_cast<const uint4*>(base + at));
-        } else {
-          alignas(16) T part[E];
-#pragma unroll
-          for (int i = 0; i < E; ++i) part[i] = at + i >= mis && at + i < i_end ? base[at + i] : T(kNegInf);
-          raw[r] = *reinterpret_cast<uint4*>(part);
-        }
-      }
-    }
-    float top = kNegInf;
-#pragma unroll
-    for (int r = 0; r < kGran; ++r) top = fmaxf(top, granule_max<T>(raw[r]));
-    const float tg = top == kNegInf ? 0.f : top;
-    float sum = 0.f;
-#pragma unroll
-    for (int r = 0; r < kGran; ++r) {
-      float part = 0.f;
-#pragma unroll
-      for (int i = 0; i < E; ++i) part += ex2((elem<T>(raw[r], i) - tg) * kLog2e);
-      sum += part;
-    }
-    // maxima of 64 sets of four threads, or of 256
-    const bool few = a.n_out <= 16;
-    float set = top;
-    if (few) {
-      set = fmaxf(set, __shfl_xor_sync(~0u, set, 1));
-      set = fmaxf(set, __shfl_xor_sync(~0u, set, 2));
-    }
-    const int n_sets = few ? kThreads / 4 : kThreads;
-    if (!few || (tid & 3) == 0) sets[few ? tid >> 2 : tid] = set;
-    // the slice's max and sum
-    float m = top, l = sum;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float mo = __shfl_xor_sync(~0u, m, o), lo = __shfl_xor_sync(~0u, l, o);
-      const float mn = fmaxf(m, mo), mg = mn == kNegInf ? 0.f : mn;
-      l = l * ex2((m - mg) * kLog2e) + lo * ex2((mo - mg) * kLog2e);
-      m = mn;
-    }
-    if (lane == 0) {
-      red_m[warp] = m;
-      red_s[warp] = l;
-    }
-    if (tid == 0) sh_n = 0;
-    __syncthreads();
-    if (tid < n_sets) {
-      int r = 0;
-      const float v = sets[tid];
+// emit(key, rank) for the `keep` largest of list[0 .. n), all different, 0 for
+// none: P threads count the larger ones of an entry.
+template <typename F>
+__device__ __forceinline__ void rank_list(const uint64_t* list, int n, int keep, F&& emit) {
+  int p = 1;
+  while (p < 32 && 2 * p * n <= kThreads) p *= 2;
+  const int sub = threadIdx.x & (p - 1), step = kThreads / p;
+  for (int c0 = 0; c0 < n; c0 += step) {
+    const int c = c0 + threadIdx.x / p;
+    const uint64_t key = c < n ? list[c] : 0;
+    int r = 0;
 #pragma unroll 4
-      for (int i = 0; i < n_sets; i += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(sets + i);
-        r += x.x > v || (x.x == v && i < tid);
-        r += x.y > v || (x.y == v && i + 1 < tid);
-        r += x.z > v || (x.z == v && i + 2 < tid);
-        r += x.w > v || (x.w == v && i + 3 < tid);
-      }
-      if (r == a.n_out - 1) sh_tau = v;
-    }
-    if (tid == kThreads - 1) {  // a warp that has no set to rank where there are 64
-      float mm = kNegInf, ll = 0.f;
-      for (int w = 0; w < kThreads / 32; ++w) {
-        const float mn = fmaxf(mm, red_m[w]), mg = mn == kNegInf ? 0.f : mn;
-        ll = ll * ex2((mm - mg) * kLog2e) + red_s[w] * ex2((red_m[w] - mg) * kLog2e);
-        mm = mn;
-      }
-      a.slice_stats[2 * srow] = mm;
-      a.slice_stats[2 * srow + 1] = ll;
-    }
-    __syncthreads();
-    const float tau = sh_tau;
+    for (int o = sub; o < n; o += p) r += list[o] > key;
+    for (int o = 1; o < p; o <<= 1) r += __shfl_xor_sync(~0u, r, o);
+    if (sub == 0 && key && r < keep) emit(key, r);
+  }
+}
+
+// max and sum of (m, l) over a warp
+__device__ __forceinline__ void warp_softmax(float& m, float& l) {
+  float top = m;
 #pragma unroll
-    for (int r = 0; r < kGran; ++r) {
-      if (!(granule_max<T>(raw[r]) >= tau)) continue;
-      const int64_t index = at0 + r * kThreads * E - mis;
-      for (int i = 0; i < E; ++i) {
-        const float x = elem<T>(raw[r], i);
-        if (x >= tau && x > kNegInf) {
-          const int at = atomicAdd(&sh_n, 1);
-          if (at < kList) list[at] = make_key(x, (uint32_t)(index + i));
-        }
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  l *= ex2((m - (top == kNegInf ? 0.f : top)) * kLog2e);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+  m = top;
+}
+
+struct BeamShared {
+  uint64_t list[kBeamMaxMerge];  // a part's candidates, then the merges'
+  uint64_t warp_key[kWarps];
+  uint64_t best[kBeamMaxOut];
+  __align__(16) float sets[256];
+  float m[kWarps], l[kWarps];
+  float tau, top, sum, log_sum;
+  int n, last;
+};
+
+// Ends a part, elements [i0, i1) of a row: its maximum, sum and best
+// candidates, then, as the last part of the row, the row's, and as the last row
+// of the group the answer. Block-wide.
+template <typename T>
+__device__ __noinline__ void finish_part(const BeamArgs& a, BeamShared& sh, int row, int64_t i0, int64_t i1, bool dead,
+                                         float m, float l, float tau) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int group = row / a.n_beams, beam = row - group * a.n_beams, parts = gridDim.x;
+  const int64_t slot0 = (int64_t)row * a.slices, slot = slot0 + blockIdx.x;
+  const float score = a.scores[row];
+  uint64_t* row_key = a.row_key + (int64_t)row * a.n_out;
+  const uint32_t index0 = (uint32_t)(beam * (int64_t)a.vocab);
+  // the best candidates of the row (logits: keys by token) as totals, into row_key
+  auto totals = [&](uint64_t* list, int n, float top, float log_sum) {
+    for (int c = tid; c < n; c += kThreads) {
+      uint64_t k = list[c];
+      if (k) {  // two logits may round to the same total
+        const float z = score + ((key_value(k) - top) - log_sum);
+        k = z > kNegInf ? make_key(z, index0 + key_index(k)) : 0;
+      }
+      list[c] = k;
+    }
+    for (int c = tid; c < a.n_out; c += kThreads) row_key[c] = 0;
+    __syncthreads();
+    rank_list(list, n, a.n_out, [&](uint64_t k, int r) { row_key[r] = k; });
+  };
+  if (dead) {
+    if (blockIdx.x == 0)
+      for (int c = tid; c < a.n_out; c += kThreads)
+        row_key[c] = c == 0 && score > kNegInf && a.finished && a.finished[row] ? make_key(score, index0 + a.pad) : 0;
+  } else {
+    warp_softmax(m, l);
+    if (lane == 0) {
+      sh.m[warp] = m;
+      sh.l[warp] = l;
+    }
+    for (int c = tid; c < a.n_out; c += kThreads) sh.best[c] = 0;
+    __syncthreads();
+    if (warp == kWarps - 1) {
+      m = lane < kWarps ? sh.m[lane] : kNegInf;
+      l = lane < kWarps ? sh.l[lane] : 0.f;
+      warp_softmax(m, l);
+      if (lane == 0) {
+        sh.top = m;
+        sh.sum = l;
+        sh.log_sum = logf(l);
       }
     }
-    __syncthreads();
-    const int found = sh_n;
-    uint64_t* keys = a.slice_key + srow * a.n_out;
+    const int found = sh.n;
     if (found <= kList) {
-      for (int i = tid; i < found; i += kThreads) {
-        const uint64_t k = list[i];
-        int r = 0;
-        for (int o = 0; o < found; ++o) r += list[o] > k;
-        if (r < a.n_out) keys[r] = k;
-      }
+      rank_list(sh.list, found, a.n_out, [&](uint64_t k, int r) { sh.best[r] = k; });
     } else {
-      // many logits equal to the bound: one best after the other, from shared memory
-      uint4* held = reinterpret_cast<uint4*>(list);
-      static_assert(sizeof(list) >= kGran * kThreads * 16, "the slice fits the list");
-#pragma unroll
-      for (int r = 0; r < kGran; ++r) held[r * kThreads + tid] = raw[r];
+      // many logits reach the bound: one best after the other, read again
+      const T* x0 = static_cast<const T*>(a.logits) + row * a.row_stride;
       uint64_t before = ~0ull;
       for (int o = 0; o < a.n_out; ++o) {
         uint64_t best = 0;
-#pragma unroll 1
-        for (int r = 0; r < kGran; ++r) {
-          const uint4 x4 = held[r * kThreads + tid];
-#pragma unroll 1
-          for (int i = 0; i < E; ++i) {
-            const float x = elem<T>(x4, i);
-            const uint64_t k = make_key(x, (uint32_t)(at0 + r * kThreads * E + i - mis));
-            if (x >= tau && k < before && k > best) best = k;
-          }
+#pragma unroll 4
+        for (int64_t i = i0 + tid; i < i1; i += kThreads) {
+          const float x = (float)x0[i];
+          const uint64_t k = make_key(x, (uint32_t)i);
+          if (x >= tau && k < before && k > best) best = k;
         }
-        before = block_max_key(best, warp_key);
-        if (tid == 0) keys[o] = before;
+        before = block_max_key(best, sh.warp_key);
+        if (tid == 0) sh.best[o] = before;
       }
     }
-    if (tid == 0) a.slice_count[srow] = min(found, a.n_out);
+    __syncthreads();
+    if (parts == 1) {
+      totals(sh.best, a.n_out, sh.top, sh.log_sum);
+    } else {
+      for (int c = tid; c < a.n_out; c += kThreads) a.slice_key[slot * a.n_out + c] = sh.best[c];
+      if (tid == 0) {
+        a.slice_stats[2 * slot] = sh.top;
+        a.slice_stats[2 * slot + 1] = sh.sum;
+      }
+    }
   }
 
   // the row
-  if (!arrive_last(a.counters + row, a.slices)) return;
-  uint64_t* row_key = a.row_key + (int64_t)row * a.n_out;
-  if (dead) {
-    if (tid == 0) {
-      const bool one = done && score > kNegInf;
-      if (one) row_key[0] = make_key(score, (uint32_t)(beam * (int64_t)a.vocab + a.pad));
-      a.row_count[row] = one;
-    }
-  } else {
-    if (warp == 0) {  // max and sum over the slices, and where each slice's candidates start
-      float m = kNegInf;
-      for (int i = lane; i < a.slices; i += 32) m = fmaxf(m, __ldcg(a.slice_stats + 2 * ((int64_t)row * a.slices + i)));
-#pragma unroll
-      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-      const float mg = m == kNegInf ? 0.f : m;
-      float l = 0.f;
-      for (int i = lane; i < a.slices; i += 32) {
-        const float* st = a.slice_stats + 2 * ((int64_t)row * a.slices + i);
-        l += __ldcg(st + 1) * ex2((__ldcg(st) - mg) * kLog2e);
+  if (parts > 1) {
+    if (!arrive_last(a.counters + row, parts, sh.last)) return;
+    if (!dead) {
+      const int all = parts * a.n_out;
+      if (warp == kWarps - 1) {  // max and sum over the parts
+        m = kNegInf;
+        l = 0.f;
+        for (int i = lane; i < parts; i += 32) {
+          const float mi = __ldcg(a.slice_stats + 2 * (slot0 + i)), li = __ldcg(a.slice_stats + 2 * (slot0 + i) + 1);
+          const float mn = fmaxf(m, mi), mg = mn == kNegInf ? 0.f : mn;
+          l = l * ex2((m - mg) * kLog2e) + li * ex2((mi - mg) * kLog2e);
+          m = mn;
+        }
+        warp_softmax(m, l);
+        if (lane == 0) {
+          sh.top = m;
+          sh.log_sum = logf(l);
+        }
       }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
-      if (lane == 0) {
-        red_m[0] = m;
-        sh_shift = logf(l);
-      }
+      for (int c = tid; c < all; c += kThreads) sh.list[c] = __ldcg(a.slice_key + slot0 * a.n_out + c);
+      __syncthreads();
+      totals(sh.list, all, sh.top, sh.log_sum);
     }
-    for (int i = tid; i < a.slices; i += kThreads) sh_at[i] = __ldcg(a.slice_count + (int64_t)row * a.slices + i);
-    if (tid == 0) sh_n = 0;
-    __syncthreads();
-    const float m = red_m[0], log_sum = sh_shift;
-    // totals; a slice's list stays sorted but for totals that round to the same value
-    for (int c = tid; c < a.slices * a.n_out; c += kThreads) {
-      const int i = c / a.n_out, o = c - i * a.n_out;
-      uint64_t k = 0;
-      if (o < sh_at[i]) {
-        const uint64_t x = __ldcg(a.slice_key + ((int64_t)row * a.slices + i) * a.n_out + o);
-        const float z = score + ((key_value(x) - m) - log_sum);
-        if (z > kNegInf) k = make_key(z, (uint32_t)(beam * (int64_t)a.vocab + key_index(x)));
-      }
-      list[c] = k;
-      if (k) atomicAdd(&sh_n, 1);
-    }
-    __syncthreads();
-    for (int c = tid; c < a.slices * a.n_out; c += kThreads) {
-      const uint64_t k = list[c];
-      if (!k) continue;
-      int r = 0;
-      for (int o = 0; o < a.slices * a.n_out; ++o) r += list[o] > k;
-      if (r < a.n_out) row_key[r] = k;
-    }
-    if (tid == 0) a.row_count[row] = min(sh_n, a.n_out);
   }
 
   // the group
-  if (!arrive_last(a.counters + a.n_groups * a.n_beams + group, a.n_beams)) return;
-  const int64_t row0 = (int64_t)group * a.n_beams;
-  for (int i = tid; i < a.n_beams; i += kThreads) sh_at[i] = __ldcg(a.row_count + row0 + i);
-  if (tid == 0) sh_n = 0;
+  if (a.n_beams > 1 && !arrive_last(a.counters + a.n_groups * a.n_beams + group, a.n_beams, sh.last)) return;
+  const int64_t row0 = (int64_t)group * a.n_beams, out0 = (int64_t)group * a.n_out;
+  const int all = a.n_beams * a.n_out;
   __syncthreads();
-  for (int c = tid; c < a.n_beams * a.n_out; c += kThreads) {
-    const int i = c / a.n_out, o = c - i * a.n_out;
-    if (o < sh_at[i]) list[c] = __ldcg(a.row_key + row0 * a.n_out + c);
+  for (int c = tid; c < all; c += kThreads) sh.list[c] = __ldcg(a.row_key + row0 * a.n_out + c);
+  for (int c = tid; c < a.n_out; c += kThreads) sh.best[c] = 0;
+  __syncthreads();
+  rank_list(sh.list, all, a.n_out, [&](uint64_t k, int r) { sh.best[r] = k; });
+  __syncthreads();
+  for (int r = tid; r < a.n_out; r += kThreads) {
+    const uint64_t k = sh.best[r];
+    const uint32_t index = key_index(k);
+    // a place with no candidate keeps a beam
+    const int p = k ? (int)(index / (uint32_t)a.vocab) : r % a.n_beams;
+    const int tok = k ? (int)(index - (uint32_t)p * (uint32_t)a.vocab) : a.pad;
+    a.scores_out[out0 + r] = k ? key_value(k) : kNegInf;
+    a.parents[out0 + r] = p;
+    a.tokens[out0 + r] = tok;
+    a.finished_out[out0 + r] = !k || tok == a.eos || (a.finished && a.finished[row0 + p]);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, kBeamPerSm) k_beam_select(const __grid_constant__ BeamArgs a) {
+  constexpr int E = 16 / sizeof(T);
+  extern __shared__ __align__(16) uint4 ring[];  // [kStages][kStage]
+  __shared__ BeamShared sh;
+  __shared__ uint64_t bars[kStages];
+  const int tid = threadIdx.x, row = blockIdx.y;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), bar = (uint32_t)__cvta_generic_to_shared(bars);
+  const int slice0 = blockIdx.x * a.per, slice1 = min(a.slices, slice0 + a.per);
+  const float score = a.scores[row];
+  const uint8_t done = a.finished ? a.finished[row] : 0;
+  // the row's first element sits at base[mis]: base is 16-byte aligned
+  const T* x0 = static_cast<const T*>(a.logits) + row * a.row_stride;
+  const int mis = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T)), off = mis * (int)sizeof(T);
+  const T* base = x0 - mis;
+  const int64_t i_end = mis + (int64_t)a.vocab;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(bar + 8 * i, 1);
+    mbar_init_fence();
+    sh.n = 0;
   }
   __syncthreads();
-  for (int c = tid; c < a.n_beams * a.n_out; c += kThreads) {
-    const int i = c / a.n_out, o = c - i * a.n_out;
-    if (o >= sh_at[i]) continue;
-    const uint64_t k = list[c];
-    int r = o;
-    for (int b = 0; b < a.n_beams && r < a.n_out; ++b)
-      if (b != i) r += count_above(list + b * a.n_out, sh_at[b], k);
-    if (r >= a.n_out) continue;
-    const uint32_t index = key_index(k), p = index / (uint32_t)a.vocab, tok = index - p * (uint32_t)a.vocab;
-    const int64_t to = (int64_t)group * a.n_out + r;
-    a.scores_out[to] = key_value(k);
-    a.parents[to] = (int32_t)p;
-    a.tokens[to] = (int32_t)tok;
-    a.finished_out[to] = (a.finished && a.finished[row0 + p]) || (int32_t)tok == a.eos;
-    atomicAdd(&sh_n, 1);
+  // slice `slice` into a stage: its whole granules by one bulk copy; those at
+  // the row's ends by hand, -inf where there is no logit
+  auto fetch = [&](int slice, int stage) {
+    if (slice >= slice1) return;
+    const int64_t at0 = (int64_t)slice * a.slice;
+    const int n = kGran * kThreads + (mis ? 1 : 0);
+    const int lo = mis && slice == 0 ? 1 : 0, hi = (int)min((int64_t)n, (i_end - at0) / E);
+    if (tid == 0) {
+      const int bytes = hi > lo ? (hi - lo) * 16 : 0;
+      mbar_expect_tx(bar + 8 * stage, bytes);
+      if (bytes) bulk_g2s(ring_at + (stage * kStage + lo) * 16, base + at0 + lo * E, bytes, bar + 8 * stage);
+    }
+    if (lo > 0 || hi < n) {
+#pragma unroll 1
+      for (int v = tid; v < n; v += kThreads) {
+        if (v >= lo && v < hi) continue;
+        const int64_t at = at0 + v * E;
+        alignas(16) T part[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) part[i] = at + i >= mis && at + i < i_end ? base[at + i] : T(kNegInf);
+        ring[stage * kStage + v] = *reinterpret_cast<uint4*>(part);
+      }
+      fence_proxy_async();  // a later slice's bulk copy may write there
+    }
+  };
+#pragma unroll 1
+  for (int i = 0; i < kStages - 1; ++i) fetch(slice0 + i, i);
+  // a finished row's logits, or those of a beam that is out, do not matter (the
+  // first slices were asked for before that was known: they are awaited)
+  const bool dead = done || !(score > kNegInf);
+  if (dead)
+    for (int i = 0; i < kStages - 1 && slice0 + i < slice1; ++i) mbar_wait(bar + 8 * i, 0);
+  float m = kNegInf, l = 0.f, tau = kNegInf;
+#pragma unroll 1
+  for (int slice = slice0, it = 0; slice < slice1 && !dead; ++slice, ++it) {
+    const int stage = it % kStages;
+    __syncthreads();  // the stage to fill has been read, and what was written by hand is there
+    fetch(slice + kStages - 1, (it + kStages - 1) % kStages);
+    if (!mbar_wait(bar + 8 * stage, it / kStages & 1)) l = NAN;  // a copy that never came: no candidates
+    const uint4* x = ring + stage * kStage + tid;
+    uint4 g[kGran];
+#pragma unroll
+    for (int r = 0; r < kGran; ++r) g[r] = x[r * kThreads];
+    if (off) {
+#pragma unroll
+      for (int r = 0; r < kGran; ++r) g[r] = shifted(g[r], x[r * kThreads + 1], off);
+    }
+    float top = kNegInf;
+#pragma unroll
+    for (int r = 0; r < kGran; ++r) top = fmaxf(top, granule_max<T>(g[r]));
+    if (top > m) {
+      l *= ex2((m - top) * kLog2e);
+      m = top;
+    }
+    const float mg = m == kNegInf ? 0.f : m;
+#pragma unroll
+    for (int r = 0; r < kGran; ++r) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) sum += ex2((elem<T>(g[r], i) - mg) * kLog2e);
+      l += sum;
+    }
+    if ((it & (it + 1)) == 0 || tau == kNegInf) {  // the bound so far
+      const int size = a.n_out <= 16 ? kThreads / 64 : kThreads / 256, n_sets = kThreads / size;
+      float set = m;
+      for (int o = 1; o < size; o <<= 1) set = fmaxf(set, __shfl_xor_sync(~0u, set, o));
+      if ((tid & (size - 1)) == 0) sh.sets[tid / size] = set;
+      __syncthreads();
+      if (tid < n_sets) {
+        int r = 0;
+        const float v = sh.sets[tid];
+#pragma unroll 4
+        for (int i = 0; i < n_sets; i += 4) {
+          const float4 y = *reinterpret_cast<const float4*>(sh.sets + i);
+          r += y.x > v || (y.x == v && i < tid);
+          r += y.y > v || (y.y == v && i + 1 < tid);
+          r += y.z > v || (y.z == v && i + 2 < tid);
+          r += y.w > v || (y.w == v && i + 3 < tid);
+        }
+        if (r == a.n_out - 1) sh.tau = v;
+      }
+      __syncthreads();
+      tau = sh.tau;
+    }
+    if (top >= tau) {
+      uint32_t hits = 0;
+#pragma unroll
+      for (int r = 0; r < kGran; ++r)
+#pragma unroll
+        for (int i = 0; i < E; ++i) hits |= (elem<T>(g[r], i) >= tau ? 1u : 0u) << (r * E + i);
+      while (hits) {
+        const int b = __ffs(hits) - 1, e = (b / E * kThreads + tid) * E + b % E;  // of the slice
+        hits &= hits - 1;
+        const float v = (float)(reinterpret_cast<const T*>(ring + stage * kStage))[e + mis];
+        if (v > kNegInf) {
+          const int at = atomicAdd(&sh.n, 1);
+          if (at < kList) sh.list[at] = make_key(v, (uint32_t)((int64_t)slice * a.slice + e));
+        }
+      }
+    }
   }
-  __syncthreads();
-  for (int r = sh_n + tid; r < a.n_out; r += kThreads) {  // places with no candidate
-    const int64_t to = (int64_t)group * a.n_out + r;
-    a.scores_out[to] = kNegInf;
-    a.parents[to] = r % a.n_beams;
-    a.tokens[to] = a.pad;
-    a.finished_out[to] = 1;
-  }
+  finish_part<T>(a, sh, row, (int64_t)slice0 * a.slice, min((int64_t)a.vocab, (int64_t)slice1 * a.slice), dead, m, l, tau);
 }
 
 }  // namespace
 
 int beam_slice(int32_t dtype) { return kThreads * kGran * (dtype == LC_F32 ? 4 : 8); }
 
-void launch_beam(const BeamArgs& a, cudaStream_t s) {
-  const dim3 grid((unsigned)a.slices, (unsigned)(a.n_groups * a.n_beams));
+void launch_beam(BeamArgs a, int device, int sms, cudaStream_t s) {
+  // as many parts a row as fill the card, of whole slices
+  const int rows = a.n_groups * a.n_beams, fill = std::max(1, kBeamPerSm * sms / rows);
+  a.per = (a.slices + fill - 1) / fill;
+  const dim3 grid((unsigned)((a.slices + a.per - 1) / a.per), (unsigned)rows);
+  constexpr int kRing = kStages * kStage * 16;
+  static_assert(kBeamPerSm * (kRing + (int)sizeof(BeamShared) + 1024) <= 228 * 1024, "the blocks fit an SM");
+  auto launch = [&](auto kernel, SmemOptIn& opt) {
+    opt(kernel, kRing, device);
+    kernel<<<grid, kThreads, kRing, s>>>(a);
+    LC_CUDA(cudaGetLastError());
+  };
+  static SmemOptIn f32, bf16, f16;
   if (a.dtype == LC_F32)
-    k_beam_select<float><<<grid, kThreads, 0, s>>>(a);
+    launch(k_beam_select<float>, f32);
   else if (a.dtype == LC_BF16)
-    k_beam_select<__nv_bfloat16><<<grid, kThreads, 0, s>>>(a);
+    launch(k_beam_select<__nv_bfloat16>, bf16);
   else
-    k_beam_select<__half><<<grid, kThreads, 0, s>>>(a);
-  LC_CUDA(cudaGetLastError());
+    launch(k_beam_select<__half>, f16);
 }
 
 }  // namespace lc

@@ -142,7 +142,7 @@ struct lc_paged {
 };
 
 struct lc_beam {
-  int32_t n_groups = 0, n_beams = 0, n_out = 0, device = 0;
+  int32_t n_groups = 0, n_beams = 0, n_out = 0, device = 0, sms = 0;
   int64_t vocab = 0;
   Order order;
   Workspace ws;
@@ -428,7 +428,7 @@ int lc_beam_create(int32_t n_groups, int32_t n_beams, int64_t vocab, int32_t n_o
     LC_REQUIRE(n_out >= 1 && n_out <= kBeamMaxOut, LC_ERR_INVALID, "n_out must be 1.." + std::to_string(kBeamMaxOut));
     LC_REQUIRE(vocab >= 1 && vocab < (1ll << 31) && (int64_t)n_beams * vocab < (1ll << 32), LC_ERR_INVALID,
                "vocab must be >= 1 and n_beams * vocab below 2^32");
-    const int64_t slices = (vocab + 7 + beam_slice(LC_F32) - 1) / beam_slice(LC_F32);
+    const int64_t slices = (vocab + beam_slice(LC_F32) - 1) / beam_slice(LC_F32);
     LC_REQUIRE(slices <= 256 && slices * n_out <= kBeamMaxMerge, LC_ERR_INVALID, "vocab too large for this n_out");
     DeviceScope scope(device);
     auto b = std::make_unique<lc_beam>();
@@ -437,18 +437,17 @@ int lc_beam_create(int32_t n_groups, int32_t n_beams, int64_t vocab, int32_t n_o
     b->n_out = n_out;
     b->device = device;
     b->vocab = vocab;
+    b->sms = sm_count(device);
     b->order.open();
     const size_t rows = (size_t)n_groups * n_beams, lists = rows * slices;
     const size_t keys = (lists + rows) * n_out;
     uint8_t* w = static_cast<uint8_t*>(
-        b->ws.get(keys * 8 + (2 * lists + lists + rows + rows + n_groups) * 4, true));
+        b->ws.get(keys * 8 + (2 * lists + rows + n_groups) * 4, true));
     BeamArgs& a = b->a;
     a.slice_key = reinterpret_cast<uint64_t*>(w);
     a.row_key = a.slice_key + lists * n_out;
     a.slice_stats = reinterpret_cast<float*>(a.row_key + rows * n_out);
-    a.slice_count = reinterpret_cast<int32_t*>(a.slice_stats + 2 * lists);
-    a.row_count = a.slice_count + lists;
-    a.counters = a.row_count + rows;
+    a.counters = reinterpret_cast<int32_t*>(a.slice_stats + 2 * lists);
     *out = b.release();
   });
 }
@@ -492,7 +491,7 @@ int lc_beam_select(lc_beam* b, int32_t n_groups, const void* logits, int32_t dty
     a.n_out = b->n_out;
     a.vocab = (int32_t)b->vocab;
     a.slice = beam_slice(dtype);
-    a.slices = (int32_t)((b->vocab + 7 + a.slice - 1) / a.slice);
+    a.slices = (int32_t)((b->vocab + a.slice - 1) / a.slice);
     a.scores = scores;
     a.finished = finished;
     a.eos = eos;
@@ -501,7 +500,7 @@ int lc_beam_select(lc_beam* b, int32_t n_groups, const void* logits, int32_t dty
     a.parents = parents;
     a.tokens = tokens;
     a.finished_out = finished_out;
-    launch_beam(a, b->order.on(stream));
+    launch_beam(a, b->device, b->sms, b->order.on(stream));
   });
 }
 

@@ -111,7 +111,7 @@ struct BeamArgs {
   const void* logits;
   int32_t dtype;
   int64_t row_stride;
-  int32_t n_groups, n_beams, n_out, vocab, slices, slice;
+  int32_t n_groups, n_beams, n_out, vocab, slices, slice, per;
   const float* scores;
   const uint8_t* finished;  // may be null
   int32_t eos, pad;
@@ -119,12 +119,10 @@ struct BeamArgs {
   int32_t* parents;
   int32_t* tokens;
   uint8_t* finished_out;
-  // workspace
+  // workspace, by the parts of a row (at most one a slice)
   float* slice_stats;    // [rows][slices][2]: max, sum exp(x - max)
-  int32_t* slice_count;  // [rows][slices]
-  uint64_t* slice_key;   // [rows][slices][n_out]: (logit, token), best first
-  uint64_t* row_key;     // [rows][n_out]: (total, flat index), best first
-  int32_t* row_count;    // [rows]
+  uint64_t* slice_key;   // [rows][slices][n_out]: (logit, token), best first, 0 for none
+  uint64_t* row_key;     // [rows][n_out]: (total, flat index), best first, 0 for none
   int32_t* counters;     // [rows + n_groups], zero between calls
 };
 
@@ -147,6 +145,6 @@ bool paged_evict_keys_in_smem(int64_t cap, int cluster);
 void launch_paged_evict(const PagedEvictArgs& a, int32_t device, int32_t sms, cudaStream_t s);
 void launch_paged_reorder(const PagedReorderArgs& a, int32_t sms, cudaStream_t s);
 int beam_slice(int32_t dtype);
-void launch_beam(const BeamArgs& a, cudaStream_t s);
+void launch_beam(BeamArgs a, int32_t device, int32_t sms, cudaStream_t s);
 
 }  // namespace lc
