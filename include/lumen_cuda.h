@@ -599,7 +599,7 @@ int lc_paged_reorder(lc_paged* p, int32_t n_groups, int32_t n_beams, const int32
 typedef struct lc_beam lc_beam;
 
 /* Workspace for lc_beam_select: up to n_groups groups of n_beams (<= 64) rows
- * of `vocab` logits, n_out (<= 64) chosen of each group. */
+ * of `vocab` (<= 2^24) logits, n_out (<= 64) chosen of each group. */
 int lc_beam_create(int32_t n_groups, int32_t n_beams, int64_t vocab, int32_t n_out, int32_t device, lc_beam** out);
 void lc_beam_destroy(lc_beam* b);
 

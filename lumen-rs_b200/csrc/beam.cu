@@ -8,19 +8,19 @@
 // n_out best.
 //
 // A block takes a part of a row (all of it where there are rows enough for the
-// card) slice by slice through a ring of shared memory that one thread fills
-// with bulk copies. Rows that begin off 16 bytes are put right as they are
-// read from the ring, so that a thread's logits, and with them the order of
-// the sums, do not depend on the row's address. A thread keeps a running
+// card) slice by slice through a ring of shared memory that one warp of its
+// own fills with bulk copies: while the memory is busy a copy's issue alone
+// takes some 900 cycles. Rows that begin off 16 bytes are put right as they
+// are read from the ring, so that a thread's logits, and with them the order
+// of the sums, do not depend on the row's address. A thread keeps a running
 // maximum and sum of its own. The n_out-th largest of the maxima of 64 (or
 // 256) disjoint sets of the logits so far is a lower bound of the n_out-th
-// largest: it is taken after 1, 2, 4 ... slices, and the logits that reach it,
-// some n_out for every doubling, are gathered, to be ranked by counting at the
-// end. The last part of a row to finish has the row's sum, turns the parts'
-// candidates into totals and ranks them; the last row of a group ranks the
-// rows' candidates and writes the answer. One launch; ranks are by value and
-// index only, so the order of arrival changes nothing. The chain of those
-// steps is what a small call takes, and a good half of a large one.
+// largest: it is taken after slices 1, 3, 8, 16 ... (only once: 51 us for 33
+// million logits; after 1, 2, 4, 8: 32; so: 31), and the logits that reach it
+// are gathered, to be ranked by counting at the end. The last block of a group turns all parts' candidates into totals,
+// ranks them and writes the answer. One launch; ranks are by value and index
+// only, so the order of arrival changes nothing. The chain of those steps is
+// what a small call takes, and a good half of a large one.
 #include <algorithm>
 
 #include "devutil.cuh"
@@ -29,7 +29,7 @@
 namespace lc {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 512;  // that compute; one more warp fetches
 constexpr int kWarps = kThreads / 32;
 constexpr int kGran = 2;      // 16-byte granules of a slice for each thread
 constexpr int kStages = 4;    // slices of the ring
@@ -107,33 +107,65 @@ __device__ __forceinline__ float granule_max<__half>(const uint4& r) {
   return fmaxf(f.x, f.y);
 }
 
+// a barrier of the computing threads
+__device__ __forceinline__ void sync_threads() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
+
+struct BeamShared {
+  uint64_t list[kBeamMaxMerge];  // a part's candidates, then the group's
+  uint64_t few[kThreads], best[kBeamMaxOut], warp_key[kWarps];
+  __align__(16) float sets[256];
+  float m[kWarps], l[kWarps], row_top[kBeamMaxBeams], row_log[kBeamMaxBeams];
+  float bound;
+  int n, last;
+};
+
 __device__ __forceinline__ uint64_t block_max_key(uint64_t k, uint64_t* warp_key) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     const uint64_t x = __shfl_xor_sync(~0u, k, o);
     k = x > k ? x : k;
   }
-  __syncthreads();
+  sync_threads();
   if ((threadIdx.x & 31) == 0) warp_key[threadIdx.x >> 5] = k;
-  __syncthreads();
+  sync_threads();
   k = warp_key[0];
 #pragma unroll
   for (int w = 1; w < kWarps; ++w) k = warp_key[w] > k ? warp_key[w] : k;
   return k;
 }
 
-// true in every thread of the block that arrives last of `of`
-__device__ __forceinline__ bool arrive_last(int* counter, int of, int& flag) {
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    __threadfence();  // the block's writes, which the barrier put before this thread
-    const bool last = atomicAdd(counter, 1) == of - 1;
-    if (last) *counter = 0;
-    __threadfence();
-    flag = last;
+// max and sum of (m, l) over a warp
+__device__ __forceinline__ void warp_softmax(float& m, float& l) {
+  float top = m;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  l *= ex2((m - (top == kNegInf ? 0.f : top)) * kLog2e);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+  m = top;
+}
+
+// A lower bound of the keep-th largest of the values whose maximum over this
+// thread's is x: the keep-th largest of the maxima of 64 or 256 sets of threads.
+__device__ __forceinline__ float set_bound(BeamShared& sh, float x, int keep) {
+  const int tid = threadIdx.x, size = keep <= 16 ? kThreads / 64 : kThreads / 256, n_sets = kThreads / size;
+  for (int o = 1; o < size; o <<= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
+  const int set = tid / size, sub = tid & (size - 1), span = n_sets / size;
+  if (sub == 0) sh.sets[set] = x;
+  sync_threads();
+  int r = 0;  // this thread counts over `span` of the sets
+#pragma unroll 2
+  for (int i = sub * span; i < (sub + 1) * span; i += 4) {
+    const float4 y = *reinterpret_cast<const float4*>(sh.sets + i);
+    r += y.x > x || (y.x == x && i < set);
+    r += y.y > x || (y.y == x && i + 1 < set);
+    r += y.z > x || (y.z == x && i + 2 < set);
+    r += y.w > x || (y.w == x && i + 3 < set);
   }
-  __syncthreads();
-  return flag;
+  for (int o = 1; o < size; o <<= 1) r += __shfl_xor_sync(~0u, r, o);
+  if (sub == 0 && r == keep - 1) sh.bound = x;
+  sync_threads();
+  return sh.bound;
 }
 
 // emit(key, rank) for the `keep` largest of list[0 .. n), all different, 0 for
@@ -154,57 +186,23 @@ __device__ __forceinline__ void rank_list(const uint64_t* list, int n, int keep,
   }
 }
 
-// max and sum of (m, l) over a warp
-__device__ __forceinline__ void warp_softmax(float& m, float& l) {
-  float top = m;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-  l *= ex2((m - (top == kNegInf ? 0.f : top)) * kLog2e);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
-  m = top;
-}
-
-struct BeamShared {
-  uint64_t list[kBeamMaxMerge];  // a part's candidates, then the merges'
-  uint64_t warp_key[kWarps];
-  uint64_t best[kBeamMaxOut];
-  __align__(16) float sets[256];
-  float m[kWarps], l[kWarps];
-  float tau, top, sum, log_sum;
-  int n, last;
-};
-
 // Ends a part, elements [i0, i1) of a row: its maximum, sum and best
-// candidates, then, as the last part of the row, the row's, and as the last row
-// of the group the answer. Block-wide.
+// candidates; then, in the last block of the group, the answer.
 template <typename T>
-__device__ __noinline__ void finish_part(const BeamArgs& a, BeamShared& sh, int row, int64_t i0, int64_t i1, bool dead,
-                                         float m, float l, float tau) {
+__device__ __noinline__ void finish(const BeamArgs& a, BeamShared& sh, int row, int64_t i0, int64_t i1, bool done,
+                                    bool dead, float m, float l, float tau) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int group = row / a.n_beams, beam = row - group * a.n_beams, parts = gridDim.x;
-  const int64_t slot0 = (int64_t)row * a.slices, slot = slot0 + blockIdx.x;
-  const float score = a.scores[row];
-  uint64_t* row_key = a.row_key + (int64_t)row * a.n_out;
-  const uint32_t index0 = (uint32_t)(beam * (int64_t)a.vocab);
-  // the best candidates of the row (logits: keys by token) as totals, into row_key
-  auto totals = [&](uint64_t* list, int n, float top, float log_sum) {
-    for (int c = tid; c < n; c += kThreads) {
-      uint64_t k = list[c];
-      if (k) {  // two logits may round to the same total
-        const float z = score + ((key_value(k) - top) - log_sum);
-        k = z > kNegInf ? make_key(z, index0 + key_index(k)) : 0;
-      }
-      list[c] = k;
-    }
-    for (int c = tid; c < a.n_out; c += kThreads) row_key[c] = 0;
-    __syncthreads();
-    rank_list(list, n, a.n_out, [&](uint64_t k, int r) { row_key[r] = k; });
-  };
+  const int group = row / a.n_beams, parts = gridDim.x;
+  const int64_t slot = (int64_t)row * parts + blockIdx.x;
+  uint64_t* keys = a.slice_key + slot * a.n_out;
   if (dead) {
-    if (blockIdx.x == 0)
-      for (int c = tid; c < a.n_out; c += kThreads)
-        row_key[c] = c == 0 && score > kNegInf && a.finished && a.finished[row] ? make_key(score, index0 + a.pad) : 0;
+    // a finished row's only total is its score: of one logit, 0, of a sum of 1
+    const bool one = done && blockIdx.x == 0;
+    for (int c = tid; c < a.n_out; c += kThreads) keys[c] = one && c == 0 ? make_key(0.f, a.pad) : 0;
+    if (tid == 0) {
+      a.slice_stats[2 * slot] = one ? 0.f : kNegInf;
+      a.slice_stats[2 * slot + 1] = one ? 1.f : 0.f;
+    }
   } else {
     warp_softmax(m, l);
     if (lane == 0) {
@@ -212,15 +210,14 @@ __device__ __noinline__ void finish_part(const BeamArgs& a, BeamShared& sh, int 
       sh.l[warp] = l;
     }
     for (int c = tid; c < a.n_out; c += kThreads) sh.best[c] = 0;
-    __syncthreads();
+    sync_threads();
     if (warp == kWarps - 1) {
       m = lane < kWarps ? sh.m[lane] : kNegInf;
       l = lane < kWarps ? sh.l[lane] : 0.f;
       warp_softmax(m, l);
       if (lane == 0) {
-        sh.top = m;
-        sh.sum = l;
-        sh.log_sum = logf(l);
+        a.slice_stats[2 * slot] = m;
+        a.slice_stats[2 * slot + 1] = l;
       }
     }
     const int found = sh.n;
@@ -242,54 +239,77 @@ __device__ __noinline__ void finish_part(const BeamArgs& a, BeamShared& sh, int 
         if (tid == 0) sh.best[o] = before;
       }
     }
-    __syncthreads();
-    if (parts == 1) {
-      totals(sh.best, a.n_out, sh.top, sh.log_sum);
-    } else {
-      for (int c = tid; c < a.n_out; c += kThreads) a.slice_key[slot * a.n_out + c] = sh.best[c];
-      if (tid == 0) {
-        a.slice_stats[2 * slot] = sh.top;
-        a.slice_stats[2 * slot + 1] = sh.sum;
-      }
-    }
+    sync_threads();
+    for (int c = tid; c < a.n_out; c += kThreads) keys[c] = sh.best[c];
   }
 
-  // the row
-  if (parts > 1) {
-    if (!arrive_last(a.counters + row, parts, sh.last)) return;
-    if (!dead) {
-      const int all = parts * a.n_out;
-      if (warp == kWarps - 1) {  // max and sum over the parts
-        m = kNegInf;
-        l = 0.f;
-        for (int i = lane; i < parts; i += 32) {
-          const float mi = __ldcg(a.slice_stats + 2 * (slot0 + i)), li = __ldcg(a.slice_stats + 2 * (slot0 + i) + 1);
-          const float mn = fmaxf(m, mi), mg = mn == kNegInf ? 0.f : mn;
-          l = l * ex2((m - mg) * kLog2e) + li * ex2((mi - mg) * kLog2e);
-          m = mn;
-        }
-        warp_softmax(m, l);
-        if (lane == 0) {
-          sh.top = m;
-          sh.log_sum = logf(l);
-        }
-      }
-      for (int c = tid; c < all; c += kThreads) sh.list[c] = __ldcg(a.slice_key + slot0 * a.n_out + c);
-      __syncthreads();
-      totals(sh.list, all, sh.top, sh.log_sum);
+  // the last block of the group goes on
+  const int64_t row0 = (int64_t)group * a.n_beams, slot0 = row0 * parts, out0 = (int64_t)group * a.n_out;
+  sync_threads();
+  if (tid == 0) {
+    const int of = a.n_beams * parts;
+    __threadfence();  // the block's writes, which the barrier put before this thread
+    sh.last = atomicAdd(a.counters + group, 1) == of - 1;
+    if (sh.last) {
+      __threadfence();
+      a.counters[group] = 0;
     }
+    sh.n = 0;
   }
-
-  // the group
-  if (a.n_beams > 1 && !arrive_last(a.counters + a.n_groups * a.n_beams + group, a.n_beams, sh.last)) return;
-  const int64_t row0 = (int64_t)group * a.n_beams, out0 = (int64_t)group * a.n_out;
-  const int all = a.n_beams * a.n_out;
-  __syncthreads();
-  for (int c = tid; c < all; c += kThreads) sh.list[c] = __ldcg(a.row_key + row0 * a.n_out + c);
+  sync_threads();
+  if (!sh.last) return;
+  const int per_row = parts * a.n_out, all = a.n_beams * per_row;
+  for (int c = tid; c < all; c += kThreads) sh.list[c] = __ldcg(a.slice_key + slot0 * a.n_out + c);
   for (int c = tid; c < a.n_out; c += kThreads) sh.best[c] = 0;
-  __syncthreads();
-  rank_list(sh.list, all, a.n_out, [&](uint64_t k, int r) { sh.best[r] = k; });
-  __syncthreads();
+  for (int b = warp; b < a.n_beams; b += kWarps) {  // the rows' maxima and sums
+    m = kNegInf;
+    l = 0.f;
+    for (int i = lane; i < parts; i += 32) {
+      const float* st = a.slice_stats + 2 * (slot0 + (int64_t)b * parts + i);
+      const float mi = __ldcg(st), li = __ldcg(st + 1);
+      const float mn = fmaxf(m, mi), mg = mn == kNegInf ? 0.f : mn;
+      l = l * ex2((m - mg) * kLog2e) + li * ex2((mi - mg) * kLog2e);
+      m = mn;
+    }
+    warp_softmax(m, l);
+    if (lane == 0) {
+      sh.row_top[b] = m;
+      sh.row_log[b] = logf(l);
+    }
+  }
+  sync_threads();
+  float top = kNegInf;
+  for (int c = tid; c < all; c += kThreads) {
+    uint64_t k = sh.list[c];
+    if (k) {
+      const int b = c / per_row;
+      const float z = a.scores[row0 + b] + ((key_value(k) - sh.row_top[b]) - sh.row_log[b]);
+      k = z > kNegInf ? make_key(z, (uint32_t)(b * (int64_t)a.vocab + key_index(k))) : 0;
+      if (k) top = fmaxf(top, z);
+    }
+    sh.list[c] = k;
+  }
+  const uint64_t* list = sh.list;
+  int n = all;
+  if (all > kThreads) {  // those that reach a bound
+    const float bound = set_bound(sh, top, a.n_out);
+    for (int c = tid; c < all; c += kThreads) {
+      const uint64_t k = sh.list[c];
+      if (k && key_value(k) >= bound) {
+        const int at = atomicAdd(&sh.n, 1);
+        if (at < kThreads) sh.few[at] = k;
+      }
+    }
+    sync_threads();
+    if (sh.n <= kThreads) {
+      list = sh.few;
+      n = sh.n;
+    }
+  } else {
+    sync_threads();
+  }
+  rank_list(list, n, a.n_out, [&](uint64_t k, int r) { sh.best[r] = k; });
+  sync_threads();
   for (int r = tid; r < a.n_out; r += kThreads) {
     const uint64_t k = sh.best[r];
     const uint32_t index = key_index(k);
@@ -304,66 +324,83 @@ __device__ __noinline__ void finish_part(const BeamArgs& a, BeamShared& sh, int 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, kBeamPerSm) k_beam_select(const __grid_constant__ BeamArgs a) {
+__global__ void __launch_bounds__(kThreads + 32, kBeamPerSm) k_beam_select(const __grid_constant__ BeamArgs a) {
   constexpr int E = 16 / sizeof(T);
   extern __shared__ __align__(16) uint4 ring[];  // [kStages][kStage]
   __shared__ BeamShared sh;
-  __shared__ uint64_t bars[kStages];
+  __shared__ uint64_t bars[2 * kStages];  // full, then empty
   const int tid = threadIdx.x, row = blockIdx.y;
-  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), bar = (uint32_t)__cvta_generic_to_shared(bars);
-  const int slice0 = blockIdx.x * a.per, slice1 = min(a.slices, slice0 + a.per);
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), full = (uint32_t)__cvta_generic_to_shared(bars);
+  const uint32_t empty = full + 8 * kStages;
+  const int slice0 = blockIdx.x * a.per, slices = min(a.slices, slice0 + a.per) - slice0;
   const float score = a.scores[row];
   const uint8_t done = a.finished ? a.finished[row] : 0;
   // the row's first element sits at base[mis]: base is 16-byte aligned
   const T* x0 = static_cast<const T*>(a.logits) + row * a.row_stride;
   const int mis = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T)), off = mis * (int)sizeof(T);
-  const T* base = x0 - mis;
-  const int64_t i_end = mis + (int64_t)a.vocab;
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) mbar_init(bar + 8 * i, 1);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, kWarps);
+    }
     mbar_init_fence();
     sh.n = 0;
   }
   __syncthreads();
-  // slice `slice` into a stage: its whole granules by one bulk copy; those at
-  // the row's ends by hand, -inf where there is no logit
-  auto fetch = [&](int slice, int stage) {
-    if (slice >= slice1) return;
-    const int64_t at0 = (int64_t)slice * a.slice;
-    const int n = kGran * kThreads + (mis ? 1 : 0);
-    const int lo = mis && slice == 0 ? 1 : 0, hi = (int)min((int64_t)n, (i_end - at0) / E);
-    if (tid == 0) {
-      const int bytes = hi > lo ? (hi - lo) * 16 : 0;
-      mbar_expect_tx(bar + 8 * stage, bytes);
-      if (bytes) bulk_g2s(ring_at + (stage * kStage + lo) * 16, base + at0 + lo * E, bytes, bar + 8 * stage);
-    }
-    if (lo > 0 || hi < n) {
-#pragma unroll 1
-      for (int v = tid; v < n; v += kThreads) {
-        if (v >= lo && v < hi) continue;
-        const int64_t at = at0 + v * E;
-        alignas(16) T part[E];
+
+  if (tid >= kThreads) {
+    // The fetching warp: a slice's whole granules by one bulk copy; those at the
+    // row's ends by hand, -inf where there is no logit.
+    const int lane = tid & 31;
+    const T* base = x0 - mis;
+    const int64_t i_end = mis + (int64_t)a.vocab;
+    int it = 0;
+    for (; it < slices; ++it) {
+      const int stage = it % kStages;
+      // the ring's first slices are asked for before it is known whether they matter
+      if (it >= kStages && (done || !(score > kNegInf) || !mbar_wait(empty + 8 * stage, (it / kStages - 1) & 1))) break;
+      const int64_t at0 = (int64_t)(slice0 + it) * a.slice;
+      const int n = kGran * kThreads + (mis ? 1 : 0);
+      const int lo = mis && slice0 + it == 0 ? 1 : 0, hi = (int)min((int64_t)n, (i_end - at0) / E);
+      if (lo > 0 || hi < n) {
+        for (int v = lane; v < n; v += 32) {
+          if (v >= lo && v < hi) {
+            v += (hi - v) / 32 * 32;  // the copy's
+            if (v < hi) continue;
+          }
+          if (v >= n) break;
+          const int64_t at = at0 + v * E;
+          alignas(16) T part[E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) part[i] = at + i >= mis && at + i < i_end ? base[at + i] : T(kNegInf);
-        ring[stage * kStage + v] = *reinterpret_cast<uint4*>(part);
+          for (int i = 0; i < E; ++i) part[i] = T(kNegInf);
+          if (at < i_end)
+            for (int i = 0; i < E; ++i)
+              if (at + i >= mis && at + i < i_end) part[i] = base[at + i];
+          ring[stage * kStage + v] = *reinterpret_cast<uint4*>(part);
+        }
+        fence_proxy_async();  // a later slice's bulk copy may write there
+        __syncwarp();
       }
-      fence_proxy_async();  // a later slice's bulk copy may write there
+      if (lane == 0) {
+        const int bytes = hi > lo ? (hi - lo) * 16 : 0;
+        mbar_expect_tx(full + 8 * stage, bytes);
+        if (bytes) bulk_g2s(ring_at + (stage * kStage + lo) * 16, base + at0 + lo * E, bytes, full + 8 * stage);
+      }
+      __syncwarp();
     }
-  };
-#pragma unroll 1
-  for (int i = 0; i < kStages - 1; ++i) fetch(slice0 + i, i);
-  // a finished row's logits, or those of a beam that is out, do not matter (the
-  // first slices were asked for before that was known: they are awaited)
+    // where no one else does, await the copies in flight
+    if (done || !(score > kNegInf))
+      for (int i = 0; i < it; ++i) mbar_wait(full + 8 * i, 0);
+    return;
+  }
+
+  // a finished row's logits, or those of a beam that is out, do not matter
   const bool dead = done || !(score > kNegInf);
-  if (dead)
-    for (int i = 0; i < kStages - 1 && slice0 + i < slice1; ++i) mbar_wait(bar + 8 * i, 0);
   float m = kNegInf, l = 0.f, tau = kNegInf;
 #pragma unroll 1
-  for (int slice = slice0, it = 0; slice < slice1 && !dead; ++slice, ++it) {
+  for (int it = 0; it < slices && !dead; ++it) {
     const int stage = it % kStages;
-    __syncthreads();  // the stage to fill has been read, and what was written by hand is there
-    fetch(slice + kStages - 1, (it + kStages - 1) % kStages);
-    if (!mbar_wait(bar + 8 * stage, it / kStages & 1)) l = NAN;  // a copy that never came: no candidates
+    if (!mbar_wait(full + 8 * stage, it / kStages & 1)) l = NAN;  // a copy that never came: no candidates
     const uint4* x = ring + stage * kStage + tid;
     uint4 g[kGran];
 #pragma unroll
@@ -387,28 +424,7 @@ __global__ void __launch_bounds__(kThreads, kBeamPerSm) k_beam_select(const __gr
       for (int i = 0; i < E; ++i) sum += ex2((elem<T>(g[r], i) - mg) * kLog2e);
       l += sum;
     }
-    if ((it & (it + 1)) == 0 || tau == kNegInf) {  // the bound so far
-      const int size = a.n_out <= 16 ? kThreads / 64 : kThreads / 256, n_sets = kThreads / size;
-      float set = m;
-      for (int o = 1; o < size; o <<= 1) set = fmaxf(set, __shfl_xor_sync(~0u, set, o));
-      if ((tid & (size - 1)) == 0) sh.sets[tid / size] = set;
-      __syncthreads();
-      if (tid < n_sets) {
-        int r = 0;
-        const float v = sh.sets[tid];
-#pragma unroll 4
-        for (int i = 0; i < n_sets; i += 4) {
-          const float4 y = *reinterpret_cast<const float4*>(sh.sets + i);
-          r += y.x > v || (y.x == v && i < tid);
-          r += y.y > v || (y.y == v && i + 1 < tid);
-          r += y.z > v || (y.z == v && i + 2 < tid);
-          r += y.w > v || (y.w == v && i + 3 < tid);
-        }
-        if (r == a.n_out - 1) sh.tau = v;
-      }
-      __syncthreads();
-      tau = sh.tau;
-    }
+    if (it == 0 || it == 2 || (it & 7) == 7 || tau == kNegInf) tau = set_bound(sh, m, a.n_out);
     if (top >= tau) {
       uint32_t hits = 0;
 #pragma unroll
@@ -421,12 +437,15 @@ __global__ void __launch_bounds__(kThreads, kBeamPerSm) k_beam_select(const __gr
         const float v = (float)(reinterpret_cast<const T*>(ring + stage * kStage))[e + mis];
         if (v > kNegInf) {
           const int at = atomicAdd(&sh.n, 1);
-          if (at < kList) sh.list[at] = make_key(v, (uint32_t)((int64_t)slice * a.slice + e));
+          if (at < kList) sh.list[at] = make_key(v, (uint32_t)((int64_t)(slice0 + it) * a.slice + e));
         }
       }
     }
+    __syncwarp();
+    if ((tid & 31) == 0) mbar_arrive(empty + 8 * stage);
   }
-  finish_part<T>(a, sh, row, (int64_t)slice0 * a.slice, min((int64_t)a.vocab, (int64_t)slice1 * a.slice), dead, m, l, tau);
+  finish<T>(a, sh, row, (int64_t)slice0 * a.slice, min((int64_t)a.vocab, (int64_t)(slice0 + slices) * a.slice), done, dead,
+            m, l, tau);
 }
 
 }  // namespace
@@ -434,15 +453,17 @@ __global__ void __launch_bounds__(kThreads, kBeamPerSm) k_beam_select(const __gr
 int beam_slice(int32_t dtype) { return kThreads * kGran * (dtype == LC_F32 ? 4 : 8); }
 
 void launch_beam(BeamArgs a, int device, int sms, cudaStream_t s) {
-  // as many parts a row as fill the card, of whole slices
+  // as many parts a row as fill the card, of whole slices, their candidates at
+  // most two for each thread of the block that ranks a group's
   const int rows = a.n_groups * a.n_beams, fill = std::max(1, kBeamPerSm * sms / rows);
-  a.per = (a.slices + fill - 1) / fill;
+  const int most = std::max(1, 2 * kThreads / (a.n_beams * a.n_out));
+  a.per = (a.slices + std::min(fill, most) - 1) / std::min(fill, most);
   const dim3 grid((unsigned)((a.slices + a.per - 1) / a.per), (unsigned)rows);
   constexpr int kRing = kStages * kStage * 16;
   static_assert(kBeamPerSm * (kRing + (int)sizeof(BeamShared) + 1024) <= 228 * 1024, "the blocks fit an SM");
   auto launch = [&](auto kernel, SmemOptIn& opt) {
     opt(kernel, kRing, device);
-    kernel<<<grid, kThreads, kRing, s>>>(a);
+    kernel<<<grid, kThreads + 32, kRing, s>>>(a);
     LC_CUDA(cudaGetLastError());
   };
   static SmemOptIn f32, bf16, f16;

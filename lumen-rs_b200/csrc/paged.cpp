@@ -426,10 +426,8 @@ int lc_beam_create(int32_t n_groups, int32_t n_beams, int64_t vocab, int32_t n_o
     LC_REQUIRE(n_groups >= 1 && n_beams >= 1 && n_beams <= kBeamMaxBeams && (int64_t)n_groups * n_beams <= 65535,
                LC_ERR_INVALID, "n_beams must be 1.." + std::to_string(kBeamMaxBeams) + " and the rows at most 65535");
     LC_REQUIRE(n_out >= 1 && n_out <= kBeamMaxOut, LC_ERR_INVALID, "n_out must be 1.." + std::to_string(kBeamMaxOut));
-    LC_REQUIRE(vocab >= 1 && vocab < (1ll << 31) && (int64_t)n_beams * vocab < (1ll << 32), LC_ERR_INVALID,
-               "vocab must be >= 1 and n_beams * vocab below 2^32");
+    LC_REQUIRE(vocab >= 1 && vocab <= (1 << 24), LC_ERR_INVALID, "vocab must be 1..2^24");
     const int64_t slices = (vocab + beam_slice(LC_F32) - 1) / beam_slice(LC_F32);
-    LC_REQUIRE(slices <= 256 && slices * n_out <= kBeamMaxMerge, LC_ERR_INVALID, "vocab too large for this n_out");
     DeviceScope scope(device);
     auto b = std::make_unique<lc_beam>();
     b->n_groups = n_groups;
@@ -439,14 +437,13 @@ int lc_beam_create(int32_t n_groups, int32_t n_beams, int64_t vocab, int32_t n_o
     b->vocab = vocab;
     b->sms = sm_count(device);
     b->order.open();
-    const size_t rows = (size_t)n_groups * n_beams, lists = rows * slices;
-    const size_t keys = (lists + rows) * n_out;
-    uint8_t* w = static_cast<uint8_t*>(
-        b->ws.get(keys * 8 + (2 * lists + rows + n_groups) * 4, true));
+    // a row has at most one part a slice, and a group no more candidates than one merge takes
+    const size_t rows = (size_t)n_groups * n_beams;
+    const size_t lists = rows * std::min<int64_t>(slices, std::max(1, kBeamMaxMerge / (n_beams * n_out)));
+    uint8_t* w = static_cast<uint8_t*>(b->ws.get(lists * n_out * 8 + (2 * lists + n_groups) * 4, true));
     BeamArgs& a = b->a;
     a.slice_key = reinterpret_cast<uint64_t*>(w);
-    a.row_key = a.slice_key + lists * n_out;
-    a.slice_stats = reinterpret_cast<float*>(a.row_key + rows * n_out);
+    a.slice_stats = reinterpret_cast<float*>(a.slice_key + lists * n_out);
     a.counters = reinterpret_cast<int32_t*>(a.slice_stats + 2 * lists);
     *out = b.release();
   });

@@ -120,10 +120,9 @@ struct BeamArgs {
   int32_t* tokens;
   uint8_t* finished_out;
   // workspace, by the parts of a row (at most one a slice)
-  float* slice_stats;    // [rows][slices][2]: max, sum exp(x - max)
-  uint64_t* slice_key;   // [rows][slices][n_out]: (logit, token), best first, 0 for none
-  uint64_t* row_key;     // [rows][n_out]: (total, flat index), best first, 0 for none
-  int32_t* counters;     // [rows + n_groups], zero between calls
+  float* slice_stats;   // [rows][parts][2]: max, sum exp(x - max)
+  uint64_t* slice_key;  // [rows][parts][n_out]: (logit, token), best first, 0 for none
+  int32_t* counters;    // [n_groups], zero between calls
 };
 
 constexpr int kPagedMaxSeqs = 2048;
