@@ -349,80 +349,94 @@ __global__ void __launch_bounds__(256, 4) k_paged_move(const PagedEvictArgs a) {
   move_pairs<U, kMoveBatch, 8>(a, blockIdx.x, a.pairs[blockIdx.x], blockIdx.y * 8 + (threadIdx.x >> 5), gridDim.y * 8);
 }
 
-// Reordering: block (row j, share of the copies). Every block works out the
-// group's mapping (who inherits which tail page) from the parents; a row's
-// first block writes its table, and where row j is a later child of its
-// parent, its blocks copy the first `fill` slots of the parent's tail page
-// into the spare tail page that it takes, four units a thread at a time.
+// Reordering: block (group, share). Every block works out the group's mapping
+// from the parents: the first child of a beam inherits its tail page, the i-th
+// later child takes that of the i-th beam without children. The tables and the
+// copies of the tail pages' first `fill` slots are shared out over the group's
+// blocks, so that they all have the same to do however the parents fall.
+constexpr int kReorderThreads = 256, kReorderUnroll = 8, kReorderChunk = 32 * kReorderUnroll * 2;
 template <typename U>
-__global__ void __launch_bounds__(256) k_paged_reorder(const PagedReorderArgs a) {
-  __shared__ int parent[kBeamMaxBeams], first[kBeamMaxBeams];
-  __shared__ int owner;
-  const int tid = threadIdx.x, w = a.n_beams;
-  const int row = blockIdx.x, g = row / w, j = row - g * w;
+__global__ void __launch_bounds__(kReorderThreads) k_paged_reorder(const PagedReorderArgs a) {
+  __shared__ int parent[kBeamMaxBeams], first[kBeamMaxBeams], owner[kBeamMaxBeams], spare[kBeamMaxBeams];
+  __shared__ int64_t src[kBeamMaxBeams], dst[kBeamMaxBeams];
+  __shared__ int extra_below, spare_below, n_copies;  // of the first 32 beams; of all
+  const int tid = threadIdx.x, lane = tid & 31, w = a.n_beams, g = blockIdx.x;
   const int cap = a.c.width * a.c.page_tokens;
-  int n = a.c.lens[g];
-  if (n < 0 || n > cap) {
-    *a.c.status = 1;
-    n = n < 0 ? 0 : cap;
-  }
-  int p = -1;
+  const int32_t* tables = a.c.tables + (int64_t)g * w * a.c.width;
+  int n = a.c.lens[g], p = 0;
   if (tid < w) {
-    first[tid] = INT32_MAX;
     p = a.parents[(int64_t)g * w + tid];
     if (p < 0 || p >= w) {
       *a.c.status = 1;
       p = tid;
     }
     parent[tid] = p;
+    first[tid] = INT32_MAX;
+  }
+  if (n < 0 || n > cap) {
+    *a.c.status = 1;
+    n = n < 0 ? 0 : cap;
   }
   __syncthreads();
   if (tid < w) atomicMin(&first[p], tid);
   __syncthreads();
-  p = parent[j];
-  if (first[p] != j && tid == 0) {  // the i-th later child takes the i-th childless beam's tail
-    int i = 0, own = -1;
-    for (int x = 0; x < j; ++x) i += first[parent[x]] != x;
-    while (i >= 0) i -= first[++own] == INT32_MAX;
-    owner = own;
-  } else if (tid == 0) {
-    owner = p;
+  const int full = n / a.c.page_tokens, fill = n - full * a.c.page_tokens;
+  if (tid < kBeamMaxBeams) {  // two warps: the i-th later child, the i-th childless beam
+    const bool extra = tid < w && first[p] != tid, childless = tid < w && first[tid] == INT32_MAX;
+    const uint32_t e = __ballot_sync(~0u, extra), s = __ballot_sync(~0u, childless), below = (1u << lane) - 1;
+    if (tid == 0) {
+      extra_below = __popc(e);
+      spare_below = __popc(s);
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(kBeamMaxBeams) : "memory");
+    const int at = __popc(e & below) + (tid >= 32 ? extra_below : 0);
+    if (childless) spare[__popc(s & below) + (tid >= 32 ? spare_below : 0)] = tid;
+    if (tid == kBeamMaxBeams - 1) n_copies = extra_below + __popc(e);
+    asm volatile("bar.sync 1, %0;" ::"n"(kBeamMaxBeams) : "memory");
+    if (tid < w) owner[tid] = extra ? spare[at] : p;
+    if (extra && fill > 0) {
+      const int from = tables[(int64_t)p * a.c.width + full], to = tables[(int64_t)spare[at] * a.c.width + full];
+      const bool bad = from < 0 || from >= a.c.n_pages || to < 0 || to >= a.c.n_pages;
+      if (bad) *a.c.status = 1;
+      src[at] = bad ? -1 : from * a.c.page;
+      dst[at] = to * a.c.page;
+    }
   }
   __syncthreads();
-  const int own = owner;
-  const int full = n / a.c.page_tokens, fill = n - full * a.c.page_tokens;
-  const int32_t* tables = a.c.tables + (int64_t)g * w * a.c.width;
-  if (blockIdx.y == 0)
-    for (int i = tid; i < a.c.width; i += 256) {
-      const int from = i < full ? p : i == full && fill > 0 ? own : j;
-      a.tables_out[(int64_t)row * a.c.width + i] = tables[(int64_t)from * a.c.width + i];
-    }
-  if (own == p || fill == 0) return;
-  const int src = tables[(int64_t)p * a.c.width + full], dst = tables[(int64_t)own * a.c.width + full];
-  if (src < 0 || src >= a.c.n_pages || dst < 0 || dst >= a.c.n_pages) {
-    if (tid == 0) *a.c.status = 1;
-    return;
+  for (int x = blockIdx.y * kReorderThreads + tid; x < w * a.c.width; x += gridDim.y * kReorderThreads) {
+    const int j = x / a.c.width, i = x - j * a.c.width;
+    const int from = i < full ? parent[j] : i == full && fill > 0 ? owner[j] : j;
+    a.tables_out[(int64_t)g * w * a.c.width + x] = tables[(int64_t)from * a.c.width + i];
   }
-  // the copy's rows, (layer, K or V, head, slot), shared out evenly
-  const uint32_t units = a.c.d, per_head = units * fill, per_pool = per_head * a.c.hkv;
-  const int64_t total = (int64_t)per_pool * 2 * a.c.n_layers, step = (int64_t)gridDim.y * 256;
-  for (int64_t x0 = (int64_t)blockIdx.y * 256 + tid; x0 < total; x0 += 4 * step) {
-    U got[4];
-    U* to[4];
+  if (fill == 0) return;
+  // the copies' chunks: (copy, layer, K or V, head, chunk of its slots' units), a warp each
+  const int units = a.c.d, per_head = units * fill, chunks = (per_head + kReorderChunk - 1) / kReorderChunk;
+  const int64_t total = (int64_t)n_copies * a.c.n_layers * 2 * a.c.hkv * chunks;
+  const bool packed = a.c.token == units;
+  for (int64_t x = (int64_t)blockIdx.y * (kReorderThreads / 32) + (tid >> 5); x < total;
+       x += (int64_t)gridDim.y * (kReorderThreads / 32)) {
+    const int64_t item = x / chunks;
+    const int chunk = (int)(x - item * chunks), pool = (int)(item / a.c.hkv), h = (int)(item - (int64_t)pool * a.c.hkv);
+    const int copy = pool / (2 * a.c.n_layers), lp = pool - copy * 2 * a.c.n_layers;
+    if (src[copy] < 0) continue;
+    U* base = static_cast<U*>(lp & 1 ? a.c.v : a.c.k) + (lp >> 1) * a.c.layer + h * a.c.head;
+    const U* from = base + src[copy];
+    U* to = base + dst[copy];
+    const int end = min(per_head, (chunk + 1) * kReorderChunk);
+    for (int z0 = chunk * kReorderChunk + lane; z0 < end; z0 += 32 * kReorderUnroll) {
+      U got[kReorderUnroll];
+      auto at = [&](int z) -> int64_t {
+        if (packed) return z;
+        const int t = z / units;
+        return t * a.c.token + (z - t * units);
+      };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t x = x0 + i * step;
-      to[i] = nullptr;
-      if (x >= total) continue;
-      const uint32_t lp = (uint32_t)(x / per_pool), y = (uint32_t)(x - (int64_t)lp * per_pool);
-      const uint32_t h = y / per_head, z = y - h * per_head, t = z / units, c = z - t * units;
-      U* base = static_cast<U*>(lp & 1 ? a.c.v : a.c.k) + (lp >> 1) * a.c.layer + h * a.c.head + t * a.c.token + c;
-      got[i] = base[src * a.c.page];
-      to[i] = base + dst * a.c.page;
+      for (int i = 0; i < kReorderUnroll; ++i)
+        if (z0 + 32 * i < end) got[i] = from[at(z0 + 32 * i)];
+#pragma unroll
+      for (int i = 0; i < kReorderUnroll; ++i)
+        if (z0 + 32 * i < end) to[at(z0 + 32 * i)] = got[i];
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (to[i]) *to[i] = got[i];
   }
 }
 
@@ -494,11 +508,12 @@ void launch_evict(PagedEvictArgs a, int device, int sms, cudaStream_t s) {
 template <typename U>
 void launch_reorder(PagedReorderArgs a, int sms, cudaStream_t s) {
   a.c = in_units<U>(a.c, a.esize);
-  // blocks a row: enough that one row in four copying fills the card, and none with less than 16 units a thread
-  const int64_t rows = (int64_t)a.n_groups * a.n_beams;
-  const int64_t units = 2ll * a.c.n_layers * a.c.hkv * a.c.page_tokens * a.c.d;
-  const int64_t y = std::max<int64_t>(1, std::min<int64_t>((units + 4095) / 4096, (32ll * sms + rows - 1) / rows));
-  k_paged_reorder<U><<<dim3((unsigned)rows, (unsigned)std::min<int64_t>(y, 65535)), 256, 0, s>>>(a);
+  // blocks of a group: all groups' as many as run at once, no more than every
+  // warp has a chunk where every beam but one is copied
+  const int64_t chunks = (a.c.page_tokens * (int64_t)a.c.d + kReorderChunk - 1) / kReorderChunk;
+  const int64_t all = 2 * chunks * a.c.n_layers * a.c.hkv * std::max(1, a.n_beams - 1);
+  const int64_t y = std::min<int64_t>((all + 7) / 8, (8ll * sms + a.n_groups - 1) / a.n_groups);
+  k_paged_reorder<U><<<dim3((unsigned)a.n_groups, (unsigned)std::min<int64_t>(y, 65535)), kReorderThreads, 0, s>>>(a);
 }
 
 }  // namespace
