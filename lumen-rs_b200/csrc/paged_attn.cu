@@ -217,40 +217,43 @@ __device__ void finish_segment(const PagedAttnArgs& a, const Segment& g, int hg_
   }
   if (g.parts > 1) {
     int* counter = a.counters + (int64_t)g.s * a.c.hkv * hg_n + g.hh;
-    __threadfence();
     __syncthreads();
-    if (tid == 0) {
+    if (tid == THREADS - 1) {  // a thread without loads in flight, which a fence would wait for
+      __threadfence();         // the block's writes, which the barrier put before this thread
       last = atomicAdd(counter, 1) == g.parts - 1;
-      if (last) *counter = 0;
+      if (last) {
+        *counter = 0;
+        __threadfence();
+      }
     }
     __syncthreads();
     if (last) {
-      __threadfence();
-      auto slot = [&](int b) { return a.part + (b == 0 ? g.slot0 : 2 * (g.first + b)) * kSlot; };
+      // In few instructions rather than unrolled: they are fetched for this one
+      // time (74 parts took 20 to 30 us with all loads of a thread unrolled).
+      const float* first_part = a.part + g.slot0 * kSlot;
+      const float* parts = a.part + 2 * g.first * kSlot;  // + 2 b kSlot: part b > 0
       for (int i = warp; i < nh; i += W) {
-        constexpr int kEach = (kPagedMaxBlocks + 31) / 32;  // parts a lane: all their loads at once
-        float m = kNegInf, l = 0.f, ms[kEach], ls[kEach];
-#pragma unroll
-        for (int b = 0; b < kEach; ++b) {
-          const bool in = b * 32 + lane < g.parts;
-          const float* from = slot(in ? b * 32 + lane : 0) + i;
-          ms[b] = in ? __ldcg(from) : kNegInf;
-          ls[b] = in ? __ldcg(from + GP) : 0.f;
+        float m = kNegInf, l = 0.f;
+#pragma unroll 1
+        for (int b = lane; b < g.parts; b += 32) {
+          const float* from = (b == 0 ? first_part : parts + 2 * b * kSlot) + i;
+          const float pm = __ldcg(from), pl = __ldcg(from + GP);
+          const float mn = fmaxf(m, pm), mg = mn == kNegInf ? 0.f : mn;
+          l = l * ex2(m - mg) + pl * ex2(pm - mg);
+          m = mn;
+          oo[b * GP + i] = pm;
         }
+        float top = m;
 #pragma unroll
-        for (int b = 0; b < kEach; ++b) m = fmaxf(m, ms[b]);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-        const float mg = m == kNegInf ? 0.f : m;
-#pragma unroll
-        for (int b = 0; b < kEach; ++b) {
-          const float f = ex2(ms[b] - mg);
-          l = fmaf(f, ls[b], l);
-          if (b * 32 + lane < g.parts) oo[(b * 32 + lane) * GP + i] = f;
-        }
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+        const float mg = top == kNegInf ? 0.f : top;
+        l *= ex2(m - mg);
 #pragma unroll
         for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
-        if (lane == 0) row_stats(i, m, l);
+        if (lane == 0) {
+          row_stats(i, top, l);
+          om[i] = mg;
+        }
       }
       __syncthreads();
       // four dimensions a thread, the parts shared out where threads are left
@@ -259,23 +262,24 @@ __device__ void finish_segment(const PagedAttnArgs& a, const Segment& g, int hg_
       const int share = kShare > 1 ? tid / kVecs : 0;
       for (int v = tid - share * kVecs; v < nh * DP / 4 && share < kShare; v += THREADS) {
         const int i = v * 4 / DP, x = v * 4 % DP;
+        const float mg = om[i];
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        constexpr int kAhead = 16;  // loads in flight
-        for (int b = share; b < g.parts; b += kShare * kAhead) {
-          float4 got[kAhead];
-#pragma unroll
-          for (int k = 0; k < kAhead; ++k)
-            if (b + k * kShare < g.parts)
-              got[k] = __ldcg(reinterpret_cast<const float4*>(slot(b + k * kShare) + 2 * GP) + v);
-#pragma unroll
-          for (int k = 0; k < kAhead; ++k)
-            if (b + k * kShare < g.parts) {
-              const float f = oo[(b + k * kShare) * GP + i];
-              o.x = fmaf(f, got[k].x, o.x);
-              o.y = fmaf(f, got[k].y, o.y);
-              o.z = fmaf(f, got[k].z, o.z);
-              o.w = fmaf(f, got[k].w, o.w);
-            }
+        if (share == 0) {
+          const float f = ex2(oo[i] - mg);
+          o = __ldcg(reinterpret_cast<const float4*>(first_part + 2 * GP) + v);
+          o.x *= f;
+          o.y *= f;
+          o.z *= f;
+          o.w *= f;
+        }
+#pragma unroll 8
+        for (int b = share == 0 ? kShare : share; b < g.parts; b += kShare) {
+          const float4 p = __ldcg(reinterpret_cast<const float4*>(parts + 2 * b * kSlot + 2 * GP) + v);
+          const float f = ex2(oo[b * GP + i] - mg);
+          o.x = fmaf(f, p.x, o.x);
+          o.y = fmaf(f, p.y, o.y);
+          o.z = fmaf(f, p.z, o.z);
+          o.w = fmaf(f, p.w, o.w);
         }
         if (kShare > 1) {
           sums[share * kVecs + v] = o;
