@@ -1040,10 +1040,11 @@ class BeamSearch:
         rows, shape = (g, beams), (g, self.n_out)
         at = _dev(scores, "scores", rows, "f32", self.device)
         fin = None if finished is None else _dev(finished, "finished", rows, "uint8", self.device)
-        new = scores.new_empty(shape)
-        parents, tokens = scores.new_empty((2,) + shape, dtype=_TORCH["int32"]).unbind(0)
+        ints = scores.new_empty((3,) + shape, dtype=_TORCH["int32"])
         done = scores.new_empty(shape, dtype=_TORCH["uint8"])
+        base, step = ints.data_ptr(), 4 * g * self.n_out
         _check(lib().lc_beam_select(self._h, g, logits.data_ptr(), _float_code(logits, "logits"), row, at, fin, eos_id, pad_id,
-                                    new.data_ptr(), parents.data_ptr(), tokens.data_ptr(), done.data_ptr(),
+                                    base, base + step, base + 2 * step, done.data_ptr(),
                                     _stream_on(stream, self.device)))
-        return new, parents, tokens, done
+        new, parents, tokens = ints.unbind(0)
+        return new.view(_TORCH["f32"]), parents, tokens, done
