@@ -1,8 +1,11 @@
 // Host side of the uncompressed paged cache (lc_paged_*) and of beam
 // selection (lc_beam_*): argument checks, workspaces, stream order.
 #include <algorithm>
+#include <map>
 #include <memory>
+#include <mutex>
 #include <string>
+#include <vector>
 
 #include "paged.h"
 
@@ -44,34 +47,84 @@ struct DeviceScope {
   int now = -1;
 };
 
-// A device buffer that grows. Growing waits for the stream order (the
-// device) that cudaFree brings, so a shorter buffer is never freed in use.
+// Workspaces come from a memory pool of the library's own for each device, which
+// keeps what is freed: a handle made for every request pays for its memory
+// once a process, not once a handle.
+cudaMemPool_t workspace_pool(int device) {
+  static std::mutex mu;
+  static std::map<int, cudaMemPool_t> pools;
+  std::lock_guard<std::mutex> lock(mu);
+  cudaMemPool_t& pool = pools[device];
+  if (!pool) {
+    cudaMemPoolProps props = {};
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = device;
+    LC_CUDA(cudaMemPoolCreate(&pool, &props));
+    uint64_t keep = UINT64_MAX;
+    LC_CUDA(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep));
+  }
+  return pool;
+}
+
+bool capturing(cudaStream_t s) {
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  LC_CUDA(cudaStreamIsCapturing(s, &capture));
+  return capture != cudaStreamCaptureStatusNone;
+}
+
+// A device buffer that grows, in the order of the handle's calls.
 struct Workspace {
   void* p = nullptr;
   size_t bytes = 0;
   ~Workspace() {
-    if (p) cudaFree(p);
+    if (p) cudaFreeAsync(p, cudaStreamLegacy);  // the device is idle: the handle is being destroyed
   }
-  void* get(size_t need, bool zeroed = false) {
+  void* get(size_t need, int device, cudaStream_t s, bool zeroed = false) {
     if (need > bytes) {
-      if (p) cudaFree(p);
+      LC_REQUIRE(!capturing(s), LC_ERR_STATE, "the first call of this size allocates: make it outside the capture");
+      if (p) LC_CUDA(cudaFreeAsync(p, s));
       p = nullptr;
       bytes = 0;
-      const cudaError_t e = cudaMalloc(&p, need);
+      const cudaError_t e = cudaMallocFromPoolAsync(&p, need, workspace_pool(device), s);
       if (e != cudaSuccess) {
         cudaGetLastError();
         p = nullptr;
         LC_THROW(LC_ERR_NOMEM, "workspace of " + std::to_string(need) + " bytes: " + cudaGetErrorString(e));
       }
       bytes = need;
-      if (zeroed) {
-        LC_CUDA(cudaMemset(p, 0, need));
-        LC_CUDA(cudaStreamSynchronize(cudaStreamLegacy));
-      }
+      if (zeroed) LC_CUDA(cudaMemsetAsync(p, 0, need, s));
     }
     return p;
   }
 };
+
+// Words of mapped host memory, one a handle, from pages that are kept.
+struct StatusWords {
+  std::mutex mu;
+  std::vector<int32_t*> free;
+  int32_t* take() {
+    std::lock_guard<std::mutex> lock(mu);
+    if (free.empty()) {
+      constexpr int kWords = 256;  // each on a cache line of its own
+      int32_t* page = nullptr;
+      LC_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&page), kWords * 64, cudaHostAllocMapped | cudaHostAllocPortable));
+      for (int i = 0; i < kWords; ++i) free.push_back(page + 16 * i);
+    }
+    int32_t* w = free.back();
+    free.pop_back();
+    *w = 0;
+    return w;
+  }
+  void give(int32_t* w) {
+    std::lock_guard<std::mutex> lock(mu);
+    free.push_back(w);
+  }
+};
+StatusWords& status_words() {
+  static auto* words = new StatusWords;  // outlives every handle
+  return *words;
+}
 
 // Calls of one handle share its workspace: a call on another stream than the
 // last one's waits for it. A stream that is being captured takes no part: a
@@ -80,21 +133,16 @@ struct Workspace {
 struct Order {
   cudaStream_t own = nullptr, last = nullptr;
   cudaEvent_t ev = nullptr;
-  void open() {
-    LC_CUDA(cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking));
-    LC_CUDA(cudaEventCreateWithFlags(&ev, cudaEventDisableTiming));
-  }
   ~Order() {
     if (ev) cudaEventDestroy(ev);
     if (own) cudaStreamDestroy(own);
   }
   cudaStream_t on(void* stream) {
+    if (!stream && !own) LC_CUDA(cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking));
     cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : own;
-    if (last == s) return s;
-    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    LC_CUDA(cudaStreamIsCapturing(s, &capture));
-    if (capture != cudaStreamCaptureStatusNone) return s;
+    if (last == s || capturing(s)) return s;
     if (last) {
+      if (!ev) LC_CUDA(cudaEventCreateWithFlags(&ev, cudaEventDisableTiming));
       LC_CUDA(cudaEventRecord(ev, last));
       LC_CUDA(cudaStreamWaitEvent(s, ev, 0));
     }
@@ -120,7 +168,7 @@ struct lc_paged {
   Workspace part, counters, scores, evict;
   int32_t* status = nullptr;  // mapped host word
   ~lc_paged() {
-    if (status) cudaFreeHost(status);
+    if (status) status_words().give(status);
   }
 
   PagedView call(const int32_t* tables, int32_t width, const int32_t* lens, int32_t rows) const {
@@ -144,9 +192,9 @@ struct lc_paged {
 struct lc_beam {
   int32_t n_groups = 0, n_beams = 0, n_out = 0, device = 0, sms = 0;
   int64_t vocab = 0;
+  size_t lists = 0;
   Order order;
   Workspace ws;
-  BeamArgs a{};
 };
 
 extern "C" {
@@ -197,9 +245,7 @@ int lc_paged_create(const lc_paged_config* config, void* k_pages, void* v_pages,
     p->cfg = c;
     p->esize = element_size(c.dtype);
     p->sms = sm_count(c.device);
-    p->order.open();
-    LC_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&p->status), 4, cudaHostAllocMapped));
-    *p->status = 0;
+    p->status = status_words().take();
     int32_t* dev_status = nullptr;
     LC_CUDA(cudaHostGetDevicePointer(reinterpret_cast<void**>(&dev_status), p->status, 0));
     p->view.k = k_pages;
@@ -215,8 +261,6 @@ int lc_paged_create(const lc_paged_config* config, void* k_pages, void* v_pages,
     p->view.n_pages = c.n_pages;
     p->view.status = dev_status;
     p->maps = make_paged_maps(p->view, c.dtype);
-    p->part.get((size_t)paged_part_floats(p->sms) * 4);
-    p->counters.get((size_t)c.max_seqs * c.max_q_heads * 4, true);
     *out = p.release();
   });
 }
@@ -299,20 +343,20 @@ static void paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t
   a.layer = layer;
   a.window = window;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
-  a.part = static_cast<float*>(p->part.p);
-  a.counters = static_cast<int32_t*>(p->counters.p);
   const int64_t cap = (int64_t)width * p->cfg.page_tokens;
+  const cudaStream_t s = p->order.on(stream);
+  a.part = static_cast<float*>(p->part.get((size_t)paged_part_floats(p->sms) * 4, p->cfg.device, s));
+  a.counters = static_cast<int32_t*>(
+      p->counters.get((size_t)p->cfg.max_seqs * p->cfg.max_q_heads * 4, p->cfg.device, s, true));
   if (acc_out) {
     check_device(acc_in, p->cfg.device, "acc_in", 4);
     check_device(acc_out, p->cfg.device, "acc_out", 4);
     LC_REQUIRE(acc_stride >= cap, LC_ERR_INVALID, "acc rows shorter than the table");
     const size_t rows = (size_t)n_seqs * n_q_heads;
     a.score_tokens = cap;
-    float* ws = static_cast<float*>(p->scores.get((rows * cap + 2 * rows) * 4));
-    a.scores = ws;
-    a.stats = ws + rows * cap;
+    a.scores = static_cast<float*>(p->scores.get((rows * cap + 2 * rows) * 4, p->cfg.device, s));
+    a.stats = a.scores + rows * cap;
   }
-  const cudaStream_t s = p->order.on(stream);
   launch_paged_attn(a, p->maps, p->cfg.dtype, p->cfg.device, p->sms, s);
   if (acc_out) {
     PagedWeightArgs w{};
@@ -387,11 +431,13 @@ int lc_paged_evict(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* ta
     a.list_cap = std::max<int64_t>(1, std::min<int64_t>(budget, cap - budget));
     const int cl = paged_evict_cluster(cap);
     const int64_t keys = paged_evict_keys_in_smem(cap, cl) ? 0 : rows * stride;
-    int32_t* ws = static_cast<int32_t*>(p->evict.get((size_t)(rows * (4 * a.list_cap + 1) + keys) * 4));
+    const cudaStream_t s = p->order.on(stream);
+    int32_t* ws = static_cast<int32_t*>(
+        p->evict.get((size_t)(rows * (4 * a.list_cap + 1) + keys) * 4, p->cfg.device, s));
     a.list = ws;
     a.pairs = ws + rows * 4 * a.list_cap;
     a.keys = reinterpret_cast<uint32_t*>(a.pairs + rows);
-    launch_paged_evict(a, p->cfg.device, p->sms, p->order.on(stream));
+    launch_paged_evict(a, p->cfg.device, p->sms, s);
   });
 }
 
@@ -436,15 +482,10 @@ int lc_beam_create(int32_t n_groups, int32_t n_beams, int64_t vocab, int32_t n_o
     b->device = device;
     b->vocab = vocab;
     b->sms = sm_count(device);
-    b->order.open();
     // a row has at most one part a slice, and a group no more candidates than one merge takes
     const size_t rows = (size_t)n_groups * n_beams;
     const size_t lists = rows * std::min<int64_t>(slices, std::max(1, kBeamMaxMerge / (n_beams * n_out)));
-    uint8_t* w = static_cast<uint8_t*>(b->ws.get(lists * n_out * 8 + (2 * lists + n_groups) * 4, true));
-    BeamArgs& a = b->a;
-    a.slice_key = reinterpret_cast<uint64_t*>(w);
-    a.slice_stats = reinterpret_cast<float*>(a.slice_key + lists * n_out);
-    a.counters = reinterpret_cast<int32_t*>(a.slice_stats + 2 * lists);
+    b->lists = lists;
     *out = b.release();
   });
 }
@@ -479,7 +520,13 @@ int lc_beam_select(lc_beam* b, int32_t n_groups, const void* logits, int32_t dty
     check_device(tokens, b->device, "tokens", 4);
     check_device(finished_out, b->device, "finished_out", 1);
     LC_REQUIRE(finished_out != finished && scores_out != scores, LC_ERR_INVALID, "outputs overlap inputs");
-    BeamArgs a = b->a;
+    const cudaStream_t s = b->order.on(stream);
+    const size_t keys = b->lists * b->n_out;
+    uint8_t* w = static_cast<uint8_t*>(b->ws.get(keys * 8 + (2 * b->lists + b->n_groups) * 4, b->device, s, true));
+    BeamArgs a{};
+    a.slice_key = reinterpret_cast<uint64_t*>(w);
+    a.slice_stats = reinterpret_cast<float*>(a.slice_key + keys);
+    a.counters = reinterpret_cast<int32_t*>(a.slice_stats + 2 * b->lists);
     a.logits = logits;
     a.dtype = dtype;
     a.row_stride = row_stride;
@@ -497,7 +544,7 @@ int lc_beam_select(lc_beam* b, int32_t n_groups, const void* logits, int32_t dty
     a.parents = parents;
     a.tokens = tokens;
     a.finished_out = finished_out;
-    launch_beam(a, b->device, b->sms, b->order.on(stream));
+    launch_beam(a, b->device, b->sms, s);
   });
 }
 

@@ -1021,10 +1021,13 @@ int64_t paged_part_floats(int32_t sms) { return 2ll * (2 * sms) * 8 * (kPagedMax
 PagedMaps make_paged_maps(const PagedView& c, int32_t dtype) {
   PagedMaps m{};
   if (dtype == LC_F32 || !vector_rows(c, 2) || c.page_tokens % 8 != 0 || c.d < 64) return m;
-  void* fn = nullptr;
-  cudaDriverEntryPointQueryResult found;
-  LC_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found));
-  LC_REQUIRE(found == cudaDriverEntryPointSuccess && fn, LC_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+  static void* const fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    LC_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found));
+    LC_REQUIRE(found == cudaDriverEntryPointSuccess && f, LC_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    return f;
+  }();
   const int box = c.page_tokens % 16 == 0 ? 16 : 8;
   const cuuint64_t dims[5] = {(cuuint64_t)c.d, (cuuint64_t)c.page_tokens, (cuuint64_t)c.hkv, (cuuint64_t)c.n_pages,
                               (cuuint64_t)c.n_layers};
