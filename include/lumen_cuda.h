@@ -530,7 +530,7 @@ typedef struct lc_paged_config {
   int32_t device;
   int32_t max_seqs;          /* rows of one call, <= 2048 */
   int32_t max_pages_per_seq; /* widest table */
-  int32_t max_q_heads;
+  int32_t max_q_heads;       /* <= 4096 */
   int32_t reserved;          /* 0 */
 } lc_paged_config;
 
@@ -555,7 +555,8 @@ int lc_paged_append(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* t
 /* Decode attention, one query token per sequence: out = softmax(scale q K^T) V
  * over the last `window` of the lens[s] slots (0: all of them), GQA as
  * lc_decode_attn; q, out [n_seqs][n_q_heads][head_dim]. Sums and softmax in
- * f32. A sequence of length 0, or without a finite score, gives zeros. */
+ * f32. A sequence of length 0, or without a finite score, gives zeros. out
+ * must not overlap q. */
 int lc_paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* tables, int32_t width,
                   const int32_t* lens, const void* q, int32_t q_dtype, int32_t n_q_heads, float scale, int32_t window,
                   void* out, int32_t out_dtype, void* stream);

@@ -33,6 +33,17 @@ void check_device(const void* p, int device, const char* what, size_t align) {
              std::string(what) + ": pointer not aligned to its elements");
 }
 
+bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + b_bytes && y < x + a_bytes;
+}
+
+// An output may be its input, not a part of it.
+void check_in_place(const void* in, const void* out, size_t bytes, const char* what) {
+  LC_REQUIRE(in == out || !overlap(in, bytes, out, bytes), LC_ERR_INVALID,
+             std::string(what) + ": output overlaps input, but is not the same");
+}
+
 // The calling thread's device, put back at the end of a call.
 struct DeviceScope {
   int before = -1;
@@ -216,8 +227,8 @@ int lc_paged_create(const lc_paged_config* config, void* k_pages, void* v_pages,
                "max_seqs must be 1.." + std::to_string(kPagedMaxSeqs));
     LC_REQUIRE(c.max_pages_per_seq >= 1 && (int64_t)c.max_pages_per_seq * c.page_tokens < (1ll << 30), LC_ERR_INVALID,
                "a sequence must hold 1..2^30-1 slots");
-    LC_REQUIRE(c.max_q_heads >= c.n_kv_heads && c.max_q_heads <= 8192, LC_ERR_INVALID,
-               "max_q_heads must be n_kv_heads..8192");
+    LC_REQUIRE(c.max_q_heads >= c.n_kv_heads && c.max_q_heads <= 4096, LC_ERR_INVALID,
+               "max_q_heads must be n_kv_heads..4096");
     LC_REQUIRE(c.reserved == 0, LC_ERR_INVALID, "reserved must be 0");
     if (!c.layer_stride && !c.page_stride && !c.head_stride && !c.token_stride) {
       c.token_stride = c.head_dim;
@@ -334,6 +345,9 @@ static void paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t
   a.c = p->call(tables, width, lens, n_seqs);
   check_device(q, p->cfg.device, "q", element_size(q_dtype));
   check_device(out, p->cfg.device, "out", element_size(out_dtype));
+  const size_t values = (size_t)n_seqs * n_q_heads * p->cfg.head_dim;
+  LC_REQUIRE(!overlap(q, values * element_size(q_dtype), out, values * element_size(out_dtype)), LC_ERR_INVALID,
+             "out overlaps q");
   a.q = q;
   a.out = out;
   a.q_dtype = q_dtype;
@@ -352,6 +366,7 @@ static void paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t
     check_device(acc_in, p->cfg.device, "acc_in", 4);
     check_device(acc_out, p->cfg.device, "acc_out", 4);
     LC_REQUIRE(acc_stride >= cap, LC_ERR_INVALID, "acc rows shorter than the table");
+    check_in_place(acc_in, acc_out, (size_t)n_seqs * p->cfg.n_kv_heads * acc_stride * 4, "acc");
     const size_t rows = (size_t)n_seqs * n_q_heads;
     a.score_tokens = cap;
     a.scores = static_cast<float*>(p->scores.get((rows * cap + 2 * rows) * 4, p->cfg.device, s));
@@ -415,6 +430,10 @@ int lc_paged_evict(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* ta
     check_device(pos_out, p->cfg.device, "pos_out", 4);
     const int64_t cap = (int64_t)width * p->cfg.page_tokens;
     LC_REQUIRE(stride >= cap, LC_ERR_INVALID, "acc and pos rows shorter than the table");
+    const size_t row_bytes = (size_t)n_seqs * p->cfg.n_kv_heads * stride * 4;
+    check_in_place(acc_in, acc_out, row_bytes, "acc");
+    check_in_place(pos_in, pos_out, row_bytes, "pos");
+    LC_REQUIRE(!overlap(acc_out, row_bytes, pos_out, row_bytes), LC_ERR_INVALID, "acc_out overlaps pos_out");
     a.layer = layer;
     a.n_seqs = n_seqs;
     a.esize = p->esize;
@@ -453,9 +472,8 @@ int lc_paged_reorder(lc_paged* p, int32_t n_groups, int32_t n_beams, const int32
     a.c = p->call(tables, width, lens, n_groups * n_beams);
     check_device(parents, p->cfg.device, "parents", 4);
     check_device(tables_out, p->cfg.device, "tables_out", 4);
-    const int64_t entries = (int64_t)n_groups * n_beams * width;
-    LC_REQUIRE(tables_out + entries <= tables || tables + entries <= tables_out, LC_ERR_INVALID,
-               "tables_out overlaps tables");
+    const size_t bytes = (size_t)n_groups * n_beams * width * 4;
+    LC_REQUIRE(!overlap(tables, bytes, tables_out, bytes), LC_ERR_INVALID, "tables_out overlaps tables");
     a.n_groups = n_groups;
     a.n_beams = n_beams;
     a.esize = p->esize;
@@ -519,7 +537,9 @@ int lc_beam_select(lc_beam* b, int32_t n_groups, const void* logits, int32_t dty
     check_device(parents, b->device, "parents", 4);
     check_device(tokens, b->device, "tokens", 4);
     check_device(finished_out, b->device, "finished_out", 1);
-    LC_REQUIRE(finished_out != finished && scores_out != scores, LC_ERR_INVALID, "outputs overlap inputs");
+    const size_t in = (size_t)n_groups * b->n_beams, out = (size_t)n_groups * b->n_out;
+    LC_REQUIRE(!overlap(scores, in * 4, scores_out, out * 4) && !(finished && overlap(finished, in, finished_out, out)),
+               LC_ERR_INVALID, "outputs overlap inputs");
     const cudaStream_t s = b->order.on(stream);
     const size_t keys = b->lists * b->n_out;
     uint8_t* w = static_cast<uint8_t*>(b->ws.get(keys * 8 + (2 * b->lists + b->n_groups) * 4, b->device, s, true));

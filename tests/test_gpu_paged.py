@@ -382,3 +382,63 @@ def test_status_tells_of_bad_tables(lc, gpu, what):
         cache.attn(0, tables, ln, torch.zeros((2, 2, 64), dtype=torch.bfloat16, device="cuda"), 1.0)
     torch.cuda.synchronize()
     assert cache.status() == lc.LC_ERR_INVALID
+
+
+def test_overlaps_are_refused(lc, gpu):
+    """Outputs may be their inputs where the header says so, and never a part of them."""
+    k = torch.zeros((1, 4, 2, 16, 64), dtype=torch.bfloat16, device="cuda")
+    cache = lc.PagedKvCache(k, k.clone(), max_seqs=2, max_pages_per_seq=2, max_q_heads=2)
+    tables = torch.zeros((2, 2), dtype=torch.int32, device="cuda")
+    ln = torch.ones(2, dtype=torch.int32, device="cuda")
+    q = torch.zeros((3, 2, 64), dtype=torch.bfloat16, device="cuda")
+    acc, pos = torch.zeros((3, 2, 32), device="cuda"), torch.zeros((3, 2, 32), dtype=torch.int32, device="cuda")
+    for f, args in ((cache.attn, (0, tables, ln, q[:2], 1.0)), ):
+        for out in (q[:2], q[1:]):
+            with pytest.raises(lc.LumenError):
+                f(*args, out=out)
+    with pytest.raises(lc.LumenError):
+        cache.attn_weights(0, tables, ln, q[:2], 1.0, acc[:2], acc[1:])
+    with pytest.raises(lc.LumenError):
+        cache.evict(0, tables, ln, 8, acc[:2], pos[:2], acc[1:])
+    with pytest.raises(lc.LumenError):
+        cache.evict(0, tables, ln, 8, acc[:2], pos[:2], None, pos[1:])
+    with pytest.raises(lc.LumenError):
+        cache.evict(0, tables, ln, 8, acc[:2], pos[:2], pos_out=acc.view(torch.int32)[:2])
+
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f32", 64), ("f16", 40)])
+def test_offsets_past_32_bits(lc, gpu, dtype, dim):
+    """Pages whose elements lie beyond 2^32 of the pool: attention, append, eviction, reordering."""
+    page, kv = 64, 2
+    need = (1 << 32) // (kv * page * dim) + 40
+    k, v = (torch.empty((1, need, kv, page, dim), dtype=ref.DTYPES[dtype], device="cuda") for _ in range(2))
+    lens = [1000, 130]
+    tables = torch.full((2, 17), -1, dtype=torch.int32)
+    tables[0, :16] = torch.arange(need - 1, need - 17, -1, dtype=torch.int32)
+    tables[1, :4] = torch.tensor([need - 20, 3, need - 30, need - 33], dtype=torch.int32)
+    tables = tables.cuda()
+    rows = ref.fill_slots(k, v, 0, tables, lens, 1)
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    cache = lc.PagedKvCache(k, v, max_seqs=2, max_pages_per_seq=17, max_q_heads=4)
+    q = queries(2, 4, dim, dtype, 2)
+    check(cache.attn(0, tables, ln, q, dim ** -0.5), ref.attn(rows, q, dim ** -0.5)[0], dtype)
+    new = torch.randn((2, kv, 1, dim), device="cuda").to(k.dtype)
+    cache.append(0, tables, ln, new, new)
+    for s, n in enumerate(lens):
+        assert torch.equal(k[0, int(tables[s, n // page]), :, n % page], new[s, :, 0])
+    span = 17 * page
+    acc = torch.rand((2, kv, span), device="cuda")
+    pos = torch.arange(span, dtype=torch.int32, device="cuda").expand(2, kv, span).contiguous()
+    a0 = acc.cpu()
+    before = [k[0, tables[s, :-(-n // page)].long()].clone() for s, n in enumerate(lens)]
+    cache.evict(0, tables, ln, 100, acc, pos)
+    for s, n in enumerate(lens):
+        for h in range(kv):
+            _, _, pairs = ref.evict_row(a0[s, h, :n].tolist(), list(range(n)), 100, 0, 0)
+            for at, to in pairs:
+                assert torch.equal(k[0, int(tables[s, to // page]), h, to % page], before[s][at // page, h, at % page])
+    tails = k[0, tables[:, 1].long()].clone()
+    out = cache.reorder(tables, torch.tensor([100], dtype=torch.int32, device="cuda"),
+                        torch.zeros((1, 2), dtype=torch.int32, device="cuda"))
+    assert out[1, 0] == tables[0, 0] and torch.equal(k[0, int(tables[1, 1]), :, :36], tails[0, :, :36])
+    assert cache.status() == lc.LC_OK
