@@ -59,8 +59,9 @@ struct DeviceScope {
 };
 
 // Workspaces come from a memory pool of the library's own for each device, which
-// keeps what is freed: a handle made for every request pays for its memory
-// once a process, not once a handle.
+// keeps up to kKeptBytes of what is freed: a handle made for every request pays
+// for its memory once a process, not once a handle.
+constexpr uint64_t kKeptBytes = 256ull << 20;
 cudaMemPool_t workspace_pool(int device) {
   static std::mutex mu;
   static std::map<int, cudaMemPool_t> pools;
@@ -72,7 +73,7 @@ cudaMemPool_t workspace_pool(int device) {
     props.location.type = cudaMemLocationTypeDevice;
     props.location.id = device;
     LC_CUDA(cudaMemPoolCreate(&pool, &props));
-    uint64_t keep = UINT64_MAX;
+    uint64_t keep = kKeptBytes;
     LC_CUDA(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep));
   }
   return pool;
@@ -324,7 +325,7 @@ int lc_paged_append(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* t
     a.pos = pos;
     a.pos0 = pos0;
     a.pos_stride = pos_stride;
-    launch_paged_append(a, p->order.on(stream));
+    launch_paged_append(a, p->sms, p->order.on(stream));
   });
 }
 

@@ -132,7 +132,7 @@ constexpr int kBeamMaxBeams = 64;
 constexpr int kBeamMaxOut = 64;
 constexpr int kBeamMaxMerge = 4096;  // candidates of one merge
 
-void launch_paged_append(const PagedAppendArgs& a, cudaStream_t s);
+void launch_paged_append(const PagedAppendArgs& a, int32_t sms, cudaStream_t s);
 // pool_dtype: LC_F32 / LC_BF16 / LC_F16.
 void launch_paged_attn(PagedAttnArgs& a, const PagedMaps& maps, int32_t pool_dtype, int32_t device, int32_t sms,
                        cudaStream_t s);

@@ -28,10 +28,10 @@ namespace {
 constexpr float kNegInf = -INFINITY;
 // What an item costs a block beyond its tiles, in tiles (see build_prefix):
 // 0, 8, 16 and 32 took 128, 119, 110 and 97 us for 32 sequences of 1 to 8192
-// slots on the tensor cores, 37, 30, 30 and 29 for a window of 1024; the
-// general kernel's tiles cost more each, and 64 sequences of 128 to 512 f32
+// slots on the tensor cores, 37, 30, 30 and 29 for a window of 1024; the FMA
+// kernel's tiles cost more each, and 64 sequences of 128 to 512 f32
 // slots took 150, 144, 156 and 180.
-constexpr int kMmaCost = 32, kGeneralCost = 8;
+constexpr int kMmaCost = 32, kFmaCost = 8;
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -324,10 +324,11 @@ __device__ __forceinline__ void cp_wait() {
 // ST > 1: f32 pools whose rows are whole 16-byte units, through ST stages of
 // cp.async a warp; per tile of 16 KB some 750 instructions (4 heads, d = 128)
 // against the 2800 that the SM issues while its share of the HBM delivers one.
-// ST = 1: any alignment and type, loaded value by value.
-template <typename T, int DP, int GP, int W, int ST>
+// ST = 1: 16-bit pools by 16-byte loads into registers (VEC), or any alignment
+// and type, value by value.
+template <typename T, int DP, int GP, int W, int ST, bool VEC>
 __global__ void __launch_bounds__(W * 32, ST > 1 ? 1 : 2) k_paged_attn(const PagedAttnArgs a) {
-  constexpr int LPT = DP / 64, TT = 32 / LPT, PITCH = DP + 4 * LPT, VL = DP / 32, kCost = kGeneralCost;
+  constexpr int LPT = DP / 64, TT = 32 / LPT, PITCH = DP + 4 * LPT, VL = DP / 32, kCost = kFmaCost;
   constexpr int TILE = TT * PITCH, CH = DP / 4;
   extern __shared__ __align__(16) uint8_t smem[];
   float* tiles = reinterpret_cast<float*>(smem);  // [W][ST][K, V][TT][PITCH]
@@ -389,8 +390,36 @@ __global__ void __launch_bounds__(W * 32, ST > 1 ? 1 : 2) k_paged_attn(const Pag
       cp_commit();
     };
 
+    // VEC: a tile's 16-byte units in registers, fetched while the one before is worked on
+    constexpr int CV = DP * (int)sizeof(T) / 16, E = 16 / (int)sizeof(T), N = VEC ? TT * CV / 32 : 1;
+    uint4 kg[N], vg[N];
+    auto fetch = [&](int j, int page) {
+      if (j >= g.j1) return;
+      const int64_t row = row_of(j, page);
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        const int e = x * 32 + lane, r = e / CV, c = e - r * CV;
+        const int64_t off = __shfl_sync(~0u, row, r);
+        kg[x] = vg[x] = make_uint4(0, 0, 0, 0);
+        if (off >= 0 && c * E < a.c.d) {
+          kg[x] = *reinterpret_cast<const uint4*>(kb + off + c * E);
+          vg[x] = *reinterpret_cast<const uint4*>(vb + off + c * E);
+        }
+      }
+    };
+    auto spread = [&](float* to, const uint4& u) {
+      const T* x = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int i = 0; i < E; i += 4)
+        *reinterpret_cast<float4*>(to + i) = make_float4(to_f32(x[i]), to_f32(x[i + 1]), to_f32(x[i + 2]), to_f32(x[i + 3]));
+    };
+
     const int first = g.j0 + warp;
     int page = page_of(first);
+    if constexpr (VEC) {
+      fetch(first, page);
+      page = page_of(first + W);
+    }
     if constexpr (ST > 1) {
 #pragma unroll
       for (int i = 0; i < ST - 1; ++i) {
@@ -422,6 +451,16 @@ __global__ void __launch_bounds__(W * 32, ST > 1 ? 1 : 2) k_paged_attn(const Pag
         __syncwarp();
         issue(j + (ST - 1) * W, fill, page);
         page = page_of(j + ST * W);
+      } else if constexpr (VEC) {
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+          const int e = x * 32 + lane, r = e / CV, c = e - r * CV;
+          spread(mine + r * PITCH + c * E, kg[x]);
+          spread(mine + TILE + r * PITCH + c * E, vg[x]);
+        }
+        __syncwarp();
+        fetch(j + W, page);
+        page = page_of(j + 2 * W);
       } else {
         const int64_t row = row_of(j, page);
         page = page_of(j + W);
@@ -733,7 +772,8 @@ __global__ void __launch_bounds__(W * 32, PER_SM)
         if (t < g.lo || t + TT > g.n) {  // rows outside: zeros in place of what memory held
           for (int e = lane; e < TT * CH; e += 32) {
             const int r = e % TT, c = e / TT;
-            if (t + r < g.lo || t + r >= g.n) *reinterpret_cast<uint4*>(smem + (vt - base) + (c >> 3) * 2048 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+            uint4* v = reinterpret_cast<uint4*>(smem + (vt - base) + (c >> 3) * 2048 + r * 128 + (c & 7) * 16);
+            if (t + r < g.lo || t + r >= g.n) *v = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async();
           __syncwarp();
@@ -764,7 +804,8 @@ __global__ void __launch_bounds__(W * 32, PER_SM)
         float* to = a.scores + (((int64_t)g.s * a.c.hkv + h) * a.score_tokens + t) * a.group + head0 + 2 * tg;
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-          if (t + (x >> 1) * 8 >= g.lo && t + (x >> 1) * 8 < g.n && 2 * tg + (x & 1) < nh) to[(x >> 1) * 8 * a.group + (x & 1)] = s[x];
+          if (t + (x >> 1) * 8 >= g.lo && t + (x >> 1) * 8 < g.n && 2 * tg + (x & 1) < nh)
+            to[(x >> 1) * 8 * a.group + (x & 1)] = s[x];
       }
       if (__any_sync(~0u, s[0] > m0 || s[2] > m0 || s[1] > m1 || s[3] > m1)) {
         float t0 = fmaxf(m0, fmaxf(s[0], s[2])), t1 = fmaxf(m1, fmaxf(s[1], s[3]));
@@ -845,29 +886,31 @@ int attn_grid(const PagedAttnArgs& a, int gp, int tile, int cost, int most) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(most, (tiles + a.min_tiles - 1) / a.min_tiles));
 }
 
-template <typename T, int DP, int GP, int ST>
+template <typename T, int DP, int GP, int ST, bool VEC>
 void launch_fma(PagedAttnArgs& a, int device, int sms, cudaStream_t s) {
   constexpr int LPT = DP / 64, TT = 32 / LPT, PITCH = DP + 4 * LPT;
   constexpr size_t fixed = (size_t)(kWarps * ST * 2 * TT * PITCH + GP * DP + kWarps * TT * GP + 2 * kWarps * GP) * 4;
   static_assert(fixed + (kPagedMaxSeqs + 1) * 4 <= 226 * 1024, "fits a block");
-  auto kernel = k_paged_attn<T, DP, GP, kWarps, ST>;
+  auto kernel = k_paged_attn<T, DP, GP, kWarps, ST, VEC>;
   static SmemOptIn opt;
   opt(kernel, fixed + (kPagedMaxSeqs + 1) * 4, device);
   a.min_tiles = kWarps;
-  const int grid = attn_grid(a, GP, TT, kGeneralCost, ST > 1 ? sms : 2 * sms);
+  const int grid = attn_grid(a, GP, TT, kFmaCost, ST > 1 ? sms : 2 * sms);
   kernel<<<grid, kWarps * 32, fixed + (size_t)(a.n_seqs + 1) * 4, s>>>(a);
 }
 
-// 16-byte rows of f32: the pipeline, for as many heads at a time as the group
-// has (up to 8). Anything else that the tensor cores do not take: the plain
-// loads.
+// Rows of 16-byte units: the pipeline for f32, for as many heads at a time as
+// the group has (up to 8), and 16-byte loads for 16-bit pools whose queries are
+// of another type. Anything else: the plain loads.
 template <typename T, int DP>
 void launch_fma(PagedAttnArgs& a, bool vec, int device, int sms, cudaStream_t s) {
   if constexpr (sizeof(T) == 4) {
-    if (vec && a.group <= 4) return launch_fma<T, DP, 4, 3>(a, device, sms, s);
-    if (vec) return launch_fma<T, DP, 8, 3>(a, device, sms, s);
+    if (vec && a.group <= 4) return launch_fma<T, DP, 4, 3, false>(a, device, sms, s);
+    if (vec) return launch_fma<T, DP, 8, 3, false>(a, device, sms, s);
+  } else {
+    if (vec) return launch_fma<T, DP, 4, 1, true>(a, device, sms, s);
   }
-  launch_fma<T, DP, 4, 1>(a, device, sms, s);
+  launch_fma<T, DP, 4, 1, false>(a, device, sms, s);
 }
 
 template <typename T>
@@ -889,7 +932,10 @@ __global__ void __launch_bounds__(256) k_paged_weights(const PagedWeightArgs a) 
   const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks, s = row / a.hkv, tid = threadIdx.x;
   const int n = min(max(a.lens[s], 0), a.cap), lo = first_slot(n, a.window);
   const int t0 = chunk * 1024 + tid;
-  if (chunk * 1024 >= n) return;
+  if (chunk * 1024 >= n) {
+    if (chunk == 0) pdl_wait();  // this kernel must not end before the attention, whatever the lengths
+    return;
+  }
   const float* acc_in = a.acc_in + row * a.acc_stride;
   float acc[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -936,28 +982,61 @@ __global__ void __launch_bounds__(256) k_paged_weights(const PagedWeightArgs a) 
   }
 }
 
-// One warp a (token, head) row: converts and writes K and V into its page.
-template <typename T>
+__device__ __forceinline__ void from_f32(float x, float& y) { y = x; }
+__device__ __forceinline__ void from_f32(float x, __nv_bfloat16& y) { y = __float2bfloat16_rn(x); }
+__device__ __forceinline__ void from_f32(float x, __half& y) { y = __float2half_rn(x); }
+
+// New tokens' K and V rows into their pages, converted. A warp takes four
+// (token, head) rows at a time, V elements of K or V a lane: V fills 16 bytes
+// of the pool where rows are whole 16-byte units. Bound by the bytes of both.
+constexpr int kAppendRows = 4;
+template <typename TI, typename TO, int V>
 __global__ void __launch_bounds__(256) k_paged_append(const PagedAppendArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = (int64_t)a.n_seqs * a.c.hkv * a.n_tokens;
-  for (int64_t r = blockIdx.x * 8ll + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8ll) {
-    const int64_t sh = r / a.n_tokens;
-    const int tok = (int)(r - sh * a.n_tokens), s = (int)(sh / a.c.hkv), h = (int)(sh - (int64_t)s * a.c.hkv);
-    const int64_t t = (int64_t)a.c.lens[s] + tok;
-    if (t < 0 || t >= (int64_t)a.c.width * a.c.page_tokens) {
-      *a.c.status = 1;
-      continue;
+  struct alignas(V * sizeof(TI) > 16 ? 16 : V * sizeof(TI)) In {
+    TI x[V];
+  };
+  struct alignas(V * sizeof(TO)) Out {
+    TO x[V];
+  };
+  const int lane = threadIdx.x & 31, units = a.c.d / V;
+  const int64_t rows = (int64_t)a.n_seqs * a.c.hkv * a.n_tokens, head0 = a.layer * a.c.layer;
+  for (int64_t r0 = (blockIdx.x * 8ll + (threadIdx.x >> 5)) * kAppendRows; r0 < rows; r0 += gridDim.x * 8ll * kAppendRows) {
+    int64_t to = -1;
+    if (lane < kAppendRows && r0 + lane < rows) {
+      const int64_t r = r0 + lane, sh = r / a.n_tokens;
+      const int tok = (int)(r - sh * a.n_tokens), s = (int)(sh / a.c.hkv), h = (int)(sh - (int64_t)s * a.c.hkv);
+      const int64_t t = (int64_t)a.c.lens[s] + tok;
+      if (t < 0 || t >= (int64_t)a.c.width * a.c.page_tokens) {
+        *a.c.status = 1;
+      } else {
+        to = row_offset(a.c, s, (int)t);
+        if (to >= 0) {
+          to += head0 + h * a.c.head;
+          if (a.pos) a.pos[sh * a.pos_stride + t] = a.pos0[s] + tok;
+        }
+      }
     }
-    const int64_t off = row_offset(a.c, s, (int)t);
-    if (off < 0) continue;
-    T* k = static_cast<T*>(a.c.k) + a.layer * a.c.layer + h * a.c.head + off;
-    T* v = static_cast<T*>(a.c.v) + a.layer * a.c.layer + h * a.c.head + off;
-    for (int x = lane; x < a.c.d; x += 32) {
-      store_f32(k, x, a.pool_dtype, load_f32(a.keys, r * a.c.d + x, a.dtype));
-      store_f32(v, x, a.pool_dtype, load_f32(a.values, r * a.c.d + x, a.dtype));
+    for (int x = lane; x < 2 * units + lane; x += 32) {  // the same count for all lanes: they shuffle
+      const bool value = x >= units;
+      const int64_t e = (int64_t)(value ? x - units : x) * V;
+      const TI* from = static_cast<const TI*>(value ? a.values : a.keys) + r0 * a.c.d + e;
+      TO* base = static_cast<TO*>(value ? a.c.v : a.c.k) + e;
+      In in[kAppendRows];
+      int64_t at[kAppendRows];
+#pragma unroll
+      for (int i = 0; i < kAppendRows; ++i) {
+        at[i] = __shfl_sync(~0u, to, i);
+        if (at[i] >= 0 && x < 2 * units) in[i] = *reinterpret_cast<const In*>(from + (int64_t)i * a.c.d);
+      }
+#pragma unroll
+      for (int i = 0; i < kAppendRows; ++i) {
+        if (at[i] < 0 || x >= 2 * units) continue;
+        Out out;
+#pragma unroll
+        for (int y = 0; y < V; ++y) from_f32(to_f32(in[i].x[y]), out.x[y]);
+        *reinterpret_cast<Out*>(base + at[i]) = out;
+      }
     }
-    if (a.pos && lane == 0) a.pos[sh * a.pos_stride + t] = a.pos0[s] + tok;
   }
 }
 
@@ -1076,16 +1155,36 @@ void launch_paged_weights(PagedWeightArgs a, cudaStream_t s) {
              2 * a.group * 4, s, a);
 }
 
-void launch_paged_append(const PagedAppendArgs& a, cudaStream_t s) {
-  const int64_t rows = (int64_t)a.n_seqs * a.c.hkv * a.n_tokens;
-  const int grid = (int)std::min<int64_t>(148 * 16, (rows + 7) / 8);
-  if (a.pool_dtype == LC_F32)
-    k_paged_append<float><<<grid, 256, 0, s>>>(a);
-  else if (a.pool_dtype == LC_BF16)
-    k_paged_append<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
+template <typename TI, typename TO>
+void launch_append(const PagedAppendArgs& a, int sms, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(TO);
+  const int64_t rows = (int64_t)a.n_seqs * a.c.hkv * a.n_tokens, per = 8 * kAppendRows;
+  const int grid = (int)std::min<int64_t>(8ll * sms, (rows + per - 1) / per);
+  const uintptr_t in = reinterpret_cast<uintptr_t>(a.keys) | reinterpret_cast<uintptr_t>(a.values);
+  if (vector_rows(a.c, sizeof(TO)) && in % std::min<size_t>(16, V * sizeof(TI)) == 0)
+    k_paged_append<TI, TO, V><<<grid, 256, 0, s>>>(a);
   else
-    k_paged_append<__half><<<grid, 256, 0, s>>>(a);
+    k_paged_append<TI, TO, 1><<<grid, 256, 0, s>>>(a);
   LC_CUDA(cudaGetLastError());
+}
+
+template <typename TO>
+void launch_append(const PagedAppendArgs& a, int sms, cudaStream_t s) {
+  if (a.dtype == LC_F32)
+    launch_append<float, TO>(a, sms, s);
+  else if (a.dtype == LC_BF16)
+    launch_append<__nv_bfloat16, TO>(a, sms, s);
+  else
+    launch_append<__half, TO>(a, sms, s);
+}
+
+void launch_paged_append(const PagedAppendArgs& a, int32_t sms, cudaStream_t s) {
+  if (a.pool_dtype == LC_F32)
+    launch_append<float>(a, sms, s);
+  else if (a.pool_dtype == LC_BF16)
+    launch_append<__nv_bfloat16>(a, sms, s);
+  else
+    launch_append<__half>(a, sms, s);
 }
 
 }  // namespace lc

@@ -442,3 +442,53 @@ def test_offsets_past_32_bits(lc, gpu, dtype, dim):
                         torch.zeros((1, 2), dtype=torch.int32, device="cuda"))
     assert out[1, 0] == tables[0, 0] and torch.equal(k[0, int(tables[1, 1]), :, :36], tails[0, :, :36])
     assert cache.status() == lc.LC_OK
+
+
+@pytest.mark.parametrize("pool,qt,dim,heads,kv,page,window", [
+    ("bf16", "f32", 64, 10, 2, 16, 0), ("f16", "f32", 136, 4, 1, 24, 100), ("bf16", "f16", 256, 3, 1, 8, 0),
+    ("f16", "bf16", 40, 4, 4, 7, 33), ("bf16", "f32", 100, 8, 2, 16, 0)])
+def test_attn_queries_of_another_type(lc, gpu, pool, qt, dim, heads, kv, page, window):
+    """16-bit pools whose slots outside the sequences hold NaN."""
+    lens = [0, 1, 17, 333, 1200]
+    cache, tables, ln, rows = make(lc, lens, heads, kv, dim, page, pool)
+    q = queries(len(lens), heads, dim, qt, 4)
+    out = torch.empty((len(lens), heads, dim), device="cuda")
+    check(cache.attn(1, tables, ln, q, dim ** -0.5, window=window, out=out), ref.attn(rows, q, dim ** -0.5, window)[0],
+          "f32")
+    assert cache.status() == lc.LC_OK
+
+
+@pytest.mark.parametrize("pool", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("src", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("dim,shift", [(128, 0), (128, 1), (128, 4), (200, 0), (36, 0)])
+def test_append_types_and_alignment(lc, gpu, pool, src, dim, shift):
+    """Sources at odd addresses, rows of odd 16-byte units, a length beyond the table."""
+    k, v = ref.pool(1, 12, 2, 16, dim, pool, 0)
+    cache = lc.PagedKvCache(k, v, max_seqs=3, max_pages_per_seq=4, max_q_heads=2)
+    tables = torch.randperm(12, device="cuda").to(torch.int32).view(3, 4)
+    lens = [13, 0, 40]
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    new = []
+    for _ in range(2):
+        flat = torch.randn(3 * 2 * 25 * dim + shift, device="cuda").to(ref.DTYPES[src])
+        new.append(flat[shift:].view(3, 2, 25, dim))
+    cache.append(0, tables, ln, *new)
+    for pool_t, x in zip((k, v), new):
+        flat = pool_t[0][tables.long()].transpose(1, 2).reshape(3, 2, 64, dim)
+        for s, n in enumerate(lens):
+            fit = min(25, 64 - n)
+            assert torch.equal(flat[s, :, n:n + fit], x[s, :, :fit].to(k.dtype))
+            assert torch.isnan(flat[s, :, :n].float()).all() and torch.isnan(flat[s, :, n + fit:].float()).all()
+    assert cache.status() == lc.LC_ERR_INVALID  # sequence 2's last token is past its table
+
+
+def test_weights_of_empty_sequences(lc, gpu):
+    """No slot anywhere: the output's zeros are there when the call's work on the stream is done."""
+    cache, tables, ln, rows = make(lc, [0, 0], 4, 2, 64, 16, "bf16")
+    tables = torch.zeros((2, 1), dtype=torch.int32, device="cuda")
+    acc = torch.ones((2, 2, 16), device="cuda")
+    q = queries(2, 4, 64, "bf16", 1)
+    for _ in range(20):
+        out = torch.full_like(q, 3.0)
+        cache.attn_weights(0, tables, ln, q, 1.0, acc, out=out)
+        assert (out.clone() == 0).all() and (acc == 1).all()
