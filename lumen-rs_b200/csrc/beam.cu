@@ -13,14 +13,21 @@
 // takes some 900 cycles. Rows that begin off 16 bytes are put right as they
 // are read from the ring, so that a thread's logits, and with them the order
 // of the sums, do not depend on the row's address. A thread keeps a running
-// maximum and sum of its own. The n_out-th largest of the maxima of 64 (or
-// 256) disjoint sets of the logits so far is a lower bound of the n_out-th
-// largest: it is taken after slices 1, 3, 8, 16 ... (only once: 51 us for 33
-// million logits; after 1, 2, 4, 8: 32; so: 31), and the logits that reach it
-// are gathered, to be ranked by counting at the end. The last block of a group turns all parts' candidates into totals,
-// ranks them and writes the answer. One launch; ranks are by value and index
-// only, so the order of arrival changes nothing. The chain of those steps is
-// what a small call takes, and a good half of a large one.
+// maximum and sum of its own.
+//
+// The n_out-th largest of the maxima of 64 (or 128) disjoint sets of the
+// logits so far is a lower bound of the n_out-th largest logit. It is taken
+// after slices 1, 3, 8, 16 ... (only once: 51 us for 33 million logits; after
+// 1, 2, 4, 8: 32; so: 31), and the logits that reach it are gathered, to be
+// ranked by counting at the end. The last block of a group turns all parts'
+// candidates into totals, cuts them by the same bound, ranks them and writes
+// the answer. One launch; ranks are by value and index only, so the order of
+// arrival changes nothing.
+//
+// 256 rows of 131072 bf16 logits take 31 us, 2.2 TB/s; 256 rows of 1000 take
+// 15.5. So half is the chain of launch, first copy, bound, ranking, the
+// counter's round trip and the merge, all of it latency; the other half runs
+// at 0.65 of the pace that a copy of the card's memory has.
 #include <algorithm>
 
 #include "devutil.cuh"
@@ -36,6 +43,9 @@ constexpr int kStages = 4;    // slices of the ring
 constexpr int kStage = kGran * kThreads + 8;  // granules of a stage: a slice, and one more for rows off 16 bytes
 constexpr int kBeamPerSm = 2;
 constexpr int kList = 1024;   // gathered candidates of a part
+// More candidates than these are cut by a bound before they are ranked: 512 of
+// 4 beams took 18.7 us uncut and 11.1 cut, 208 13.8 and 13.0; 128 15.5 and 16.4.
+constexpr int kRankAll = 128;
 constexpr float kNegInf = -INFINITY;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -107,13 +117,35 @@ __device__ __forceinline__ float granule_max<__half>(const uint4& r) {
   return fmaxf(f.x, f.y);
 }
 
+// two f32 at a time
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t x;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(lo), "f"(hi));
+  return x;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t x) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(x));
+  return f;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t x;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(a), "l"(b));
+  return x;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t x;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(a), "l"(b));
+  return x;
+}
+
 // a barrier of the computing threads
 __device__ __forceinline__ void sync_threads() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 
 struct BeamShared {
   uint64_t list[kBeamMaxMerge];  // a part's candidates, then the group's
   uint64_t few[kThreads], best[kBeamMaxOut], warp_key[kWarps];
-  __align__(16) float sets[256];
+  __align__(16) float sets[128];
   float m[kWarps], l[kWarps], row_top[kBeamMaxBeams], row_log[kBeamMaxBeams];
   float bound;
   int n, last;
@@ -146,9 +178,9 @@ __device__ __forceinline__ void warp_softmax(float& m, float& l) {
 }
 
 // A lower bound of the keep-th largest of the values whose maximum over this
-// thread's is x: the keep-th largest of the maxima of 64 or 256 sets of threads.
+// thread's is x: the keep-th largest of the maxima of 64 or 128 sets of threads.
 __device__ __forceinline__ float set_bound(BeamShared& sh, float x, int keep) {
-  const int tid = threadIdx.x, size = keep <= 16 ? kThreads / 64 : kThreads / 256, n_sets = kThreads / size;
+  const int tid = threadIdx.x, size = keep <= 16 ? kThreads / 64 : kThreads / 128, n_sets = kThreads / size;
   for (int o = 1; o < size; o <<= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
   const int set = tid / size, sub = tid & (size - 1), span = n_sets / size;
   if (sub == 0) sh.sets[set] = x;
@@ -291,7 +323,7 @@ __device__ __noinline__ void finish(const BeamArgs& a, BeamShared& sh, int row, 
   }
   const uint64_t* list = sh.list;
   int n = all;
-  if (all > kThreads) {  // those that reach a bound
+  if (all > kRankAll) {  // those that reach a bound
     const float bound = set_bound(sh, top, a.n_out);
     for (int c = tid; c < all; c += kThreads) {
       const uint64_t k = sh.list[c];
@@ -396,11 +428,13 @@ __global__ void __launch_bounds__(kThreads + 32, kBeamPerSm) k_beam_select(const
 
   // a finished row's logits, or those of a beam that is out, do not matter
   const bool dead = done || !(score > kNegInf);
-  float m = kNegInf, l = 0.f, tau = kNegInf;
+  float m = kNegInf, tau = kNegInf;
+  uint64_t l = pack2(0.f, 0.f);  // the sum in two halves
+  const uint64_t log2e = pack2(kLog2e, kLog2e);
 #pragma unroll 1
   for (int it = 0; it < slices && !dead; ++it) {
     const int stage = it % kStages;
-    if (!mbar_wait(full + 8 * stage, it / kStages & 1)) l = NAN;  // a copy that never came: no candidates
+    if (!mbar_wait(full + 8 * stage, it / kStages & 1)) l = pack2(NAN, NAN);  // a copy that never came: no candidates
     const uint4* x = ring + stage * kStage + tid;
     uint4 g[kGran];
 #pragma unroll
@@ -413,16 +447,21 @@ __global__ void __launch_bounds__(kThreads + 32, kBeamPerSm) k_beam_select(const
 #pragma unroll
     for (int r = 0; r < kGran; ++r) top = fmaxf(top, granule_max<T>(g[r]));
     if (top > m) {
-      l *= ex2((m - top) * kLog2e);
+      const float f = ex2((m - top) * kLog2e);
+      l = mul2(l, pack2(f, f));
       m = top;
     }
     const float mg = m == kNegInf ? 0.f : m;
+    const uint64_t less = pack2(-mg, -mg);
 #pragma unroll
     for (int r = 0; r < kGran; ++r) {
-      float sum = 0.f;
+      uint64_t sum = 0;  // two zeros; products by twos: 31.1 us against 31.7 one by one
 #pragma unroll
-      for (int i = 0; i < E; ++i) sum += ex2((elem<T>(g[r], i) - mg) * kLog2e);
-      l += sum;
+      for (int i = 0; i < E; i += 2) {
+        const float2 y = unpack2(mul2(add2(pack2(elem<T>(g[r], i), elem<T>(g[r], i + 1)), less), log2e));
+        sum = add2(sum, pack2(ex2(y.x), ex2(y.y)));
+      }
+      l = add2(l, sum);
     }
     if (it == 0 || it == 2 || (it & 7) == 7 || tau == kNegInf) tau = set_bound(sh, m, a.n_out);
     if (top >= tau) {
@@ -444,8 +483,9 @@ __global__ void __launch_bounds__(kThreads + 32, kBeamPerSm) k_beam_select(const
     __syncwarp();
     if ((tid & 31) == 0) mbar_arrive(empty + 8 * stage);
   }
+  const float2 halves = unpack2(l);
   finish<T>(a, sh, row, (int64_t)slice0 * a.slice, min((int64_t)a.vocab, (int64_t)(slice0 + slices) * a.slice), done, dead,
-            m, l, tau);
+            m, halves.x + halves.y, tau);
 }
 
 }  // namespace
