@@ -841,7 +841,7 @@ def _need_torch():
 
         _FLOAT_CODES.update({torch.float32: LC_F32, torch.bfloat16: LC_BF16, torch.float16: LC_F16})
         _TORCH.update({"f32": torch.float32, "int32": torch.int32, "uint8": torch.uint8,
-                       "raw_stream": torch._C._cuda_getCurrentRawStream})
+                       "empty_like": torch.empty_like, "raw_stream": torch._C._cuda_getCurrentRawStream})
 
 
 def _dev(x, name: str, shape, dtype, device: int) -> int:
@@ -943,11 +943,12 @@ class PagedKvCache:
         n, t, width, ln = self._rows(tables, lens)
         heads = q.shape[1]
         shape = (n, heads, self.head_dim)
+        at = _dev(q, "q", shape, None, self.device)
         if out is None:
-            out = q.new_empty(shape)
-        _check(lib().lc_paged_attn(self._h, layer, n, t, width, ln, _dev(q, "q", shape, None, self.device),
-                                   _float_code(q, "q"), heads, scale, window, _dev(out, "out", shape, None, self.device),
-                                   _float_code(out, "out"), _stream_on(stream, self.device)))
+            out = _TORCH["empty_like"](q)
+        _check(lib().lc_paged_attn(self._h, layer, n, t, width, ln, at, _float_code(q, "q"), heads, scale, window,
+                                   _dev(out, "out", shape, None, self.device), _float_code(out, "out"),
+                                   _stream_on(stream, self.device)))
         return out
 
     def attn_weights(self, layer: int, tables, lens, q, scale: float, acc_in, acc_out=None, decay: float = 1.0,
@@ -957,12 +958,13 @@ class PagedKvCache:
         n, t, width, ln = self._rows(tables, lens)
         heads, span = q.shape[1], acc_in.shape[2]
         shape, rows = (n, heads, self.head_dim), (n, self.n_kv_heads, span)
+        at = _dev(q, "q", shape, None, self.device)
         if out is None:
-            out = q.new_empty(shape)
+            out = _TORCH["empty_like"](q)
         acc_out = acc_in if acc_out is None else acc_out
         _check(lib().lc_paged_attn_weights(
-            self._h, layer, n, t, width, ln, _dev(q, "q", shape, None, self.device), _float_code(q, "q"), heads, scale,
-            window, _dev(out, "out", shape, None, self.device), _float_code(out, "out"),
+            self._h, layer, n, t, width, ln, at, _float_code(q, "q"), heads, scale, window,
+            _dev(out, "out", shape, None, self.device), _float_code(out, "out"),
             _dev(acc_in, "acc_in", rows, "f32", self.device), _dev(acc_out, "acc_out", rows, "f32", self.device), span,
             decay, _stream_on(stream, self.device)))
         return out
@@ -1008,6 +1010,7 @@ class BeamSearch:
         _need_torch()
         self.n_groups, self.n_beams, self.vocab, self.device = n_groups, n_beams, vocab, device
         self.n_out = n_beams if n_out is None else n_out
+        self._like = [None]  # tensors like a call's outputs
         h = C.c_void_p()
         _check(lib().lc_beam_create(n_groups, n_beams, vocab, self.n_out, device, C.byref(h)))
         self._h = h
@@ -1040,11 +1043,10 @@ class BeamSearch:
         rows, shape = (g, beams), (g, self.n_out)
         at = _dev(scores, "scores", rows, "f32", self.device)
         fin = None if finished is None else _dev(finished, "finished", rows, "uint8", self.device)
-        ints = scores.new_empty((3,) + shape, dtype=_TORCH["int32"])
-        done = scores.new_empty(shape, dtype=_TORCH["uint8"])
-        base, step = ints.data_ptr(), 4 * g * self.n_out
-        _check(lib().lc_beam_select(self._h, g, logits.data_ptr(), _float_code(logits, "logits"), row, at, fin, eos_id, pad_id,
-                                    base, base + step, base + 2 * step, done.data_ptr(),
+        if self._like[0] is None or self._like[0].shape != shape:  # empty_like takes half of new_empty's time
+            self._like = [scores.new_empty(shape, dtype=_TORCH[t]) for t in ("f32", "int32", "int32", "uint8")]
+        new, parents, tokens, done = map(_TORCH["empty_like"], self._like)
+        _check(lib().lc_beam_select(self._h, g, logits.data_ptr(), _float_code(logits, "logits"), row, at, fin, eos_id,
+                                    pad_id, new.data_ptr(), parents.data_ptr(), tokens.data_ptr(), done.data_ptr(),
                                     _stream_on(stream, self.device)))
-        new, parents, tokens = ints.unbind(0)
-        return new.view(_TORCH["f32"]), parents, tokens, done
+        return new, parents, tokens, done

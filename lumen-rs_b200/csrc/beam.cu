@@ -365,8 +365,6 @@ __global__ void __launch_bounds__(kThreads + 32, kBeamPerSm) k_beam_select(const
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), full = (uint32_t)__cvta_generic_to_shared(bars);
   const uint32_t empty = full + 8 * kStages;
   const int slice0 = blockIdx.x * a.per, slices = min(a.slices, slice0 + a.per) - slice0;
-  const float score = a.scores[row];
-  const uint8_t done = a.finished ? a.finished[row] : 0;
   // the row's first element sits at base[mis]: base is 16-byte aligned
   const T* x0 = static_cast<const T*>(a.logits) + row * a.row_stride;
   const int mis = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T)), off = mis * (int)sizeof(T);
@@ -379,6 +377,10 @@ __global__ void __launch_bounds__(kThreads + 32, kBeamPerSm) k_beam_select(const
     sh.n = 0;
   }
   __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
+  const float score = a.scores[row];
+  const uint8_t done = a.finished ? a.finished[row] : 0;
 
   if (tid >= kThreads) {
     // The fetching warp: a slice's whole granules by one bulk copy; those at the
@@ -503,8 +505,7 @@ void launch_beam(BeamArgs a, int device, int sms, cudaStream_t s) {
   static_assert(kBeamPerSm * (kRing + (int)sizeof(BeamShared) + 1024) <= 228 * 1024, "the blocks fit an SM");
   auto launch = [&](auto kernel, SmemOptIn& opt) {
     opt(kernel, kRing, device);
-    kernel<<<grid, kThreads + 32, kRing, s>>>(a);
-    LC_CUDA(cudaGetLastError());
+    launch_pdl(kernel, grid, dim3(kThreads + 32), kRing, s, a);
   };
   static SmemOptIn f32, bf16, f16;
   if (a.dtype == LC_F32)

@@ -343,7 +343,8 @@ __global__ void __launch_bounds__(W * 32, ST > 1 ? 1 : 2) k_paged_attn(const Pag
   static_assert(ST == 1 || sizeof(T) == 4, "cp.async does not convert");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hg_n = (a.group + GP - 1) / GP, hh_n = a.c.hkv * hg_n;
-  if (a.scores) pdl_launch_dependents();
+  pdl_wait();
+  pdl_launch_dependents();
   build_prefix<W * 32>(a, TT, kCost, prefix);
   const int total = prefix[a.n_seqs] * hh_n;
   const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, a.min_tiles);
@@ -648,13 +649,14 @@ __global__ void __launch_bounds__(W * 32, PER_SM)
                 "the warps' outputs, and the joins' weights and sums, fit the stages");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, tg = lane & 3;
   const int hg_n = (a.group + GP - 1) / GP, hh_n = a.c.hkv * hg_n;
-  if (a.scores) pdl_launch_dependents();
   const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars + warp * ST);
   if (TMA && lane == 0) {
 #pragma unroll
     for (int i = 0; i < ST; ++i) mbar_init(bar + 8 * i, 1);
     mbar_init_fence();
   }
+  pdl_wait();
+  pdl_launch_dependents();
   build_prefix<W * 32>(a, TT, kCost, prefix);
   const int total = prefix[a.n_seqs] * hh_n;
   const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, a.min_tiles);
@@ -896,7 +898,7 @@ void launch_fma(PagedAttnArgs& a, int device, int sms, cudaStream_t s) {
   opt(kernel, fixed + (kPagedMaxSeqs + 1) * 4, device);
   a.min_tiles = kWarps;
   const int grid = attn_grid(a, GP, TT, kFmaCost, ST > 1 ? sms : 2 * sms);
-  kernel<<<grid, kWarps * 32, fixed + (size_t)(a.n_seqs + 1) * 4, s>>>(a);
+  launch_pdl(kernel, dim3(grid), dim3(kWarps * 32), fixed + (size_t)(a.n_seqs + 1) * 4, s, a);
 }
 
 // Rows of 16-byte units: the pipeline for f32, for as many heads at a time as
@@ -930,7 +932,7 @@ template <bool VEC>
 __global__ void __launch_bounds__(256) k_paged_weights(const PagedWeightArgs a) {
   extern __shared__ float st[];  // [group][2]
   const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks, s = row / a.hkv, tid = threadIdx.x;
-  const int n = min(max(a.lens[s], 0), a.cap), lo = first_slot(n, a.window);
+  const int n = min(max(__ldcg(a.lens + s), 0), a.cap), lo = first_slot(n, a.window);
   const int t0 = chunk * 1024 + tid;
   if (chunk * 1024 >= n) {
     if (chunk == 0) pdl_wait();  // this kernel must not end before the attention, whatever the lengths
@@ -940,8 +942,10 @@ __global__ void __launch_bounds__(256) k_paged_weights(const PagedWeightArgs a) 
   float acc[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (t0 + i * 256 < n) acc[i] = acc_in[t0 + i * 256];
-  pdl_wait();  // what follows reads the attention's scores and statistics
+    if (t0 + i * 256 < n) acc[i] = __ldcg(acc_in + t0 + i * 256);
+  // The attention has waited for what came before it when it lets this kernel
+  // in, so lengths and acc_in (from L2) are final; what follows is its own.
+  pdl_wait();
   for (int i = tid; i < 2 * a.group; i += 256) st[i] = a.stats[2ll * row * a.group + i];
   const float* sc = a.scores + (int64_t)row * a.score_tokens * a.group;
   if (VEC) {
@@ -998,6 +1002,8 @@ __global__ void __launch_bounds__(256) k_paged_append(const PagedAppendArgs a) {
   struct alignas(V * sizeof(TO)) Out {
     TO x[V];
   };
+  pdl_wait();
+  pdl_launch_dependents();
   const int lane = threadIdx.x & 31, units = a.c.d / V;
   const int64_t rows = (int64_t)a.n_seqs * a.c.hkv * a.n_tokens, head0 = a.layer * a.c.layer;
   for (int64_t r0 = (blockIdx.x * 8ll + (threadIdx.x >> 5)) * kAppendRows; r0 < rows; r0 += gridDim.x * 8ll * kAppendRows) {
@@ -1049,7 +1055,8 @@ void launch_mma(PagedAttnArgs& a, const PagedMaps& maps, int device, int sms, cu
   opt(kernel, fixed + (kPagedMaxSeqs + 1) * 4, device);
   a.min_tiles = W;
   a.box = maps.box;
-  kernel<<<attn_grid(a, 8, 16, kMmaCost, PER_SM * sms), W * 32, fixed + (size_t)(a.n_seqs + 1) * 4, s>>>(a, maps.k, maps.v);
+  const int grid = attn_grid(a, 8, 16, kMmaCost, PER_SM * sms);
+  launch_pdl(kernel, dim3(grid), dim3(W * 32), fixed + (size_t)(a.n_seqs + 1) * 4, s, a, maps.k, maps.v);
 }
 
 template <typename T>
@@ -1162,10 +1169,9 @@ void launch_append(const PagedAppendArgs& a, int sms, cudaStream_t s) {
   const int grid = (int)std::min<int64_t>(8ll * sms, (rows + per - 1) / per);
   const uintptr_t in = reinterpret_cast<uintptr_t>(a.keys) | reinterpret_cast<uintptr_t>(a.values);
   if (vector_rows(a.c, sizeof(TO)) && in % std::min<size_t>(16, V * sizeof(TI)) == 0)
-    k_paged_append<TI, TO, V><<<grid, 256, 0, s>>>(a);
+    launch_pdl(k_paged_append<TI, TO, V>, dim3(grid), dim3(256), 0, s, a);
   else
-    k_paged_append<TI, TO, 1><<<grid, 256, 0, s>>>(a);
-  LC_CUDA(cudaGetLastError());
+    launch_pdl(k_paged_append<TI, TO, 1>, dim3(grid), dim3(256), 0, s, a);
 }
 
 template <typename TO>

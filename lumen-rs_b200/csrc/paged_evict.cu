@@ -145,6 +145,10 @@ __global__ void __launch_bounds__(THREADS, CL ? 2 : 1)
   const int* pos_in = a.pos_in + row * a.stride;
   float* acc_out = a.acc_out + row * a.stride;
   int* pos_out = a.pos_out + row * a.stride;
+#pragma unroll
+  for (int i = tid; i < 3 * kBins / 4; i += THREADS) reinterpret_cast<int4*>(hist)[i] = make_int4(0, 0, 0, 0);
+  if (tid == 0) sh_max = INT32_MIN;
+  pdl_wait();
   // a row's only block need not wait for its length to read ahead
   float held_acc[kHeld];
   int held_pos[kHeld];
@@ -159,9 +163,6 @@ __global__ void __launch_bounds__(THREADS, CL ? 2 : 1)
     }
   }
   int n = a.c.lens[s];
-  if (tid == 0) sh_max = INT32_MIN;
-#pragma unroll
-  for (int i = tid; i < 3 * kBins / 4; i += THREADS) reinterpret_cast<int4*>(hist)[i] = make_int4(0, 0, 0, 0);
   if (n < 0 || n > cap) {
     *a.c.status = 1;
     n = n < 0 ? 0 : cap;
@@ -346,6 +347,7 @@ __global__ void __launch_bounds__(THREADS, CL ? 2 : 1)
 template <typename U>
 __global__ void __launch_bounds__(256, 4) k_paged_move(const PagedEvictArgs a) {
   pdl_wait();
+  pdl_launch_dependents();
   move_pairs<U, kMoveBatch, 8>(a, blockIdx.x, a.pairs[blockIdx.x], blockIdx.y * 8 + (threadIdx.x >> 5), gridDim.y * 8);
 }
 
@@ -361,6 +363,8 @@ __global__ void __launch_bounds__(kReorderThreads) k_paged_reorder(const PagedRe
   __shared__ int64_t src[kBeamMaxBeams], dst[kBeamMaxBeams];
   __shared__ int extra_below, spare_below, n_copies;  // of the first 32 beams; of all
   const int tid = threadIdx.x, lane = tid & 31, w = a.n_beams, g = blockIdx.x;
+  pdl_wait();
+  pdl_launch_dependents();
   const int cap = a.c.width * a.c.page_tokens;
   const int32_t* tables = a.c.tables + (int64_t)g * w * a.c.width;
   int n = a.c.lens[g], p = 0;
@@ -477,7 +481,7 @@ void launch_evict(PagedEvictArgs a, int device, int sms, cudaStream_t s) {
   if (cl == 1) {
     auto one = [&](auto kernel, int threads, SmemOptIn& opt) {
       opt(kernel, kEvictSmemKeys * 4, device);
-      kernel<<<rows, threads, smem, s>>>(a, 1, in_smem);
+      launch_pdl(kernel, dim3(rows), dim3(threads), smem, s, a, 1, (int)in_smem);
     };
     static SmemOptIn small, large;
     if (cap <= 2048)
@@ -495,12 +499,14 @@ void launch_evict(PagedEvictArgs a, int device, int sms, cudaStream_t s) {
   cfg.blockDim = dim3(512);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = cl;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   LC_CUDA(cudaLaunchKernelEx(&cfg, k_paged_evict<U, 512, true>, a, cl, in_smem ? 1 : 0));
   launch_move<U>(a, rows, sms, s);
 }
@@ -513,7 +519,8 @@ void launch_reorder(PagedReorderArgs a, int sms, cudaStream_t s) {
   const int64_t chunks = (a.c.page_tokens * (int64_t)a.c.d + kReorderChunk - 1) / kReorderChunk;
   const int64_t all = 2 * chunks * a.c.n_layers * a.c.hkv * std::max(1, a.n_beams - 1);
   const int64_t y = std::min<int64_t>((all + 7) / 8, (8ll * sms + a.n_groups - 1) / a.n_groups);
-  k_paged_reorder<U><<<dim3((unsigned)a.n_groups, (unsigned)std::min<int64_t>(y, 65535)), kReorderThreads, 0, s>>>(a);
+  launch_pdl(k_paged_reorder<U>, dim3((unsigned)a.n_groups, (unsigned)std::min<int64_t>(y, 65535)), dim3(kReorderThreads),
+             0, s, a);
 }
 
 }  // namespace
