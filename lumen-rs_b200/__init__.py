@@ -841,7 +841,8 @@ def _need_torch():
 
         _FLOAT_CODES.update({torch.float32: LC_F32, torch.bfloat16: LC_BF16, torch.float16: LC_F16})
         _TORCH.update({"f32": torch.float32, "int32": torch.int32, "uint8": torch.uint8,
-                       "empty_like": torch.empty_like, "raw_stream": torch._C._cuda_getCurrentRawStream})
+                       "empty": torch.empty, "empty_like": torch.empty_like,
+                       "raw_stream": torch._C._cuda_getCurrentRawStream})
 
 
 def _dev(x, name: str, shape, dtype, device: int) -> int:
@@ -1010,10 +1011,13 @@ class BeamSearch:
         _need_torch()
         self.n_groups, self.n_beams, self.vocab, self.device = n_groups, n_beams, vocab, device
         self.n_out = n_beams if n_out is None else n_out
-        self._like = [None]  # tensors like a call's outputs
         h = C.c_void_p()
         _check(lib().lc_beam_create(n_groups, n_beams, vocab, self.n_out, device, C.byref(h)))
         self._h = h
+        # a call's outputs are made like these: empty_like takes half of empty's time
+        scores, ints, flags = (_TORCH["empty"]((n_groups, self.n_out), dtype=_TORCH[t], device=f"cuda:{device}")
+                               for t in ("f32", "int32", "uint8"))
+        self._like = [scores, ints, ints, flags]
 
     def close(self):
         h = getattr(self, "_h", None)
@@ -1043,8 +1047,8 @@ class BeamSearch:
         rows, shape = (g, beams), (g, self.n_out)
         at = _dev(scores, "scores", rows, "f32", self.device)
         fin = None if finished is None else _dev(finished, "finished", rows, "uint8", self.device)
-        if self._like[0] is None or self._like[0].shape != shape:  # empty_like takes half of new_empty's time
-            self._like = [scores.new_empty(shape, dtype=_TORCH[t]) for t in ("f32", "int32", "int32", "uint8")]
+        if self._like[0].shape != shape:
+            self._like = [x.new_empty(shape) for x in self._like]
         new, parents, tokens, done = map(_TORCH["empty_like"], self._like)
         _check(lib().lc_beam_select(self._h, g, logits.data_ptr(), _float_code(logits, "logits"), row, at, fin, eos_id,
                                     pad_id, new.data_ptr(), parents.data_ptr(), tokens.data_ptr(), done.data_ptr(),

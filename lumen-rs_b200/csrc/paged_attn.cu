@@ -16,7 +16,9 @@
 // (no host copy, and a captured graph follows them). An item that lies in
 // one run is finished by its block; of one that spans several, each block
 // leaves (m, l, o) in its slot and the last to arrive joins them, in slot
-// order, so results do not depend on the order of arrival.
+// order, so results do not depend on the order of arrival. Of one item alone
+// (one sequence, one kv head) the parts are joined through one SM: 131072
+// slots of 128 bf16 take 30 us, 10 of them the bytes.
 #include <algorithm>
 
 #include "devutil.cuh"
@@ -324,8 +326,12 @@ __device__ __forceinline__ void cp_wait() {
 // ST > 1: f32 pools whose rows are whole 16-byte units, through ST stages of
 // cp.async a warp; per tile of 16 KB some 750 instructions (4 heads, d = 128)
 // against the 2800 that the SM issues while its share of the HBM delivers one.
+// One sequence of 65536 slots, 8 heads of 128: 99 us, 5.4 TB/s; one of 19, 2
+// heads of 80: 5.9 us, which is the launch and one tile's latency.
 // ST = 1: 16-bit pools by 16-byte loads into registers (VEC), or any alignment
-// and type, value by value.
+// and type, value by value: 32 sequences of 2048 slots, 8 heads of 128 bf16
+// under f32 queries take 129 us so and 470 value by value, bound by their
+// instructions (the tensor cores take 53 under bf16 queries).
 template <typename T, int DP, int GP, int W, int ST, bool VEC>
 __global__ void __launch_bounds__(W * 32, ST > 1 ? 1 : 2) k_paged_attn(const PagedAttnArgs a) {
   constexpr int LPT = DP / 64, TT = 32 / LPT, PITCH = DP + 4 * LPT, VL = DP / 32, kCost = kFmaCost;
@@ -634,6 +640,14 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
 // rows with 16 bytes of padding. The latter's addresses are half of the
 // instructions of a tile, and a warp that has eight to share an SM with must
 // not take longer than the SM's share of the HBM does.
+//
+// 32 sequences of 8192 slots, 8 kv heads of 128 bf16: 176 us, 6.1 TB/s, 0.93 of
+// a plain copy; the tensor pipe is busy 16 % and the issue slots 24 %. One of
+// 131072: 94 us, 5.7 TB/s. What is left is the first loads' latency (4.5 us),
+// items' ends and beginnings (3.7 us each) and SMs that reach the memory at
+// different speeds (blocks with equal shares end between 0.75 and 1 of the
+// whole time). 16 sequences of up to 4096 under a window of 1024, 8 heads of
+// 256 f16: 28.6 us, 4.0 TB/s, where the first two are a third.
 template <typename T, int DP, int W, int ST, bool TMA, int PER_SM>
 __global__ void __launch_bounds__(W * 32, PER_SM)
     k_paged_attn_mma(const PagedAttnArgs a, const __grid_constant__ CUtensorMap k_map,
@@ -927,7 +941,9 @@ void launch_fma(PagedAttnArgs& a, bool vec, int device, int sms, cudaStream_t s)
 
 // acc_out[s, h, t] = decay acc_in + sum_g exp2(score_gt - m_g) / l_g. A block
 // does 1024 slots of a row, four a thread, so that a thread has all its loads
-// in flight at once; 4 (group + 2) bytes a slot, the scores still in L2.
+// in flight at once; 4 (group + 2) bytes a slot, the scores still in L2. 24
+// sequences of 1000 to 6000 slots, 8 kv heads of 4 query heads: 7 us after the
+// attention's 66, of which its blocks' start and first loads are hidden.
 template <bool VEC>
 __global__ void __launch_bounds__(256) k_paged_weights(const PagedWeightArgs a) {
   extern __shared__ float st[];  // [group][2]
@@ -992,7 +1008,9 @@ __device__ __forceinline__ void from_f32(float x, __half& y) { y = __float2half_
 
 // New tokens' K and V rows into their pages, converted. A warp takes four
 // (token, head) rows at a time, V elements of K or V a lane: V fills 16 bytes
-// of the pool where rows are whole 16-byte units. Bound by the bytes of both.
+// of the pool where rows are whole 16-byte units. Bound by the bytes of both:
+// 32 x 2048 tokens of 8 heads of 128 bf16 take 110 us, 4.9 TB/s read and
+// written; value by value (head dimension 100) 194 us, 2.2 TB/s.
 constexpr int kAppendRows = 4;
 template <typename TI, typename TO, int V>
 __global__ void __launch_bounds__(256) k_paged_append(const PagedAppendArgs a) {
