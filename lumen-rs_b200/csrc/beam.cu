@@ -144,11 +144,11 @@ __device__ __forceinline__ void sync_threads() { asm volatile("bar.sync 1, %0;" 
 
 struct BeamShared {
   uint64_t list[kBeamMaxMerge];  // a part's candidates, then the group's
-  uint64_t few[kThreads], best[kBeamMaxOut], warp_key[kWarps];
+  uint64_t few[kThreads], best[kBeamMaxOut], warp_key[kWarps], key_sets[128], key_bound;
   __align__(16) float sets[128];
   float m[kWarps], l[kWarps], row_top[kBeamMaxBeams], row_log[kBeamMaxBeams];
   float bound;
-  int n, last;
+  int n, n_few, last;
 };
 
 __device__ __forceinline__ uint64_t block_max_key(uint64_t k, uint64_t* warp_key) {
@@ -200,10 +200,71 @@ __device__ __forceinline__ float set_bound(BeamShared& sh, float x, int keep) {
   return sh.bound;
 }
 
-// emit(key, rank) for the `keep` largest of list[0 .. n), all different, 0 for
-// none: P threads count the larger ones of an entry.
+// The same of keys, which are all different; 0 where the sets with one are fewer.
+__device__ __forceinline__ uint64_t set_bound_key(BeamShared& sh, uint64_t x, int keep) {
+  const int tid = threadIdx.x, size = keep <= 16 ? kThreads / 64 : kThreads / 128, n_sets = kThreads / size;
+  for (int o = 1; o < size; o <<= 1) {
+    const uint64_t y = __shfl_xor_sync(~0u, x, o);
+    x = y > x ? y : x;
+  }
+  const int set = tid / size, sub = tid & (size - 1), span = n_sets / size;
+  if (sub == 0) sh.key_sets[set] = x;
+  if (tid == 0) sh.key_bound = sh.n_few = 0;
+  sync_threads();
+  int r = 0;
+#pragma unroll 4
+  for (int i = sub * span; i < (sub + 1) * span; ++i) r += sh.key_sets[i] > x;
+  for (int o = 1; o < size; o <<= 1) r += __shfl_xor_sync(~0u, r, o);
+  if (sub == 0 && x && r == keep - 1) sh.key_bound = x;
+  sync_threads();
+  return sh.key_bound;
+}
+
+// emit(key, rank) for the `keep` largest of sh.list[0 .. n), all different, 0
+// for none: cut by a bound where they are many, then P threads count the
+// larger ones of an entry. The bound is of values, which takes half a
+// microsecond less than one of keys; that one follows where too many values
+// are equal. A merge's list is sorted by parts, so for the bound neighbours go
+// to sets far from each other (37 * 429 = 1 mod 512): taken in order, the best
+// of 64 rows fell into 8 sets, too many reached the bound, and 4 groups of 64
+// beams to 64 took 580 us; they take 24.
 template <typename F>
-__device__ __forceinline__ void rank_list(const uint64_t* list, int n, int keep, F&& emit) {
+__device__ __forceinline__ void rank_list(BeamShared& sh, int n, int keep, F&& emit) {
+  const uint64_t* list = sh.list;
+  if (n > kRankAll) {
+    auto best_of_mine = [&] {
+      uint64_t top = 0;
+      for (int c0 = 0; c0 < n; c0 += kThreads) {
+        const int c = c0 + ((429 * threadIdx.x + c0 / 64) & (kThreads - 1));
+        if (c < n && list[c] > top) top = list[c];
+      }
+      return top;
+    };
+    auto cut = [&](auto&& reaches) {
+      for (int c = threadIdx.x; c < n; c += kThreads) {
+        const uint64_t k = list[c];
+        if (k && reaches(k)) {
+          const int at = atomicAdd(&sh.n_few, 1);
+          if (at < kThreads) sh.few[at] = k;
+        }
+      }
+      sync_threads();
+    };
+    if (threadIdx.x == 0) sh.n_few = 0;
+    const uint64_t top = best_of_mine();
+    const float bound = set_bound(sh, top ? key_value(top) : kNegInf, keep);
+    cut([&](uint64_t k) { return key_value(k) >= bound; });
+    const int reached = sh.n_few;
+    sync_threads();  // read by all before it is set anew
+    if (reached > kThreads) {
+      const uint64_t key_bound = set_bound_key(sh, best_of_mine(), keep);
+      cut([&](uint64_t k) { return k >= key_bound; });
+    }
+    if (sh.n_few <= kThreads) {
+      list = sh.few;
+      n = sh.n_few;
+    }
+  }
   int p = 1;
   while (p < 32 && 2 * p * n <= kThreads) p *= 2;
   const int sub = threadIdx.x & (p - 1), step = kThreads / p;
@@ -254,7 +315,7 @@ __device__ __noinline__ void finish(const BeamArgs& a, BeamShared& sh, int row, 
     }
     const int found = sh.n;
     if (found <= kList) {
-      rank_list(sh.list, found, a.n_out, [&](uint64_t k, int r) { sh.best[r] = k; });
+      rank_list(sh, found, a.n_out, [&](uint64_t k, int r) { sh.best[r] = k; });
     } else {
       // many logits reach the bound: one best after the other, read again
       const T* x0 = static_cast<const T*>(a.logits) + row * a.row_stride;
@@ -286,7 +347,6 @@ __device__ __noinline__ void finish(const BeamArgs& a, BeamShared& sh, int row, 
       __threadfence();
       a.counters[group] = 0;
     }
-    sh.n = 0;
   }
   sync_threads();
   if (!sh.last) return;
@@ -310,37 +370,17 @@ __device__ __noinline__ void finish(const BeamArgs& a, BeamShared& sh, int row, 
     }
   }
   sync_threads();
-  float top = kNegInf;
   for (int c = tid; c < all; c += kThreads) {
     uint64_t k = sh.list[c];
     if (k) {
       const int b = c / per_row;
       const float z = a.scores[row0 + b] + ((key_value(k) - sh.row_top[b]) - sh.row_log[b]);
       k = z > kNegInf ? make_key(z, (uint32_t)(b * (int64_t)a.vocab + key_index(k))) : 0;
-      if (k) top = fmaxf(top, z);
     }
     sh.list[c] = k;
   }
-  const uint64_t* list = sh.list;
-  int n = all;
-  if (all > kRankAll) {  // those that reach a bound
-    const float bound = set_bound(sh, top, a.n_out);
-    for (int c = tid; c < all; c += kThreads) {
-      const uint64_t k = sh.list[c];
-      if (k && key_value(k) >= bound) {
-        const int at = atomicAdd(&sh.n, 1);
-        if (at < kThreads) sh.few[at] = k;
-      }
-    }
-    sync_threads();
-    if (sh.n <= kThreads) {
-      list = sh.few;
-      n = sh.n;
-    }
-  } else {
-    sync_threads();
-  }
-  rank_list(list, n, a.n_out, [&](uint64_t k, int r) { sh.best[r] = k; });
+  sync_threads();
+  rank_list(sh, all, a.n_out, [&](uint64_t k, int r) { sh.best[r] = k; });
   sync_threads();
   for (int r = tid; r < a.n_out; r += kThreads) {
     const uint64_t k = sh.best[r];

@@ -118,3 +118,18 @@ def test_select_refusals(lc, gpu):
         beam.select(x, s.double())
     with pytest.raises((ValueError, TypeError)):
         beam.select(x, s, s)
+
+
+@pytest.mark.parametrize("beams,n_out,vocab", [(64, 64, 5000), (16, 32, 700), (12, 12, 700), (33, 40, 9001)])
+def test_select_many_candidates(lc, gpu, beams, n_out, vocab):
+    """Merges of many candidates: all totals equal, all but the last beam's equal, one beam far ahead,
+    every beam alike up to its score."""
+    x = torch.zeros((4, beams, vocab), device="cuda")
+    x[1, -1] = torch.linspace(-3, 3, vocab, device="cuda")
+    x[2] = torch.randn((beams, vocab), generator=torch.Generator().manual_seed(1)).cuda()
+    x[3] = torch.linspace(0, 40, vocab, device="cuda").flip(0)
+    scores = np.zeros((4, beams), np.float32)
+    scores[2] = -30
+    scores[2, beams // 2] = 0
+    scores[3] = -np.arange(beams, dtype=np.float32) * np.float32(0.37)
+    check(lc, x, scores, None, n_out)
