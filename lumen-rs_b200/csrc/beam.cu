@@ -42,7 +42,7 @@ constexpr int kGran = 2;      // 16-byte granules of a slice for each thread
 constexpr int kStages = 4;    // slices of the ring
 constexpr int kStage = kGran * kThreads + 8;  // granules of a stage: a slice, and one more for rows off 16 bytes
 constexpr int kBeamPerSm = 2;
-constexpr int kList = 1024;   // gathered candidates of a part
+constexpr int kList = kBeamMaxMerge;  // gathered candidates of a part
 // More candidates than these are cut by a bound before they are ranked: 512 of
 // 4 beams took 18.7 us uncut and 11.1 cut, 208 13.8 and 13.0; 128 15.5 and 16.4.
 constexpr int kRankAll = 128;
@@ -142,6 +142,24 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 // a barrier of the computing threads
 __device__ __forceinline__ void sync_threads() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 
+// of which x holds for so many
+__device__ __forceinline__ int count_threads(bool x) {
+  int n;
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.popc.aligned.u32 %0, 1, %2, p;\n}\n"
+      : "=r"(n)
+      : "r"((uint32_t)x), "n"(kThreads)
+      : "memory");
+  return n;
+}
+
+// The next larger value; not of NaN.
+__device__ __forceinline__ float next_up(float x) {
+  if (x == 0.f) return __uint_as_float(1u);
+  const uint32_t u = __float_as_uint(x);
+  return x > 0.f ? (x < INFINITY ? __uint_as_float(u + 1) : NAN) : __uint_as_float(u - 1);
+}
+
 struct BeamShared {
   uint64_t list[kBeamMaxMerge];  // a part's candidates, then the group's
   uint64_t few[kThreads], best[kBeamMaxOut], warp_key[kWarps], key_sets[128], key_bound;
@@ -198,6 +216,37 @@ __device__ __forceinline__ float set_bound(BeamShared& sh, float x, int keep) {
   if (sub == 0 && r == keep - 1) sh.bound = x;
   sync_threads();
   return sh.bound;
+}
+
+// Of a slice's marked logits (bit r * e + i: value i of granule r) those that
+// are not among the first `keep` of all threads' in the order of tokens.
+__device__ __noinline__ uint32_t past_first(BeamShared& sh, uint32_t marked, int e, int keep) {
+  static_assert(kGran == 2, "two counts in a word");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t low = marked & ((1u << e) - 1), high = marked >> e;
+  const uint32_t own = __popc(low) | __popc(high) << 16;
+  uint32_t inc = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t up = __shfl_up_sync(~0u, inc, o);
+    if (lane >= o) inc += up;
+  }
+  if (lane == 31) sh.warp_key[warp] = inc;
+  sync_threads();
+  uint32_t before = inc - own, all = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    const uint32_t x = (uint32_t)sh.warp_key[w];
+    if (w < warp) before += x;
+    all += x;
+  }
+  sync_threads();
+  int at[2] = {(int)(before & 0xffff), (int)((all & 0xffff) + (before >> 16))};
+  uint32_t past = 0;
+  for (uint32_t rest = marked; rest; rest &= rest - 1) {
+    const int bit = __ffs(rest) - 1;
+    if (at[bit >= e]++ >= keep) past |= 1u << bit;
+  }
+  return past;
 }
 
 // The same of keys, which are all different; 0 where the sets with one are fewer.
@@ -470,7 +519,7 @@ __global__ void __launch_bounds__(kThreads + 32, kBeamPerSm) k_beam_select(const
 
   // a finished row's logits, or those of a beam that is out, do not matter
   const bool dead = done || !(score > kNegInf);
-  float m = kNegInf, tau = kNegInf;
+  float m = kNegInf, tau = kNegInf, least = next_up(kNegInf);  // least: of the logits to gather
   uint64_t l = pack2(0.f, 0.f);  // the sum in two halves
   const uint64_t log2e = pack2(kLog2e, kLog2e);
 #pragma unroll 1
@@ -505,22 +554,41 @@ __global__ void __launch_bounds__(kThreads + 32, kBeamPerSm) k_beam_select(const
       }
       l = add2(l, sum);
     }
-    if (it == 0 || it == 2 || (it & 7) == 7 || tau == kNegInf) tau = set_bound(sh, m, a.n_out);
-    if (top >= tau) {
-      uint32_t hits = 0;
+    bool rose = false;
+    if (it == 0 || it == 2 || (it & 7) == 7 || tau == kNegInf) {
+      const float before = tau;
+      tau = set_bound(sh, m, a.n_out);
+      rose = tau > before;
+      if (rose) least = tau;
+    }
+    uint32_t hits = 0;
+    if (top >= least) {
 #pragma unroll
       for (int r = 0; r < kGran; ++r)
 #pragma unroll
-        for (int i = 0; i < E; ++i) hits |= (elem<T>(g[r], i) >= tau ? 1u : 0u) << (r * E + i);
-      while (hits) {
-        const int b = __ffs(hits) - 1, e = (b / E * kThreads + tid) * E + b % E;  // of the slice
-        hits &= hits - 1;
-        const float v = (float)(reinterpret_cast<const T*>(ring + stage * kStage))[e + mis];
-        if (v > kNegInf) {
-          const int at = atomicAdd(&sh.n, 1);
-          if (at < kList) sh.list[at] = make_key(v, (uint32_t)((int64_t)(slice0 + it) * a.slice + e));
+        for (int i = 0; i < E; ++i) hits |= (elem<T>(g[r], i) >= least ? 1u : 0u) << (r * E + i);
+    }
+    if (rose) {
+      // Logits equal to the bound matter in the slice that raised it alone (n_out
+      // others with lower tokens reach it for later ones), and of these the first
+      // n_out: of 256 rows masked with the lowest value all were gathered, and
+      // then read again and again, in 689 us.
+      if (count_threads(hits != 0) > kThreads / 4) {
+        uint32_t equal = 0;
+        for (uint32_t rest = hits; rest; rest &= rest - 1) {
+          const int b = __ffs(rest) - 1, e = (b / E * kThreads + tid) * E + b % E;
+          const float v = (float)(reinterpret_cast<const T*>(ring + stage * kStage))[e + mis];
+          if (v == tau) equal |= 1u << b;
         }
+        hits &= ~past_first(sh, equal, E, a.n_out);
       }
+      least = next_up(tau);
+    }
+    for (; hits; hits &= hits - 1) {
+      const int b = __ffs(hits) - 1, e = (b / E * kThreads + tid) * E + b % E;  // of the slice
+      const float v = (float)(reinterpret_cast<const T*>(ring + stage * kStage))[e + mis];
+      const int at = atomicAdd(&sh.n, 1);
+      if (at < kList) sh.list[at] = make_key(v, (uint32_t)((int64_t)(slice0 + it) * a.slice + e));
     }
     __syncwarp();
     if ((tid & 31) == 0) mbar_arrive(empty + 8 * stage);

@@ -8,9 +8,9 @@ import paged_ref as ref
 pytestmark = pytest.mark.gpu
 
 
-def check(lc, logits, scores, finished, n_out, eos=2, pad=0):
+def check(lc, logits, scores, finished, n_out, eos=2, pad=0, rtol=0.0):
     """logits [groups, beams, vocab] on the GPU. Totals in f32 are off by about
-    four roundings of values below 100: 3e-5."""
+    four roundings of values below 100: 3e-5 (larger ones: rtol, of three roundings to 24 bits)."""
     g, beams, vocab = logits.shape
     beam = lc.BeamSearch(g, beams, vocab, n_out)
     fin = None if finished is None else torch.from_numpy(finished).cuda()
@@ -24,7 +24,7 @@ def check(lc, logits, scores, finished, n_out, eos=2, pad=0):
         assert [int(v) for v in f[i]] == [w[3] for w in want]
         a, b = s[i].astype(np.float64), np.array([w[0] for w in want])
         assert np.array_equal(np.isinf(a), np.isinf(b))
-        assert np.allclose(a[np.isfinite(a)], b[np.isfinite(b)], rtol=0, atol=3e-5)
+        assert np.allclose(a[np.isfinite(a)], b[np.isfinite(b)], rtol=rtol, atol=3e-5)
 
 
 def inputs(groups, beams, vocab, dtype, seed, spread=3.0):
@@ -133,3 +133,22 @@ def test_select_many_candidates(lc, gpu, beams, n_out, vocab):
     scores[2, beams // 2] = 0
     scores[3] = -np.arange(beams, dtype=np.float32) * np.float32(0.37)
     check(lc, x, scores, None, n_out)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("mask", ["-inf", "lowest"])
+@pytest.mark.parametrize("vocab,kept", [(30011, 5), (30011, 40), (70000, 3000), (9000, 0)])
+def test_select_masked_vocabulary(lc, gpu, dtype, mask, vocab, kept):
+    """All tokens but a few at -inf or at the type's lowest value: spread, in one run at the end, and in
+    rows of their own; ties of the lowest go to the lowest tokens."""
+    x, scores, r = inputs(3, 4, vocab, dtype, vocab + kept)
+    fill = -float("inf") if mask == "-inf" else torch.finfo(x.dtype).min
+    y = torch.full_like(x, fill)
+    spread = torch.from_numpy(r.permutation(vocab)[:kept]).cuda()
+    y[0][:, spread] = x[0][:, spread]
+    y[1][:, vocab - kept:] = x[1][:, vocab - kept:]
+    y[2, 1] = x[2, 1]
+    if kept == 0:  # a maximum of the lowest value: log of a count
+        scores[:] = np.float32(-1.5)
+    check(lc, y, scores, None, 8, rtol=2.0 ** -22)
+    check(lc, y, scores, None, 24, rtol=2.0 ** -22)
