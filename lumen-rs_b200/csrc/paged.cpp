@@ -449,7 +449,7 @@ int lc_paged_evict(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* ta
     // at most min(budget, cap - budget) slots move in a row
     const int64_t rows = (int64_t)n_seqs * p->cfg.n_kv_heads;
     a.list_cap = std::max<int64_t>(1, std::min<int64_t>(budget, cap - budget));
-    const int cl = paged_evict_cluster(cap);
+    const int cl = paged_evict_cluster(cap, (int)rows, p->sms);
     const int64_t keys = paged_evict_keys_in_smem(cap, cl) ? 0 : rows * stride;
     const cudaStream_t s = p->order.on(stream);
     int32_t* ws = static_cast<int32_t*>(

@@ -144,7 +144,7 @@ void launch_paged_attn(PagedAttnArgs& a, const PagedMaps& maps, int32_t pool_dty
 PagedMaps make_paged_maps(const PagedView& c, int32_t dtype);
 int64_t paged_part_floats(int32_t sms);
 void launch_paged_weights(PagedWeightArgs a, cudaStream_t s);
-int paged_evict_cluster(int64_t cap);
+int paged_evict_cluster(int64_t cap, int rows, int sms);
 bool paged_evict_keys_in_smem(int64_t cap, int cluster);
 void launch_paged_evict(const PagedEvictArgs& a, int32_t device, int32_t sms, cudaStream_t s);
 void launch_paged_reorder(const PagedReorderArgs& a, int32_t sms, cudaStream_t s);

@@ -12,9 +12,9 @@
 //
 // A block owns a row: keys in shared memory, a radix select of the budget-th
 // largest over histograms of 11, 11 and 10 bits, and a prefix sum over runs of
-// slots for the order. Where a row's keys are more than one block's shared
-// memory takes, a cluster of up to 8 blocks has a range of slots each and they
-// read one another's histograms and counts; past that keys are in global
+// slots for the order. Of long rows a cluster of up to 8 blocks has a range of
+// slots each and they read one another's histograms and counts; where a row's
+// keys are more than their shared memory takes, keys are in global
 // memory. Short lists are moved by the row's own blocks, long ones by a second
 // kernel over the whole card.
 //
@@ -37,9 +37,11 @@ namespace {
 constexpr int kBins = 2048;  // 11 + 11 + 10 bits of the key
 constexpr int kEvictMaxCluster = 8;
 constexpr int64_t kEvictSmemKeys = 40 * 1024;  // 160 KB of keys a block
+constexpr int64_t kEvictBlockSlots = 12288;    // see paged_evict_cluster
 constexpr int kFusedMoves = 64;  // longest list that a row's own blocks move (a second launch costs more)
-constexpr int kMoveBatch = 16;   // pairs a warp looks up at a time: 16 and 8 took 35.2 us, 4 took 35.7 (64 rows of up to 8192)
-constexpr int kHeld = 8;  // slots whose acc and pos a thread of a row's only block holds in registers
+// pairs a warp looks up at a time: 16 and 8 took 35.2 us, 4 took 35.7 (64 rows of up to 8192)
+constexpr int kMoveBatch = 16;
+constexpr int kHeld = 8;  // slots whose acc and pos a thread holds in registers
 
 // Monotone map to unsigned; NaN below everything, -0 as 0.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -127,7 +129,7 @@ __device__ __forceinline__ void move_pairs(const PagedEvictArgs& a, int row, int
 // CL: the row has a cluster of blocks (else one). U: the unit of a copy, in
 // which the view's strides and d are given.
 template <typename U, int THREADS, bool CL>
-__global__ void __launch_bounds__(THREADS, CL ? 2 : 1)
+__global__ void __launch_bounds__(THREADS, 1)
     k_paged_evict(const PagedEvictArgs a, const int cl_arg, const int use_smem) {
   extern __shared__ uint32_t smem_keys[];
   __shared__ __align__(16) int hist[3][kBins];
@@ -155,33 +157,32 @@ __global__ void __launch_bounds__(THREADS, CL ? 2 : 1)
   for (int i = tid; i < 3 * kBins / 4; i += THREADS) reinterpret_cast<int4*>(hist)[i] = make_int4(0, 0, 0, 0);
   if (tid == 0) sh_max = INT32_MIN;
   pdl_wait();
-  // a row's only block need not wait for its length to read ahead
   float held_acc[kHeld];
   int held_pos[kHeld];
-  if (!CL) {
+  auto hold = [&](int from, int end) {
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
-      const int t = tid + i * THREADS;
-      if (t < cap) {
+      const int t = from + tid + i * THREADS;
+      if (t < end) {
         held_acc[i] = acc_in[t];
         held_pos[i] = pos_in[t];
       }
     }
-  }
+  };
+  if (!CL) hold(0, cap);  // a row's only block need not wait for its length to read ahead
   int n = a.c.lens[s];
   if (n < 0 || n > cap) {
     *a.c.status = 1;
     n = n < 0 ? 0 : cap;
   }
   const int per = CL ? (n + cl - 1) / cl : n, b = min(n, rank * per), e = min(n, b + per);
+  if (CL) hold(b, e);
   // each slot of the block's range, in strides: f(slot, acc, pos)
   auto each = [&](auto&& f) {
     int t = b + tid;
-    if (!CL) {
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i, t += THREADS)
-        if (t < e) f(t, held_acc[i], held_pos[i]);
-    }
+    for (int i = 0; i < kHeld; ++i, t += THREADS)
+      if (t < e) f(t, held_acc[i], held_pos[i]);
     // four loads before the first f, which may write where the compiler cannot tell them apart
     for (; t < e; t += 4 * THREADS) {
       float acc[4];
@@ -482,7 +483,7 @@ void launch_move(const PagedEvictArgs& a, int rows, int sms, cudaStream_t s) {
 template <typename U>
 void launch_evict(PagedEvictArgs a, int device, int sms, cudaStream_t s) {
   const int64_t cap = std::min<int64_t>((int64_t)a.c.width * a.c.page_tokens, a.stride);
-  const int rows = a.n_seqs * a.c.hkv, cl = paged_evict_cluster(cap);
+  const int rows = a.n_seqs * a.c.hkv, cl = paged_evict_cluster(cap, rows, sms);
   const bool in_smem = paged_evict_keys_in_smem(cap, cl);
   const size_t smem = in_smem ? (size_t)((cap + cl - 1) / cl) * 4 : 0;
   a.c = in_units<U>(a.c, a.esize);
@@ -502,10 +503,10 @@ void launch_evict(PagedEvictArgs a, int device, int sms, cudaStream_t s) {
     return;
   }
   static SmemOptIn opt;
-  opt(k_paged_evict<U, 512, true>, kEvictSmemKeys * 4, device);
+  opt(k_paged_evict<U, 1024, true>, kEvictSmemKeys * 4, device);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * cl));
-  cfg.blockDim = dim3(512);
+  cfg.blockDim = dim3(1024);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[2];
@@ -516,7 +517,7 @@ void launch_evict(PagedEvictArgs a, int device, int sms, cudaStream_t s) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  LC_CUDA(cudaLaunchKernelEx(&cfg, k_paged_evict<U, 512, true>, a, cl, in_smem ? 1 : 0));
+  LC_CUDA(cudaLaunchKernelEx(&cfg, k_paged_evict<U, 1024, true>, a, cl, in_smem ? 1 : 0));
   launch_move<U>(a, rows, sms, s);
 }
 
@@ -534,13 +535,16 @@ void launch_reorder(PagedReorderArgs a, int sms, cudaStream_t s) {
 
 }  // namespace
 
-// Blocks per row: one where it holds the row's keys in shared memory. A
-// cluster's barriers cost more than its blocks bring while one block can do
-// it: 8 rows of 8192 slots took 18 us with one block each, 22 with 2 and 28
-// with 4; 8 rows of 32768, 42, 40 and 37.
-int paged_evict_cluster(int64_t cap) {
+// Blocks per row: one up to 12288 slots, more of longer ones while all rows'
+// blocks run at once, and as many as hold the row's keys in shared memory. A
+// cluster's barriers cost what its blocks bring for shorter rows: with one, two
+// and four blocks 32 rows of 12000 slots took 14, 16 and 19 us, 16 of 16384
+// 29, 26 and 25, 8 of 32768 51, 40 and 28 (36 with eight).
+int paged_evict_cluster(int64_t cap, int rows, int sms) {
   int cl = 1;
-  while (cl < kEvictMaxCluster && !paged_evict_keys_in_smem(cap, cl)) cl *= 2;
+  while (cl < kEvictMaxCluster &&
+         (!paged_evict_keys_in_smem(cap, cl) || (cap > cl * kEvictBlockSlots && 2 * cl * rows <= sms)))
+    cl *= 2;
   return cl;
 }
 

@@ -492,3 +492,13 @@ def test_weights_of_empty_sequences(lc, gpu):
         out = torch.full_like(q, 3.0)
         cache.attn_weights(0, tables, ln, q, 1.0, acc, out=out)
         assert (out.clone() == 0).all() and (acc == 1).all()
+
+
+@pytest.mark.parametrize("lens,budget", [([13000], 12999), ([13000, 9, 12500, 0], 3000), ([30000, 25001], 9000),
+                                         ([60000], 20000)])
+@pytest.mark.parametrize("inplace", [False, True])
+def test_evict_rows_of_a_cluster(lc, gpu, lens, budget, inplace):
+    """Rows of 2, 4 and 8 blocks, ragged, some of no more than the budget, with equal weights."""
+    g = torch.Generator().manual_seed(len(lens))
+    acc = torch.randint(0, 900, (len(lens), 2, span_for(max(lens), 64)), generator=g).float()
+    run_evict(lc, lens, budget, 4, 100, kv=2, page=64, dim=8, acc=acc, inplace=inplace)
