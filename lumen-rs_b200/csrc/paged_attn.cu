@@ -318,23 +318,27 @@ __device__ __forceinline__ void cp_wait() {
 
 // The FMA kernel: products and sums in f32 for pools of any of the three
 // types, head dimension up to DP. A warp owns whole tiles of TT = 32 / LPT
-// slots: LPT = DP / 64 lanes share a slot's dot product, 16 bytes at a time in
-// turn, and for the values the lanes own dimensions. Rows sit in shared memory
-// as f32 with 4 LPT words of padding, which keeps the eight lanes of a 16-byte
-// read phase on different banks.
+// slots: LPT lanes share a slot's dot product, 16 bytes at a time in turn, and
+// for the values the lanes own dimensions. Rows sit in shared memory as f32
+// with 4 LPT words of padding, which keeps the eight lanes of a 16-byte read
+// phase on different banks.
 //
 // ST > 1: f32 pools whose rows are whole 16-byte units, through ST stages of
-// cp.async a warp; per tile of 16 KB some 750 instructions (4 heads, d = 128)
-// against the 2800 that the SM issues while its share of the HBM delivers one.
-// One sequence of 65536 slots, 8 heads of 128: 99 us, 5.4 TB/s; one of 19, 2
-// heads of 80: 5.9 us, which is the launch and one tile's latency.
+// cp.async a warp. What a warp waits for its own products bounds it, so as many
+// warps as shared memory takes with two stages of small tiles: one sequence of
+// 65536 slots, 8 heads of 128 under 32 queries takes 92 us, 5.9 TB/s, with 11
+// warps, 93 with 10, 96 with 8, and 98 with 4 of three stages of tiles twice
+// as long; one of 131072, 4 heads of 256, 167 and 201. Under 8 queries a head
+// the products themselves do: 4 of 81000 slots, 2 heads of 96, 165 us, of which
+// 76 the bytes. One of 19 slots, 2 heads of 80: 5.5, the launch and one tile.
 // ST = 1: 16-bit pools by 16-byte loads into registers (VEC), or any alignment
 // and type, value by value: 32 sequences of 2048 slots, 8 heads of 128 bf16
 // under f32 queries take 129 us so and 470 value by value, bound by their
 // instructions (the tensor cores take 53 under bf16 queries).
 template <typename T, int DP, int GP, int W, int ST, bool VEC>
 __global__ void __launch_bounds__(W * 32, ST > 1 ? 1 : 2) k_paged_attn(const PagedAttnArgs a) {
-  constexpr int LPT = DP / 64, TT = 32 / LPT, PITCH = DP + 4 * LPT, VL = DP / 32, kCost = kFmaCost;
+  constexpr int LPT = ST > 1 ? DP / 32 : DP / 64, TT = 32 / LPT, PITCH = DP + 4 * LPT, VL = DP / 32;
+  constexpr int kCost = ST > 1 ? 2 * kFmaCost : kFmaCost;
   constexpr int TILE = TT * PITCH, CH = DP / 4;
   extern __shared__ __align__(16) uint8_t smem[];
   float* tiles = reinterpret_cast<float*>(smem);  // [W][ST][K, V][TT][PITCH]
@@ -493,7 +497,7 @@ __global__ void __launch_bounds__(W * 32, ST > 1 ? 1 : 2) k_paged_attn(const Pag
 #pragma unroll
       for (int i = 0; i < GP; ++i) s[i] = 0.f;
 #pragma unroll 4
-      for (int c = 0; c < 16; ++c) {
+      for (int c = 0; c < DP / (4 * LPT); ++c) {
         const int x = 4 * (c * LPT + part);
         const float4 kk = *reinterpret_cast<const float4*>(kw + tok * PITCH + x);
 #pragma unroll
@@ -888,7 +892,6 @@ __global__ void __launch_bounds__(W * 32, PER_SM)
   }
 }
 
-constexpr int kWarps = 4;
 
 // Blocks for the call: as many as run at once, fewer where even the table's
 // full width holds less than min_tiles places of the list for each.
@@ -904,14 +907,14 @@ int attn_grid(const PagedAttnArgs& a, int gp, int tile, int cost, int most) {
 
 template <typename T, int DP, int GP, int ST, bool VEC>
 void launch_fma(PagedAttnArgs& a, int device, int sms, cudaStream_t s) {
-  constexpr int LPT = DP / 64, TT = 32 / LPT, PITCH = DP + 4 * LPT;
+  constexpr int LPT = ST > 1 ? DP / 32 : DP / 64, TT = 32 / LPT, PITCH = DP + 4 * LPT, kWarps = ST > 1 ? 11 : 4;
   constexpr size_t fixed = (size_t)(kWarps * ST * 2 * TT * PITCH + GP * DP + kWarps * TT * GP + 2 * kWarps * GP) * 4;
   static_assert(fixed + (kPagedMaxSeqs + 1) * 4 <= 226 * 1024, "fits a block");
   auto kernel = k_paged_attn<T, DP, GP, kWarps, ST, VEC>;
   static SmemOptIn opt;
   opt(kernel, fixed + (kPagedMaxSeqs + 1) * 4, device);
   a.min_tiles = kWarps;
-  const int grid = attn_grid(a, GP, TT, kFmaCost, ST > 1 ? sms : 2 * sms);
+  const int grid = attn_grid(a, GP, TT, ST > 1 ? 2 * kFmaCost : kFmaCost, ST > 1 ? sms : 2 * sms);
   launch_pdl(kernel, dim3(grid), dim3(kWarps * 32), fixed + (size_t)(a.n_seqs + 1) * 4, s, a);
 }
 
@@ -921,8 +924,8 @@ void launch_fma(PagedAttnArgs& a, int device, int sms, cudaStream_t s) {
 template <typename T, int DP>
 void launch_fma(PagedAttnArgs& a, bool vec, int device, int sms, cudaStream_t s) {
   if constexpr (sizeof(T) == 4) {
-    if (vec && a.group <= 4) return launch_fma<T, DP, 4, 3, false>(a, device, sms, s);
-    if (vec) return launch_fma<T, DP, 8, 3, false>(a, device, sms, s);
+    if (vec && a.group <= 4) return launch_fma<T, DP, 4, 2, false>(a, device, sms, s);
+    if (vec) return launch_fma<T, DP, 8, 2, false>(a, device, sms, s);
   } else {
     if (vec) return launch_fma<T, DP, 4, 1, true>(a, device, sms, s);
   }
