@@ -422,7 +422,8 @@ __global__ void __launch_bounds__(W * 32, ST > 1 ? 1 : 2) k_paged_attn(const Pag
       const T* x = reinterpret_cast<const T*>(&u);
 #pragma unroll
       for (int i = 0; i < E; i += 4)
-        *reinterpret_cast<float4*>(to + i) = make_float4(to_f32(x[i]), to_f32(x[i + 1]), to_f32(x[i + 2]), to_f32(x[i + 3]));
+        *reinterpret_cast<float4*>(to + i) =
+            make_float4(to_f32(x[i]), to_f32(x[i + 1]), to_f32(x[i + 2]), to_f32(x[i + 3]));
     };
 
     const int first = g.j0 + warp;
@@ -1027,7 +1028,8 @@ __global__ void __launch_bounds__(256) k_paged_append(const PagedAppendArgs a) {
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, units = a.c.d / V;
   const int64_t rows = (int64_t)a.n_seqs * a.c.hkv * a.n_tokens, head0 = a.layer * a.c.layer;
-  for (int64_t r0 = (blockIdx.x * 8ll + (threadIdx.x >> 5)) * kAppendRows; r0 < rows; r0 += gridDim.x * 8ll * kAppendRows) {
+  const int64_t step = gridDim.x * 8ll * kAppendRows;
+  for (int64_t r0 = (blockIdx.x * 8ll + (threadIdx.x >> 5)) * kAppendRows; r0 < rows; r0 += step) {
     int64_t to = -1;
     if (lane < kAppendRows && r0 + lane < rows) {
       const int64_t r = r0 + lane, sh = r / a.n_tokens;
@@ -1085,7 +1087,8 @@ void launch_mma(PagedAttnArgs& a, const PagedMaps& maps, int device, int sms, cu
   // More short items than SMs: two blocks an SM of half the warps each, whose
   // items' beginnings and ends overlap (64 sequences of 1 to 64 slots: 12 us
   // against 18.5; one 131072-slot sequence 96 against 94).
-  const int64_t cap = (int64_t)a.c.width * a.c.page_tokens, seen = a.window > 0 ? std::min<int64_t>(cap, a.window) : cap;
+  const int64_t cap = (int64_t)a.c.width * a.c.page_tokens;
+  const int64_t seen = a.window > 0 ? std::min<int64_t>(cap, a.window) : cap;
   const bool halves = seen <= 256 && (int64_t)a.n_seqs * a.c.hkv > sms;
   if (maps.box && halves) {
     if (a.c.d <= 64)
@@ -1160,7 +1163,8 @@ PagedMaps make_paged_maps(const PagedView& c, int32_t dtype) {
 void launch_paged_attn(PagedAttnArgs& a, const PagedMaps& maps, int32_t pool_dtype, int32_t device, int32_t sms,
                        cudaStream_t s) {
   const bool vec = vector_rows(a.c, pool_dtype == LC_F32 ? 4 : 2);
-  const bool mma = pool_dtype != LC_F32 && a.q_dtype == pool_dtype && vec && (reinterpret_cast<uintptr_t>(a.q) & 3) == 0;
+  const bool mma =
+      pool_dtype != LC_F32 && a.q_dtype == pool_dtype && vec && (reinterpret_cast<uintptr_t>(a.q) & 3) == 0;
   if (mma && pool_dtype == LC_BF16)
     launch_mma<__nv_bfloat16>(a, maps, device, sms, s);
   else if (mma)

@@ -529,8 +529,8 @@ void launch_reorder(PagedReorderArgs a, int sms, cudaStream_t s) {
   const int64_t chunks = (a.c.page_tokens * (int64_t)a.c.d + kReorderChunk - 1) / kReorderChunk;
   const int64_t all = 2 * chunks * a.c.n_layers * a.c.hkv * std::max(1, a.n_beams - 1);
   const int64_t y = std::min<int64_t>((all + 7) / 8, (8ll * sms + a.n_groups - 1) / a.n_groups);
-  launch_pdl(k_paged_reorder<U>, dim3((unsigned)a.n_groups, (unsigned)std::min<int64_t>(y, 65535)), dim3(kReorderThreads),
-             0, s, a);
+  const dim3 grid((unsigned)a.n_groups, (unsigned)std::min<int64_t>(y, 65535));
+  launch_pdl(k_paged_reorder<U>, grid, dim3(kReorderThreads), 0, s, a);
 }
 
 }  // namespace
