@@ -502,3 +502,30 @@ def test_evict_rows_of_a_cluster(lc, gpu, lens, budget, inplace):
     g = torch.Generator().manual_seed(len(lens))
     acc = torch.randint(0, 900, (len(lens), 2, span_for(max(lens), 64)), generator=g).float()
     run_evict(lc, lens, budget, 4, 100, kv=2, page=64, dim=8, acc=acc, inplace=inplace)
+
+
+def two_slots(lc, dtype, dim, page, low, high):
+    """Sequences of two slots: one of V 0 and one of V 1, whose score is `low` to `high` smaller in log2
+    (head i's query picks dimension i, so scores are single products). The f32 outputs, and p / (1 + p) in f64."""
+    seqs, heads = 48, 8
+    cache, tables, ln, _ = make(lc, [2] * seqs, heads, 1, dim, page, dtype, layers=1, layer=0)
+    g = torch.Generator().manual_seed(dim + page)
+    less = ((low + (high - low) * torch.rand((seqs, heads), generator=g)) / 1.4426950408889634).to(ref.DTYPES[dtype])
+    for pool_t, first, second in ((cache.k_pages, 0.0, -less), (cache.v_pages, 0.0, torch.ones_like(less))):
+        for s in range(seqs):
+            pool_t[0, int(tables[s, 0]), 0, :2] = first
+            pool_t[0, int(tables[s, 0]), 0, 1, :heads] = second[s].cuda()
+    q = torch.zeros((seqs, heads, dim), dtype=ref.DTYPES[dtype], device="cuda")
+    q[:, range(heads), range(heads)] = 1.0
+    out = cache.attn(0, tables, ln, q, 1.0, out=torch.empty((seqs, heads, dim), device="cuda"))
+    p = torch.exp(-less.double())
+    return out[:, range(heads), range(heads)].double().cpu(), p / (1 + p)
+
+
+@pytest.mark.parametrize("dtype", ["bf16"])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 7), (128, 8), (192, 16), (256, 16), (256, 3)])
+def test_attn_weights_keep_24_bits(lc, gpu, dtype, dim, page):
+    """A score below 8 (log2) is off by its factor's and its product's rounding, 8 * 2^-24 each, a weight
+    by ln 2 of that, 2^-22 of exp2 and 2^-24 three times (sum, reciprocal, product): 1.2e-6 in all, below 2^-19."""
+    got, want = two_slots(lc, dtype, dim, page, 0.0, 8.0)
+    assert ((got - want).abs() <= 2.0 ** -19 * want).all()
