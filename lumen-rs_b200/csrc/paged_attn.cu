@@ -595,11 +595,18 @@ __device__ __forceinline__ void mma_16(float* c, const uint32_t (&a)[4], uint32_
 }
 // (x, y) as a sum of parts of 16 bits, the largest first. Three of bf16 hold all
 // 24 bits of an f32; of two, outputs were off by 2^-17 and differed from those of
-// f32 weights in 1e-4 of their norm. Two of f16 hold 22 bits.
+// f32 weights in 1e-4 of their norm. Two of f16 hold 22 bits, of numbers up to 1
+// scaled by 2^15 (f16 ends at 65504) down to 2^-18 of it; below, they are off by
+// 2^-40, the half step of f16's least numbers. Unscaled that was 2^-25: a slot of
+// a 2^20-th of the largest weight had 5 bits, and those below 2^-25 were lost.
 template <typename T>
 constexpr int kParts = 2;
 template <>
 constexpr int kParts<__nv_bfloat16> = 3;
+template <typename T>
+constexpr float kScale = 32768.f;
+template <>
+constexpr float kScale<__nv_bfloat16> = 1.f;
 __device__ __forceinline__ void split_16(float x, float y, uint32_t (&part)[2], __half) {
   const __half2 h = __floats2half2_rn(x, y);
   const float2 f = __half22float2(h);
@@ -863,8 +870,8 @@ __global__ void __launch_bounds__(W * 32, PER_SM)
       l0 += p0 + p2;
       l1 += p1 + p3;
       uint32_t w0[kParts<T>], w1[kParts<T>];
-      split_16(p0, p1, w0, T());
-      split_16(p2, p3, w1, T());
+      split_16(p0 * kScale<T>, p1 * kScale<T>, w0, T());
+      split_16(p2 * kScale<T>, p3 * kScale<T>, w1, T());
 #pragma unroll
       for (int x = 0; x < kParts<T>; ++x) {
         w0[x] = transpose_8x8(w0[x]);
@@ -895,7 +902,7 @@ __global__ void __launch_bounds__(W * 32, PER_SM)
     for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
       for (int x = 0; x < 4; ++x)
-        oo[(warp * GP + 2 * tg + (x & 1)) * DP + i * 16 + gr + (x >> 1) * 8] = o[i][x];
+        oo[(warp * GP + 2 * tg + (x & 1)) * DP + i * 16 + gr + (x >> 1) * 8] = o[i][x] * (1.f / kScale<T>);
     finish_segment<W * 32, GP, DP>(a, g, hg_n, om, ol, oo);
     if (TMA && u < u_end) {  // the sums were written where the next loads go
       fence_proxy_async();

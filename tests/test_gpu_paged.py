@@ -522,10 +522,19 @@ def two_slots(lc, dtype, dim, page, low, high):
     return out[:, range(heads), range(heads)].double().cpu(), p / (1 + p)
 
 
-@pytest.mark.parametrize("dtype", ["bf16"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("dim,page", [(64, 16), (128, 7), (128, 8), (192, 16), (256, 16), (256, 3)])
 def test_attn_weights_keep_24_bits(lc, gpu, dtype, dim, page):
     """A score below 8 (log2) is off by its factor's and its product's rounding, 8 * 2^-24 each, a weight
     by ln 2 of that, 2^-22 of exp2 and 2^-24 three times (sum, reciprocal, product): 1.2e-6 in all, below 2^-19."""
     got, want = two_slots(lc, dtype, dim, page, 0.0, 8.0)
     assert ((got - want).abs() <= 2.0 ** -19 * want).all()
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 7), (256, 16)])
+@pytest.mark.parametrize("low,high", [(8.0, 18.0), (18.0, 28.0)])
+def test_attn_small_weights_under_a_large_one(lc, gpu, dim, page, low, high):
+    """f16: a slot far below one whose V is 0. Scores below 28: 28 * 2^-24 twice, times ln 2, and 2^-22 and 3 * 2^-24
+    as above, 2.8e-6, below 2^-18; two parts: 2^-22; and 2^-40 of the largest weight, two of them for two parts."""
+    got, want = two_slots(lc, "f16", dim, page, low, high)
+    assert ((got - want).abs() <= (2.0 ** -18 + 2.0 ** -22) * want + 2.0 ** -39).all()
