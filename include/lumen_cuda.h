@@ -513,7 +513,9 @@ void lc_ring_destroy(lc_ring* ring);
  * [n_seqs]. Pools, tables, lens and every tensor of these calls are memory of
  * the handle's device (LC_ERR_INVALID for host memory); nothing is copied to
  * the host and no call synchronises, so calls can be captured in a CUDA graph
- * after a first one outside (which may allocate the handle's workspace).
+ * after a first one of their size outside (which may allocate the handle's
+ * workspace). A captured call's workspace is kept until the handle is
+ * destroyed, whatever larger calls follow; its graph must not be replayed after.
  * Lengths and page ids are read on the device: a length beyond the table is
  * cut to it, a page id outside the pool is not accessed, and both are told by
  * lc_paged_status. Calls of one handle are ordered across streams (replays of

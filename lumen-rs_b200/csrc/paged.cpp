@@ -85,19 +85,28 @@ bool capturing(cudaStream_t s) {
   return capture != cudaStreamCaptureStatusNone;
 }
 
-// A device buffer that grows, in the order of the handle's calls.
+// A device buffer that grows, in the order of the handle's calls. One that a
+// captured call was given is kept when it is outgrown, until the handle is
+// destroyed: the graph has its address.
 struct Workspace {
   void* p = nullptr;
   size_t bytes = 0;
-  ~Workspace() {
-    if (p) cudaFreeAsync(p, cudaStreamLegacy);  // the device is idle: the handle is being destroyed
+  bool in_graph = false;
+  std::vector<void*> outgrown;
+  ~Workspace() {  // the device is idle: the handle is being destroyed
+    if (p) cudaFreeAsync(p, cudaStreamLegacy);
+    for (void* x : outgrown) cudaFreeAsync(x, cudaStreamLegacy);
   }
-  void* get(size_t need, int device, cudaStream_t s, bool zeroed = false) {
+  void* get(size_t need, int device, cudaStream_t s, bool captured, bool zeroed = false) {
     if (need > bytes) {
-      LC_REQUIRE(!capturing(s), LC_ERR_STATE, "the first call of this size allocates: make it outside the capture");
-      if (p) LC_CUDA(cudaFreeAsync(p, s));
+      LC_REQUIRE(!captured, LC_ERR_STATE, "the first call of this size allocates: make it outside the capture");
+      if (p && in_graph)
+        outgrown.push_back(p);
+      else if (p)
+        LC_CUDA(cudaFreeAsync(p, s));
       p = nullptr;
       bytes = 0;
+      in_graph = false;
       const cudaError_t e = cudaMallocFromPoolAsync(&p, need, workspace_pool(device), s);
       if (e != cudaSuccess) {
         cudaGetLastError();
@@ -107,6 +116,7 @@ struct Workspace {
       bytes = need;
       if (zeroed) LC_CUDA(cudaMemsetAsync(p, 0, need, s));
     }
+    in_graph |= captured;
     return p;
   }
 };
@@ -149,10 +159,12 @@ struct Order {
     if (ev) cudaEventDestroy(ev);
     if (own) cudaStreamDestroy(own);
   }
+  bool captured = false;  // the call that on() was last asked for
   cudaStream_t on(void* stream) {
     if (!stream && !own) LC_CUDA(cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking));
     cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : own;
-    if (last == s || capturing(s)) return s;
+    captured = capturing(s);
+    if (last == s || captured) return s;
     if (last) {
       if (!ev) LC_CUDA(cudaEventCreateWithFlags(&ev, cudaEventDisableTiming));
       LC_CUDA(cudaEventRecord(ev, last));
@@ -360,9 +372,9 @@ static void paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   const int64_t cap = (int64_t)width * p->cfg.page_tokens;
   const cudaStream_t s = p->order.on(stream);
-  a.part = static_cast<float*>(p->part.get((size_t)paged_part_floats(p->sms) * 4, p->cfg.device, s));
-  a.counters = static_cast<int32_t*>(
-      p->counters.get((size_t)p->cfg.max_seqs * p->cfg.max_q_heads * 4, p->cfg.device, s, true));
+  a.part = static_cast<float*>(p->part.get((size_t)paged_part_floats(p->sms) * 4, p->cfg.device, s, p->order.captured));
+  a.counters = static_cast<int32_t*>(p->counters.get((size_t)p->cfg.max_seqs * p->cfg.max_q_heads * 4, p->cfg.device, s,
+                                                     p->order.captured, true));
   if (acc_out) {
     check_device(acc_in, p->cfg.device, "acc_in", 4);
     check_device(acc_out, p->cfg.device, "acc_out", 4);
@@ -370,7 +382,8 @@ static void paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t
     check_in_place(acc_in, acc_out, (size_t)n_seqs * p->cfg.n_kv_heads * acc_stride * 4, "acc");
     const size_t rows = (size_t)n_seqs * n_q_heads;
     a.score_tokens = cap;
-    a.scores = static_cast<float*>(p->scores.get((rows * cap + 2 * rows) * 4, p->cfg.device, s));
+    a.scores =
+        static_cast<float*>(p->scores.get((rows * cap + 2 * rows) * 4, p->cfg.device, s, p->order.captured));
     a.stats = a.scores + rows * cap;
   }
   launch_paged_attn(a, p->maps, p->cfg.dtype, p->cfg.device, p->sms, s);
@@ -453,7 +466,7 @@ int lc_paged_evict(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* ta
     const int64_t keys = paged_evict_keys_in_smem(cap, cl) ? 0 : rows * stride;
     const cudaStream_t s = p->order.on(stream);
     int32_t* ws = static_cast<int32_t*>(
-        p->evict.get((size_t)(rows * (4 * a.list_cap + 1) + keys) * 4, p->cfg.device, s));
+        p->evict.get((size_t)(rows * (4 * a.list_cap + 1) + keys) * 4, p->cfg.device, s, p->order.captured));
     a.list = ws;
     a.pairs = ws + rows * 4 * a.list_cap;
     a.keys = reinterpret_cast<uint32_t*>(a.pairs + rows);
@@ -543,7 +556,8 @@ int lc_beam_select(lc_beam* b, int32_t n_groups, const void* logits, int32_t dty
                LC_ERR_INVALID, "outputs overlap inputs");
     const cudaStream_t s = b->order.on(stream);
     const size_t keys = b->lists * b->n_out;
-    uint8_t* w = static_cast<uint8_t*>(b->ws.get(keys * 8 + (2 * b->lists + b->n_groups) * 4, b->device, s, true));
+    uint8_t* w = static_cast<uint8_t*>(
+        b->ws.get(keys * 8 + (2 * b->lists + b->n_groups) * 4, b->device, s, b->order.captured, true));
     BeamArgs a{};
     a.slice_key = reinterpret_cast<uint64_t*>(w);
     a.slice_stats = reinterpret_cast<float*>(a.slice_key + keys);

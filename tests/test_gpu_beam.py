@@ -152,3 +152,22 @@ def test_select_masked_vocabulary(lc, gpu, dtype, mask, vocab, kept):
         scores[:] = np.float32(-1.5)
     check(lc, y, scores, None, 8, rtol=2.0 ** -22)
     check(lc, y, scores, None, 24, rtol=2.0 ** -22)
+
+
+def test_select_captured(lc, gpu):
+    """A graph's replay after larger and smaller calls of its handle, with other logits in place."""
+    x, scores, _ = inputs(4, 4, 30011, "f32", 3)
+    beam = lc.BeamSearch(4, 4, 30011, 6)
+    s = torch.from_numpy(scores).cuda()
+    a, b = x[:2].clone(), x[2:].clone()
+    wants = [[t.clone() for t in beam.select(y, s[:2])] for y in (a, b)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = beam.select(a, s[:2])
+    for y, want in ((a.clone(), wants[0]), (b, wants[1])):
+        beam.select(x, s)
+        beam.select(x[:1], s[:1])
+        a.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))

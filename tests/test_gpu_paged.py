@@ -538,3 +538,98 @@ def test_attn_small_weights_under_a_large_one(lc, gpu, dim, page, low, high):
     as above, 2.8e-6, below 2^-18; two parts: 2^-22; and 2^-40 of the largest weight, two of them for two parts."""
     got, want = two_slots(lc, "f16", dim, page, low, high)
     assert ((got - want).abs() <= (2.0 ** -18 + 2.0 ** -22) * want + 2.0 ** -39).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_captured_calls_after_larger_ones(lc, gpu, dtype):
+    """Graphs of attn_weights and evict of two sequences, replayed after calls of the same handle that need
+    more workspace and after those of another handle, whose answers they leave alone."""
+    heads, kv, dim, page, lens = 8, 2, 64, 16, [2000, 1500, 90, 70]
+    cache, tables, ln, _ = make(lc, lens, heads, kv, dim, page, dtype, seed=5)
+    span = tables.shape[1] * page
+    q = queries(4, heads, dim, dtype, 3)
+    g = torch.Generator().manual_seed(6)
+    acc = torch.rand((4, kv, span), generator=g).cuda()
+    pos = torch.arange(span, dtype=torch.int32, device="cuda").expand(4, kv, span).contiguous()
+    k0, v0 = cache.k_pages.clone(), cache.v_pages.clone()
+
+    class Call:
+        """attn_weights or evict of the rows from `first` on of a handle, and all that it wrote."""
+
+        def __init__(self, handle, name, first, budget=0):
+            self.handle, self.name, self.budget = handle, name, budget
+            self.t, self.n, self.q, self.acc, self.pos = (x[first:].clone() for x in (tables, ln, q, acc, pos))
+            self.out, self.acc_out, self.pos_out = (torch.empty_like(x) for x in (self.q, self.acc, self.pos))
+
+        def reset(self):
+            self.handle.k_pages.copy_(k0)
+            self.handle.v_pages.copy_(v0)
+            for x in (self.out, self.acc_out, self.pos_out):
+                x.fill_(3)
+
+        def run(self):
+            if self.name == "weights":
+                self.handle.attn_weights(1, self.t, self.n, self.q, 0.125, self.acc, self.acc_out, out=self.out)
+            else:
+                self.handle.evict(1, self.t, self.n, self.budget, self.acc, self.pos, self.acc_out, self.pos_out)
+
+        def wrote(self):
+            torch.cuda.synchronize()
+            k, v = self.handle.k_pages, self.handle.v_pages
+            return [x.clone() for x in (self.out, self.acc_out, self.pos_out, k.contiguous().view(torch.uint8),
+                                        v.contiguous().view(torch.uint8))]
+
+        def eager(self):
+            self.reset()
+            self.run()
+            return self.wrote()
+
+    small = [Call(cache, "weights", 2), Call(cache, "evict", 2, 40), Call(cache, "evict", 2, 60)]
+    want = [c.eager() for c in small]
+    graphs = []
+    for c in small:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            c.run()
+    for c in (Call(cache, "weights", 0), Call(cache, "evict", 0, 700)):
+        c.eager()
+    other = lc.PagedKvCache(k0.clone(), v0.clone(), max_seqs=4, max_pages_per_seq=tables.shape[1], max_q_heads=heads)
+    theirs = [Call(other, "weights", 1), Call(other, "evict", 1, 300), Call(other, "weights", 0), Call(other, "evict", 0, 700)]
+    wanted = [c.eager() for c in theirs]
+    for _ in range(2):
+        for c, graph, w in zip(small, graphs, want):
+            c.reset()
+            graph.replay()
+            assert all(torch.equal(a, b) for a, b in zip(c.wrote(), w))
+        for c, w in zip(theirs, wanted):
+            assert all(torch.equal(a, b) for a, b in zip(c.eager(), w))
+
+
+def test_captured_append_and_reorder(lc, gpu):
+    """Graphs of the two calls without a workspace do what the calls do."""
+    k, v = ref.pool(2, 16, 2, 16, 64, "bf16", 0)
+    for x in (k, v):
+        x.copy_(torch.randn(x.shape, device="cuda"))
+    cache = lc.PagedKvCache(k, v, max_seqs=4, max_pages_per_seq=4, max_q_heads=2)
+    tables = torch.randperm(16, device="cuda").to(torch.int32).view(4, 4)
+    ln = torch.tensor([37, 37, 37, 37], dtype=torch.int32, device="cuda")
+    parents = torch.tensor([[2, 0, 2, 2]], dtype=torch.int32, device="cuda")
+    new = torch.randn((4, 2, 1, 64), device="cuda").to(k.dtype)
+    k0, v0, out = k.clone(), v.clone(), torch.empty_like(tables)
+
+    def calls():
+        cache.reorder(tables, ln[:1], parents, out)
+        cache.append(0, out, ln, new, new)
+
+    calls()
+    want = [x.clone() for x in (out, k, v)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls()
+    for _ in range(2):
+        for x, x0 in ((k, k0), (v, v0)):
+            x.copy_(x0)
+        out.fill_(-1)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((out, k, v), want))
