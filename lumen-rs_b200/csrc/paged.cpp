@@ -148,31 +148,48 @@ StatusWords& status_words() {
   return *words;
 }
 
-// Calls of one handle share its workspace: a call on another stream than the
-// last one's waits for it. A stream that is being captured takes no part: a
-// graph may not wait for work outside it, so its replays are the caller's to
-// order.
+// Calls of one handle share its workspace and write its pools: a call on another
+// stream than the last one's waits for that call's event. The event is recorded
+// behind every call (0.4 us of its issue; kernels overlap across it as
+// before), so that the last one's stream is not touched again: it may have been
+// destroyed since, or be in capture, which a later record would join. A stream
+// that is being captured takes no part: a graph may not wait for work outside
+// it, so its replays are the caller's to order.
 struct Order {
-  cudaStream_t own = nullptr, last = nullptr;
-  cudaEvent_t ev = nullptr;
+  cudaStream_t own = nullptr;
+  unsigned long long last = 0;  // the last call's stream by its id, which no other stream is given
+  cudaEvent_t ev = nullptr;     // null before the first call
   ~Order() {
     if (ev) cudaEventDestroy(ev);
     if (own) cudaStreamDestroy(own);
   }
-  bool captured = false;  // the call that on() was last asked for
-  cudaStream_t on(void* stream) {
-    if (!stream && !own) LC_CUDA(cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking));
-    cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : own;
-    captured = capturing(s);
-    if (last == s || captured) return s;
-    if (last) {
-      if (!ev) LC_CUDA(cudaEventCreateWithFlags(&ev, cudaEventDisableTiming));
-      LC_CUDA(cudaEventRecord(ev, last));
-      LC_CUDA(cudaStreamWaitEvent(s, ev, 0));
+};
+
+// One call's place in the order, from its first launch to its last.
+struct Turn {
+  Order& order;
+  cudaStream_t s;
+  bool captured = false;
+  Turn(Order& o, void* stream) : order(o) {
+    if (!stream && !o.own) LC_CUDA(cudaStreamCreateWithFlags(&o.own, cudaStreamNonBlocking));
+    s = stream ? static_cast<cudaStream_t>(stream) : o.own;
+    unsigned long long id = s == o.own ? ~0ull : ~1ull;  // these two are no one's to capture or destroy
+    if (s != o.own && s != cudaStreamLegacy) {
+      captured = capturing(s);
+      if (captured) return;
+      LC_CUDA(cudaStreamGetId(s, &id));
     }
-    last = s;
-    return s;
+    if (!o.ev)
+      LC_CUDA(cudaEventCreateWithFlags(&o.ev, cudaEventDisableTiming));
+    else if (o.last != id)
+      LC_CUDA(cudaStreamWaitEvent(s, o.ev, 0));
+    o.last = id;
   }
+  ~Turn() {
+    if (!captured) cudaEventRecord(order.ev, s);
+  }
+  Turn(const Turn&) = delete;
+  Turn& operator=(const Turn&) = delete;
 };
 
 int sm_count(int device) {
@@ -337,7 +354,8 @@ int lc_paged_append(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* t
     a.pos = pos;
     a.pos0 = pos0;
     a.pos_stride = pos_stride;
-    launch_paged_append(a, p->sms, p->order.on(stream));
+    const Turn turn(p->order, stream);
+    launch_paged_append(a, p->sms, turn.s);
   });
 }
 
@@ -371,10 +389,11 @@ static void paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t
   a.window = window;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   const int64_t cap = (int64_t)width * p->cfg.page_tokens;
-  const cudaStream_t s = p->order.on(stream);
-  a.part = static_cast<float*>(p->part.get((size_t)paged_part_floats(p->sms) * 4, p->cfg.device, s, p->order.captured));
+  const Turn turn(p->order, stream);
+  const cudaStream_t s = turn.s;
+  a.part = static_cast<float*>(p->part.get((size_t)paged_part_floats(p->sms) * 4, p->cfg.device, s, turn.captured));
   a.counters = static_cast<int32_t*>(p->counters.get((size_t)p->cfg.max_seqs * p->cfg.max_q_heads * 4, p->cfg.device, s,
-                                                     p->order.captured, true));
+                                                     turn.captured, true));
   if (acc_out) {
     check_device(acc_in, p->cfg.device, "acc_in", 4);
     check_device(acc_out, p->cfg.device, "acc_out", 4);
@@ -383,7 +402,7 @@ static void paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t
     const size_t rows = (size_t)n_seqs * n_q_heads;
     a.score_tokens = cap;
     a.scores =
-        static_cast<float*>(p->scores.get((rows * cap + 2 * rows) * 4, p->cfg.device, s, p->order.captured));
+        static_cast<float*>(p->scores.get((rows * cap + 2 * rows) * 4, p->cfg.device, s, turn.captured));
     a.stats = a.scores + rows * cap;
   }
   launch_paged_attn(a, p->maps, p->cfg.dtype, p->cfg.device, p->sms, s);
@@ -464,9 +483,10 @@ int lc_paged_evict(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* ta
     a.list_cap = std::max<int64_t>(1, std::min<int64_t>(budget, cap - budget));
     const int cl = paged_evict_cluster(cap, (int)rows, p->sms);
     const int64_t keys = paged_evict_keys_in_smem(cap, cl) ? 0 : rows * stride;
-    const cudaStream_t s = p->order.on(stream);
+    const Turn turn(p->order, stream);
+    const cudaStream_t s = turn.s;
     int32_t* ws = static_cast<int32_t*>(
-        p->evict.get((size_t)(rows * (4 * a.list_cap + 1) + keys) * 4, p->cfg.device, s, p->order.captured));
+        p->evict.get((size_t)(rows * (4 * a.list_cap + 1) + keys) * 4, p->cfg.device, s, turn.captured));
     a.list = ws;
     a.pairs = ws + rows * 4 * a.list_cap;
     a.keys = reinterpret_cast<uint32_t*>(a.pairs + rows);
@@ -493,7 +513,8 @@ int lc_paged_reorder(lc_paged* p, int32_t n_groups, int32_t n_beams, const int32
     a.esize = p->esize;
     a.parents = parents;
     a.tables_out = tables_out;
-    launch_paged_reorder(a, p->sms, p->order.on(stream));
+    const Turn turn(p->order, stream);
+    launch_paged_reorder(a, p->sms, turn.s);
   });
 }
 
@@ -554,10 +575,11 @@ int lc_beam_select(lc_beam* b, int32_t n_groups, const void* logits, int32_t dty
     const size_t in = (size_t)n_groups * b->n_beams, out = (size_t)n_groups * b->n_out;
     LC_REQUIRE(!overlap(scores, in * 4, scores_out, out * 4) && !(finished && overlap(finished, in, finished_out, out)),
                LC_ERR_INVALID, "outputs overlap inputs");
-    const cudaStream_t s = b->order.on(stream);
+    const Turn turn(b->order, stream);
+    const cudaStream_t s = turn.s;
     const size_t keys = b->lists * b->n_out;
     uint8_t* w = static_cast<uint8_t*>(
-        b->ws.get(keys * 8 + (2 * b->lists + b->n_groups) * 4, b->device, s, b->order.captured, true));
+        b->ws.get(keys * 8 + (2 * b->lists + b->n_groups) * 4, b->device, s, turn.captured, true));
     BeamArgs a{};
     a.slice_key = reinterpret_cast<uint64_t*>(w);
     a.slice_stats = reinterpret_cast<float*>(a.slice_key + keys);

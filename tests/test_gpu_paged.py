@@ -633,3 +633,85 @@ def test_captured_append_and_reorder(lc, gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip((out, k, v), want))
+
+
+def test_order_with_the_last_stream_in_capture(lc, gpu):
+    """The last call's stream is being captured: a call on another stream runs at once, outside of that capture."""
+    lens = [700, 90]
+    cache, tables, ln, _ = make(lc, lens, 8, 2, 128, 32, "bf16")
+    q = queries(2, 8, 128, "bf16", 11)
+    want = cache.attn(1, tables, ln, q, 0.1)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    first, inside, outside = (torch.zeros_like(q) for _ in range(3))
+    torch.cuda.synchronize()
+    cache.attn(1, tables, ln, q, 0.1, out=first, stream=a)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=a):
+        cache.attn(1, tables, ln, q, 0.1, out=inside, stream=a)
+        cache.attn(1, tables, ln, q, 0.1, out=outside, stream=b)
+    torch.cuda.synchronize()
+    assert torch.equal(first, want) and torch.equal(outside, want) and (inside == 0).all()
+    outside.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(inside, want) and (outside == 0).all()
+
+
+@pytest.mark.parametrize("handle", ["paged", "beam"])
+def test_order_after_a_destroyed_stream(lc, gpu, handle):
+    """Streams that are destroyed between the calls, whose values later ones may be given again."""
+    import ctypes
+
+    cudart = torch.cuda.cudart()
+    lens = [700, 90]
+    cache, tables, ln, _ = make(lc, lens, 8, 2, 128, 32, "bf16")
+    q = queries(2, 8, 128, "bf16", 11)
+    beam = lc.BeamSearch(2, 4, 30011)
+    x, scores = torch.randn((2, 4, 30011), device="cuda"), torch.zeros((2, 4), device="cuda")
+
+    def call(stream=None):
+        if handle == "paged":
+            return [cache.attn(1, tables, ln, q, 0.1, stream=stream)]
+        return beam.select(x, scores, stream=stream)
+
+    want = call()
+    torch.cuda.synchronize()
+    for _ in range(4):
+        raw = ctypes.c_ulonglong()
+        assert int(cudart.cudaStreamCreate(ctypes.addressof(raw))) == 0
+        got = [call(raw.value)]
+        torch.cuda.ExternalStream(raw.value).synchronize()
+        assert int(cudart.cudaStreamDestroy(raw.value)) == 0
+        got.append(call())
+        torch.cuda.synchronize()
+        for g in got:
+            assert all(torch.equal(u, w) for u, w in zip(g, want))
+
+
+def test_calls_on_streams_in_turn(lc, gpu):
+    """Append, attention and eviction of one handle, each on another stream than the call before, no other wait between."""
+    lens = [5000, 3000]
+    cache, tables, ln, _ = make(lc, lens, 8, 2, 128, 32, "bf16")
+    span = tables.shape[1] * 32
+    new = torch.randn((2, 2, 1, 128), device="cuda").to(torch.bfloat16)
+    q = queries(2, 8, 128, "bf16", 12)
+    acc = torch.rand((2, 2, span), device="cuda")
+    pos = torch.arange(span, dtype=torch.int32, device="cuda").expand(2, 2, span).contiguous()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    k0, v0 = cache.k_pages.clone(), cache.v_pages.clone()
+    n1, n2 = ln + 1, torch.clamp(ln + 1, max=1000)
+    outs = []
+    for order in ([None] * 4, [streams[0], None, streams[1], streams[2]], [streams[2], streams[0], streams[1], None]):
+        cache.k_pages.copy_(k0)
+        cache.v_pages.copy_(v0)
+        a, p, out = acc.clone(), pos.clone(), torch.empty_like(q)
+        torch.cuda.synchronize()
+        cache.append(1, tables, ln, new, new, stream=order[0])
+        cache.attn_weights(1, tables, n1, q, 0.1, a, stream=order[1], out=torch.empty_like(q))
+        cache.evict(1, tables, n1, 1000, a, p, n_recent=10, stream=order[2])
+        cache.attn(1, tables, n2, q, 0.1, out=out, stream=order[3])
+        torch.cuda.synchronize()
+        outs.append((out, a, p))
+    for got in outs[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(got, outs[0]))
