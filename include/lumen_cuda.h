@@ -607,7 +607,7 @@ int lc_beam_create(int32_t n_groups, int32_t n_beams, int64_t vocab, int32_t n_o
 void lc_beam_destroy(lc_beam* b);
 
 /* Of every group's totals scores[b] + log_softmax(logits[b])[v] the n_out
- * largest, best first, equal ones by lower b * vocab + v: scores_out, parents,
+ * largest (as f32), best first, equal ones by lower b * vocab + v: scores_out, parents,
  * tokens, finished_out [n_groups][n_out]. logits [n_groups * n_beams] rows
  * row_stride elements apart, scores f32. A row with finished set (may be NULL)
  * has the one candidate (pad, its score); -inf and NaN totals are none.

@@ -15,8 +15,8 @@
 // of the sums, do not depend on the row's address. A thread keeps a running
 // maximum and sum of its own.
 //
-// The n_out-th largest of the maxima of 64 (or 128) disjoint sets of the
-// logits so far is a lower bound of the n_out-th largest logit. It is taken
+// The largest but n_out of the maxima of 64 (or 128) disjoint sets of the
+// logits so far is a lower bound of the largest but n_out logit. It is taken
 // after slices 1, 3, 8, 16 ... (only once: 51 us for 33 million logits; after
 // 1, 2, 4, 8: 32; so: 31), and the logits that reach it are gathered, to be
 // ranked by counting at the end. The last block of a group turns all parts'
@@ -24,10 +24,17 @@
 // the answer. One launch; ranks are by value and index only, so the order of
 // arrival changes nothing.
 //
-// 256 rows of 131072 bf16 logits take 32 us, 2.1 TB/s; 256 rows of 1000 take
-// 15.5; 4 of 50021 f32 13.3. So half is the chain of launch, first copy, bound, ranking, the
-// counter's round trip and the merge, all of it latency; the other half runs
-// at 0.65 of the pace that a copy of the card's memory has.
+// Totals are rounded, so different logits of a row may have equal ones, of
+// which the lower token goes first: next to its n_out best logits a part keeps
+// the one after them. Only where that has the total of the answer's last place,
+// the first such part is read again (see repair).
+//
+// 256 rows of 131072 bf16 logits take 32.4 us, 2.1 TB/s; 64 groups of 4 rows of
+// 1000 f32 13.3; 4 rows of 50021 f32 14.0. So half is the chain of launch, first
+// copy, bound, ranking, the counter's round trip and the merge, all of it
+// latency; the other half runs at 0.65 of the pace that a copy of the card's
+// memory has. Looking for a part to read again is 0.7 of these, reading one to
+// its end is 45 us for all of 256 rows of 131072 f32 at once.
 #include <algorithm>
 
 #include "devutil.cuh"
@@ -160,13 +167,29 @@ __device__ __forceinline__ float next_up(float x) {
   return x > 0.f ? (x < INFINITY ? __uint_as_float(u + 1) : NAN) : __uint_as_float(u - 1);
 }
 
+// The next larger (or smaller) value of type T to x, itself one and finite.
+template <typename T>
+__device__ __forceinline__ float neighbour(float x, bool larger) {
+  if constexpr (sizeof(T) == 4) {
+    return larger ? next_up(x) : -next_up(-x);
+  } else {
+    const T t = T(x);
+    unsigned short u = *reinterpret_cast<const unsigned short*>(&t);
+    if ((u & 0x7fff) == 0)
+      u = larger ? 1 : 0x8001;
+    else
+      u += larger == !(u & 0x8000) ? 1 : -1;
+    return (float)*reinterpret_cast<const T*>(&u);
+  }
+}
+
 struct BeamShared {
   uint64_t list[kBeamMaxMerge];  // a part's candidates, then the group's
-  uint64_t few[kThreads], best[kBeamMaxOut], warp_key[kWarps], key_sets[128], key_bound;
+  uint64_t few[kThreads], best[kBeamMaxOut + 1], warp_key[kWarps], key_sets[128], key_bound;
   __align__(16) float sets[128];
-  float m[kWarps], l[kWarps], row_top[kBeamMaxBeams], row_log[kBeamMaxBeams];
+  float m[kWarps], l[kWarps], row_top[kBeamMaxBeams], row_log[kBeamMaxBeams], row_next[kBeamMaxBeams];
   float bound;
-  int n, n_few, last;
+  int n, n_few, last, again;
 };
 
 __device__ __forceinline__ uint64_t block_max_key(uint64_t k, uint64_t* warp_key) {
@@ -198,7 +221,7 @@ __device__ __forceinline__ void warp_softmax(float& m, float& l) {
 // A lower bound of the keep-th largest of the values whose maximum over this
 // thread's is x: the keep-th largest of the maxima of 64 or 128 sets of threads.
 __device__ __forceinline__ float set_bound(BeamShared& sh, float x, int keep) {
-  const int tid = threadIdx.x, size = keep <= 16 ? kThreads / 64 : kThreads / 128, n_sets = kThreads / size;
+  const int tid = threadIdx.x, size = keep <= 17 ? kThreads / 64 : kThreads / 128, n_sets = kThreads / size;
   for (int o = 1; o < size; o <<= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
   const int set = tid / size, sub = tid & (size - 1), span = n_sets / size;
   if (sub == 0) sh.sets[set] = x;
@@ -251,7 +274,7 @@ __device__ __noinline__ uint32_t past_first(BeamShared& sh, uint32_t marked, int
 
 // The same of keys, which are all different; 0 where the sets with one are fewer.
 __device__ __forceinline__ uint64_t set_bound_key(BeamShared& sh, uint64_t x, int keep) {
-  const int tid = threadIdx.x, size = keep <= 16 ? kThreads / 64 : kThreads / 128, n_sets = kThreads / size;
+  const int tid = threadIdx.x, size = keep <= 17 ? kThreads / 64 : kThreads / 128, n_sets = kThreads / size;
   for (int o = 1; o < size; o <<= 1) {
     const uint64_t y = __shfl_xor_sync(~0u, x, o);
     x = y > x ? y : x;
@@ -276,7 +299,7 @@ __device__ __forceinline__ uint64_t set_bound_key(BeamShared& sh, uint64_t x, in
 // are equal. A merge's list is sorted by parts, so for the bound neighbours go
 // to sets far from each other (37 * 429 = 1 mod 512): taken in order, the best
 // of 64 rows fell into 8 sets, too many reached the bound, and 4 groups of 64
-// beams to 64 took 580 us; they take 24.
+// beams to 64 took 580 us; they take 27.
 template <typename F>
 __device__ __forceinline__ void rank_list(BeamShared& sh, int n, int keep, F&& emit) {
   const uint64_t* list = sh.list;
@@ -328,6 +351,62 @@ __device__ __forceinline__ void rank_list(BeamShared& sh, int n, int keep, F&& e
   }
 }
 
+// The answer's places of total z, its lowest, where a part may have missed a
+// token of that total. All that such a part listed have z or more, so that the
+// first of them has enough for the places after those of earlier parts: its
+// first tokens of total z, in order.
+template <typename T>
+__device__ __noinline__ void repair(const BeamArgs& a, BeamShared& sh, int64_t row0, int64_t slot0, int parts, float z) {
+  constexpr int kLoads = 16;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) sh.again = INT32_MAX;
+  sync_threads();
+  for (int c = tid; c < a.n_beams * parts; c += kThreads) {
+    const float next = __ldcg(a.slice_next + 2 * (slot0 + c)), least = __ldcg(a.slice_next + 2 * (slot0 + c) + 1);
+    const int b = c / parts;
+    auto total = [&](float x) { return a.scores[row0 + b] + ((x - sh.row_top[b]) - sh.row_log[b]); };
+    // Logits equal to the least listed have higher tokens than it: none is missed
+    // where no other value has their total.
+    if (next > kNegInf && total(next) >= z &&
+        (next < least || total(neighbour<T>(least, false)) >= z || total(neighbour<T>(least, true)) <= z))
+      atomicMin(&sh.again, c);
+  }
+  sync_threads();
+  if (sh.again == INT32_MAX) return;
+  const int b = sh.again / parts;
+  const int64_t i0 = (int64_t)(sh.again - b * parts) * a.per * a.slice;
+  const int64_t i1 = min((int64_t)a.vocab, i0 + (int64_t)a.per * a.slice);
+  const uint32_t base = (uint32_t)(b * (int64_t)a.vocab);
+  const T* x0 = static_cast<const T*>(a.logits) + (row0 + b) * a.row_stride;
+  const float score = a.scores[row0 + b], top = sh.row_top[b], log = sh.row_log[b];
+  const uint64_t mine = tid < a.n_out ? sh.best[tid] : 0;
+  int have = count_threads(mine && (key_value(mine) > z || key_index(mine) < base + (uint32_t)i0));
+  for (int64_t i = i0; i < i1 && have < a.n_out; i += kLoads * kThreads) {
+    T x[kLoads];
+#pragma unroll
+    for (int r = 0; r < kLoads; ++r)
+      if (i + r * kThreads + tid < i1) x[r] = x0[i + r * kThreads + tid];
+    uint32_t hits = 0;
+#pragma unroll
+    for (int r = 0; r < kLoads; ++r)
+      if (i + r * kThreads + tid < i1 && score + (((float)x[r] - top) - log) == z) hits |= 1u << r;
+    if (!count_threads(hits != 0)) continue;
+    for (int r = 0; r < kLoads && have < a.n_out; ++r) {
+      const uint32_t found = __ballot_sync(~0u, hits >> r & 1);
+      if (lane == 0) sh.warp_key[warp] = __popc(found);
+      sync_threads();
+      int at = have + __popc(found & ((1u << lane) - 1));
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) at += (int)sh.warp_key[w];
+        have += (int)sh.warp_key[w];
+      }
+      if ((hits >> r & 1) && at < a.n_out) sh.best[at] = make_key(z, base + (uint32_t)(i + r * kThreads + tid));
+      sync_threads();
+    }
+  }
+  sync_threads();
+}
+
 // Ends a part, elements [i0, i1) of a row: its maximum, sum and best
 // candidates; then, in the last block of the group, the answer.
 template <typename T>
@@ -344,6 +423,7 @@ __device__ __noinline__ void finish(const BeamArgs& a, BeamShared& sh, int row, 
     if (tid == 0) {
       a.slice_stats[2 * slot] = one ? 0.f : kNegInf;
       a.slice_stats[2 * slot + 1] = one ? 1.f : 0.f;
+      a.slice_next[2 * slot] = kNegInf;
     }
   } else {
     warp_softmax(m, l);
@@ -351,7 +431,7 @@ __device__ __noinline__ void finish(const BeamArgs& a, BeamShared& sh, int row, 
       sh.m[warp] = m;
       sh.l[warp] = l;
     }
-    for (int c = tid; c < a.n_out; c += kThreads) sh.best[c] = 0;
+    for (int c = tid; c <= a.n_out; c += kThreads) sh.best[c] = 0;
     sync_threads();
     if (warp == kWarps - 1) {
       m = lane < kWarps ? sh.m[lane] : kNegInf;
@@ -364,12 +444,12 @@ __device__ __noinline__ void finish(const BeamArgs& a, BeamShared& sh, int row, 
     }
     const int found = sh.n;
     if (found <= kList) {
-      rank_list(sh, found, a.n_out, [&](uint64_t k, int r) { sh.best[r] = k; });
+      rank_list(sh, found, a.n_out + 1, [&](uint64_t k, int r) { sh.best[r] = k; });
     } else {
       // many logits reach the bound: one best after the other, read again
       const T* x0 = static_cast<const T*>(a.logits) + row * a.row_stride;
       uint64_t before = ~0ull;
-      for (int o = 0; o < a.n_out; ++o) {
+      for (int o = 0; o <= a.n_out; ++o) {
         uint64_t best = 0;
 #pragma unroll 4
         for (int64_t i = i0 + tid; i < i1; i += kThreads) {
@@ -383,6 +463,10 @@ __device__ __noinline__ void finish(const BeamArgs& a, BeamShared& sh, int row, 
     }
     sync_threads();
     for (int c = tid; c < a.n_out; c += kThreads) keys[c] = sh.best[c];
+    if (tid == 0) {
+      a.slice_next[2 * slot] = sh.best[a.n_out] ? key_value(sh.best[a.n_out]) : kNegInf;
+      a.slice_next[2 * slot + 1] = sh.best[a.n_out] ? key_value(sh.best[a.n_out - 1]) : kNegInf;
+    }
   }
 
   // the last block of the group goes on
@@ -405,17 +489,25 @@ __device__ __noinline__ void finish(const BeamArgs& a, BeamShared& sh, int row, 
   for (int b = warp; b < a.n_beams; b += kWarps) {  // the rows' maxima and sums
     m = kNegInf;
     l = 0.f;
+    const float score = a.scores[row0 + b];
+    float next = kNegInf;
     for (int i = lane; i < parts; i += 32) {
-      const float* st = a.slice_stats + 2 * (slot0 + (int64_t)b * parts + i);
+      const int64_t part = slot0 + (int64_t)b * parts + i;
+      const float* st = a.slice_stats + 2 * part;
       const float mi = __ldcg(st), li = __ldcg(st + 1);
+      next = fmaxf(next, __ldcg(a.slice_next + 2 * part));
       const float mn = fmaxf(m, mi), mg = mn == kNegInf ? 0.f : mn;
       l = l * ex2((m - mg) * kLog2e) + li * ex2((mi - mg) * kLog2e);
       m = mn;
     }
     warp_softmax(m, l);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) next = fmaxf(next, __shfl_xor_sync(~0u, next, o));
     if (lane == 0) {
+      const float log = logf(l);
       sh.row_top[b] = m;
-      sh.row_log[b] = logf(l);
+      sh.row_log[b] = log;
+      sh.row_next[b] = next > kNegInf ? score + ((next - m) - log) : kNegInf;
     }
   }
   sync_threads();
@@ -431,6 +523,12 @@ __device__ __noinline__ void finish(const BeamArgs& a, BeamShared& sh, int row, 
   sync_threads();
   rank_list(sh, all, a.n_out, [&](uint64_t k, int r) { sh.best[r] = k; });
   sync_threads();
+  if (sh.best[a.n_out - 1]) {  // else every candidate has a place
+    const float z = key_value(sh.best[a.n_out - 1]);
+    bool tied = false;
+    for (int b = lane; b < a.n_beams; b += 32) tied |= sh.row_next[b] >= z;
+    if (__any_sync(~0u, tied)) repair<T>(a, sh, row0, slot0, parts, z);
+  }
   for (int r = tid; r < a.n_out; r += kThreads) {
     const uint64_t k = sh.best[r];
     const uint32_t index = key_index(k);
@@ -557,7 +655,7 @@ __global__ void __launch_bounds__(kThreads + 32, kBeamPerSm) k_beam_select(const
     bool rose = false;
     if (it == 0 || it == 2 || (it & 7) == 7 || tau == kNegInf) {
       const float before = tau;
-      tau = set_bound(sh, m, a.n_out);
+      tau = set_bound(sh, m, a.n_out + 1);
       rose = tau > before;
       if (rose) least = tau;
     }
@@ -569,9 +667,9 @@ __global__ void __launch_bounds__(kThreads + 32, kBeamPerSm) k_beam_select(const
         for (int i = 0; i < E; ++i) hits |= (elem<T>(g[r], i) >= least ? 1u : 0u) << (r * E + i);
     }
     if (rose) {
-      // Logits equal to the bound matter in the slice that raised it alone (n_out
+      // Logits equal to the bound matter in the slice that raised it alone (n_out + 1
       // others with lower tokens reach it for later ones), and of these the first
-      // n_out: of 256 rows masked with the lowest value all were gathered, and
+      // n_out + 1: of 256 rows masked with the lowest value all were gathered, and
       // then read again and again, in 689 us.
       if (count_threads(hits != 0) > kThreads / 4) {
         uint32_t equal = 0;
@@ -580,7 +678,7 @@ __global__ void __launch_bounds__(kThreads + 32, kBeamPerSm) k_beam_select(const
           const float v = (float)(reinterpret_cast<const T*>(ring + stage * kStage))[e + mis];
           if (v == tau) equal |= 1u << b;
         }
-        hits &= ~past_first(sh, equal, E, a.n_out);
+        hits &= ~past_first(sh, equal, E, a.n_out + 1);
       }
       least = next_up(tau);
     }

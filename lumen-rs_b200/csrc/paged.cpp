@@ -579,11 +579,12 @@ int lc_beam_select(lc_beam* b, int32_t n_groups, const void* logits, int32_t dty
     const cudaStream_t s = turn.s;
     const size_t keys = b->lists * b->n_out;
     uint8_t* w = static_cast<uint8_t*>(
-        b->ws.get(keys * 8 + (2 * b->lists + b->n_groups) * 4, b->device, s, turn.captured, true));
+        b->ws.get(keys * 8 + (4 * b->lists + b->n_groups) * 4, b->device, s, turn.captured, true));
     BeamArgs a{};
     a.slice_key = reinterpret_cast<uint64_t*>(w);
     a.slice_stats = reinterpret_cast<float*>(a.slice_key + keys);
-    a.counters = reinterpret_cast<int32_t*>(a.slice_stats + 2 * b->lists);
+    a.slice_next = a.slice_stats + 2 * b->lists;
+    a.counters = reinterpret_cast<int32_t*>(a.slice_next + 2 * b->lists);
     a.logits = logits;
     a.dtype = dtype;
     a.row_stride = row_stride;

@@ -121,6 +121,7 @@ struct BeamArgs {
   uint8_t* finished_out;
   // workspace, by the parts of a row (at most one a slice)
   float* slice_stats;   // [rows][parts][2]: max, sum exp(x - max)
+  float* slice_next;    // [rows][parts][2]: the largest logit that is not listed (-inf: none), the least listed
   uint64_t* slice_key;  // [rows][parts][n_out]: (logit, token), best first, 0 for none
   int32_t* counters;    // [n_groups], zero between calls
 };

@@ -171,3 +171,65 @@ def test_select_captured(lc, gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def check_f32(lc, x, scores, n_out, pad=0):
+    """Against the definition in f32, whose totals the kernel's are equal to where the sums' logarithms are: rows
+    whose other logits are 150 and more below one (its sum is 1), or totals whose steps are far above the logarithm."""
+    g, beams, vocab = x.shape
+    got = [t.cpu().numpy() for t in lc.BeamSearch(g, beams, vocab, n_out).select(x, torch.from_numpy(scores).cuda(), pad_id=pad)]
+    xs = x.float().cpu().numpy()
+    for i in range(g):
+        d = xs[i] - xs[i].max(1, keepdims=True)
+        z = scores[i][:, None] + (d - np.log(np.exp(d.astype(np.float64)).sum(1, keepdims=True)).astype(np.float32))
+        assert z.dtype == np.float32
+        z = z.reshape(-1)
+        order = np.argsort(-z, kind="stable")[:n_out]
+        m = len(order)
+        np.testing.assert_array_equal(got[0][i, :m], z[order])
+        np.testing.assert_array_equal(got[1][i, :m], order // vocab)
+        np.testing.assert_array_equal(got[2][i, :m], order % vocab)
+        assert np.isinf(got[0][i, m:]).all() and (got[3][i, m:] == 1).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("score", [-0.5, -300.0, -1e4, -1e9])
+@pytest.mark.parametrize("groups,beams,vocab,n_out", [(1, 1, 30011, 1), (1, 1, 30011, 2), (2, 4, 30011, 9), (3, 8, 9001, 64),
+                                                      (60, 4, 20001, 5), (300, 1, 9000, 7), (2, 2, 3, 5)])
+def test_select_equal_totals_of_different_logits(lc, gpu, dtype, score, groups, beams, vocab, n_out):
+    """Logits that differ by less than a step of their totals: the lower token goes first."""
+    g = torch.Generator().manual_seed(vocab + n_out)
+    x = (-200 - torch.rand((groups, beams, vocab), generator=g)).cuda()
+    x.scatter_(2, torch.randint(0, vocab, (groups, beams, 1), generator=g).cuda(), 0.0)
+    # all beams alike, or one far ahead, or steps apart that are a few of a total's
+    scores = np.full((groups, beams), score, np.float32)
+    scores[1::3] = np.float32(-1e9)
+    scores[1::3, beams // 2] = np.float32(score)
+    scores[2::3] = score * (1 + 2.0 ** -20 * np.arange(beams, dtype=np.float32))
+    check_f32(lc, x.to(ref.DTYPES[dtype]), scores, n_out)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_select_equal_logits_beside_equal_totals(lc, gpu, dtype):
+    """More equal logits than places, with a larger logit of the same total behind them."""
+    x = torch.full((2, 1, 20000), -200.0, device="cuda")
+    x[:, 0, 5] = 0.0
+    x[0, 0, 1000::9] = -199.0
+    x[0, 0, 15000] = -198.0
+    x[1, 0, :3] = -250.0
+    x[1, 0, 19999] = -199.0
+    x = x.to(ref.DTYPES[dtype])
+    for score in (-1.0, -1e9):
+        for n_out in (1, 2, 3, 12):
+            check_f32(lc, x, np.full((2, 1), score, np.float32), n_out)
+
+
+def test_select_infinite_and_huge_scores(lc, gpu):
+    """Scores that leave every candidate of a beam the same total."""
+    x, _, _ = inputs(3, 3, 5001, "f32", 8)
+    scores = np.array([[1e30, -1e30, -3e38], [np.inf, 0, np.inf], [-1e9, 0, -1e9]], np.float32)
+    for n_out in (1, 4, 40):
+        check_f32(lc, x[:2].contiguous(), scores[:2], n_out)
+    few = x[2:, :, :5].contiguous()
+    few[0, 1] = torch.tensor([0.0, -200, -201, -202, -203])
+    check_f32(lc, few, scores[2:], 12)
