@@ -541,8 +541,10 @@ int lc_paged_create(const lc_paged_config* config, void* k_pages, void* v_pages,
 void lc_paged_destroy(lc_paged* p);
 
 /* LC_ERR_INVALID once a call met a length beyond its table, a page id outside
- * the pool or a parent outside its group (that call's output is unspecified).
- * Reads a host word: synchronise first to hear of calls in flight. */
+ * the pool or a parent outside its group (that call's output is unspecified);
+ * LC_ERR_TIMEOUT once a bounded wait for a copy ran out (the output is NaN
+ * where the copy's slots count). It stays so for the handle's life. Reads host
+ * words: synchronise first to hear of calls in flight. */
 int lc_paged_status(const lc_paged* p);
 
 /* Write keys / values [n_seqs][n_kv_heads][n_tokens][head_dim] of `dtype` to
@@ -605,6 +607,10 @@ typedef struct lc_beam lc_beam;
  * of `vocab` (<= 2^24) logits, n_out (<= 64) chosen of each group. */
 int lc_beam_create(int32_t n_groups, int32_t n_beams, int64_t vocab, int32_t n_out, int32_t device, lc_beam** out);
 void lc_beam_destroy(lc_beam* b);
+
+/* LC_ERR_TIMEOUT once a bounded wait for a copy ran out (that row gave no
+ * candidates); as lc_paged_status. */
+int lc_beam_status(const lc_beam* b);
 
 /* Of every group's totals scores[b] + log_softmax(logits[b])[v] the n_out
  * largest (as f32), best first, equal ones by lower b * vocab + v: scores_out, parents,

@@ -57,7 +57,8 @@ ABI_SYMBOLS = [
     "lc_ring_update", "lc_ring_truncate_to", "lc_ring_counters", "lc_ring_read", "lc_ring_clear",
     "lc_ring_deep_clone", "lc_ring_destroy", "lc_version", "lc_save_lkv2", "lc_load_lkv2", "lc_lkv2_info",
     "lc_paged_create", "lc_paged_destroy", "lc_paged_status", "lc_paged_append", "lc_paged_attn", "lc_paged_attn_weights",
-    "lc_paged_evict", "lc_paged_reorder", "lc_beam_create", "lc_beam_destroy", "lc_beam_select",
+    "lc_paged_evict", "lc_paged_reorder", "lc_beam_create", "lc_beam_destroy", "lc_beam_status",
+    "lc_beam_select",
 ]
 
 
@@ -171,6 +172,7 @@ def lib():
         "lc_paged_reorder": (C.c_int, [vp, i32, i32, vp, i32, vp, vp, vp, vp]),
         "lc_beam_create": (C.c_int, [i32, i32, i64, i32, i32, pp]),
         "lc_beam_destroy": (None, [vp]),
+        "lc_beam_status": (C.c_int, [vp]),
         "lc_beam_select": (C.c_int, [vp, i32, vp, i32, i64, vp, vp, i32, i32, vp, vp, vp, vp, vp]),
     }
     for name, (res, args) in sig.items():
@@ -917,7 +919,8 @@ class PagedKvCache:
             _dev(lens, "lens", (n,), "int32", self.device)
 
     def status(self) -> int:
-        """LC_OK, or LC_ERR_INVALID once a finished call met a length, page id or parent out of range."""
+        """LC_OK, LC_ERR_INVALID once a finished call met a length, page id or parent out of range, or
+        LC_ERR_TIMEOUT once a copy did not end in time (outputs are NaN then)."""
         return lib().lc_paged_status(self._h)
 
     def append(self, layer: int, tables, lens, keys, values, pos=None, pos0=None, stream=None):
@@ -1026,6 +1029,10 @@ class BeamSearch:
             self._h = None
 
     __del__ = close
+
+    def status(self) -> int:
+        """LC_OK, or LC_ERR_TIMEOUT once a copy of a finished call did not end in time (its row gave no candidates)."""
+        return lib().lc_beam_status(self._h)
 
     def select(self, logits, scores, finished=None, *, eos_id: int = -1, pad_id: int = 0, stream=None):
         """The n_out best totals scores + log_softmax(logits) of each group, best first: (scores f32,

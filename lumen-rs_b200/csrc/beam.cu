@@ -29,7 +29,7 @@
 // the one after them. Only where that has the total of the answer's last place,
 // the first such part is read again (see repair).
 //
-// 256 rows of 131072 bf16 logits take 32.4 us, 2.1 TB/s; 64 groups of 4 rows of
+// 256 rows of 131072 bf16 logits take 32.7 us, 2.1 TB/s; 64 groups of 4 rows of
 // 1000 f32 13.3; 4 rows of 50021 f32 14.0. So half is the chain of launch, first
 // copy, bound, ranking, the counter's round trip and the merge, all of it
 // latency; the other half runs at 0.65 of the pace that a copy of the card's
@@ -609,9 +609,8 @@ __global__ void __launch_bounds__(kThreads + 32, kBeamPerSm) k_beam_select(const
       }
       __syncwarp();
     }
-    // where no one else does, await the copies in flight
-    if (done || !(score > kNegInf))
-      for (int i = 0; i < it; ++i) mbar_wait(full + 8 * i, 0);
+    // the copies in flight, which no one may be waiting for
+    for (int i = max(0, it - kStages); i < it; ++i) mbar_wait(full + 8 * (i % kStages), i / kStages & 1);
     return;
   }
 
@@ -619,11 +618,15 @@ __global__ void __launch_bounds__(kThreads + 32, kBeamPerSm) k_beam_select(const
   const bool dead = done || !(score > kNegInf);
   float m = kNegInf, tau = kNegInf, least = next_up(kNegInf);  // least: of the logits to gather
   uint64_t l = pack2(0.f, 0.f);  // the sum in two halves
+  bool lost = false;
   const uint64_t log2e = pack2(kLog2e, kLog2e);
 #pragma unroll 1
   for (int it = 0; it < slices && !dead; ++it) {
     const int stage = it % kStages;
-    if (!mbar_wait(full + 8 * stage, it / kStages & 1)) l = pack2(NAN, NAN);  // a copy that never came: no candidates
+    if (!lost && !mbar_wait(full + 8 * stage, it / kStages & 1)) {  // a copy that did not come: no candidates
+      lost = true;
+      a.status[kTimedOut] = 1;
+    }
     const uint4* x = ring + stage * kStage + tid;
     uint4 g[kGran];
 #pragma unroll
@@ -693,7 +696,7 @@ __global__ void __launch_bounds__(kThreads + 32, kBeamPerSm) k_beam_select(const
   }
   const float2 halves = unpack2(l);
   finish<T>(a, sh, row, (int64_t)slice0 * a.slice, min((int64_t)a.vocab, (int64_t)(slice0 + slices) * a.slice), done, dead,
-            m, halves.x + halves.y, tau);
+            m, lost ? NAN : halves.x + halves.y, tau);
 }
 
 }  // namespace

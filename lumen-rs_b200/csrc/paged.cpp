@@ -121,21 +121,21 @@ struct Workspace {
   }
 };
 
-// Words of mapped host memory, one a handle, from pages that are kept.
+// Status words in mapped host memory, a cache line a handle, from pages that are kept.
 struct StatusWords {
   std::mutex mu;
   std::vector<int32_t*> free;
   int32_t* take() {
     std::lock_guard<std::mutex> lock(mu);
     if (free.empty()) {
-      constexpr int kWords = 256;  // each on a cache line of its own
+      constexpr int kLines = 256;
       int32_t* page = nullptr;
-      LC_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&page), kWords * 64, cudaHostAllocMapped | cudaHostAllocPortable));
-      for (int i = 0; i < kWords; ++i) free.push_back(page + 16 * i);
+      LC_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&page), kLines * 64, cudaHostAllocMapped | cudaHostAllocPortable));
+      for (int i = 0; i < kLines; ++i) free.push_back(page + 16 * i);
     }
     int32_t* w = free.back();
     free.pop_back();
-    *w = 0;
+    std::fill(w, w + kStatusBits, 0);
     return w;
   }
   void give(int32_t* w) {
@@ -192,6 +192,23 @@ struct Turn {
   Turn& operator=(const Turn&) = delete;
 };
 
+// A handle's status words and their address on the device.
+struct Status {
+  int32_t* words = nullptr;
+  int32_t* on_device = nullptr;
+  ~Status() {
+    if (words) status_words().give(words);
+  }
+  void make() {
+    words = status_words().take();
+    LC_CUDA(cudaHostGetDevicePointer(reinterpret_cast<void**>(&on_device), words, 0));
+  }
+  void check() const {
+    const int code = status_code(words);
+    LC_REQUIRE(code == LC_OK, code, status_message(code));
+  }
+};
+
 int sm_count(int device) {
   int n = 0;
   LC_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device));
@@ -207,10 +224,7 @@ struct lc_paged {
   int sms = 0, esize = 0;
   Order order;
   Workspace part, counters, scores, evict;
-  int32_t* status = nullptr;  // mapped host word
-  ~lc_paged() {
-    if (status) status_words().give(status);
-  }
+  Status status;
 
   PagedView call(const int32_t* tables, int32_t width, const int32_t* lens, int32_t rows) const {
     LC_REQUIRE(rows >= 1 && rows <= cfg.max_seqs, LC_ERR_INVALID,
@@ -236,6 +250,7 @@ struct lc_beam {
   size_t lists = 0;
   Order order;
   Workspace ws;
+  Status status;
 };
 
 extern "C" {
@@ -286,9 +301,7 @@ int lc_paged_create(const lc_paged_config* config, void* k_pages, void* v_pages,
     p->cfg = c;
     p->esize = element_size(c.dtype);
     p->sms = sm_count(c.device);
-    p->status = status_words().take();
-    int32_t* dev_status = nullptr;
-    LC_CUDA(cudaHostGetDevicePointer(reinterpret_cast<void**>(&dev_status), p->status, 0));
+    p->status.make();
     p->view.k = k_pages;
     p->view.v = v_pages;
     p->view.layer = c.n_layers == 1 ? 0 : c.layer_stride;
@@ -300,7 +313,7 @@ int lc_paged_create(const lc_paged_config* config, void* k_pages, void* v_pages,
     p->view.d = c.head_dim;
     p->view.page_tokens = c.page_tokens;
     p->view.n_pages = c.n_pages;
-    p->view.status = dev_status;
+    p->view.status = p->status.on_device;
     p->maps = make_paged_maps(p->view, c.dtype);
     *out = p.release();
   });
@@ -320,8 +333,7 @@ void lc_paged_destroy(lc_paged* p) {
 int lc_paged_status(const lc_paged* p) {
   return abi_guard([&] {
     LC_REQUIRE(p, LC_ERR_INVALID, "null handle");
-    LC_REQUIRE(*static_cast<volatile int32_t*>(p->status) == 0, LC_ERR_INVALID,
-               "a call met a length beyond its table, a page id outside the pool or a parent outside its group");
+    p->status.check();
   });
 }
 
@@ -539,6 +551,7 @@ int lc_beam_create(int32_t n_groups, int32_t n_beams, int64_t vocab, int32_t n_o
     const size_t rows = (size_t)n_groups * n_beams;
     const size_t lists = rows * std::min<int64_t>(slices, std::max(1, kBeamMaxMerge / (n_beams * n_out)));
     b->lists = lists;
+    b->status.make();
     *out = b.release();
   });
 }
@@ -552,6 +565,13 @@ void lc_beam_destroy(lc_beam* b) {
   cudaDeviceSynchronize();
   delete b;
   if (before >= 0 && before != device) cudaSetDevice(before);
+}
+
+int lc_beam_status(const lc_beam* b) {
+  return abi_guard([&] {
+    LC_REQUIRE(b, LC_ERR_INVALID, "null handle");
+    b->status.check();
+  });
 }
 
 int lc_beam_select(lc_beam* b, int32_t n_groups, const void* logits, int32_t dtype, int64_t row_stride,
@@ -602,6 +622,7 @@ int lc_beam_select(lc_beam* b, int32_t n_groups, const void* logits, int32_t dty
     a.parents = parents;
     a.tokens = tokens;
     a.finished_out = finished_out;
+    a.status = b->status.on_device;
     launch_beam(a, b->device, b->sms, s);
   });
 }

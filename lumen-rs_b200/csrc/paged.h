@@ -9,6 +9,7 @@
 #include <atomic>
 
 #include "common.h"
+#include "status.h"
 
 namespace lc {
 
@@ -36,7 +37,7 @@ struct PagedView {
   const int32_t* tables;  // [rows][width]
   const int32_t* lens;
   int32_t width;
-  int32_t* status;  // mapped host word: set when a length or a page id is out of range
+  int32_t* status;  // mapped host words, by StatusBit
 };
 
 // TMA descriptors of the two pools; box: slots of a load, 0 where there are none.
@@ -115,6 +116,7 @@ struct BeamArgs {
   const float* scores;
   const uint8_t* finished;  // may be null
   int32_t eos, pad;
+  int32_t* status;  // mapped host words, by StatusBit
   float* scores_out;
   int32_t* parents;
   int32_t* tokens;

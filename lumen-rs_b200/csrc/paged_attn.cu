@@ -58,7 +58,7 @@ __device__ __forceinline__ void store_f32(void* p, int64_t i, int dtype, float x
 __device__ __forceinline__ int clamp_len(const PagedView& c, int s) {
   const int cap = c.width * c.page_tokens, n = c.lens[s];
   if (n < 0 || n > cap) {
-    *c.status = 1;
+    c.status[kBadInput] = 1;
     return n < 0 ? 0 : cap;
   }
   return n;
@@ -71,7 +71,7 @@ __device__ __forceinline__ int first_slot(int n, int window) { return window > 0
 __device__ __forceinline__ int64_t row_offset(const PagedView& c, int s, int t) {
   const int page = c.tables[(int64_t)s * c.width + t / c.page_tokens];
   if (page < 0 || page >= c.n_pages) {
-    *c.status = 1;
+    c.status[kBadInput] = 1;
     return -1;
   }
   return page * c.page + (int64_t)(t % c.page_tokens) * c.token;
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(W * 32, ST > 1 ? 1 : 2) k_paged_attn(const Pag
     auto row_of = [&](int j, int page) -> int64_t {
       const int t = g.t0 + j * TT + lane;
       if (page >= 0 && page < a.c.n_pages) return page * a.c.page + (int64_t)(t % a.c.page_tokens) * a.c.token;
-      if (page != INT32_MIN) *a.c.status = 1;
+      if (page != INT32_MIN) a.c.status[kBadInput] = 1;
       return -1;
     };
     auto issue = [&](int j, int stage, int page) {
@@ -669,7 +669,7 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
 // items' ends and beginnings (3.7 us each) and SMs that reach the memory at
 // different speeds (blocks with equal shares end between 0.75 and 1 of the
 // whole time). 16 sequences of up to 4096 under a window of 1024, 8 heads of
-// 256 f16: 28.6 us, 4.0 TB/s, where the first two are a third.
+// 256 f16: 28.8 us, 4.0 TB/s, where the first two are a third.
 template <typename T, int DP, int W, int ST, bool TMA, int PER_SM>
 __global__ void __launch_bounds__(W * 32, PER_SM)
     k_paged_attn_mma(const PagedAttnArgs a, const __grid_constant__ CUtensorMap k_map,
@@ -710,6 +710,7 @@ __global__ void __launch_bounds__(W * 32, PER_SM)
   auto k_frag = [&](int i) -> uint32_t { return TMA ? (i >> 2) * 2048 + k_at[i & (TMA ? 3 : 0)] : k_at[0] + i * 32; };
   auto v_frag = [&](int i) -> uint32_t { return TMA ? (i >> 2) * 2048 + v_at[i & (TMA ? 3 : 0)] : v_at[0] + i * 32; };
   uint32_t phases = 0;
+  bool lost = false;  // TMA: a copy of this warp's did not come; it loads no more, and its sums are NaN
   for (int u = blockIdx.x * per; u < u_end;) {
     const Segment g = find_segment(a, prefix, TT, kCost, hh_n, per, u, u_end);
     u = g.next;
@@ -732,9 +733,9 @@ __global__ void __launch_bounds__(W * 32, PER_SM)
     auto issue = [&](int j, int stage, int page) {
       const uint32_t to = stages + stage * 2 * TILE;
       if constexpr (TMA) {
-        if (j >= g.j1) return;
+        if (j >= g.j1 || lost) return;
         if (page < 0 || page >= a.c.n_pages) {
-          *a.c.status = 1;
+          a.c.status[kBadInput] = 1;
           page = 0;
         }
         const int page1 = __shfl_sync(~0u, page, 1);
@@ -758,7 +759,7 @@ __global__ void __launch_bounds__(W * 32, PER_SM)
           if (page >= 0 && page < a.c.n_pages)
             off = page * a.c.page + (int64_t)(t % a.c.page_tokens) * a.c.token;
           else if (page != INT32_MIN)
-            *a.c.status = 1;
+            a.c.status[kBadInput] = 1;
 #pragma unroll
           for (int x = 0; x < TT * CH / 32; ++x) {
             const int e = x * 32 + lane, r = e / CH, c = e - r * CH;
@@ -799,12 +800,20 @@ __global__ void __launch_bounds__(W * 32, PER_SM)
       issue(first + i * W, i, now);
     }
     int stage = 0, fill = ST - 1;
-    for (int j = first; j < g.j1; j += W) {
+    for (int j = first; j < g.j1 && !lost; j += W) {
       const uint32_t kt = stages + stage * 2 * TILE, vt = kt + TILE;
       if constexpr (TMA) {
         __syncwarp();  // the stage to fill has been read
         issue(j + (ST - 1) * W, fill, page);
-        if (!mbar_wait(bar + 8 * stage, phases >> stage & 1)) *a.c.status = 2;
+        if (!__all_sync(~0u, mbar_wait(bar + 8 * stage, phases >> stage & 1))) {
+          a.c.status[kTimedOut] = 1;
+          lost = true;
+          for (int i = 1, at = stage; i < ST; ++i) {  // the others in flight, as long again each
+            at = at + 1 == ST ? 0 : at + 1;
+            if (j + i * W < g.j1) mbar_wait(bar + 8 * at, phases >> at & 1);
+          }
+          break;
+        }
         phases ^= 1u << stage;
         const int t = g.t0 + j * TT;
         if (t < g.lo || t + TT > g.n) {  // rows outside: zeros in place of what memory held
@@ -886,6 +895,7 @@ __global__ void __launch_bounds__(W * 32, PER_SM)
       }
     }
     if constexpr (!TMA) cp_wait<0>();
+    if (TMA && lost) l0 = l1 = NAN;
 #pragma unroll
     for (int b = 4; b < 32; b <<= 1) {
       l0 += __shfl_xor_sync(~0u, l0, b);
@@ -1054,7 +1064,7 @@ __global__ void __launch_bounds__(256) k_paged_append(const PagedAppendArgs a) {
       const int tok = (int)(r - sh * a.n_tokens), s = (int)(sh / a.c.hkv), h = (int)(sh - (int64_t)s * a.c.hkv);
       const int64_t t = (int64_t)a.c.lens[s] + tok;
       if (t < 0 || t >= (int64_t)a.c.width * a.c.page_tokens) {
-        *a.c.status = 1;
+        a.c.status[kBadInput] = 1;
       } else {
         to = row_offset(a.c, s, (int)t);
         if (to >= 0) {

@@ -80,7 +80,7 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t x, uint64_t* warp_sum, u
 __device__ __forceinline__ int64_t page_row(const PagedView& c, int s, int t) {
   const int page = c.tables[(int64_t)s * c.width + t / c.page_tokens];
   if (page < 0 || page >= c.n_pages) {
-    *c.status = 1;
+    c.status[kBadInput] = 1;
     return -1;
   }
   return page * c.page + (int64_t)(t % c.page_tokens) * c.token;
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (!CL) hold(0, cap);  // a row's only block need not wait for its length to read ahead
   int n = a.c.lens[s];
   if (n < 0 || n > cap) {
-    *a.c.status = 1;
+    a.c.status[kBadInput] = 1;
     n = n < 0 ? 0 : cap;
   }
   const int per = CL ? (n + cl - 1) / cl : n, b = min(n, rank * per), e = min(n, b + per);
@@ -381,14 +381,14 @@ __global__ void __launch_bounds__(kReorderThreads) k_paged_reorder(const PagedRe
   if (tid < w) {
     p = a.parents[(int64_t)g * w + tid];
     if (p < 0 || p >= w) {
-      *a.c.status = 1;
+      a.c.status[kBadInput] = 1;
       p = tid;
     }
     parent[tid] = p;
     first[tid] = INT32_MAX;
   }
   if (n < 0 || n > cap) {
-    *a.c.status = 1;
+    a.c.status[kBadInput] = 1;
     n = n < 0 ? 0 : cap;
   }
   __syncthreads();
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kReorderThreads) k_paged_reorder(const PagedRe
     if (extra && fill > 0) {
       const int from = tables[(int64_t)p * a.c.width + full], to = tables[(int64_t)spare[at] * a.c.width + full];
       const bool bad = from < 0 || from >= a.c.n_pages || to < 0 || to >= a.c.n_pages;
-      if (bad) *a.c.status = 1;
+      if (bad) a.c.status[kBadInput] = 1;
       src[at] = bad ? -1 : from * a.c.page;
       dst[at] = to * a.c.page;
     }
