@@ -891,6 +891,8 @@ class PagedKvCache:
             raise ValueError("k_pages and v_pages must be on one GPU")
         if v_pages.stride() != k_pages.stride() or (k_pages.shape[4] > 1 and k_pages.stride(4) != 1):
             raise ValueError("k_pages and v_pages must have the same strides, 1 in the last dimension")
+        if not any(k_pages.stride()[:4]) and k_pages.shape[:4].numel() > 1:  # to lc_paged_create: contiguous
+            raise ValueError("k_pages and v_pages must not be expanded from a single row")
         self.k_pages, self.v_pages = k_pages, v_pages
         self.n_layers, self.n_pages, self.n_kv_heads, self.page_tokens, self.head_dim = k_pages.shape
         self.device = k_pages.device.index

@@ -715,3 +715,13 @@ def test_calls_on_streams_in_turn(lc, gpu):
         outs.append((out, a, p))
     for got in outs[1:]:
         assert all(torch.equal(x, y) for x, y in zip(got, outs[0]))
+
+
+def test_expanded_pools_are_refused(lc, gpu):
+    """Strides of zero everywhere stand for a contiguous pool at the C entry, of which these have one row."""
+    row = torch.zeros((1, 1, 1, 1, 64), dtype=torch.bfloat16, device="cuda")
+    for shape in ((2, 4, 2, 16, 64), (1, 1, 1, 16, 64), (1, 8, 1, 1, 64)):
+        with pytest.raises((ValueError, lc.LumenError)):
+            lc.PagedKvCache(row.expand(shape), row.clone().expand(shape), max_seqs=1, max_pages_per_seq=1, max_q_heads=2)
+    lone = torch.zeros(64, dtype=torch.bfloat16, device="cuda").as_strided((1, 1, 1, 1, 64), (0, 0, 0, 0, 1))
+    lc.PagedKvCache(lone, lone.clone().as_strided((1, 1, 1, 1, 64), (0, 0, 0, 0, 1)), max_seqs=1, max_pages_per_seq=1, max_q_heads=1)
