@@ -928,7 +928,8 @@ int attn_grid(const PagedAttnArgs& a, int gp, int tile, int cost, int most) {
   const int64_t cap = (int64_t)a.c.width * a.c.page_tokens;
   const int64_t seen = a.window > 0 ? std::min<int64_t>(cap, a.window) : cap;
   const int64_t items = (int64_t)a.n_seqs * a.c.hkv * ((a.group + gp - 1) / gp);
-  const int64_t tiles = items * ((seen + tile - 1) / tile + cost);
+  // a window may begin inside a tile, and so reach one more
+  const int64_t tiles = items * ((seen + tile - 1) / tile + (a.window > 0 ? 1 : 0) + cost);
   LC_REQUIRE(tiles < (1ll << 31) - (1 << 20), LC_ERR_INVALID, "more slots than one call can split");
   most = std::min(most, kPagedMaxBlocks);
   return (int)std::max<int64_t>(1, std::min<int64_t>(most, (tiles + a.min_tiles - 1) / a.min_tiles));

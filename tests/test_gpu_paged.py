@@ -725,3 +725,18 @@ def test_expanded_pools_are_refused(lc, gpu):
             lc.PagedKvCache(row.expand(shape), row.clone().expand(shape), max_seqs=1, max_pages_per_seq=1, max_q_heads=2)
     lone = torch.zeros(64, dtype=torch.bfloat16, device="cuda").as_strided((1, 1, 1, 1, 64), (0, 0, 0, 0, 1))
     lc.PagedKvCache(lone, lone.clone().as_strided((1, 1, 1, 1, 64), (0, 0, 0, 0, 1)), max_seqs=1, max_pages_per_seq=1, max_q_heads=1)
+
+
+def test_too_many_slots_for_a_call(lc, gpu):
+    """2^21 items of 991 tiles and, where their window begins inside one, 992, of 16 slots: with what an item costs
+    beside, one more than 31 bits count, and refused; a little shorter windows fit, here of lengths 0."""
+    seqs, kv, page, dim = 2048, 1024, 4096, 8
+    k, v = (torch.zeros((1, 1, kv, page, dim), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    cache = lc.PagedKvCache(k, v, max_seqs=seqs, max_pages_per_seq=5, max_q_heads=kv)
+    tables = torch.zeros((seqs, 5), dtype=torch.int32, device="cuda")
+    ln = torch.zeros(seqs, dtype=torch.int32, device="cuda")
+    q = torch.ones((seqs, kv, dim), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(lc.LumenError) as e:
+        cache.attn(0, tables, ln, q, 1.0, window=991 * 16)
+    assert e.value.code == lc.LC_ERR_INVALID
+    assert (cache.attn(0, tables, ln, q, 1.0, window=989 * 16) == 0).all()
