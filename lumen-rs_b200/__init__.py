@@ -844,7 +844,7 @@ def _need_torch():
         _FLOAT_CODES.update({torch.float32: LC_F32, torch.bfloat16: LC_BF16, torch.float16: LC_F16})
         _TORCH.update({"f32": torch.float32, "int32": torch.int32, "uint8": torch.uint8,
                        "empty": torch.empty, "empty_like": torch.empty_like,
-                       "raw_stream": torch._C._cuda_getCurrentRawStream})
+                       "raw_stream": torch._C._cuda_getCurrentRawStream, "cuda": torch.cuda})
 
 
 def _dev(x, name: str, shape, dtype, device: int) -> int:
@@ -876,12 +876,23 @@ def _stream_on(stream, device: int) -> int:
     return stream if stream else CUDA_STREAM_LEGACY
 
 
+def _new_like(x, stream):
+    """An output like x from the memory that torch keeps for the stream it is written on: of the current stream's,
+    it could be a block that earlier work there has yet to write."""
+    if stream is None:
+        return _TORCH["empty_like"](x)
+    cuda, raw = _TORCH["cuda"], getattr(stream, "cuda_stream", stream)
+    with cuda.stream(cuda.ExternalStream(raw, x.device) if raw > CUDA_STREAM_LEGACY else cuda.default_stream(x.device)):
+        return _TORCH["empty_like"](x)
+
+
 class PagedKvCache:
     """Decode over an uncompressed paged cache (lc_paged): pools k_pages and
     v_pages [n_layers, n_pages, n_kv_heads, page_tokens, head_dim] on the GPU,
     contiguous in the last dimension (a permuted view of another page layout
     will do), owned by the caller and borrowed by this object. In every call
-    tables is int32 [n_seqs, pages] and lens int32 [n_seqs], on the GPU."""
+    tables is int32 [n_seqs, pages] and lens int32 [n_seqs], on the GPU. Outputs
+    that a call makes are torch's memory of the stream that it runs on."""
 
     def __init__(self, k_pages, v_pages, *, max_seqs: int, max_pages_per_seq: int, max_q_heads: int):
         _need_torch()
@@ -951,7 +962,7 @@ class PagedKvCache:
         shape = (n, heads, self.head_dim)
         at = _dev(q, "q", shape, None, self.device)
         if out is None:
-            out = _TORCH["empty_like"](q)
+            out = _new_like(q, stream)
         _check(lib().lc_paged_attn(self._h, layer, n, t, width, ln, at, _float_code(q, "q"), heads, scale, window,
                                    _dev(out, "out", shape, None, self.device), _float_code(out, "out"),
                                    _stream_on(stream, self.device)))
@@ -966,7 +977,7 @@ class PagedKvCache:
         shape, rows = (n, heads, self.head_dim), (n, self.n_kv_heads, span)
         at = _dev(q, "q", shape, None, self.device)
         if out is None:
-            out = _TORCH["empty_like"](q)
+            out = _new_like(q, stream)
         acc_out = acc_in if acc_out is None else acc_out
         _check(lib().lc_paged_attn_weights(
             self._h, layer, n, t, width, ln, at, _float_code(q, "q"), heads, scale, window,
@@ -999,7 +1010,7 @@ class PagedKvCache:
         shape = (groups * beams, tables.shape[1])
         t = _dev(tables, "tables", shape, "int32", self.device)
         if tables_out is None:
-            tables_out = tables.new_empty(shape)
+            tables_out = _new_like(tables, stream)
         _check(lib().lc_paged_reorder(self._h, groups, beams, t, shape[1],
                                       _dev(lens, "lens", (groups,), "int32", self.device),
                                       _dev(parents, "parents", (groups, beams), "int32", self.device),
@@ -1010,7 +1021,8 @@ class PagedKvCache:
 
 class BeamSearch:
     """Beam search's selection over beams and vocabulary (lc_beam), for up to
-    n_groups groups of n_beams rows; n_out (n_beams unless given) are chosen."""
+    n_groups groups of n_beams rows; n_out (n_beams unless given) are chosen.
+    Outputs are torch's memory of the stream that a call runs on."""
 
     def __init__(self, n_groups: int, n_beams: int, vocab: int, n_out: Optional[int] = None, device: int = 0):
         _need_torch()
@@ -1058,7 +1070,7 @@ class BeamSearch:
         fin = None if finished is None else _dev(finished, "finished", rows, "uint8", self.device)
         if self._like[0].shape != shape:
             self._like = [x.new_empty(shape) for x in self._like]
-        new, parents, tokens, done = map(_TORCH["empty_like"], self._like)
+        new, parents, tokens, done = [_new_like(x, stream) for x in self._like]
         _check(lib().lc_beam_select(self._h, g, logits.data_ptr(), _float_code(logits, "logits"), row, at, fin, eos_id,
                                     pad_id, new.data_ptr(), parents.data_ptr(), tokens.data_ptr(), done.data_ptr(),
                                     _stream_on(stream, self.device)))

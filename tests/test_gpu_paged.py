@@ -740,3 +740,40 @@ def test_too_many_slots_for_a_call(lc, gpu):
         cache.attn(0, tables, ln, q, 1.0, window=991 * 16)
     assert e.value.code == lc.LC_ERR_INVALID
     assert (cache.attn(0, tables, ln, q, 1.0, window=989 * 16) == 0).all()
+
+
+@pytest.mark.parametrize("name", ["attn", "weights", "reorder", "select"])
+def test_outputs_made_for_another_stream(lc, gpu, name):
+    """The current stream has yet to write blocks that are free by now; outputs of calls on other streams are not those."""
+    lens = [700, 90]
+    cache, tables, ln, _ = make(lc, lens, 8, 2, 128, 32, "bf16")
+    q = queries(2, 8, 128, "bf16", 11)
+    acc = torch.rand((2, 2, tables.shape[1] * 32), device="cuda")
+    beam = lc.BeamSearch(2, 4, 3011)
+    x, scores = torch.randn((2, 4, 3011), device="cuda"), torch.zeros((2, 4), device="cuda")
+    parents = torch.zeros((1, 2), dtype=torch.int32, device="cuda")
+
+    def call(stream):
+        if name == "attn":
+            return [cache.attn(1, tables, ln, q, 0.1, stream=stream)]
+        if name == "weights":
+            return [cache.attn_weights(1, tables, ln, q, 0.1, acc, acc.clone() if stream is None else more, stream=stream)]
+        if name == "reorder":
+            return [cache.reorder(tables, full, parents, stream=stream)]
+        return beam.select(x, scores, stream=stream)
+
+    full, more = torch.tensor([64], dtype=torch.int32, device="cuda"), acc.clone()
+    want = [t.clone() for t in call(None)]
+    side = torch.cuda.Stream()
+    for stream in (side, side.cuda_stream):
+        torch.cuda.synchronize()
+        torch.cuda._sleep(100_000_000)
+        late = [torch.empty_like(t) for t in want for _ in range(64)]
+        for t in late:
+            t.fill_(1)
+        del late, t
+        got = call(stream)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for stream in (0, 1, torch.cuda.current_stream()):
+        assert all(torch.equal(a, b) for a, b in zip(call(stream), want))
