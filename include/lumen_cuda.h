@@ -583,7 +583,7 @@ int lc_paged_attn_weights(lc_paged* p, int32_t layer, int32_t n_seqs, const int3
  * longer names the newest tokens). acc_out and pos_out of slots budget ..
  * lens[s] - 1 become 0 and -1; shorter sequences are copied. The new length,
  * min(lens[s], budget), is the caller's to set once all layers are cut.
- * acc, pos: [n_seqs][n_kv_heads][stride]; the outputs may be the inputs. Pages
+ * acc, pos: [n_seqs][n_kv_heads][stride]; the outputs may be their inputs. Pages
  * must not be shared between sequences. */
 int lc_paged_evict(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* tables, int32_t width,
                    const int32_t* lens, int32_t budget, int32_t n_sink, int32_t n_recent, const float* acc_in,
@@ -596,7 +596,7 @@ int lc_paged_evict(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* ta
  * tail page (where it is partly filled) is every row's own: a parent's first
  * child keeps it; the i-th other child takes the tail page of the i-th row
  * without children, into which the parent's tokens are copied (all layers and
- * heads). Later pages stay with row j. tables_out must not overlap tables. */
+ * heads). Later pages stay with row j. tables_out must not overlap the inputs. */
 int lc_paged_reorder(lc_paged* p, int32_t n_groups, int32_t n_beams, const int32_t* tables, int32_t width,
                      const int32_t* lens, const int32_t* parents, int32_t* tables_out, void* stream);
 
@@ -619,7 +619,7 @@ int lc_beam_status(const lc_beam* b);
  * has the one candidate (pad, its score); -inf and NaN totals are none.
  * finished_out: the parent was finished, or the token is eos. A place without
  * a candidate holds -inf, parent place % n_beams, pad, finished. All tensors
- * are device memory; outputs must not overlap inputs. */
+ * are device memory; outputs must not overlap inputs or each other. */
 int lc_beam_select(lc_beam* b, int32_t n_groups, const void* logits, int32_t dtype, int64_t row_stride,
                    const float* scores, const uint8_t* finished, int32_t eos, int32_t pad, float* scores_out,
                    int32_t* parents, int32_t* tokens, uint8_t* finished_out, void* stream);

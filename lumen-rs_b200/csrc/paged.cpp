@@ -389,8 +389,8 @@ static void paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t
   check_device(q, p->cfg.device, "q", element_size(q_dtype));
   check_device(out, p->cfg.device, "out", element_size(out_dtype));
   const size_t values = (size_t)n_seqs * n_q_heads * p->cfg.head_dim;
-  LC_REQUIRE(!overlap(q, values * element_size(q_dtype), out, values * element_size(out_dtype)), LC_ERR_INVALID,
-             "out overlaps q");
+  const size_t out_bytes = values * element_size(out_dtype);
+  LC_REQUIRE(!overlap(q, values * element_size(q_dtype), out, out_bytes), LC_ERR_INVALID, "out overlaps q");
   a.q = q;
   a.out = out;
   a.q_dtype = q_dtype;
@@ -410,7 +410,11 @@ static void paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t
     check_device(acc_in, p->cfg.device, "acc_in", 4);
     check_device(acc_out, p->cfg.device, "acc_out", 4);
     LC_REQUIRE(acc_stride >= cap, LC_ERR_INVALID, "acc rows shorter than the table");
-    check_in_place(acc_in, acc_out, (size_t)n_seqs * p->cfg.n_kv_heads * acc_stride * 4, "acc");
+    const size_t acc_bytes = (size_t)n_seqs * p->cfg.n_kv_heads * acc_stride * 4;
+    check_in_place(acc_in, acc_out, acc_bytes, "acc");
+    LC_REQUIRE(!overlap(out, out_bytes, acc_in, acc_bytes) && !overlap(out, out_bytes, acc_out, acc_bytes) &&
+                   !overlap(q, values * element_size(q_dtype), acc_out, acc_bytes),
+               LC_ERR_INVALID, "acc overlaps q or out");
     const size_t rows = (size_t)n_seqs * n_q_heads;
     a.score_tokens = cap;
     a.scores =
@@ -479,6 +483,8 @@ int lc_paged_evict(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* ta
     check_in_place(acc_in, acc_out, row_bytes, "acc");
     check_in_place(pos_in, pos_out, row_bytes, "pos");
     LC_REQUIRE(!overlap(acc_out, row_bytes, pos_out, row_bytes), LC_ERR_INVALID, "acc_out overlaps pos_out");
+    LC_REQUIRE(!overlap(acc_out, row_bytes, pos_in, row_bytes) && !overlap(pos_out, row_bytes, acc_in, row_bytes),
+               LC_ERR_INVALID, "an output overlaps the other's input");
     a.layer = layer;
     a.n_seqs = n_seqs;
     a.esize = p->esize;
@@ -519,7 +525,10 @@ int lc_paged_reorder(lc_paged* p, int32_t n_groups, int32_t n_beams, const int32
     check_device(parents, p->cfg.device, "parents", 4);
     check_device(tables_out, p->cfg.device, "tables_out", 4);
     const size_t bytes = (size_t)n_groups * n_beams * width * 4;
-    LC_REQUIRE(!overlap(tables, bytes, tables_out, bytes), LC_ERR_INVALID, "tables_out overlaps tables");
+    LC_REQUIRE(!overlap(tables, bytes, tables_out, bytes) &&
+                   !overlap(parents, (size_t)n_groups * n_beams * 4, tables_out, bytes) &&
+                   !overlap(lens, (size_t)n_groups * 4, tables_out, bytes),
+               LC_ERR_INVALID, "tables_out overlaps an input");
     a.n_groups = n_groups;
     a.n_beams = n_beams;
     a.esize = p->esize;
@@ -593,8 +602,17 @@ int lc_beam_select(lc_beam* b, int32_t n_groups, const void* logits, int32_t dty
     check_device(tokens, b->device, "tokens", 4);
     check_device(finished_out, b->device, "finished_out", 1);
     const size_t in = (size_t)n_groups * b->n_beams, out = (size_t)n_groups * b->n_out;
-    LC_REQUIRE(!overlap(scores, in * 4, scores_out, out * 4) && !(finished && overlap(finished, in, finished_out, out)),
-               LC_ERR_INVALID, "outputs overlap inputs");
+    const std::pair<const void*, size_t> ins[3] = {
+        {logits, ((in - 1) * row_stride + b->vocab) * element_size(dtype)}, {scores, in * 4}, {finished, in}};
+    const std::pair<const void*, size_t> outs[4] = {
+        {scores_out, out * 4}, {parents, out * 4}, {tokens, out * 4}, {finished_out, out}};
+    for (int o = 0; o < 4; ++o) {
+      for (const auto& [p, bytes] : ins)
+        LC_REQUIRE(!p || !overlap(p, bytes, outs[o].first, outs[o].second), LC_ERR_INVALID, "outputs overlap inputs");
+      for (int other = 0; other < o; ++other)
+        LC_REQUIRE(!overlap(outs[other].first, outs[other].second, outs[o].first, outs[o].second), LC_ERR_INVALID,
+                   "outputs overlap each other");
+    }
     const Turn turn(b->order, stream);
     const cudaStream_t s = turn.s;
     const size_t keys = b->lists * b->n_out;

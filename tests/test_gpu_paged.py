@@ -777,3 +777,41 @@ def test_outputs_made_for_another_stream(lc, gpu, name):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     for stream in (0, 1, torch.cuda.current_stream()):
         assert all(torch.equal(a, b) for a, b in zip(call(stream), want))
+
+
+def test_overlaps_with_other_inputs_are_refused(lc, gpu):
+    """An output in the place of an input that is not its own, or of another output."""
+    k = torch.zeros((1, 4, 2, 16, 64), dtype=torch.bfloat16, device="cuda")
+    cache = lc.PagedKvCache(k, k.clone(), max_seqs=2, max_pages_per_seq=2, max_q_heads=2)
+    tables = torch.zeros((2, 2), dtype=torch.int32, device="cuda")
+    ln = torch.ones(2, dtype=torch.int32, device="cuda")
+    acc, pos = torch.zeros((2, 2, 32), device="cuda"), torch.zeros((2, 2, 32), dtype=torch.int32, device="cuda")
+    both = torch.zeros((2, 2, 64), device="cuda")  # q or out, and in its storage rows of weights
+    rows, ints = both.view(-1)[:128].view(2, 2, 32), torch.zeros(16, dtype=torch.int32, device="cuda")
+
+    def refused(f, *args, **kw):
+        with pytest.raises(lc.LumenError) as e:
+            f(*args, **kw)
+        assert e.value.code == lc.LC_ERR_INVALID
+
+    refused(cache.evict, 0, tables, ln, 8, acc, pos, pos.view(torch.float32), torch.empty_like(pos))
+    refused(cache.evict, 0, tables, ln, 8, acc, pos, torch.empty_like(acc), acc.view(torch.int32))
+    refused(cache.attn_weights, 0, tables, ln, both, 1.0, acc, rows)
+    refused(cache.attn_weights, 0, tables, ln, torch.ones_like(both), 1.0, acc, rows, out=both)
+    refused(cache.attn_weights, 0, tables, ln, torch.ones_like(both), 1.0, rows, acc, out=both)
+    refused(cache.reorder, tables, ln[:1], ints[:2].view(1, 2), ints[1:5].view(2, 2))
+    refused(cache.reorder, tables, ints[:1], ints[8:10].view(1, 2), ints[:4].view(2, 2))
+    # the selection's, at the C entry
+    logits, scores = torch.zeros((1, 2, 100), device="cuda"), torch.zeros((1, 2), device="cuda")
+    beam, outs = lc.BeamSearch(1, 2, 100), torch.zeros(64, device="cuda")
+    at = [outs.data_ptr(), outs.data_ptr() + 32, outs.data_ptr() + 64, outs.data_ptr() + 96]
+
+    def select(a):
+        return lc.lib().lc_beam_select(beam._h, 1, logits.data_ptr(), lc.LC_F32, 100, scores.data_ptr(), None, -1, 0, *a, None)
+
+    torch.cuda.synchronize()
+    assert select(at) == lc.LC_OK
+    for o in range(4):
+        for other in (logits.data_ptr() + 796, scores.data_ptr() + 4, at[(o + 1) % 4]):
+            assert select(at[:o] + [other] + at[o + 1:]) == lc.LC_ERR_INVALID
+    torch.cuda.synchronize()
