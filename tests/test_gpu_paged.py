@@ -815,3 +815,39 @@ def test_overlaps_with_other_inputs_are_refused(lc, gpu):
         for other in (logits.data_ptr() + 796, scores.data_ptr() + 4, at[(o + 1) % 4]):
             assert select(at[:o] + [other] + at[o + 1:]) == lc.LC_ERR_INVALID
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("slots", [3000, 20000, 140000])
+def test_tables_much_wider_than_the_sequences(lc, gpu, dtype, slots):
+    """Tables for up to `slots`, none of their unused pages in the pool: the same answers as under tight ones."""
+    lens, page, kv, dim = [1025, 0, 700, 64], 32, 2, 64
+    cache, tables, ln, rows = make(lc, lens, 8, kv, dim, page, dtype, seed=9)
+    width = slots // page
+    wide = torch.full((4, width), -1, dtype=torch.int32, device="cuda")
+    wide[:, :tables.shape[1]] = tables
+    k0, v0 = cache.k_pages.clone(), cache.v_pages.clone()
+    q = queries(4, 8, dim, dtype, 3)
+    g = torch.Generator().manual_seed(2)
+    acc = torch.rand((4, kv, tables.shape[1] * page), generator=g).cuda()
+    pos = torch.arange(acc.shape[2], dtype=torch.int32, device="cuda").expand_as(acc).contiguous()
+    got = []
+    for t in (tables, wide):
+        handle = lc.PagedKvCache(k0.clone(), v0.clone(), max_seqs=4, max_pages_per_seq=width, max_q_heads=8)
+        a, p = (torch.zeros((4, kv, t.shape[1] * page), dtype=x.dtype, device="cuda") for x in (acc, pos))
+        a[:, :, :acc.shape[2]], p[:, :, :acc.shape[2]] = acc, pos
+        for window in (0, 100):
+            check(handle.attn(1, t, ln, q, 0.125, window=window), ref.attn(rows, q, 0.125, window)[0], dtype)
+        add = torch.zeros_like(a)
+        check(handle.attn_weights(1, t, ln, q, 0.125, add), ref.attn(rows, q, 0.125)[0], dtype)
+        handle.evict(1, t, ln, 600, a, p, n_sink=4, n_recent=30)
+        handle.evict(1, t, torch.clamp(ln, max=600), 599, a, p, n_sink=4, n_recent=30)
+        assert handle.status() == lc.LC_OK
+        n = acc.shape[2]
+        got.append([a[:, :, :n], p[:, :, :n]] + [x.contiguous().view(torch.uint8) for x in (handle.k_pages, handle.v_pages)])
+        w = ref.attn(rows, q, 0.125)[1]
+        for s, m in enumerate(lens):
+            want = w[s].view(kv, 4, m).sum(1)
+            # as in test_weights_match_plain
+            assert ((add[s, :, :m].double().cpu() - want).abs() <= 1e-4 * want + 2e-6).all()
+    assert all(torch.equal(x, y) for x, y in zip(*got))
