@@ -40,6 +40,13 @@ struct PagedView {
   int32_t* status;  // mapped host words, by StatusBit
 };
 
+// Rows and strides of whole 16-byte units.
+inline bool vector_rows(const PagedView& c, int esize) {
+  const int64_t e = 16 / esize;
+  return c.d % e == 0 && c.layer % e == 0 && c.page % e == 0 && c.head % e == 0 && c.token % e == 0 &&
+         (reinterpret_cast<uintptr_t>(c.k) & 15) == 0 && (reinterpret_cast<uintptr_t>(c.v) & 15) == 0;
+}
+
 // TMA descriptors of the two pools; box: slots of a load, 0 where there are none.
 struct PagedMaps {
   CUtensorMap k, v;

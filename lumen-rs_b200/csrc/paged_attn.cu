@@ -1144,13 +1144,6 @@ void launch_mma(PagedAttnArgs& a, const PagedMaps& maps, int device, int sms, cu
   }
 }
 
-// Rows and strides of whole 16-byte units.
-bool vector_rows(const PagedView& c, int esize) {
-  const int64_t e = 16 / esize;
-  return c.d % e == 0 && c.layer % e == 0 && c.page % e == 0 && c.head % e == 0 && c.token % e == 0 &&
-         (reinterpret_cast<uintptr_t>(c.k) & 15) == 0 && (reinterpret_cast<uintptr_t>(c.v) & 15) == 0;
-}
-
 }  // namespace
 
 int64_t paged_part_floats(int32_t sms) { return 2ll * (2 * sms) * 8 * (kPagedMaxDim + 2); }

@@ -454,13 +454,6 @@ __global__ void __launch_bounds__(kReorderThreads) k_paged_reorder(const PagedRe
   }
 }
 
-// Rows and strides of whole 16-byte units.
-bool vector_rows(const PagedView& c, int esize) {
-  const int64_t e = 16 / esize;
-  return c.d % e == 0 && c.layer % e == 0 && c.page % e == 0 && c.head % e == 0 && c.token % e == 0 &&
-         (reinterpret_cast<uintptr_t>(c.k) & 15) == 0 && (reinterpret_cast<uintptr_t>(c.v) & 15) == 0;
-}
-
 // The view with strides and d in units of U.
 template <typename U>
 PagedView in_units(PagedView c, int esize) {
