@@ -568,7 +568,8 @@ int lc_paged_attn(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* tab
 /* lc_paged_attn, and acc_out[s][h][t] = decay * acc_in[s][h][t] + the sum over
  * kv head h's query heads of slot t's attention weight, for t < lens[s] (other
  * entries are not written). acc: f32 [n_seqs][n_kv_heads][acc_stride]; acc_out
- * may be acc_in. */
+ * may be acc_in. Its workspace holds n_seqs * n_q_heads * width * page_tokens
+ * floats: give tables no wider than the longest sequence needs. */
 int lc_paged_attn_weights(lc_paged* p, int32_t layer, int32_t n_seqs, const int32_t* tables, int32_t width,
                           const int32_t* lens, const void* q, int32_t q_dtype, int32_t n_q_heads, float scale,
                           int32_t window, void* out, int32_t out_dtype, const float* acc_in, float* acc_out,

@@ -329,8 +329,10 @@ __device__ __forceinline__ void cp_wait() {
 // 65536 slots, 8 heads of 128 under 32 queries takes 92 us, 5.9 TB/s, with 11
 // warps, 93 with 10, 96 with 8, and 98 with 4 of three stages of tiles twice
 // as long; one of 131072, 4 heads of 256, 167 and 201. Under 8 queries a head
-// the products themselves do: 4 of 81000 slots, 2 heads of 96, 165 us, of which
-// 76 the bytes. One of 19 slots, 2 heads of 80: 5.5, the launch and one tile.
+// the reads of q do, eight of 16 bytes for one of K: 4 of 81000 slots, 2 heads
+// of 96, 165 us, of which 76 the bytes; shared memory's port is busy 72 % of
+// it, the FMA pipes 28 %. One of 19 slots, 2 heads of 80: 5.4, the launch and
+// one tile.
 // ST = 1: 16-bit pools by 16-byte loads into registers (VEC), or any alignment
 // and type, value by value: 32 sequences of 2048 slots, 8 heads of 128 bf16
 // under f32 queries take 129 us so and 470 value by value, bound by their
@@ -667,13 +669,13 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
 // instructions of a tile, and a warp that has eight to share an SM with must
 // not take longer than the SM's share of the HBM does.
 //
-// 32 sequences of 8192 slots, 8 kv heads of 128 bf16: 176 us, 6.1 TB/s, 0.93 of
-// a plain copy; the tensor pipe is busy 16 % and the issue slots 24 %. One of
-// 131072: 94 us, 5.7 TB/s. What is left is the first loads' latency (4.5 us),
+// 32 sequences of 8192 slots, 8 kv heads of 128 bf16: 174 us, 6.2 TB/s, 0.94 of
+// a plain copy; the tensor pipe is busy 21 % and the issue slots 28 %. One of
+// 131072: 95 us, 5.7 TB/s. What is left is the first loads' latency (4.5 us),
 // items' ends and beginnings (3.7 us each) and SMs that reach the memory at
 // different speeds (blocks with equal shares end between 0.75 and 1 of the
 // whole time). 16 sequences of up to 4096 under a window of 1024, 8 heads of
-// 256 f16: 28.8 us, 4.0 TB/s, where the first two are a third.
+// 256 f16: 29.1 us, 3.9 TB/s, where the first two are a third.
 template <typename T, int DP, int W, int ST, bool TMA, int PER_SM>
 __global__ void __launch_bounds__(W * 32, PER_SM)
     k_paged_attn_mma(const PagedAttnArgs a, const __grid_constant__ CUtensorMap k_map,
@@ -1054,7 +1056,7 @@ __device__ __forceinline__ void from_f32(float x, __half& y) { y = __float2half_
 // New tokens' K and V rows into their pages, converted. A warp takes four
 // (token, head) rows at a time, V elements of K or V a lane: V fills 16 bytes
 // of the pool where rows are whole 16-byte units. Bound by the bytes of both:
-// 32 x 2048 tokens of 8 heads of 128 bf16 take 110 us, 4.9 TB/s read and
+// 32 x 2048 tokens of 8 heads of 128 bf16 take 108 us, 5.0 TB/s read and
 // written; value by value (head dimension 100) 194 us, 2.2 TB/s.
 constexpr int kAppendRows = 4;
 template <typename TI, typename TO, int V>
